@@ -8,7 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_size_t, c_void_p
+from ctypes import (POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t,
+                    c_void_p)
 
 MAX_LEVELS = 8
 MAX_EDGES = 56
@@ -52,11 +53,27 @@ class GpaStateRef(ctypes.Structure):
                 ("moment", c_void_p * MAX_LEVELS)]
 
 
+class GpaNormArgs(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("residual", "update", "gate", "weight", "post_weight",
+                                        "scale")] + [
+        ("outer", c_int64), ("inner", c_int64), ("residual_stride", c_int64 * 2),
+        ("update_stride", c_int64 * 2), ("gate_stride", c_int64 * 2), ("width", c_int32),
+        ("stream_dtype", c_int32), ("update_dtype", c_int32), ("gate_dtype", c_int32),
+        ("out_dtype", c_int32), ("gate_mode", c_int32), ("eps", c_float),
+        ("scale_const", c_float)]
+
+
+class GpaNormGrads(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("dresidual", "dupdate", "dgate", "dweight",
+                                        "dpost_weight", "dscale")]
+
+
 EXPORTS = ("gpa_b200_saved_bytes", "gpa_b200_scratch_bytes", "gpa_b200_forward",
            "gpa_b200_backward", "gpa_b200_routes", "gpa_b200_last_error",
            "gpa_b200_abi_version", "gpa_b200_launch_count", "gpa_b200_profile_start",
            "gpa_b200_profile_stop", "gpa_b200_forward_noalloc", "gpa_b200_noalloc_capacity",
-           "gpa_b200_step", "gpa_b200_umma_selftest", "gpa_b200_device_status")
+           "gpa_b200_step", "gpa_b200_umma_selftest", "gpa_b200_device_status",
+           "gpa_b200_norm_forward", "gpa_b200_norm_scratch_bytes", "gpa_b200_norm_backward")
 
 _lib = None
 
@@ -98,6 +115,13 @@ def load():
     lib.gpa_b200_noalloc_capacity.restype = c_size_t
     lib.gpa_b200_routes.argtypes = [POINTER(GpaDims), c_void_p, POINTER(c_void_p), c_void_p]
     lib.gpa_b200_routes.restype = c_int
+    lib.gpa_b200_norm_forward.argtypes = [POINTER(GpaNormArgs), c_void_p, c_void_p, c_void_p]
+    lib.gpa_b200_norm_forward.restype = c_int
+    lib.gpa_b200_norm_scratch_bytes.argtypes = [POINTER(GpaNormArgs)]
+    lib.gpa_b200_norm_scratch_bytes.restype = c_size_t
+    lib.gpa_b200_norm_backward.argtypes = [POINTER(GpaNormArgs), c_void_p, c_void_p, c_void_p,
+                                           POINTER(GpaNormGrads), c_void_p, c_size_t, c_void_p]
+    lib.gpa_b200_norm_backward.restype = c_int
     lib.gpa_b200_last_error.argtypes = [c_char_p, c_size_t]
     lib.gpa_b200_last_error.restype = c_int
     lib.gpa_b200_abi_version.argtypes = []

@@ -20,6 +20,7 @@
 #include "decode.cuh"
 #include "gdn.cuh"
 #include "level.cuh"
+#include "norm.cuh"
 
 namespace gpa {
 
@@ -1096,6 +1097,25 @@ int gpa_b200_routes(const GpaDims* dims, const void* saved, void* const* routes,
     CK(launch_to_bthx(s.route[j], routes[j], g.dt, g.B, g.T, g.H, g.M[j], st));
   }
   return GPA_B200_OK;
+}
+
+int gpa_b200_norm_forward(const GpaNormArgs* args, void* stream_out, void* normed, void* stream) {
+  g_last_error.clear();
+  const char* why = "";
+  const int rc = gpa::norm_forward(args, stream_out, normed, static_cast<cudaStream_t>(stream), &why);
+  return rc ? fail(rc, why) : rc;
+}
+
+size_t gpa_b200_norm_scratch_bytes(const GpaNormArgs* args) { return gpa::norm_scratch_bytes(args); }
+
+int gpa_b200_norm_backward(const GpaNormArgs* args, const void* stream_in, const void* dstream,
+                           const void* dnormed, const GpaNormGrads* grads, void* scratch,
+                           size_t scratch_bytes, void* stream) {
+  g_last_error.clear();
+  const char* why = "";
+  const int rc = gpa::norm_backward(args, stream_in, dstream, dnormed, grads, scratch, scratch_bytes,
+                                    static_cast<cudaStream_t>(stream), &why);
+  return rc ? fail(rc, why) : rc;
 }
 
 int gpa_b200_last_error(char* buf, size_t len) {

@@ -1,0 +1,619 @@
+// Norms round a residual block (rows of `width` channels, all arithmetic in fp32):
+//   u = y r_y wp           r_y = rsqrt(mean y^2 + eps)      (u = y without a post weight)
+//   h' = h + c s(a) u      c: constant times an optional scale of every channel, s: sigmoid of an
+//                          optional gate (one value per channel or one per row); h' is rounded
+//                          once, to the stream's type
+//   n  = h' r w            r = rsqrt(mean h'^2 + eps), from the rounded h'
+// and, without a stream, n = y r w (plain RMS norm).  Backward, with G the gradient of h':
+//   G  = dh' + r (w dn - h' r^2 mean(w dn h'))    dh = G      dw = sum_rows dn h' r
+//   du = G c s     da = G c u s (1 - s)     dc = sum_rows G s u
+//   dy = r_y (wp du - y r_y^2 mean(wp du y))      dwp = sum_rows du y r_y
+// The statistics are formed again from the rows themselves, which the backward reads anyway.
+//
+// A group of G threads owns a row, each thread VEC consecutive channels at a time: sub-warp
+// groups for narrow rows (several rows per warp), whole blocks for wide ones.  Rows are read
+// once; the bound is the bytes moved.  Column sums of the backward stay in registers over a
+// block's rows, go to one partial row per block and are added in block order by a second
+// kernel, so results do not depend on scheduling.
+#include "../../include/gpa_b200.h"
+#include "common.cuh"
+#include "norm.cuh"
+
+#include <algorithm>
+
+namespace gpa {
+namespace {
+
+struct Rows {  // row r of a strided [outer, inner, width] tensor, unit stride along the width
+  int64_t so, si;
+};
+
+struct Fwd {
+  const void *h, *y, *gate;
+  const float *w, *wp, *scale;
+  void *stream, *out;
+  Rows rh, ry, rg;
+  uint32_t rows, inner;
+  int width, h_dt, y_dt, g_dt, out_dt, gate_full;
+  float eps, c;
+};
+
+struct Bwd {
+  Fwd f;                  // stream: the rounded h' of the forward (NULL for the plain norm)
+  const void *dn, *ds;    // contiguous gradients of n and h' (either may be NULL)
+  void *dh, *dy, *dgate;
+  float *part;            // [blocks][sums][width]
+  int sum_w, sum_p, sum_c, sums;  // slot of dw / dwp / dc in a partial row, or -1
+};
+
+template <int VEC>
+GPA_DEV void ldv(const void* p, int64_t i, int dt, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = load_in(p, i, dt);
+  } else {
+    if (dt == kF32) {
+      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+      const float4 a = q[0], b = q[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+      const uint32_t s[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float2 f;
+        if (dt == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&s[k]));
+        else f = __half22float2(*reinterpret_cast<const __half2*>(&s[k]));
+        v[2 * k] = f.x, v[2 * k + 1] = f.y;
+      }
+    }
+  }
+}
+
+template <int VEC>
+GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    store_out(p, i, v[0], dt);
+  } else {
+    if (dt == kF32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+      q[0] = make_float4(v[0], v[1], v[2], v[3]);
+      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t s[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (dt == kBF16) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+          s[k] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          const __half2 b = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+          s[k] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(s[0], s[1], s[2], s[3]);
+    }
+  }
+}
+
+GPA_DEV float round_to(float x, int dt) {
+  if (dt == kBF16) return __bfloat162float(__float2bfloat16(x));
+  if (dt == kF16) return __half2float(__float2half(x));
+  return x;
+}
+
+// Sums of NV values over the group: shuffles inside a warp (G <= 32), or shuffles and one pass
+// through shared memory (G == 0: the whole block).  `buf` alternates between two shared arrays,
+// so one barrier per sum is enough.
+template <int G, int NV>
+GPA_DEV void group_sum(float (&v)[NV], float (*sm)[3][32], int& buf) {
+  constexpr int kW = G == 0 ? 32 : G;
+#pragma unroll
+  for (int o = kW / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < NV; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if constexpr (G == 0) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
+    if (nw > 1) {
+      if (lane == 0)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) sm[buf][k][warp] = v[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float s = lane < nw ? sm[buf][k][lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        v[k] = s;
+      }
+      buf ^= 1;
+    }
+  }
+}
+
+GPA_DEV int64_t row_at(const Rows& r, uint32_t row, uint32_t inner) {
+  if (r.so == r.si * (int64_t)inner) return (int64_t)row * r.si;
+  const uint32_t o = row / inner;
+  return (int64_t)o * r.so + (int64_t)(row - o * inner) * r.si;
+}
+
+template <int G, int VEC, int ITER, int MT>
+__global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
+  __shared__ float sm[2][3][32];
+  int buf = 0;
+  const int g = G == 0 ? (int)blockDim.x : G;
+  const int t = G == 0 ? (int)threadIdx.x : (int)(threadIdx.x % G);
+  const uint32_t per = G == 0 ? 1u : blockDim.x / G;
+  const uint32_t row = blockIdx.x * per + (G == 0 ? 0u : threadIdx.x / G);
+  const bool live = row < p.rows;  // idle groups of a warp still take part in its shuffles
+  const bool plain = p.h == nullptr;
+  const float inv = 1.f / (float)p.width;
+  float x[ITER][VEC];
+  const int64_t oy = live ? row_at(p.ry, row, p.inner) : 0;
+  float s1[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * g + t) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[i][k] = 0.f;
+    if (live && c < p.width) ldv<VEC>(p.y, oy + c, p.y_dt, x[i]);
+  }
+  const int64_t at = (int64_t)row * p.width;
+  if (!plain) {
+    float ry = 1.f;
+    if (p.wp) {
+#pragma unroll
+      for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s1[0] += x[i][k] * x[i][k];
+      group_sum<G, 1>(s1, sm, buf);
+      ry = rsqrtf(s1[0] * inv + p.eps);
+    }
+    const int64_t oh = live ? row_at(p.rh, row, p.inner) : 0;
+    const int64_t og = live && p.gate ? row_at(p.rg, row, p.inner) : 0;
+    float gr = p.c;
+    if (live && p.gate && !p.gate_full) gr *= sigmoid(load_in(p.gate, og, p.g_dt));
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * g + t) * VEC;
+      if (!live || c >= p.width) continue;
+      float h[VEC], m[VEC];
+      ldv<VEC>(p.h, oh + c, p.h_dt, h);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) m[k] = gr;
+      if (p.gate && p.gate_full) {
+        float a[VEC];
+        ldv<VEC>(p.gate, og + c, p.g_dt, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m[k] *= sigmoid(a[k]);
+      }
+      if (p.scale) {
+        float a[VEC];
+        ldv<VEC>(p.scale, c, kF32, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m[k] *= a[k];
+      }
+      if (p.wp) {
+        float a[VEC];
+        ldv<VEC>(p.wp, c, kF32, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[i][k] *= ry * a[k];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[i][k] = round_to(fmaf(m[k], x[i][k], h[k]), p.h_dt);
+      stv<VEC>(p.stream, at + c, p.h_dt, x[i]);
+    }
+  }
+  float s2[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < ITER; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s2[0] += x[i][k] * x[i][k];
+  group_sum<G, 1>(s2, sm, buf);
+  const float r = rsqrtf(s2[0] * inv + p.eps);
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * g + t) * VEC;
+    if (!live || c >= p.width) continue;
+    float w[VEC];
+    ldv<VEC>(p.w, c, kF32, w);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) w[k] *= x[i][k] * r;
+    stv<VEC>(p.out, at + c, p.out_dt, w);
+  }
+}
+
+template <int G, int VEC, int ITER, int MT>
+__global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
+  const Fwd& p = b.f;
+  __shared__ float sm[2][3][32];
+  extern __shared__ float fold[];  // sub-warp groups: [blockDim / G][G * VEC * ITER]
+  int buf = 0;
+  const int g = G == 0 ? (int)blockDim.x : G;
+  const int t = G == 0 ? (int)threadIdx.x : (int)(threadIdx.x % G);
+  const uint32_t per = G == 0 ? 1u : blockDim.x / G;
+  const uint32_t mine = G == 0 ? 0u : threadIdx.x / G;
+  const bool plain = p.h_dt < 0;
+  const float inv = 1.f / (float)p.width;
+  float aw[ITER][VEC], ap[ITER][VEC], ac[ITER][VEC];
+#pragma unroll
+  for (int i = 0; i < ITER; ++i)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) aw[i][k] = ap[i][k] = ac[i][k] = 0.f;
+  const uint32_t step = gridDim.x * per;
+  for (uint32_t base = blockIdx.x * per; base < p.rows; base += step) {
+    const uint32_t row = base + mine;
+    const bool live = row < p.rows;
+    const int64_t at = (int64_t)row * p.width;
+    const int64_t oy = live ? row_at(p.ry, row, p.inner) : 0;
+    const int64_t og = live && p.gate ? row_at(p.rg, row, p.inner) : 0;
+    const bool use_y = !plain && p.y != nullptr;
+    float x[ITER][VEC], d[ITER][VEC], y[ITER][VEC];
+    float s[3] = {0.f, 0.f, 0.f};  // x^2, w dn x, y^2
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * g + t) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[i][k] = d[i][k] = y[i][k] = 0.f;
+      if (!live || c >= p.width) continue;
+      if (plain) ldv<VEC>(p.y, oy + c, p.y_dt, x[i]);
+      else ldv<VEC>(p.stream, at + c, p.h_dt, x[i]);
+      if (b.dn) ldv<VEC>(b.dn, at + c, p.out_dt, d[i]);
+      if (use_y) ldv<VEC>(p.y, oy + c, p.y_dt, y[i]);
+      float w[VEC];
+      ldv<VEC>(p.w, c, kF32, w);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        s[0] += x[i][k] * x[i][k];
+        s[1] += w[k] * d[i][k] * x[i][k];
+        s[2] += y[i][k] * y[i][k];
+      }
+    }
+    group_sum<G, 3>(s, sm, buf);
+    const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
+    const float ry = p.wp ? rsqrtf(s[2] * inv + p.eps) : 1.f;
+    float gr = 1.f;
+    if (live && p.gate && !p.gate_full) gr = sigmoid(load_in(p.gate, og, p.g_dt));
+    float s2[2] = {0.f, 0.f};  // wp du y, row-gate gradient
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * g + t) * VEC;
+      if (!live || c >= p.width) continue;
+      float w[VEC], a[VEC];
+      ldv<VEC>(p.w, c, kF32, w);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        aw[i][k] += d[i][k] * x[i][k] * r;
+        d[i][k] = r * (w[k] * d[i][k] - x[i][k] * q);
+      }
+      if (b.ds) {
+        ldv<VEC>(b.ds, at + c, p.h_dt, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) d[i][k] += a[k];
+      }
+      if (plain) {
+        stv<VEC>(b.dy, at + c, p.y_dt, d[i]);
+        continue;
+      }
+      if (b.dh) stv<VEC>(b.dh, at + c, p.h_dt, d[i]);
+      float wp[VEC], cs[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) wp[k] = 1.f, cs[k] = p.c;
+      if (p.wp) ldv<VEC>(p.wp, c, kF32, wp);
+      if (p.scale) {
+        ldv<VEC>(p.scale, c, kF32, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) cs[k] *= a[k];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) a[k] = gr;
+      if (p.gate && p.gate_full) {
+        ldv<VEC>(p.gate, og + c, p.g_dt, a);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) a[k] = sigmoid(a[k]);
+      }
+      float dg[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float u = y[i][k] * ry * wp[k], G_ = d[i][k];
+        ac[i][k] += G_ * a[k] * u * p.c;
+        dg[k] = G_ * cs[k] * u * a[k] * (1.f - a[k]);
+        s2[1] += dg[k];
+        const float du = G_ * cs[k] * a[k];
+        ap[i][k] += du * y[i][k] * ry;
+        d[i][k] = du * wp[k];
+        s2[0] += d[i][k] * y[i][k];
+      }
+      if (p.gate && p.gate_full && b.dgate) stv<VEC>(b.dgate, at + c, p.g_dt, dg);
+    }
+    if (plain) continue;
+    const bool row_gate = p.gate && !p.gate_full && b.dgate;
+    if (p.wp || row_gate) group_sum<G, 2>(s2, sm, buf);
+    if (row_gate && live && t == 0) store_out(b.dgate, row, s2[1], p.g_dt);
+    if (!b.dy) continue;
+    const float qy = p.wp ? s2[0] * inv * ry * ry : 0.f;
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * g + t) * VEC;
+      if (!live || c >= p.width) continue;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) d[i][k] = ry * (d[i][k] - y[i][k] * qy);
+      stv<VEC>(b.dy, at + c, p.y_dt, d[i]);
+    }
+  }
+  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
+  auto emit = [&](int slot, const float (&a)[ITER][VEC]) {
+    if (slot < 0) return;
+    float* dst = part + (int64_t)slot * p.width;
+    if constexpr (G == 0) {
+#pragma unroll
+      for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const int c = (i * g + t) * VEC + k;
+          if (c < p.width) dst[c] = a[i][k];
+        }
+    } else {
+      constexpr int kCols = G * VEC * ITER;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ITER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) fold[mine * kCols + (i * G + t) * VEC + k] = a[i][k];
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
+        float s = 0.f;
+        for (uint32_t j = 0; j < per; ++j) s += fold[j * kCols + c];
+        dst[c] = s;
+      }
+    }
+  };
+  emit(b.sum_w, aw);
+  emit(b.sum_p, ap);
+  emit(b.sum_c, ac);
+}
+
+// out[c] = sum over blocks of part[block][c], always in the same order: 8 lanes for 32 columns,
+// each adding every eighth block, then the lanes one after another.
+__global__ void k_norm_fold(const float* part, int blocks, int64_t pitch, int cols, float* out) {
+  __shared__ float sm[8][33];
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < cols)
+    for (int b = threadIdx.y; b < blocks; b += 8) s += part[b * pitch + c];
+  sm[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < cols) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += sm[j][threadIdx.x];
+    out[c] = s;
+  }
+}
+
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool strides8(const Rows& r) { return r.so % 8 == 0 && r.si % 8 == 0; }
+
+// Threads of a row: 8 consecutive channels each where every row starts on a 16-byte boundary
+// (one or two 16-byte accesses), else one channel each.
+struct Shape {
+  int vec, group, iter, threads;  // group 0: the block
+};
+
+Shape shape_of(const Fwd& f, bool vec) {
+  Shape s;
+  s.vec = vec ? 8 : 1;
+  const int n = (f.width + s.vec - 1) / s.vec;  // thread-sized pieces of a row
+  if (n <= 32) {
+    s.group = 1;
+    while (s.group < n) s.group *= 2;
+    if (s.group < 4) s.group = 4;
+    s.iter = 1;
+    s.threads = 128;
+  } else {
+    s.group = 0;
+    s.iter = 1;
+    while ((n + s.iter - 1) / s.iter > 1024) s.iter *= 2;
+    s.threads = ((n + s.iter - 1) / s.iter + 31) / 32 * 32;
+  }
+  return s;
+}
+
+constexpr int kMaxWidth = 16384;
+
+}  // namespace
+
+// (group, vec, iter, most threads) of every shape that shape_of can return
+#define NORM_DISPATCH(S, CALL)                                      \
+  do {                                                              \
+    if ((S).vec == 8) {                                             \
+      if ((S).group == 4) { CALL(4, 8, 1, 128); }                   \
+      else if ((S).group == 8) { CALL(8, 8, 1, 128); }              \
+      else if ((S).group == 16) { CALL(16, 8, 1, 128); }            \
+      else if ((S).group == 32) { CALL(32, 8, 1, 128); }            \
+      else if ((S).iter == 1 && (S).threads <= 256) { CALL(0, 8, 1, 256); } \
+      else if ((S).iter == 1) { CALL(0, 8, 1, 1024); }              \
+      else { CALL(0, 8, 2, 1024); }                                 \
+    } else {                                                        \
+      if ((S).group == 4) { CALL(4, 1, 1, 128); }                   \
+      else if ((S).group == 8) { CALL(8, 1, 1, 128); }              \
+      else if ((S).group == 16) { CALL(16, 1, 1, 128); }            \
+      else if ((S).group == 32) { CALL(32, 1, 1, 128); }            \
+      else if ((S).iter == 1) { CALL(0, 1, 1, 1024); }              \
+      else if ((S).iter == 2) { CALL(0, 1, 2, 1024); }              \
+      else if ((S).iter == 4) { CALL(0, 1, 4, 1024); }              \
+      else if ((S).iter == 8) { CALL(0, 1, 8, 1024); }              \
+      else { CALL(0, 1, 16, 1024); }                                \
+    }                                                               \
+  } while (0)
+
+namespace {
+
+const char* fill(const GpaNormArgs* a, Fwd* f) {
+  if (!a) return "args is NULL";
+  if (a->outer < 0 || a->inner < 0 || a->width < 1) return "outer, inner and width must not be negative, width at least 1";
+  for (int dt : {a->stream_dtype, a->update_dtype, a->gate_dtype, a->out_dtype})
+    if (dt < 0 || dt > 2) return "dtypes must be F32, BF16 or F16";
+  if (!a->update && !a->residual) return "update must not be NULL";
+  if (a->gate_mode < 0 || a->gate_mode > 2) return "gate_mode must be 0, 1 or 2";
+  if (a->gate_mode && !a->gate) return "gate_mode needs a gate";
+  if (!a->residual && (a->gate_mode || a->post_weight || a->scale))
+    return "a norm without a residual takes no post weight, gate or scale";
+  if (!a->weight) return "weight must not be NULL";
+  f->h = a->residual;
+  f->y = a->update;
+  f->gate = a->gate_mode ? a->gate : nullptr;
+  f->w = a->weight;
+  f->wp = a->post_weight;
+  f->scale = a->scale;
+  f->stream = nullptr;
+  f->out = nullptr;
+  f->rh = {a->residual_stride[0], a->residual_stride[1]};
+  f->ry = {a->update_stride[0], a->update_stride[1]};
+  f->rg = {a->gate_stride[0], a->gate_stride[1]};
+  f->rows = (uint32_t)(a->outer * a->inner);
+  f->inner = (uint32_t)std::max<int64_t>(a->inner, 1);
+  f->width = a->width;
+  f->h_dt = a->residual ? a->stream_dtype : -1;
+  f->y_dt = a->update_dtype;
+  f->g_dt = a->gate_dtype;
+  f->out_dt = a->out_dtype;
+  f->gate_full = a->gate_mode == 2;
+  f->eps = a->eps;
+  f->c = a->scale_const;
+  return nullptr;
+}
+
+bool too_large(const GpaNormArgs* a) {
+  return a->width > kMaxWidth || (a->inner && a->outer > (int64_t)0x7fffffff / a->inner);
+}
+
+bool vec_ok(const Fwd& f) {
+  return f.width % 8 == 0 && aligned8(f.h) && aligned8(f.y) && aligned8(f.w) && aligned8(f.wp) &&
+         aligned8(f.scale) && aligned8(f.stream) && aligned8(f.out) &&
+         (!f.h || strides8(f.rh)) && strides8(f.ry) &&
+         (!f.gate_full || (aligned8(f.gate) && strides8(f.rg)));
+}
+
+// Blocks of the backward: a few per SM, each with many rows, so that its column sums are added
+// in registers and few partial rows are left.
+int bwd_blocks(const Shape& s, uint32_t rows) {
+  const uint32_t per = s.group ? s.threads / s.group : 1;
+  const uint32_t need = (rows + per - 1) / per;
+  const uint32_t most = 148u * (s.threads <= 128 ? 8u : s.threads <= 256 ? 4u : s.threads <= 512 ? 2u : 1u);
+  return (int)std::max(1u, std::min(need, most));
+}
+
+}  // namespace
+
+int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStream_t st, const char** why) {
+  Fwd f;
+  if ((*why = fill(a, &f))) return GPA_B200_BAD_ARGUMENT;
+  if (too_large(a)) {
+    *why = "at most 16384 channels and 2^31 - 1 rows";
+    return GPA_B200_UNSUPPORTED;
+  }
+  if (f.rows == 0) return GPA_B200_OK;
+  if (!f.y || !normed || (f.h && !stream_out)) {
+    *why = "update and the outputs must not be NULL";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  f.stream = stream_out;
+  f.out = normed;
+  const Shape s = shape_of(f, vec_ok(f));
+  const uint32_t per = s.group ? s.threads / s.group : 1;
+  const uint32_t grid = (f.rows + per - 1) / per;
+  Launch scope("norm_fwd", st);
+#define CALL(G, V, I, M) k_norm_fwd<G, V, I, M><<<grid, s.threads, 0, st>>>(f)
+  NORM_DISPATCH(s, CALL);
+#undef CALL
+  if (cudaGetLastError() == cudaSuccess) return GPA_B200_OK;
+  *why = "norm_fwd launch failed";
+  return GPA_B200_LAUNCH_FAILURE;
+}
+
+namespace {
+// whichever variant runs, its partial rows fit: the larger grid of the two
+size_t partial_floats(const Fwd& f) {
+  const int b = std::max(bwd_blocks(shape_of(f, true), f.rows), bwd_blocks(shape_of(f, false), f.rows));
+  return (size_t)b * 3 * f.width;
+}
+}  // namespace
+
+size_t norm_scratch_bytes(const GpaNormArgs* a) {
+  Fwd f;
+  if (fill(a, &f) || too_large(a)) return 0;
+  return partial_floats(f) * sizeof(float);
+}
+
+int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstream, const void* dnormed,
+                  const GpaNormGrads* g, void* scratch, size_t scratch_bytes, cudaStream_t st,
+                  const char** why) {
+  Bwd b;
+  if ((*why = fill(a, &b.f))) return GPA_B200_BAD_ARGUMENT;
+  if (too_large(a)) {
+    *why = "at most 16384 channels and 2^31 - 1 rows";
+    return GPA_B200_UNSUPPORTED;
+  }
+  Fwd& f = b.f;
+  const bool plain = f.h == nullptr;
+  if (!g || (!plain && !stream_in) || (plain && (!f.y || !g->dupdate)) ||
+      (!f.y && (f.wp || f.scale || f.gate))) {
+    *why = "a tensor that the gradients need is NULL";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  b.sums = 0;
+  b.sum_w = g->dweight ? b.sums++ : -1;
+  b.sum_p = g->dpost_weight ? b.sums++ : -1;
+  b.sum_c = g->dscale ? b.sums++ : -1;
+  float* out[3] = {g->dweight, g->dpost_weight, g->dscale};
+  if (f.rows == 0) {
+    for (float* o : out)
+      if (o && cudaMemsetAsync(o, 0, sizeof(float) * f.width, st) != cudaSuccess) {
+        *why = "clearing the weight gradients failed";
+        return GPA_B200_LAUNCH_FAILURE;
+      }
+    return GPA_B200_OK;
+  }
+  if (b.sums && (!scratch || scratch_bytes < partial_floats(f) * sizeof(float))) {
+    *why = "scratch is smaller than gpa_b200_norm_scratch_bytes";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  f.stream = const_cast<void*>(stream_in);
+  f.h = nullptr;  // the backward reads the stream, not the residual that went in
+  b.dn = dnormed;
+  b.ds = dstream;
+  b.dh = g->dresidual;
+  b.dy = g->dupdate;
+  b.dgate = g->dgate;
+  b.part = static_cast<float*>(scratch);
+  const bool vec = vec_ok(f) && aligned8(dnormed) && aligned8(dstream) && aligned8(g->dresidual) &&
+                   aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate));
+  const Shape s = shape_of(f, vec);
+  const int blocks = bwd_blocks(s, f.rows);
+  {
+    Launch scope("norm_bwd", st);
+    const size_t smem = s.group ? sizeof(float) * s.threads * s.vec * s.iter : 0;
+#define CALL(G, V, I, M) k_norm_bwd<G, V, I, M><<<blocks, s.threads, smem, st>>>(b)
+    NORM_DISPATCH(s, CALL);
+#undef CALL
+    if (cudaGetLastError() != cudaSuccess) {
+      *why = "norm_bwd launch failed";
+      return GPA_B200_LAUNCH_FAILURE;
+    }
+  }
+  if (!b.sums) return GPA_B200_OK;
+  // the sums of all wanted weights lie next to one another in a partial row
+  for (int k = 0, slot = 0; k < 3; ++k) {
+    if (!out[k]) continue;
+    Launch scope("norm_fold", st);
+    k_norm_fold<<<(f.width + 31) / 32, dim3(32, 8), 0, st>>>(b.part + (int64_t)slot * f.width, blocks,
+                                                           (int64_t)b.sums * f.width, f.width, out[k]);
+    ++slot;
+    if (cudaGetLastError() != cudaSuccess) {
+      *why = "norm_fold launch failed";
+      return GPA_B200_LAUNCH_FAILURE;
+    }
+  }
+  return GPA_B200_OK;
+}
+
+}  // namespace gpa

@@ -1,0 +1,291 @@
+"""Operators of a language model round the DenseGPA core, as hand-written sm_100a kernels.
+
+* :func:`residual_norm` -- the norm after a block, its gate and residual scale, the residual
+  addition and the norm before the next block in one pass over the rows;
+* :func:`rms_norm` -- the same norm without a residual stream.
+
+Both take CUDA tensors in float32, bfloat16 or float16 (any mix of them), compute in fp32, run on
+the current stream without synchronising, allocate through PyTorch, can be captured in a CUDA
+graph and have first-order gradients.  They raise ``ValueError`` for arguments they refuse.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_NORM_WIDTH = 16384
+
+
+def _call(fn, device, *args):
+    """`fn(*args, stream)` on the current stream of `device`, made current for the call."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, fn.__name__)
+
+
+def _rows(t: Tensor):
+    """`t` with unit stride along its last axis and its other axes as outer x inner rows:
+    (tensor, outer stride, inner stride).  Copies only what these two strides cannot describe."""
+    width = t.shape[-1]
+    if t.is_contiguous():
+        return t, (t.shape[-2] if t.ndim > 1 else 1) * width, width
+    if t.stride(-1) == 1 or width == 1:
+        outer, span = 0, None
+        for size, stride in zip(reversed(t.shape[:-2]), reversed(t.stride()[:-2])):
+            if size == 1:
+                continue
+            if span is None:
+                outer, span = stride, stride * size
+            elif stride == span:
+                span = stride * size
+            else:
+                break
+        else:
+            return t, outer, t.stride(-2) if t.ndim > 1 else 0
+    return _rows(t.contiguous())
+
+
+def _check_tensor(name: str, t: Tensor, device=None):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (B200, sm_100a)")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+
+
+def _vector(name: str, t: Tensor, width: int, device) -> Tensor:
+    """A weight as the contiguous fp32 vector the kernels read (gradients flow back through)."""
+    _check_tensor(name, t, device)
+    if t.shape != (width,):
+        raise ValueError(f"{name} must have shape [{width}], not {list(t.shape)}")
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def _check_width(width: int):
+    if not 1 <= width <= MAX_NORM_WIDTH:
+        raise ValueError(f"the norms take 1 to {MAX_NORM_WIDTH} channels, not {width}")
+
+
+def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, stream_dtype,
+               out_dtype, shape):
+    """(GpaNormArgs, tensors that must outlive the launch)."""
+    a = _lib.GpaNormArgs()
+    keep = []
+    width = shape[-1]
+    a.width = width
+    a.inner = shape[-2] if len(shape) > 1 else 1
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    a.outer = rows // a.inner if a.inner else 0
+    a.stream_dtype = _DTYPES[stream_dtype]
+    a.out_dtype = _DTYPES[out_dtype]
+    a.eps, a.scale_const = eps, const
+    if residual is not None:
+        t, so, si = _rows(residual)
+        keep.append(t)
+        a.residual = t.data_ptr()
+        a.residual_stride[0], a.residual_stride[1] = so, si
+    if update is not None:
+        t, so, si = _rows(update)
+        keep.append(t)
+        a.update, a.update_dtype = t.data_ptr(), _DTYPES[update.dtype]
+        a.update_stride[0], a.update_stride[1] = so, si
+    if gate is not None:
+        t, so, si = _rows(gate)
+        keep.append(t)
+        a.gate, a.gate_dtype = t.data_ptr(), _DTYPES[gate.dtype]
+        a.gate_stride[0], a.gate_stride[1] = so, si
+        a.gate_mode = 2 if gate.shape[-1] == width else 1
+    a.weight = weight.data_ptr()
+    if post_weight is not None:
+        a.post_weight = post_weight.data_ptr()
+    if scale is not None:
+        a.scale = scale.data_ptr()
+    return a, keep
+
+
+def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
+    lib = _lib.load()
+    nbytes = lib.gpa_b200_norm_scratch_bytes(a)
+    scratch = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    g = _lib.GpaNormGrads(*[None if t is None else t.data_ptr() for t in grads])
+    _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
+          _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
+
+
+def _rms_forward(x, weight, eps, out_dtype):
+    out = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+    if out.numel():
+        a, keep = _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, out_dtype, x.shape)
+        _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
+    return out
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, eps, out_dtype):
+        ctx.save_for_backward(x, weight)
+        ctx.eps, ctx.out_dtype = eps, out_dtype
+        return _rms_forward(x, weight, eps, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, weight = ctx.saved_tensors
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        if not x.numel():
+            return dx, torch.zeros_like(weight), None, None
+        dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
+        a, keep = _norm_args(None, x, weight, None, None, None, ctx.eps, 1., x.dtype,
+                             ctx.out_dtype, x.shape)
+        _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
+        return dx, dw, None, None
+
+
+def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, *,
+             out_dtype: torch.dtype | None = None) -> Tensor:
+    """``x / sqrt(mean(x^2, -1) + eps) * weight`` over the last axis, rounded once.
+
+    x [..., D] (strided views are read in place where two strides describe their rows), weight
+    [D], D up to 16384; returns a contiguous tensor of x's shape in ``out_dtype`` (x's dtype by
+    default).  Gradients: x (in x's dtype) and weight.
+    """
+    _check_tensor("x", x)
+    if x.ndim < 1:
+        raise ValueError("x must have at least one axis")
+    _check_width(x.shape[-1])
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    weight = _vector("weight", weight, x.shape[-1], x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _RMSNorm.apply(x, weight, float(eps), out_dtype)
+    return _rms_forward(x, weight, eps, out_dtype)
+
+
+def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, const, out_dtype):
+    stream = torch.empty(residual.shape, device=residual.device, dtype=residual.dtype)
+    normed = torch.empty(residual.shape, device=residual.device, dtype=out_dtype)
+    if stream.numel():
+        a, keep = _norm_args(residual, update, weight, post_weight, gate, scale, eps, const,
+                             residual.dtype, out_dtype, residual.shape)
+        _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
+              normed.data_ptr())
+    return stream, normed
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, residual, update, weight, post_weight, gate, scale, eps, const, out_dtype):
+        stream, normed = _residual_forward(residual, update, weight, post_weight, gate, scale, eps,
+                                           const, out_dtype)
+        # the update itself is needed only where the residual's share depends on it
+        read = post_weight is not None or gate is not None or scale is not None
+        ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
+        ctx.update_dtype = update.dtype
+        ctx.eps, ctx.const, ctx.out_dtype = eps, const, out_dtype
+        ctx.set_materialize_grads(False)
+        return stream, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dstream, dnormed):
+        if dstream is None and dnormed is None:
+            return (None,) * 9
+        stream, update, weight, post_weight, gate, scale = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dev, shape = stream.device, stream.shape
+
+        def new(i, like_shape, dtype):
+            return torch.empty(like_shape, device=dev, dtype=dtype) if need[i] else None
+
+        dres = new(0, shape, stream.dtype)
+        dupd = new(1, shape, ctx.update_dtype)
+        dw = new(2, weight.shape, torch.float32)
+        dpw = new(3, weight.shape, torch.float32)
+        dgate = None if gate is None else new(4, gate.shape, gate.dtype)
+        dscale = new(5, weight.shape, torch.float32)
+        if not stream.numel():
+            for t in (dw, dpw, dscale):
+                if t is not None:
+                    t.zero_()
+            return dres, dupd, dw, dpw, dgate, dscale, None, None, None
+        dstream = None if dstream is None else dstream.contiguous()
+        dnormed = None if dnormed is None else dnormed.contiguous()
+        a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
+                             stream.dtype, ctx.out_dtype, shape)
+        if update is None:
+            a.update_dtype = _DTYPES[ctx.update_dtype]
+        _norm_backward(a, dev, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
+        return dres, dupd, dw, dpw, dgate, dscale, None, None, None
+
+
+def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float = 1e-6, *,
+                  post_weight: Tensor | None = None, gate: Tensor | None = None,
+                  scale: Tensor | float | None = None,
+                  out_dtype: torch.dtype | None = None) -> tuple[Tensor, Tensor]:
+    """The residual addition between two blocks, with the norms on both sides of it.
+
+    With ``rms(x) = sqrt(mean(x^2, -1) + eps)``::
+
+        u      = update / rms(update) * post_weight     (update itself without post_weight)
+        stream = residual + scale * sigmoid(gate) * u   (rounded to residual's dtype)
+        normed = stream / rms(stream) * weight          (rounded to out_dtype)
+
+    residual, update [..., D] with D up to 16384; weight, post_weight [D]; gate broadcastable to
+    update, with a last axis of D (one gate for each channel) or 1 (one for each row); scale a
+    number, or a tensor of D values or one.  ``out_dtype`` defaults to update's dtype.  Returns
+    ``(stream, normed)``, both contiguous and of residual's shape; ``normed`` is computed from
+    the rounded stream.  Gradients: every tensor argument.
+    """
+    _check_tensor("residual", residual)
+    dev = residual.device
+    _check_tensor("update", update, dev)
+    if residual.ndim < 1 or residual.shape != update.shape:
+        raise ValueError(f"residual {list(residual.shape)} and update {list(update.shape)} must "
+                         "have the same shape [..., D]")
+    width = residual.shape[-1]
+    _check_width(width)
+    out_dtype = update.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    weight = _vector("weight", weight, width, dev)
+    if post_weight is not None:
+        post_weight = _vector("post_weight", post_weight, width, dev)
+    if gate is not None:
+        _check_tensor("gate", gate, dev)
+        if gate.ndim < 1 or gate.shape[-1] not in (1, width):
+            raise ValueError(f"gate {list(gate.shape)} must end in 1 or {width}")
+        want = update.shape[:-1] + gate.shape[-1:]
+        if gate.shape != want:
+            try:
+                gate = gate.expand(want)
+            except RuntimeError:
+                raise ValueError(f"gate {list(gate.shape)} does not broadcast to update "
+                                 f"{list(update.shape)}") from None
+    const = 1.
+    if isinstance(scale, Tensor):
+        _check_tensor("scale", scale, dev)
+        if scale.numel() == 1:
+            scale = scale.reshape(1).expand(width)
+        scale = _vector("scale", scale, width, dev)
+    elif scale is not None:
+        const, scale = float(scale), None
+    args = (residual, update, weight, post_weight, gate, scale, float(eps), const, out_dtype)
+    if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in args):
+        return _ResidualNorm.apply(*args)
+    return _residual_forward(*args)
+
+
+__all__ = ["rms_norm", "residual_norm"]

@@ -206,6 +206,48 @@ int gpa_b200_umma_selftest(int M, int mma_m, int N, int Kd, int a_mn, int b_mn, 
                            const void* A, const void* B, const void* A_tiled, float* D,
                            int* status, void* stream);
 
+/* Arguments of the norms round a residual block, over outer x inner rows of `width`
+ * channels (row r lies at (r / inner) * stride[0] + (r % inner) * stride[1] elements, unit
+ * stride along the channels; outputs and gradients are contiguous):
+ *   u = update / rms(update) * post_weight        (post_weight NULL: u = update)
+ *   h = residual + scale_const * scale * sigmoid(gate) * u, rounded to stream_dtype
+ *   n = h / rms(h) * weight, rounded to out_dtype;     rms(x) = sqrt(mean x^2 + eps)
+ * residual NULL: the plain norm n = update / rms(update) * weight.  Arithmetic is fp32.
+ * No counterpart in the reference, whose wrapper composes PyTorch operations
+ * (src/gpa/hf_qwen.py:132-407). */
+typedef struct GpaNormArgs {
+  const void* residual;     /* stream_dtype, or NULL */
+  const void* update;       /* update_dtype */
+  const void* gate;         /* gate_dtype, or NULL */
+  const float* weight;      /* [width] */
+  const float* post_weight; /* [width] or NULL */
+  const float* scale;       /* [width] or NULL */
+  int64_t outer, inner;
+  int64_t residual_stride[2], update_stride[2], gate_stride[2];
+  int32_t width;            /* 1 .. 16384 */
+  int32_t stream_dtype, update_dtype, gate_dtype, out_dtype; /* GPA_B200_F32 / _BF16 / _F16 */
+  int32_t gate_mode;        /* 0 none, 1 one value per row, 2 one value per channel */
+  float eps, scale_const;
+} GpaNormArgs;
+
+/* Gradients of the norms; members left NULL are not computed (dupdate is required for the
+ * plain norm).  dgate: [rows] or [rows, width]. */
+typedef struct GpaNormGrads {
+  void *dresidual, *dupdate, *dgate;
+  float *dweight, *dpost_weight, *dscale; /* [width], overwritten */
+} GpaNormGrads;
+
+/* stream [rows, width] (stream_dtype; ignored for the plain norm), normed [rows, width]. */
+int gpa_b200_norm_forward(const GpaNormArgs* args, void* stream_out, void* normed, void* stream);
+/* Bytes of the backward's scratch (0 for arguments the entry points refuse). */
+size_t gpa_b200_norm_scratch_bytes(const GpaNormArgs* args);
+/* stream_in: the forward's stream_out.  dstream / dnormed may be NULL (zero).  args->update is
+ * read only for the plain norm or with a post weight, gate or scale vector; args->residual is
+ * only compared with NULL. */
+int gpa_b200_norm_backward(const GpaNormArgs* args, const void* stream_in, const void* dstream,
+                           const void* dnormed, const GpaNormGrads* grads, void* scratch,
+                           size_t scratch_bytes, void* stream);
+
 /* Message of the last failure on the calling thread (0 if none). */
 int gpa_b200_last_error(char* buf, size_t len);
 

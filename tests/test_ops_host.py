@@ -1,0 +1,73 @@
+"""Refusals of the language-model operators: checked on the host, before any CUDA call."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from gpa_b200 import _lib, residual_norm, rms_norm
+
+
+def _message():
+    buf = ctypes.create_string_buffer(256)
+    _lib.load().gpa_b200_last_error(buf, 256)
+    return buf.value.decode()
+
+
+def _args(**kw):
+    a = _lib.GpaNormArgs()
+    a.update = a.weight = 16
+    a.outer, a.inner, a.width = 2, 3, 8
+    a.update_stride[0], a.update_stride[1] = 24, 8
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_norms_refuse_cpu_tensors():
+    x, w = torch.ones(2, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="CUDA"):
+        rms_norm(x, w)
+    with pytest.raises(ValueError, match="CUDA"):
+        residual_norm(x, x, w)
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(weight=None), 1, "weight"), (dict(update=None), 1, "update"),
+    (dict(update_dtype=3), 1, "dtypes"), (dict(out_dtype=-1), 1, "dtypes"),
+    (dict(width=0), 1, "width"), (dict(outer=-1), 1, "outer"),
+    (dict(gate_mode=1), 1, "without a residual"), (dict(gate_mode=3), 1, "gate_mode"),
+    (dict(scale=16), 1, "without a residual"), (dict(post_weight=16), 1, "without a residual"),
+    (dict(residual=16, gate_mode=2), 1, "needs a gate"),
+    (dict(width=16385), 2, "16384"), (dict(outer=1 << 31), 2, "rows"),
+])
+def test_norm_entry_points_refuse_bad_arguments(change, code, word):
+    lib = _lib.load()
+    if change.get("gate_mode") == 1:
+        change = {**change, "gate": 16}
+    a = _args(**change)
+    assert lib.gpa_b200_norm_forward(a, None, 16, None) == code
+    assert word in _message(), _message()
+    g = _lib.GpaNormGrads()
+    g.dupdate = 16
+    assert lib.gpa_b200_norm_backward(a, None, None, None, g, None, 0, None) == code
+    assert word in _message(), _message()
+    assert lib.gpa_b200_norm_scratch_bytes(a) == 0
+
+
+def test_norm_entry_points_refuse_missing_tensors():
+    lib = _lib.load()
+    assert lib.gpa_b200_norm_forward(None, None, None, None) == 1
+    assert lib.gpa_b200_norm_forward(_args(), None, None, None) == 1 and "outputs" in _message()
+    assert lib.gpa_b200_norm_forward(_args(residual=16), None, 16, None) == 1
+    g = _lib.GpaNormGrads()
+    assert lib.gpa_b200_norm_backward(_args(), None, None, None, None, None, 0, None) == 1
+    assert lib.gpa_b200_norm_backward(_args(), None, None, None, g, None, 0, None) == 1  # no dupdate
+    g.dresidual = 16
+    assert lib.gpa_b200_norm_backward(_args(residual=16), None, None, None, g, None, 0, None) == 1
+    g.dweight = 16  # a weight gradient needs scratch
+    assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, None, 0, None) == 1
+    assert "scratch" in _message()
+    a = _args()
+    assert lib.gpa_b200_norm_scratch_bytes(a) >= 2 * 8 * 4
