@@ -11,9 +11,9 @@ the C ABI of ``include/gpa_b200.h``).
 """
 from .config import GPAConfig
 from .core import DenseGPA, edges_of
-from .ops import residual_norm, rms_norm
+from .ops import linear_cross_entropy, residual_norm, rms_norm
 from .state import GPAState, LevelState, RelationState, ResidualSnapshot, tensors
 
 __all__ = ["DenseGPA", "GPAConfig", "GPAState", "LevelState", "RelationState",
-           "ResidualSnapshot", "edges_of", "residual_norm", "rms_norm", "tensors"]
+           "ResidualSnapshot", "edges_of", "linear_cross_entropy", "residual_norm", "rms_norm", "tensors"]
 __version__ = "0.1.0"

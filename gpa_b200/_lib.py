@@ -13,7 +13,7 @@ from ctypes import (POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_
 
 MAX_LEVELS = 8
 MAX_EDGES = 56
-ABI_VERSION = 2
+ABI_VERSION = 3
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgpa_b200.so")
 
 STATUS = {0: "ok", 1: "bad argument", 2: "unsupported configuration", 3: "CUDA launch failure",
@@ -68,12 +68,21 @@ class GpaNormGrads(ctypes.Structure):
                                         "dpost_weight", "dscale")]
 
 
+class GpaLossArgs(ctypes.Structure):
+    _fields_ = [("hidden", c_void_p), ("weight", c_void_p), ("labels", c_void_p),
+                ("outer", c_int64), ("inner", c_int64), ("hidden_stride", c_int64 * 2),
+                ("weight_stride", c_int64), ("vocab", c_int64), ("ignore_index", c_int64),
+                ("width", c_int32), ("dtype", c_int32), ("reduction", c_int32)]
+
+
 EXPORTS = ("gpa_b200_saved_bytes", "gpa_b200_scratch_bytes", "gpa_b200_forward",
            "gpa_b200_backward", "gpa_b200_routes", "gpa_b200_last_error",
            "gpa_b200_abi_version", "gpa_b200_launch_count", "gpa_b200_profile_start",
            "gpa_b200_profile_stop", "gpa_b200_forward_noalloc", "gpa_b200_noalloc_capacity",
            "gpa_b200_step", "gpa_b200_umma_selftest", "gpa_b200_device_status",
-           "gpa_b200_norm_forward", "gpa_b200_norm_scratch_bytes", "gpa_b200_norm_backward")
+           "gpa_b200_norm_forward", "gpa_b200_norm_scratch_bytes", "gpa_b200_norm_backward",
+           "gpa_b200_loss_saved_bytes", "gpa_b200_loss_scratch_bytes", "gpa_b200_loss_forward",
+           "gpa_b200_loss_backward")
 
 _lib = None
 
@@ -122,6 +131,16 @@ def load():
     lib.gpa_b200_norm_backward.argtypes = [POINTER(GpaNormArgs), c_void_p, c_void_p, c_void_p,
                                            POINTER(GpaNormGrads), c_void_p, c_size_t, c_void_p]
     lib.gpa_b200_norm_backward.restype = c_int
+    lib.gpa_b200_loss_saved_bytes.argtypes = [POINTER(GpaLossArgs)]
+    lib.gpa_b200_loss_saved_bytes.restype = c_size_t
+    lib.gpa_b200_loss_scratch_bytes.argtypes = [POINTER(GpaLossArgs), c_int]
+    lib.gpa_b200_loss_scratch_bytes.restype = c_size_t
+    lib.gpa_b200_loss_forward.argtypes = [POINTER(GpaLossArgs), c_void_p, c_void_p, c_size_t,
+                                          c_void_p, c_size_t, c_void_p]
+    lib.gpa_b200_loss_forward.restype = c_int
+    lib.gpa_b200_loss_backward.argtypes = [POINTER(GpaLossArgs), c_void_p, c_size_t, c_void_p,
+                                           c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.gpa_b200_loss_backward.restype = c_int
     lib.gpa_b200_last_error.argtypes = [c_char_p, c_size_t]
     lib.gpa_b200_last_error.restype = c_int
     lib.gpa_b200_abi_version.argtypes = []

@@ -21,6 +21,7 @@
 #include "gdn.cuh"
 #include "level.cuh"
 #include "norm.cuh"
+#include "vocab_loss.cuh"
 
 namespace gpa {
 
@@ -1118,6 +1119,31 @@ int gpa_b200_norm_backward(const GpaNormArgs* args, const void* stream_in, const
   return rc ? fail(rc, why) : rc;
 }
 
+size_t gpa_b200_loss_saved_bytes(const GpaLossArgs* args) { return gpa::loss_saved_bytes(args); }
+
+size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward) {
+  return gpa::loss_scratch_bytes(args, backward);
+}
+
+int gpa_b200_loss_forward(const GpaLossArgs* args, float* loss, void* saved, size_t saved_bytes,
+                          void* scratch, size_t scratch_bytes, void* stream) {
+  g_last_error.clear();
+  const char* why = "";
+  const int rc = gpa::loss_forward(args, loss, saved, saved_bytes, scratch, scratch_bytes,
+                                   static_cast<cudaStream_t>(stream), &why);
+  return rc ? fail(rc, why) : rc;
+}
+
+int gpa_b200_loss_backward(const GpaLossArgs* args, const void* saved, size_t saved_bytes,
+                           const float* dloss, void* dhidden, void* dweight, void* scratch,
+                           size_t scratch_bytes, void* stream) {
+  g_last_error.clear();
+  const char* why = "";
+  const int rc = gpa::loss_backward(args, saved, saved_bytes, dloss, dhidden, dweight, scratch,
+                                    scratch_bytes, static_cast<cudaStream_t>(stream), &why);
+  return rc ? fail(rc, why) : rc;
+}
+
 int gpa_b200_last_error(char* buf, size_t len) {
   if (buf && len) {
     std::snprintf(buf, len, "%s", g_last_error.c_str());
@@ -1125,7 +1151,7 @@ int gpa_b200_last_error(char* buf, size_t len) {
   return g_last_error.empty() ? 0 : 1;
 }
 
-int gpa_b200_abi_version(void) { return 2; }
+int gpa_b200_abi_version(void) { return 3; }
 
 long long gpa_b200_launch_count(void) { return g_launches.load(); }
 

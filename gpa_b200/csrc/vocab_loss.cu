@@ -1,0 +1,646 @@
+// Softmax cross entropy of z = x W^T over a large vocabulary, in pieces of it, without keeping z:
+//   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_{i, y_i}
+//   P_iv = (exp(z_iv - lse_i) - [v = y_i]) r_i        dx = s P W        dW = s P^T x
+// with the upstream gradient of row i written as s r_i, |r_i| <= 1 (s carries the scalar of a
+// mean or sum, or the largest of a vector).
+//
+// Rows without a label are dropped first: the labelled ones are packed (k_rows, k_gather), so
+// masked tokens cost nothing and whatever they hold (NaN included) reaches no product.
+//   forward:  each tile of z leaves (max, sum of exp) per row, k_join puts the tiles together
+//   backward: the vocabulary goes by in pieces; z of a piece is formed again and turned into P
+//             (in the piece's buffer), then dx += P W over the piece and dW of the piece = P^T x.
+// Every sum runs in a fixed order.  dx is added up in fp32 over the pieces (and over parts of a
+// piece where the tiles of dx alone would not fill the GPU) and rounded once by k_finish.
+#include "vocab_loss.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace gpa {
+namespace vloss {
+namespace {
+
+// ------------------------------------------------------------------ rows
+// Packs the labelled rows: row[j] = index of the j-th row with a label, label[j] its label (-1
+// outside the vocabulary).  One block; each thread owns a run of rows.
+__global__ void __launch_bounds__(1024) k_rows(const int64_t* labels, int n, int64_t ignore,
+                                               int64_t vocab, int* row, int* label, int* n_rows,
+                                               float* loss_each) {
+  __shared__ int sums[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = (n + 1023) / 1024;
+  const int64_t b = (int64_t)threadIdx.x * run;
+  const int begin = (int)(b < n ? b : n), end = begin + (run < n - begin ? run : n - begin);
+  int mine = 0;
+  for (int i = begin; i < end; ++i) mine += labels[i] != ignore;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int s = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += v;
+    }
+    sums[lane] = s;
+  }
+  __syncthreads();
+  int at = incl - mine + (warp ? sums[warp - 1] : 0);
+  for (int i = begin; i < end; ++i) {
+    const int64_t y = labels[i];
+    if (y != ignore) {
+      row[at] = i;
+      label[at++] = y >= 0 && y < vocab ? (int)y : -1;
+    } else if (loss_each) {
+      loss_each[i] = 0.f;
+    }
+  }
+  if (threadIdx.x == 0) *n_rows = sums[31];
+}
+
+// Packed copy of the labelled rows (row == NULL: of all rows), zero in the padding channels and
+// behind the last row up to the end of its tile.
+template <typename T>
+__global__ void k_gather(const T* src, int64_t so, int64_t si, int64_t inner, const int* row,
+                         const int* n_rows, int64_t n, int width, int pitch, T* dst, bool vec) {
+  constexpr int kV = 16 / sizeof(T);
+  const int64_t j = blockIdx.x;
+  const int64_t rows = n_rows ? *n_rows : n;
+  if (j >= up(rows, kTile)) return;
+  T* d = dst + j * pitch;
+  if (j >= rows) {
+    for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = T(0.f);
+    return;
+  }
+  const int64_t i = row ? row[j] : j;
+  const T* s = src + (i / inner) * so + (i % inner) * si;
+  if (vec) {
+    for (int c = threadIdx.x * kV; c < width; c += blockDim.x * kV)
+      *reinterpret_cast<uint4*>(d + c) = *reinterpret_cast<const uint4*>(s + c);
+  } else {
+    for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = c < width ? s[c] : T(0.f);
+  }
+}
+
+// ------------------------------------------------------------------ joins
+// lse and loss of each packed row from the (max, sum) pairs of its tiles: 32 rows a block, 8
+// lanes of tiles.
+__global__ void k_join(const float2* part, int tiles, int64_t n_pad, const int* n_rows, const int* row,
+                       const int* label, const float* z_label, float* lse, float* loss_each,
+                       float* loss_packed) {
+  __shared__ float sm[8][33], ss[8][33];
+  const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  const bool live = j < *n_rows;
+  float m = -INFINITY, s = 0.f;
+  if (live) {
+    for (int t = threadIdx.y; t < tiles; t += 8) {
+      const float2 p = part[t * n_pad + j];
+      const float big = fmaxf(m, p.x), safe = big == -INFINITY ? 0.f : big;
+      s = s * expf(m - safe) + p.y * expf(p.x - safe);
+      m = big;
+    }
+  }
+  sm[threadIdx.y][threadIdx.x] = m;
+  ss[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y || !live) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    const float m2 = sm[k][threadIdx.x], s2 = ss[k][threadIdx.x];
+    const float big = fmaxf(m, m2), safe = big == -INFINITY ? 0.f : big;
+    s = s * expf(m - safe) + s2 * expf(m2 - safe);
+    m = big;
+  }
+  const float log_s = logf(s);
+  lse[j] = m + log_s;
+  const float l = label[j] < 0 ? NAN : (m - z_label[j]) + log_s;
+  if (loss_each) loss_each[row[j]] = l;
+  if (loss_packed) loss_packed[j] = l;
+}
+
+// mean / sum of the packed losses, added in double by one block in a fixed order
+__global__ void __launch_bounds__(1024) k_total(const float* loss, const int* n_rows, bool mean, float* out) {
+  __shared__ double sm[32];
+  const int n = *n_rows;
+  double s = 0.;
+  for (int i = threadIdx.x; i < n; i += 1024) s += (double)loss[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = sm[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) *out = (float)(mean ? s / (double)(n > 0 ? n : 1) : s);
+  }
+}
+
+// Row factors of the gradient: s in *scale, r_i per packed row (see the file comment).  A label
+// outside the vocabulary makes its row NaN.
+__global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, int reduction, const int* n_rows,
+                                                    const int* row, const int* label, float* r,
+                                                    float* scale) {
+  __shared__ float sm[32];
+  const int n = *n_rows;
+  float s = 1.f;
+  if (reduction == GPA_B200_LOSS_NONE) {
+    float big = 0.f;
+    for (int j = threadIdx.x; j < n; j += 1024) big = fmaxf(big, fabsf(dloss[row[j]]));
+    big = warp_max(big);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = big;
+    __syncthreads();
+    big = warp_max(sm[threadIdx.x & 31]);
+    s = big > 0.f && big < INFINITY ? big : 1.f;
+  }
+  for (int j = threadIdx.x; j < n; j += 1024)
+    r[j] = label[j] < 0 ? NAN : reduction == GPA_B200_LOSS_NONE ? dloss[row[j]] / s : 1.f;
+  if (threadIdx.x == 0)
+    *scale = reduction == GPA_B200_LOSS_NONE ? s
+             : reduction == GPA_B200_LOSS_MEAN ? *dloss / (float)(n > 0 ? n : 1) : *dloss;
+}
+
+// dx of the caller's rows: the parts added in order, scaled, rounded and put back in place.
+template <typename T>
+__global__ void k_finish(const float* part, int parts, int64_t part_stride, int pitch, const int* n_rows,
+                         const int* row, const float* scale, int width, T* dx) {
+  const int64_t j = blockIdx.x;
+  if (j >= *n_rows) return;
+  const float s = *scale;
+  T* out = dx + (int64_t)row[j] * width;
+  const float* p = part + j * pitch;
+  for (int c = threadIdx.x; c < width; c += blockDim.x) {
+    float v = p[c];
+    for (int k = 1; k < parts; ++k) v += p[k * part_stride + c];
+    out[c] = T(v * s);
+  }
+}
+
+// ------------------------------------------------------------------ products without tensor cores
+// C (128 x 128 per block, 8 x 8 per thread) = A B over k, fp32 multiply-adds.  An operand is
+// K-major (k contiguous) or MN-major; both are read 4 elements at a time.
+constexpr int kB = 128, kBK = 16;
+
+template <typename T>
+GPA_DEV void ld4(const T* p, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)e[i];
+  }
+}
+
+template <typename T>
+struct Operand {
+  const T* p;
+  int64_t pitch;
+  int64_t mn, k;  // extents: reads outside give zero (whole groups of 4 along the contiguous axis)
+};
+
+template <typename T, bool KMAJOR>
+GPA_DEV void fetch(const Operand<T>& o, int64_t mn0, int64_t k0, float (&v)[2][4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = threadIdx.x + h * 256;  // 512 groups of 4 of a 128 x 16 tile
+    const int64_t mn = mn0 + (KMAJOR ? i >> 2 : (i & 31) * 4), k = k0 + (KMAJOR ? (i & 3) * 4 : i >> 5);
+    v[h][0] = v[h][1] = v[h][2] = v[h][3] = 0.f;
+    if (mn < o.mn && k < o.k) ld4(o.p + (KMAJOR ? mn * o.pitch + k : k * o.pitch + mn), v[h]);
+  }
+}
+
+template <bool KMAJOR>
+GPA_DEV void put(float (*s)[kB + 4], const float (&v)[2][4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = threadIdx.x + h * 256;
+    if (KMAJOR) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[(i & 3) * 4 + e][i >> 2] = v[h][e];
+    } else {
+      *reinterpret_cast<float4*>(&s[i >> 5][(i & 31) * 4]) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
+    }
+  }
+}
+
+// acc[i][j]: row m0 + (ty * 4 + i % 4) + 64 * (i / 4), column n0 + (tx * 4 + j % 4) + 64 * (j / 4)
+template <typename TA, typename TB, bool AK, bool BK_>
+GPA_DEV void product(const Operand<TA>& a, const Operand<TB>& b, int64_t m0, int64_t n0, int64_t k0,
+                     int64_t k1, float (&acc)[8][8]) {
+  __shared__ float sa[2][kBK][kB + 4], sb[2][kBK][kB + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+  float va[2][4], vb[2][4];
+  if (k0 < k1) {
+    fetch<TA, AK>(a, m0, k0, va);
+    fetch<TB, BK_>(b, n0, k0, vb);
+  }
+  int s = 0;
+  for (int64_t k = k0; k < k1; k += kBK, s ^= 1) {
+    put<AK>(sa[s], va);
+    put<BK_>(sb[s], vb);
+    __syncthreads();
+    if (k + kBK < k1) {
+      fetch<TA, AK>(a, m0, k + kBK, va);
+      fetch<TB, BK_>(b, n0, k + kBK, vb);
+    }
+#pragma unroll
+    for (int kk = 0; kk < kBK; ++kk) {
+      float fa[8], fb[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        *reinterpret_cast<float4*>(fa + 4 * h) = *reinterpret_cast<const float4*>(&sa[s][kk][ty * 4 + 64 * h]);
+        *reinterpret_cast<float4*>(fb + 4 * h) = *reinterpret_cast<const float4*>(&sb[s][kk][tx * 4 + 64 * h]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+    }
+  }
+}
+
+GPA_DEV int at8(int t, int i) { return t * 4 + (i & 3) + 64 * (i >> 2); }
+
+template <typename T>
+__global__ void __launch_bounds__(256, 2) k_stats(const Call c, float2* part, float* z_label) {
+  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
+  if (m0 >= *c.n_rows) return;
+  float acc[8][8];
+  product<T, T, true, true>({static_cast<const T*>(c.x), c.pitch, c.n_pad, c.pitch},
+                            {static_cast<const T*>(c.w), c.w_pitch, c.vocab, c.pitch}, m0, n0, 0, c.pitch, acc);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t m = m0 + at8(ty, i);
+    const bool live = m < *c.n_rows;
+    const int y = live ? c.label[m] : -1;
+    float big = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t v = n0 + at8(tx, j);
+      if (v >= c.vocab) acc[i][j] = -INFINITY;
+      else if (v == y) z_label[m] = acc[i][j];
+      big = fmaxf(big, acc[i][j]);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    const float safe = big == -INFINITY ? 0.f : big;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += expf(acc[i][j] - safe);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (tx == 0 && live) part[blockIdx.x * c.n_pad + m] = make_float2(big, s);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int64_t vn, const float* lse,
+                                                  const float* r, float* p, int64_t p_pitch) {
+  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
+  if (m0 >= up(*c.n_rows, kTile)) return;
+  float acc[8][8];
+  product<T, T, true, true>({static_cast<const T*>(c.x), c.pitch, c.n_pad, c.pitch},
+                            {static_cast<const T*>(c.w) + v0 * c.w_pitch, c.w_pitch, vn, c.pitch}, m0, n0, 0,
+                            c.pitch, acc);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t m = m0 + at8(ty, i);
+    const bool live = m < *c.n_rows;
+    const float l = live ? lse[m] : 0.f, ri = live ? r[m] : 0.f;
+    const int64_t y = live ? c.label[m] - v0 : -1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t v = n0 + at8(tx, j);
+      p[m * p_pitch + v] = live && v < vn ? (expf(acc[i][j] - l) - (v == y ? 1.f : 0.f)) * ri : 0.f;
+    }
+  }
+}
+
+// part[z] (+)= P[:, k of part z] W
+template <typename T>
+__global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int64_t p_pitch, int64_t v0,
+                                               int64_t vn, int64_t k_part, bool add, float* part,
+                                               int64_t part_stride) {
+  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
+  if (m0 >= *c.n_rows) return;
+  const int64_t k0 = blockIdx.z * k_part, k1 = k0 + k_part < vn ? k0 + k_part : vn;
+  float acc[8][8];
+  product<float, T, true, false>({p, p_pitch, c.n_pad, p_pitch},
+                                 {static_cast<const T*>(c.w) + v0 * c.w_pitch, c.w_pitch, c.pitch, vn}, m0, n0,
+                                 k0, k1, acc);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  float* o = part + blockIdx.z * part_stride;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t m = m0 + at8(ty, i);
+    if (m >= *c.n_rows) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t d = n0 + at8(tx, j);
+      if (d < c.pitch) o[m * c.pitch + d] = add ? o[m * c.pitch + d] + acc[i][j] : acc[i][j];
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int64_t p_pitch, int64_t v0,
+                                               int64_t vn, const float* scale, T* dw) {
+  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
+  const int64_t rows = up(*c.n_rows, kTile);
+  float acc[8][8];
+  product<float, T, false, false>({p, p_pitch, p_pitch, rows}, {static_cast<const T*>(c.x), c.pitch, c.pitch, rows},
+                                  m0, n0, 0, rows, acc);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const float s = *scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t v = m0 + at8(ty, i);
+    if (v >= vn) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t d = n0 + at8(tx, j);
+      if (d < c.width) dw[(v0 + v) * c.width + d] = T(acc[i][j] * s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ plan of a call
+constexpr int64_t kPieceBytes = int64_t(1) << 30;  // of P at a time
+
+struct Plan {
+  Call c;
+  bool copy_w;             // weight rows that cannot be read 16 bytes at a time are copied first
+  int es;                  // bytes of an element of x and W
+  int tiles_v, tiles_m;    // 128 x 128 tiles
+  int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
+  int parts;               // parts of dx
+  // saved
+  int64_t s_rows, s_label, s_lse, s_bytes;
+  // scratch
+  int64_t x, w, part, z_label, loss, fwd_bytes;
+  int64_t p, dxp, r, scale, bwd_bytes;
+};
+
+const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
+  *code = GPA_B200_BAD_ARGUMENT;
+  if (!a) return "args is NULL";
+  if (a->outer < 0 || a->inner < 0 || a->width < 1 || a->vocab < 1)
+    return "outer and inner must not be negative, width and vocab at least 1";
+  if (a->dtype < 0 || a->dtype > 2) return "dtype must be F32, BF16 or F16";
+  if (a->reduction < 0 || a->reduction > 2) return "reduction must be GPA_B200_LOSS_MEAN, _SUM or _NONE";
+  if (a->weight_stride < a->width && a->vocab > 1) return "weight rows must not overlap";
+  *code = GPA_B200_UNSUPPORTED;
+  if (a->width > 65536) return "at most 65536 channels";
+  if (a->vocab > (int64_t(1) << 30)) return "at most 2^30 vocabulary entries";
+  if (a->inner && a->outer > (int64_t(1) << 22) / a->inner) return "at most 2^22 rows in a call";
+  Call& c = p->c;
+  c.n = a->outer * a->inner;
+  c.vocab = a->vocab;
+  c.width = a->width;
+  c.dtype = a->dtype;
+  p->es = a->dtype == GPA_B200_F32 ? 4 : 2;
+  const int unit = 16 / p->es;
+  c.pitch = (int)up(a->width, unit);
+  c.n_pad = up(std::max<int64_t>(c.n, 1), kTile);
+  p->copy_w = a->width % unit || a->weight_stride % unit || (reinterpret_cast<uintptr_t>(a->weight) & 15);
+  c.w = a->weight;
+  c.w_pitch = p->copy_w ? c.pitch : a->vocab > 1 ? a->weight_stride : c.pitch;
+  p->tiles_v = (int)((c.vocab + kB - 1) / kB);
+  p->tiles_m = (int)(c.n_pad / kB);
+  const int64_t most = std::max<int64_t>(kTile, kPieceBytes / (c.n_pad * 4) / kTile * kTile);
+  p->piece = std::min(up(c.vocab, kTile), most);
+  const int tiles_d = (c.pitch + kB - 1) / kB;
+  // enough parts of at least 512 entries to give every SM two tiles
+  const int64_t want = (2 * 148 + (int64_t)tiles_d * p->tiles_m - 1) / ((int64_t)tiles_d * p->tiles_m);
+  p->parts = (int)std::max<int64_t>(1, std::min(want, p->piece / 512));
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  take(256);  // n_rows
+  p->s_rows = take(4 * c.n);
+  p->s_label = take(4 * c.n);
+  p->s_lse = take(4 * c.n);
+  p->s_bytes = at;
+  at = 0;
+  p->x = take(c.n_pad * c.pitch * p->es);
+  p->w = take(p->copy_w ? c.vocab * c.pitch * p->es : 0);
+  const int64_t common = at;
+  p->part = take((int64_t)p->tiles_v * c.n_pad * 8);
+  p->z_label = take(4 * c.n);
+  p->loss = take(4 * c.n);
+  p->fwd_bytes = at;
+  at = common;
+  p->p = take(c.n_pad * p->piece * 4);
+  p->dxp = take((int64_t)p->parts * c.n_pad * c.pitch * 4);
+  p->r = take(4 * c.n);
+  p->scale = take(4);
+  p->bwd_bytes = at;
+  return nullptr;
+}
+
+template <typename T>
+cudaError_t gather(const GpaLossArgs* a, const Plan& p, const int* row, char* scratch, cudaStream_t st) {
+  const Call& c = p.c;
+  constexpr int kV = 16 / sizeof(T);
+  {
+    const bool vec = a->width % kV == 0 && a->hidden_stride[0] % kV == 0 && a->hidden_stride[1] % kV == 0 &&
+                     (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
+    Launch scope("loss_gather", st);
+    k_gather<T><<<(unsigned)c.n_pad, 128, 0, st>>>(
+        static_cast<const T*>(a->hidden), a->hidden_stride[0], a->hidden_stride[1], a->inner, row, c.n_rows, c.n,
+        c.width, c.pitch, reinterpret_cast<T*>(scratch + p.x), vec);
+  }
+  if (p.copy_w) {
+    Launch scope("loss_gather", st);
+    k_gather<T><<<(unsigned)c.vocab, 128, 0, st>>>(static_cast<const T*>(a->weight), 0, a->weight_stride, c.vocab,
+                                                   nullptr, nullptr, c.vocab, c.width, c.pitch,
+                                                   reinterpret_cast<T*>(scratch + p.w), false);
+  }
+  return cudaGetLastError();
+}
+
+void bind(Plan* p, const void* saved, char* scratch) {
+  const char* s = static_cast<const char*>(saved);
+  p->c.n_rows = reinterpret_cast<const int*>(s);
+  p->c.label = reinterpret_cast<const int*>(s + p->s_label);
+  p->c.x = scratch + p->x;
+  if (p->copy_w) p->c.w = scratch + p->w;
+}
+
+#define BY_TYPE(DT, CALL)                                  \
+  do {                                                     \
+    if ((DT) == GPA_B200_F32) { using T = float; CALL; }   \
+    else if ((DT) == GPA_B200_BF16) { using T = __nv_bfloat16; CALL; } \
+    else { using T = __half; CALL; }                       \
+  } while (0)
+
+#define OK_OR(MSG)                                   \
+  do {                                               \
+    if (cudaGetLastError() != cudaSuccess) {         \
+      *why = MSG;                                    \
+      return GPA_B200_LAUNCH_FAILURE;                \
+    }                                                \
+  } while (0)
+
+}  // namespace
+}  // namespace vloss
+
+using namespace vloss;
+
+size_t loss_saved_bytes(const GpaLossArgs* a) {
+  Plan p;
+  int code;
+  return plan_of(a, &p, &code) ? 0 : p.s_bytes;
+}
+
+size_t loss_scratch_bytes(const GpaLossArgs* a, int backward) {
+  Plan p;
+  int code;
+  return plan_of(a, &p, &code) ? 0 : backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_bytes, void* scratch,
+                 size_t scratch_bytes, cudaStream_t st, const char** why) {
+  Plan p;
+  int code;
+  if ((*why = plan_of(a, &p, &code))) return code;
+  const Call& c = p.c;
+  const bool none = a->reduction == GPA_B200_LOSS_NONE;
+  if (!a->weight || !saved || !scratch || (c.n && (!a->hidden || !a->labels)) || (!loss && !(none && !c.n))) {
+    *why = "a tensor is NULL";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  if (saved_bytes < (size_t)p.s_bytes || scratch_bytes < (size_t)p.fwd_bytes) {
+    *why = "saved or scratch is smaller than its size query";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  char* sv = static_cast<char*>(saved);
+  char* sc = static_cast<char*>(scratch);
+  bind(&p, saved, sc);
+  int* row = reinterpret_cast<int*>(sv + p.s_rows);
+  float* each = none ? loss : nullptr;
+  float* packed = none ? nullptr : reinterpret_cast<float*>(sc + p.loss);
+  float* z_label = reinterpret_cast<float*>(sc + p.z_label);
+  float2* part = reinterpret_cast<float2*>(sc + p.part);
+  {
+    Launch scope("loss_rows", st);
+    k_rows<<<1, 1024, 0, st>>>(a->labels, (int)c.n, a->ignore_index, c.vocab, row,
+                               reinterpret_cast<int*>(sv + p.s_label), reinterpret_cast<int*>(sv), each);
+    OK_OR("loss_rows launch failed");
+  }
+  if (c.n) {
+    BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
+    OK_OR("loss_gather launch failed");
+    {
+      Launch scope("loss_stats", st);
+      BY_TYPE(a->dtype, (k_stats<T><<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label)));
+      OK_OR("loss_stats launch failed");
+    }
+    Launch scope("loss_join", st);
+    k_join<<<(unsigned)((c.n + 31) / 32), dim3(32, 8), 0, st>>>(part, p.tiles_v, c.n_pad, c.n_rows, row, c.label,
+                                                               z_label, reinterpret_cast<float*>(sv + p.s_lse),
+                                                               each, packed);
+    OK_OR("loss_join launch failed");
+  }
+  if (!none) {
+    Launch scope("loss_total", st);
+    k_total<<<1, 1024, 0, st>>>(packed, c.n_rows, a->reduction == GPA_B200_LOSS_MEAN, loss);
+    OK_OR("loss_total launch failed");
+  }
+  return GPA_B200_OK;
+}
+
+int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, const float* dloss,
+                  void* dhidden, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t st,
+                  const char** why) {
+  Plan p;
+  int code;
+  if ((*why = plan_of(a, &p, &code))) return code;
+  const Call& c = p.c;
+  if (!a->weight || !saved || !scratch || (c.n && (!a->hidden || !dloss)) || (!dhidden && !dweight)) {
+    *why = "a tensor is NULL";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  if (saved_bytes < (size_t)p.s_bytes || scratch_bytes < (size_t)p.bwd_bytes) {
+    *why = "saved or scratch is smaller than its size query";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  if (dhidden && cudaMemsetAsync(dhidden, 0, (size_t)c.n * c.width * p.es, st) != cudaSuccess) {
+    *why = "clearing dhidden failed";
+    return GPA_B200_LAUNCH_FAILURE;
+  }
+  if (!c.n) {
+    if (dweight && cudaMemsetAsync(dweight, 0, (size_t)c.vocab * c.width * p.es, st) != cudaSuccess) {
+      *why = "clearing dweight failed";
+      return GPA_B200_LAUNCH_FAILURE;
+    }
+    return GPA_B200_OK;
+  }
+  const char* sv = static_cast<const char*>(saved);
+  char* sc = static_cast<char*>(scratch);
+  bind(&p, saved, sc);
+  const int* row = reinterpret_cast<const int*>(sv + p.s_rows);
+  const float* lse = reinterpret_cast<const float*>(sv + p.s_lse);
+  float* r = reinterpret_cast<float*>(sc + p.r);
+  float* scale = reinterpret_cast<float*>(sc + p.scale);
+  float* pr = reinterpret_cast<float*>(sc + p.p);
+  float* dxp = reinterpret_cast<float*>(sc + p.dxp);
+  BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
+  OK_OR("loss_gather launch failed");
+  {
+    Launch scope("loss_row_scale", st);
+    k_row_scale<<<1, 1024, 0, st>>>(dloss, a->reduction, c.n_rows, row, c.label, r, scale);
+    OK_OR("loss_row_scale launch failed");
+  }
+  const int64_t part_stride = c.n_pad * c.pitch;
+  const unsigned tiles_d = (unsigned)((c.pitch + kB - 1) / kB);
+  const int64_t k_part = up((p.piece + p.parts - 1) / p.parts, kBK);
+  for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
+    const int64_t vn = std::min(p.piece, c.vocab - v0);
+    const unsigned tv = (unsigned)(up(vn, kTile) / kB);
+    {
+      Launch scope("loss_probs", st);
+      BY_TYPE(a->dtype, (k_probs<T><<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, r, pr, p.piece)));
+      OK_OR("loss_probs launch failed");
+    }
+    if (dhidden) {
+      Launch scope("loss_dx", st);
+      BY_TYPE(a->dtype, (k_dx<T><<<dim3(tiles_d, p.tiles_m, p.parts), 256, 0, st>>>(
+                            c, pr, p.piece, v0, vn, k_part, v0 > 0, dxp, part_stride)));
+      OK_OR("loss_dx launch failed");
+    }
+    if (dweight) {
+      Launch scope("loss_dw", st);
+      BY_TYPE(a->dtype, (k_dw<T><<<dim3(tiles_d, tv), 256, 0, st>>>(c, pr, p.piece, v0, vn, scale,
+                                                                  static_cast<T*>(dweight))));
+      OK_OR("loss_dw launch failed");
+    }
+  }
+  if (dhidden) {
+    Launch scope("loss_finish", st);
+    BY_TYPE(a->dtype, (k_finish<T><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, part_stride, c.pitch, c.n_rows, row,
+                                                                scale, c.width, static_cast<T*>(dhidden))));
+    OK_OR("loss_finish launch failed");
+  }
+  return GPA_B200_OK;
+}
+
+}  // namespace gpa

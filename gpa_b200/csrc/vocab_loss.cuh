@@ -1,0 +1,39 @@
+// Softmax cross entropy over a vocabulary: shapes and buffers shared by its kernels
+// (vocab_loss.cu: rows, joins and the fp32 products; see there for the formulas).
+#pragma once
+#include "../../include/gpa_b200.h"
+#include "common.cuh"
+
+namespace gpa {
+namespace vloss {
+
+constexpr int kTile = 256;       // rows and vocabulary entries are padded to tiles of this
+
+// One call, as its kernels see it.  Rows are the labelled rows only, packed to the front; their
+// number is known on the device alone (n_rows).
+struct Call {
+  int64_t n;          // rows of the caller (an upper bound of the packed ones)
+  int64_t vocab;
+  int width, pitch;   // channels, and the element pitch of the packed rows
+  int dtype;
+  const int* n_rows;  // device: packed rows
+  const int* label;   // [n] label of a packed row, -1 when outside the vocabulary
+  const void* x;      // packed rows [pad(n)][pitch], zero behind the last one's tile
+  const void* w;      // weight [vocab][w_pitch]
+  int64_t w_pitch;
+  int64_t n_pad;      // n rounded up to tiles
+};
+
+__host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+}  // namespace vloss
+
+int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_bytes, void* scratch,
+                 size_t scratch_bytes, cudaStream_t st, const char** why);
+int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, const float* dloss,
+                  void* dhidden, void* dweight, void* scratch, size_t scratch_bytes, cudaStream_t st,
+                  const char** why);
+size_t loss_saved_bytes(const GpaLossArgs* a);
+size_t loss_scratch_bytes(const GpaLossArgs* a, int backward);
+
+}  // namespace gpa

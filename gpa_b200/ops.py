@@ -2,9 +2,11 @@
 
 * :func:`residual_norm` -- the norm after a block, its gate and residual scale, the residual
   addition and the norm before the next block in one pass over the rows;
-* :func:`rms_norm` -- the same norm without a residual stream.
+* :func:`rms_norm` -- the same norm without a residual stream;
+* :func:`linear_cross_entropy` -- softmax cross entropy over a large vocabulary, in pieces of it
+  and without keeping the logits.
 
-Both take CUDA tensors in float32, bfloat16 or float16 (any mix of them), compute in fp32, run on
+They take CUDA tensors in float32, bfloat16 or float16 (the norms any mix of them), sum in fp32, run on
 the current stream without synchronising, allocate through PyTorch, can be captured in a CUDA
 graph and have first-order gradients.  They raise ``ValueError`` for arguments they refuse.
 """
@@ -118,7 +120,7 @@ def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, s
 def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
     lib = _lib.load()
     nbytes = lib.gpa_b200_norm_scratch_bytes(a)
-    scratch = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    scratch = _scratch(nbytes, device)
     g = _lib.GpaNormGrads(*[None if t is None else t.data_ptr() for t in grads])
     _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
           _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
@@ -288,4 +290,105 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
     return _residual_forward(*args)
 
 
-__all__ = ["rms_norm", "residual_norm"]
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+def _loss_args(hidden, weight, labels, ignore_index, reduction):
+    a = _lib.GpaLossArgs()
+    x, so, si = _rows(hidden)
+    w = weight if weight.stride(-1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
+    a.hidden, a.weight, a.labels = x.data_ptr(), w.data_ptr(), labels.data_ptr()
+    a.width, a.vocab = hidden.shape[-1], weight.shape[0]
+    a.inner = hidden.shape[-2] if hidden.ndim > 1 else 1
+    a.outer = labels.numel() // a.inner if a.inner else 0
+    a.hidden_stride[0], a.hidden_stride[1] = so, si
+    a.weight_stride = w.stride(0)
+    a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[hidden.dtype], reduction
+    return a, (x, w)
+
+
+def _scratch(nbytes, device):
+    return torch.empty(nbytes, device=device, dtype=torch.uint8)
+
+
+def _loss_forward(hidden, weight, labels, ignore_index, reduction):
+    lib = _lib.load()
+    dev = hidden.device
+    a, keep = _loss_args(hidden, weight, labels, ignore_index, reduction)
+    loss = torch.empty(labels.shape if reduction == 2 else (), device=dev, dtype=torch.float32)
+    sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
+    saved, scratch = (_scratch(n, dev) for n in sizes)
+    _call(lib.gpa_b200_loss_forward, dev, a, loss.data_ptr(), saved.data_ptr(), sizes[0],
+          scratch.data_ptr(), sizes[1])
+    return loss, saved
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, labels, ignore_index, reduction):
+        loss, saved = _loss_forward(hidden, weight, labels, ignore_index, reduction)
+        ctx.save_for_backward(hidden, weight, labels)
+        ctx.saved_ws, ctx.ignore_index, ctx.reduction = saved, ignore_index, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        hidden, weight, labels = ctx.saved_tensors
+        lib = _lib.load()
+        dev = hidden.device
+        a, keep = _loss_args(hidden, weight, labels, ctx.ignore_index, ctx.reduction)
+        dx, dw = (torch.empty(t.shape, device=dev, dtype=t.dtype) if need else None
+                  for t, need in zip((hidden, weight), ctx.needs_input_grad))
+        dloss = dloss.contiguous()
+        nbytes = lib.gpa_b200_loss_scratch_bytes(a, 1)
+        scratch = _scratch(nbytes, dev)
+        _call(lib.gpa_b200_loss_backward, dev, a, ctx.saved_ws.data_ptr(), ctx.saved_ws.numel(),
+              dloss.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), scratch.data_ptr(), nbytes)
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
+                         ignore_index: int = -100, reduction: str = "mean") -> Tensor:
+    """Softmax cross entropy of the logits ``hidden @ weight.T`` against ``labels``, in fp32.
+
+    hidden [..., D] and weight [V, D] of one dtype (float32, bfloat16, float16), labels [...]
+    integers; D up to 65536, V up to 2^30, 2^22 tokens.  The logits are formed tile by tile and
+    never stored; the backward forms them again.  Tokens labelled ``ignore_index`` have no loss
+    and zero gradients, cost nothing and are not read.  A label outside [0, V) makes its loss,
+    and every gradient it reaches, NaN.
+
+    ``reduction``: "mean" over the labelled tokens (0 when there is none), "sum", or "none" (a
+    loss for each token, 0 where ignored).  Gradients: hidden and weight, rounded once to their
+    dtype; with 16-bit inputs the gradient of each logit is rounded to that type on the way.
+    """
+    _check_tensor("hidden", hidden)
+    dev = hidden.device
+    _check_tensor("weight", weight, dev)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
+    if hidden.dtype != weight.dtype:
+        raise ValueError(f"hidden ({hidden.dtype}) and weight ({weight.dtype}) must share a dtype")
+    if hidden.ndim < 1 or weight.ndim != 2 or weight.shape[1] != hidden.shape[-1]:
+        raise ValueError(f"expected hidden [..., D] and weight [V, D], not {list(hidden.shape)} and "
+                         f"{list(weight.shape)}")
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError(f"labels {list(labels.shape)} must have hidden's leading shape "
+                         f"{list(hidden.shape[:-1])}")
+    if labels.device != dev:
+        raise ValueError(f"labels is on {labels.device}, the other tensors are on {dev}")
+    if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise ValueError(f"labels must be integers, not {labels.dtype}")
+    if not 1 <= hidden.shape[-1] <= 65536 or not 1 <= weight.shape[0] <= 1 << 30:
+        raise ValueError(f"1 to 65536 channels and 1 to 2^30 vocabulary entries, not {weight.shape[1]} "
+                         f"and {weight.shape[0]}")
+    if labels.numel() > 1 << 22:
+        raise ValueError(f"at most 2^22 tokens in a call, not {labels.numel()}")
+    labels = labels.long().contiguous()
+    args = (hidden, weight, labels, int(ignore_index), _REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        return _LinearCrossEntropy.apply(*args)
+    return _loss_forward(*args)[0]
+
+
+__all__ = ["linear_cross_entropy", "rms_norm", "residual_norm"]

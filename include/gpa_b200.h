@@ -248,10 +248,42 @@ int gpa_b200_norm_backward(const GpaNormArgs* args, const void* stream_in, const
                            const void* dnormed, const GpaNormGrads* grads, void* scratch,
                            size_t scratch_bytes, void* stream);
 
+/* Softmax cross entropy of hidden W^T over a vocabulary, without keeping the logits:
+ *   z = hidden W^T (fp32),  loss_i = log sum_v exp z_iv - z_{i, labels_i}
+ * over outer x inner rows of `width` channels (hidden row r at (r / inner) * stride[0] +
+ * (r % inner) * stride[1] elements, unit stride along the channels; weight row v at
+ * v * weight_stride).  Rows whose label is ignore_index have no loss and no gradient and what
+ * they hold is not read; a label outside [0, vocab) makes its row's loss NaN and the gradients NaN.
+ * GPA_B200_LOSS_MEAN divides by the number of labelled rows (by 1 if there is none).  Replaces the
+ * loss of the reference's wrapper (src/gpa/hf_qwen.py:388-401). */
+#define GPA_B200_LOSS_MEAN 0
+#define GPA_B200_LOSS_SUM 1
+#define GPA_B200_LOSS_NONE 2
+typedef struct GpaLossArgs {
+  const void* hidden;      /* dtype */
+  const void* weight;      /* [vocab, width], dtype */
+  const int64_t* labels;   /* [rows] */
+  int64_t outer, inner, hidden_stride[2], weight_stride, vocab, ignore_index;
+  int32_t width, dtype, reduction;
+} GpaLossArgs;
+
+/* Bytes of the buffer that the forward leaves for the backward, and of either call's scratch
+ * (0 for arguments the entry points refuse). */
+size_t gpa_b200_loss_saved_bytes(const GpaLossArgs* args);
+size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward);
+/* loss: one fp32, or one per row for GPA_B200_LOSS_NONE (0 for rows without a label). */
+int gpa_b200_loss_forward(const GpaLossArgs* args, float* loss, void* saved, size_t saved_bytes,
+                          void* scratch, size_t scratch_bytes, void* stream);
+/* dloss: fp32, loss's shape.  dhidden [rows, width], dweight [vocab, width]: contiguous, dtype,
+ * overwritten; either may be NULL. */
+int gpa_b200_loss_backward(const GpaLossArgs* args, const void* saved, size_t saved_bytes,
+                           const float* dloss, void* dhidden, void* dweight, void* scratch,
+                           size_t scratch_bytes, void* stream);
+
 /* Message of the last failure on the calling thread (0 if none). */
 int gpa_b200_last_error(char* buf, size_t len);
 
-/* ABI version of this header: 2 (GpaDims.reader_mode, positional_moments and
+/* ABI version of this header: 3 (the norm and loss entry points; 2: GpaDims.reader_mode, positional_moments and
  * position; GpaParams / GpaParamGrads.moment_gain; GpaStateRef.moment; a third
  * offset word of gpa_b200_step). */
 int gpa_b200_abi_version(void);

@@ -1,0 +1,303 @@
+"""linear_cross_entropy on the GPU against float64 on the CPU.
+
+Bounds (U = 2^-24, fp32's rounding; HALF[t] half a step of type t).  A logit is a sum of D exact
+products (16-bit inputs; each rounded once more for fp32 ones) whose additions lose at most 2 U of
+the running magnitude each, whether they round or truncate: Ez = 2 (D + 2) U sum |x| |w|.  The
+loss takes two logits and an exp / log of relative error below 64 U.  A gradient of a logit is
+P = exp(z - lse) - [v = y]: its exp part is off by that relative error plus 2 max Ez, and P is
+rounded once to the input's type when that has 16 bits.  The products with P then add
+2 (n + 2) U sum |P| |w| over their n terms, and the result is rounded once.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gpa_b200 import _lib, linear_cross_entropy
+from norm_reference import HALF, TINY, U
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _inputs(seed, lead, width, vocab, dtype, masked=0.0, spread=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*lead, width, generator=g).to(dtype).cuda()
+    w = (torch.randn(vocab, width, generator=g) * spread / width ** .5).to(dtype).cuda()
+    y = torch.randint(0, vocab, lead, generator=g)
+    if masked:
+        y[torch.rand(lead, generator=g) < masked] = -100
+    return x, w, y.cuda()
+
+
+def _reference(x, w, y, up, reduction):
+    """({name: (value, bound)}) in float64 on the CPU; `up` is the gradient of the loss."""
+    dtype, shape = x.dtype, x.shape
+    x, w, y = x.detach().double().cpu().flatten(0, -2), w.detach().double().cpu(), y.cpu().flatten()
+    keep = y != -100
+    xk, yk = x[keep], y[keep]
+    n, v, d = xk.shape[0], w.shape[0], w.shape[1]
+    z = xk @ w.T
+    ez = 2 * (d + 2) * U * (xk.abs() @ w.abs().T)
+    worst = ez.amax(-1, keepdim=True) if n else torch.zeros(0, 1, dtype=torch.float64)
+    lse = torch.logsumexp(z, -1, keepdim=True)
+    picked = z.gather(-1, yk[:, None])
+    loss = (lse - picked)[:, 0]
+    e_loss = (2 * worst + 64 * U + 4 * U * (lse.abs() + picked.abs()))[:, 0]
+    out = {}
+    if reduction == "none":
+        full, bound = torch.zeros(len(y), dtype=torch.float64), torch.zeros(len(y), dtype=torch.float64)
+        full[keep], bound[keep] = loss, e_loss + U * loss.abs()
+        out["loss"] = (full, bound)
+        g = up.double().cpu().flatten()[keep][:, None]
+    else:
+        k = max(n, 1) if reduction == "mean" else 1
+        out["loss"] = (loss.sum() / k, (e_loss.sum() + 4 * U * loss.abs().sum()) / k)
+        g = torch.full((n, 1), float(up) / k, dtype=torch.float64)
+    soft = (z - lse).exp()
+    hot = torch.zeros_like(z).scatter_(-1, yk[:, None], 1.0)
+    ep = soft * (2 * worst + 64 * U) + U * (soft + hot)
+    p = soft - hot
+    if dtype != F32:
+        # rounded once to the type, with the row's factor g / max g in it: fp16 underflows at
+        # 2^-25 of the scale 2^14 that keeps small probabilities in range
+        ep = ep + HALF[dtype] * (p.abs() + ep)
+        if dtype == F16:
+            big = g.abs().max() if n else 1.0
+            ep = ep + 2.0 ** -39 * big / g.abs().clamp_min(1e-300)
+    p, ep = p * g, ep * g.abs() * (1 + 4 * U)
+    dx, ex = p @ w, ep @ w.abs() + 2 * (v + 2) * U * (p.abs() @ w.abs())
+    dw, ew = p.T @ xk, ep.T @ xk.abs() + 2 * (n + 2) * U * (p.abs().T @ xk.abs())
+    fx, fe = torch.zeros_like(x), torch.zeros_like(x)
+    fx[keep], fe[keep] = dx, ex + (HALF[dtype] + 4 * U) * (dx.abs() + ex) + TINY[dtype]
+    out["dhidden"] = (fx.view(shape), fe.view(shape))
+    out["dweight"] = (dw, ew + (HALF[dtype] + 4 * U) * (dw.abs() + ew) + TINY[dtype])
+    return out
+
+
+def _check(name, got, want):
+    value, bound = want
+    got = got.detach().double().cpu().view(value.shape)
+    bad = ~((got - value).abs() <= bound)
+    assert not bad.any(), (name, int(bad.sum()), bad.numel(),
+                           float(((got - value).abs() / bound.clamp_min(1e-300)).max()))
+
+
+def _run(x, w, y, reduction, seed=0):
+    x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(x, w, y, reduction=reduction)
+    assert loss.dtype == F32 and loss.shape == (y.shape if reduction == "none" else ())
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x, w, y, reduction=reduction), loss)
+    g = torch.Generator().manual_seed(seed + 99)
+    up = torch.randn(loss.shape, generator=g).cuda()
+    dx, dw = torch.autograd.grad(loss, (x, w), up)
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype and dx.shape == x.shape and dw.shape == w.shape
+    return loss, dx, dw, up
+
+
+def _case(seed, lead, width, vocab, dtype, reduction, masked=0.0):
+    x, w, y = _inputs(seed, lead, width, vocab, dtype, masked)
+    loss, dx, dw, up = _run(x, w, y, reduction, seed)
+    want = _reference(x, w, y, up, reduction)
+    _check("loss", loss, want["loss"])
+    _check("dhidden", dx, want["dhidden"])
+    _check("dweight", dw, want["dweight"])
+
+
+DTYPES = [BF16, F16, F32]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead,width,vocab", [
+    ((1,), 64, 256), ((1,), 1, 1), ((3, 5), 8, 7), ((2, 130), 128, 500), ((257,), 64, 257), ((255,), 192, 511),
+    ((256,), 256, 512), ((3, 171), 72, 1003), ((700,), 40, 300), ((64,), 520, 2000), ((5,), 1000, 1500),
+    ((2, 33), 61, 129), ((130,), 1024, 300), ((2, 3, 50), 320, 777), ((1300,), 96, 96), ((40,), 2050, 700),
+])
+def test_sizes(dtype, lead, width, vocab):
+    _case(width + vocab, lead, width, vocab, dtype, "mean")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("masked", [0.0, 0.3, 0.97])
+def test_reductions_and_masks(dtype, reduction, masked):
+    _case(11, (4, 150), 136, 900, dtype, reduction, masked)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_labelled_token_and_no_token(dtype, reduction):
+    x, w, y = _inputs(3, (2, 9), 64, 300, dtype)
+    y.fill_(-100)
+    loss, dx, dw, _ = _run(x, w, y, reduction)
+    assert not loss.any() and not dx.any() and not dw.any()
+    loss, dx, dw, _ = _run(x[:, :0], w, y[:, :0], reduction)
+    assert not loss.any() and dx.shape == (2, 0, 64) and not dw.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_tokens_are_not_read(dtype):
+    x, w, y = _inputs(5, (3, 100), 128, 400, dtype, 0.4)
+    want = _run(x, w, y, "mean")
+    dirty = x.clone()
+    dirty[y == -100] = float("nan")
+    got = _run(dirty, w, y, "mean")
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_ignore_index_may_be_a_token():
+    x, w, y = _inputs(6, (50,), 64, 100, BF16)
+    y[::3] = 7
+    other = torch.where(y == 7, -100, y)
+    a = linear_cross_entropy(x, w, y, ignore_index=7)
+    assert torch.equal(a, linear_cross_entropy(x, w, other))
+    assert torch.equal(a, linear_cross_entropy(x, w, other.int()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_label_outside_the_vocabulary_gives_nan_there(dtype):
+    x, w, y = _inputs(7, (20,), 64, 100, dtype)
+    y[4], y[9] = 100, -3
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    assert loss[4].isnan() and loss[9].isnan() and int(loss.isnan().sum()) == 2
+    xr = x.detach().requires_grad_()
+    (dx,) = torch.autograd.grad(linear_cross_entropy(xr, w, y, reduction="sum"), xr)
+    rows = dx.isnan().any(-1)
+    assert rows[4] and rows[9] and int(rows.sum()) == 2
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_extreme_logits(dtype):
+    """Logits of +-200 and rows whose probability sits on one entry: finite, and within bounds."""
+    x, w, y = _inputs(8, (60,), 64, 513, dtype, spread=60.0)
+    loss, dx, dw, up = _run(x, w, y, "none")
+    assert loss.isfinite().all() and dx.isfinite().all() and dw.isfinite().all()
+    _check("loss", loss, _reference(x, w, y, up, "none")["loss"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nan_in_one_token_stays_in_its_loss(dtype):
+    x, w, y = _inputs(9, (6,), 64, 300, dtype)
+    x[2, 5] = float("nan")
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    assert loss[2].isnan() and int(loss.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strided_and_misaligned_inputs(dtype):
+    x, w, y = _inputs(10, (3, 40), 96, 333, dtype, 0.2)
+    want = _run(x, w, y, "mean")
+    wide = torch.zeros(3, 41, 107, device="cuda", dtype=dtype)
+    wide[:, :40, 3:99] = x
+    tall = torch.zeros(333, 107, device="cuda", dtype=dtype)
+    tall[:, 5:101] = w
+    strided = (wide[:, :40, 3:99], tall[:, 5:101])
+    assert not strided[0].is_contiguous()
+    for a, b in zip(want, _run(*strided, y, "mean")):
+        assert torch.equal(a, b)
+    flipped = w.T.contiguous().T  # no unit stride along the channels
+    for a, b in zip(want, _run(x.transpose(0, 1).contiguous().transpose(0, 1), flipped, y, "mean")):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_only_one_gradient_is_wanted(dtype):
+    x, w, y = _inputs(12, (70,), 64, 600, dtype)
+    _, dx, dw, _ = _run(x, w, y, "sum")
+    up = torch.randn((), generator=torch.Generator().manual_seed(99)).cuda()
+    xr, wr = x.detach().requires_grad_(), w.detach().requires_grad_()
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(xr, w, y, reduction="sum"), xr, up)[0], dx)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, wr, y, reduction="sum"), wr, up)[0], dw)
+
+
+def test_many_rows_and_a_large_vocabulary_in_pieces():
+    """More rows than one piece of the vocabulary holds: the pieces' gradients add up.  The plain
+    form in fp32 on the GPU stands in for float64 here, at bf16's rounding of P and the result."""
+    x, w, y = _inputs(13, (2, 4100), 128, 70001, BF16, 0.1)
+    loss, dx, dw, up = _run(x, w, y, "mean")
+    x, w = x.float().flatten(0, 1), w.float()
+    keep = y.flatten() != -100
+    z = x @ w.T
+    lse = torch.logsumexp(z, -1, keepdim=True)
+    at = y.flatten().clamp_min(0)[:, None]
+    ref = ((lse - z.gather(-1, at))[:, 0] * keep).sum() / keep.sum()
+    assert abs(float(loss - ref)) <= 1e-5 * float(ref)
+    z = (z - lse).exp_()
+    z.scatter_add_(-1, at, torch.full_like(lse, -1.0))
+    z *= (keep.float() / keep.sum())[:, None] * up
+    rx, rw = z @ w, z.T @ x
+    # two roundings of relative size 2^-8 at most: norm-wise below the sum of both
+    assert float((dx.float().flatten(0, 1) - rx).norm() / rx.norm()) <= 2 * HALF[BF16]
+    assert float((dw.float() - rw).norm() / rw.norm()) <= 2 * HALF[BF16]
+
+
+def test_gradient_against_differences():
+    """Along random directions in fp32; the float64 quotients at two steps bound the curvature."""
+    x, w, y = _inputs(14, (30,), 24, 90, F32, 0.2)
+    loss, dx, dw, _ = _run(x, w, y, "mean")
+    one = torch.ones((), device="cuda")
+    xr, wr = x.detach().requires_grad_(), w.detach().requires_grad_()
+    dx, dw = torch.autograd.grad(linear_cross_entropy(xr, wr, y), (xr, wr), one)
+    g = torch.Generator().manual_seed(1)
+    ex, ew = torch.randn(x.shape, generator=g).cuda(), torch.randn(w.shape, generator=g).cuda()
+
+    def quotient(h, double):
+        vals = []
+        for s in (1, -1):
+            a, b = x + s * h * ex, w + s * h * ew
+            if double:
+                vals.append(torch.nn.functional.cross_entropy(a.double() @ b.double().T, y))
+            else:
+                vals.append(linear_cross_entropy(a, b, y).double())
+        return float(vals[0] - vals[1]) / (2 * h)
+
+    h = 2.0 ** -6
+    q, half = quotient(h, True), quotient(h / 2, True)
+    along = float((dx * ex).double().sum() + (dw * ew).double().sum())
+    noise = float(_reference(x, w, y, one, "mean")["loss"][1]) * 2
+    assert abs(quotient(h, False) - q) <= noise / h
+    # inputs x + h e are rounded to fp32 in both quotients: U (|x| + h |e|) times the gradient
+    moved = U / h * float((dx.abs() * (x.abs() + ex.abs())).sum() + (dw.abs() * (w.abs() + ew.abs())).sum())
+    assert abs(along - half) <= abs(q - half) + 2 * moved + 1e-6 * abs(q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_other_stream_repeats_and_replays(dtype):
+    x, w, y = _inputs(15, (2, 200), 192, 1100, dtype, 0.1)
+    x2, w2, y2 = _inputs(16, (2, 200), 192, 1100, dtype, 0.5)
+    want, want2 = _run(x, w, y, "mean"), _run(x2, w2, y2, "mean")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _run(x, w, y, "mean")
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    sx, sw, sy, up = x.clone().requires_grad_(), w.clone().requires_grad_(), y.clone(), want[3]
+
+    def step():
+        loss = linear_cross_entropy(sx, sw, sy)
+        return (loss.detach(), *torch.autograd.grad(loss, (sx, sw), up))
+
+    graphs = []
+    for _ in range(2):  # two graphs of the same step: each has its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got))
+    for values, ref in (((x2, w2, y2), want2), ((x, w, y), want)):
+        with torch.no_grad():
+            for s, v in zip((sx, sw, sy), values):
+                s.copy_(v)
+        for graph, _ in graphs:
+            graph.replay()
+        for _, got in graphs:
+            for a, b in zip(got, ref):
+                assert torch.equal(a, b)
+
+
+def test_no_tensor_core_kernel_timed_out():
+    assert _lib.device_status() == 0

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 import torch
 
-from gpa_b200 import _lib, residual_norm, rms_norm
+from gpa_b200 import _lib, linear_cross_entropy, residual_norm, rms_norm
 
 
 def _message():
@@ -71,3 +71,57 @@ def test_norm_entry_points_refuse_missing_tensors():
     assert "scratch" in _message()
     a = _args()
     assert lib.gpa_b200_norm_scratch_bytes(a) >= 2 * 8 * 4
+
+
+def _loss_args(**kw):
+    a = _lib.GpaLossArgs()
+    a.hidden = a.weight = a.labels = 16
+    a.outer, a.inner, a.width, a.vocab, a.weight_stride, a.dtype = 1, 3, 8, 10, 8, 1
+    a.hidden_stride[0], a.hidden_stride[1] = 24, 8
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_loss_refuses_cpu_tensors():
+    x, w, y = torch.ones(2, 8), torch.ones(5, 8), torch.zeros(2, dtype=torch.long)
+    with pytest.raises(ValueError, match="CUDA"):
+        linear_cross_entropy(x, w, y)
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(dtype=3), 1, "dtype"), (dict(reduction=3), 1, "reduction"), (dict(width=0), 1, "width"),
+    (dict(vocab=0), 1, "vocab"), (dict(outer=-1), 1, "outer"), (dict(weight_stride=7), 1, "overlap"),
+    (dict(width=65537, weight_stride=65537), 2, "channels"), (dict(vocab=(1 << 30) + 1), 2, "vocabulary"),
+    (dict(outer=1 << 21), 2, "rows"), (dict(weight=None), 1, "NULL"), (dict(hidden=None), 1, "NULL"),
+])
+def test_loss_entry_points_refuse_bad_arguments(change, code, word):
+    lib = _lib.load()
+    a = _loss_args(**change)
+    assert lib.gpa_b200_loss_forward(a, 16, 16, 1 << 40, 16, 1 << 40, None) == code
+    assert word in _message(), _message()
+    assert lib.gpa_b200_loss_backward(a, 16, 1 << 40, 16, 16, 16, 16, 1 << 40, None) == code
+    assert word in _message(), _message()
+    if word != "NULL":
+        assert lib.gpa_b200_loss_saved_bytes(a) == 0
+        assert lib.gpa_b200_loss_scratch_bytes(a, 0) == 0 and lib.gpa_b200_loss_scratch_bytes(a, 1) == 0
+
+
+def test_loss_entry_points_refuse_small_workspaces():
+    lib = _lib.load()
+    a = _loss_args()
+    saved, fwd, bwd = (lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0),
+                       lib.gpa_b200_loss_scratch_bytes(a, 1))
+    assert saved > 0 and fwd > 0 and bwd > 0
+    assert lib.gpa_b200_loss_forward(a, 16, 16, saved - 1, 16, fwd, None) == 1 and "size" in _message()
+    assert lib.gpa_b200_loss_forward(a, 16, 16, saved, 16, fwd - 1, None) == 1
+    assert lib.gpa_b200_loss_forward(a, None, 16, saved, 16, fwd, None) == 1
+    assert lib.gpa_b200_loss_backward(a, 16, saved, 16, 16, 16, 16, bwd - 1, None) == 1
+    assert lib.gpa_b200_loss_backward(a, 16, saved, 16, None, None, 16, bwd, None) == 1
+
+
+def test_loss_workspace_of_a_training_step_stays_small():
+    """65536 tokens against 151936 entries: logits would take 19.9 GB in 16 bits."""
+    lib = _lib.load()
+    a = _loss_args(outer=8, inner=8192, width=1024, vocab=151936, weight_stride=1024)
+    assert lib.gpa_b200_loss_scratch_bytes(a, 0) < 2.5e9 and lib.gpa_b200_loss_scratch_bytes(a, 1) < 2.5e9
