@@ -169,10 +169,10 @@ __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, int redu
 // dx of the caller's rows: the parts added in order, scaled, rounded and put back in place.
 template <typename T>
 __global__ void k_finish(const float* part, int parts, int64_t part_stride, int pitch, const int* n_rows,
-                         const int* row, const float* scale, int width, T* dx) {
+                         const int* row, const float* scale, float unit, int width, T* dx) {
   const int64_t j = blockIdx.x;
   if (j >= *n_rows) return;
-  const float s = *scale;
+  const float s = *scale * unit;
   T* out = dx + (int64_t)row[j] * width;
   const float* p = part + j * pitch;
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
@@ -183,38 +183,29 @@ __global__ void k_finish(const float* part, int parts, int64_t part_stride, int 
 }
 
 // ------------------------------------------------------------------ products without tensor cores
-// C (128 x 128 per block, 8 x 8 per thread) = A B over k, fp32 multiply-adds.  An operand is
-// K-major (k contiguous) or MN-major; both are read 4 elements at a time.
+// fp32 inputs: C (128 x 128 per block, 8 x 8 per thread) = A B over k, fp32 multiply-adds.  An
+// operand is K-major (k contiguous) or MN-major; both are read 4 elements at a time.  Tensor cores
+// would take three bf16 parts of each operand and six products for the same precision, and lose
+// it again over reductions as long as the vocabulary.
 constexpr int kB = 128, kBK = 16;
 
-template <typename T>
-GPA_DEV void ld4(const T* p, float (&v)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 f = *reinterpret_cast<const float4*>(p);
-    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)e[i];
-  }
-}
-
-template <typename T>
 struct Operand {
-  const T* p;
+  const float* p;
   int64_t pitch;
   int64_t mn, k;  // extents: reads outside give zero (whole groups of 4 along the contiguous axis)
 };
 
-template <typename T, bool KMAJOR>
-GPA_DEV void fetch(const Operand<T>& o, int64_t mn0, int64_t k0, float (&v)[2][4]) {
+template <bool KMAJOR>
+GPA_DEV void fetch(const Operand& o, int64_t mn0, int64_t k0, float (&v)[2][4]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = threadIdx.x + h * 256;  // 512 groups of 4 of a 128 x 16 tile
     const int64_t mn = mn0 + (KMAJOR ? i >> 2 : (i & 31) * 4), k = k0 + (KMAJOR ? (i & 3) * 4 : i >> 5);
     v[h][0] = v[h][1] = v[h][2] = v[h][3] = 0.f;
-    if (mn < o.mn && k < o.k) ld4(o.p + (KMAJOR ? mn * o.pitch + k : k * o.pitch + mn), v[h]);
+    if (mn < o.mn && k < o.k) {
+      const float4 f = *reinterpret_cast<const float4*>(o.p + (KMAJOR ? mn * o.pitch + k : k * o.pitch + mn));
+      v[h][0] = f.x, v[h][1] = f.y, v[h][2] = f.z, v[h][3] = f.w;
+    }
   }
 }
 
@@ -233,8 +224,8 @@ GPA_DEV void put(float (*s)[kB + 4], const float (&v)[2][4]) {
 }
 
 // acc[i][j]: row m0 + (ty * 4 + i % 4) + 64 * (i / 4), column n0 + (tx * 4 + j % 4) + 64 * (j / 4)
-template <typename TA, typename TB, bool AK, bool BK_>
-GPA_DEV void product(const Operand<TA>& a, const Operand<TB>& b, int64_t m0, int64_t n0, int64_t k0,
+template <bool AK, bool BK_>
+GPA_DEV void product(const Operand& a, const Operand& b, int64_t m0, int64_t n0, int64_t k0,
                      int64_t k1, float (&acc)[8][8]) {
   __shared__ float sa[2][kBK][kB + 4], sb[2][kBK][kB + 4];
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
@@ -244,8 +235,8 @@ GPA_DEV void product(const Operand<TA>& a, const Operand<TB>& b, int64_t m0, int
     for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
   float va[2][4], vb[2][4];
   if (k0 < k1) {
-    fetch<TA, AK>(a, m0, k0, va);
-    fetch<TB, BK_>(b, n0, k0, vb);
+    fetch<AK>(a, m0, k0, va);
+    fetch<BK_>(b, n0, k0, vb);
   }
   int s = 0;
   for (int64_t k = k0; k < k1; k += kBK, s ^= 1) {
@@ -253,8 +244,8 @@ GPA_DEV void product(const Operand<TA>& a, const Operand<TB>& b, int64_t m0, int
     put<BK_>(sb[s], vb);
     __syncthreads();
     if (k + kBK < k1) {
-      fetch<TA, AK>(a, m0, k + kBK, va);
-      fetch<TB, BK_>(b, n0, k + kBK, vb);
+      fetch<AK>(a, m0, k + kBK, va);
+      fetch<BK_>(b, n0, k + kBK, vb);
     }
 #pragma unroll
     for (int kk = 0; kk < kBK; ++kk) {
@@ -274,13 +265,12 @@ GPA_DEV void product(const Operand<TA>& a, const Operand<TB>& b, int64_t m0, int
 
 GPA_DEV int at8(int t, int i) { return t * 4 + (i & 3) + 64 * (i >> 2); }
 
-template <typename T>
 __global__ void __launch_bounds__(256, 2) k_stats(const Call c, float2* part, float* z_label) {
   const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
   if (m0 >= *c.n_rows) return;
   float acc[8][8];
-  product<T, T, true, true>({static_cast<const T*>(c.x), c.pitch, c.n_pad, c.pitch},
-                            {static_cast<const T*>(c.w), c.w_pitch, c.vocab, c.pitch}, m0, n0, 0, c.pitch, acc);
+  product<true, true>({static_cast<const float*>(c.x), c.pitch, c.n_pad, c.pitch},
+                            {static_cast<const float*>(c.w), c.w_pitch, c.vocab, c.pitch}, m0, n0, 0, c.pitch, acc);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -307,14 +297,13 @@ __global__ void __launch_bounds__(256, 2) k_stats(const Call c, float2* part, fl
   }
 }
 
-template <typename T>
 __global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int64_t vn, const float* lse,
                                                   const float* r, float* p, int64_t p_pitch) {
   const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
   if (m0 >= up(*c.n_rows, kTile)) return;
   float acc[8][8];
-  product<T, T, true, true>({static_cast<const T*>(c.x), c.pitch, c.n_pad, c.pitch},
-                            {static_cast<const T*>(c.w) + v0 * c.w_pitch, c.w_pitch, vn, c.pitch}, m0, n0, 0,
+  product<true, true>({static_cast<const float*>(c.x), c.pitch, c.n_pad, c.pitch},
+                            {static_cast<const float*>(c.w) + v0 * c.w_pitch, c.w_pitch, vn, c.pitch}, m0, n0, 0,
                             c.pitch, acc);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
@@ -332,7 +321,6 @@ __global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int6
 }
 
 // part[z] (+)= P[:, k of part z] W
-template <typename T>
 __global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int64_t p_pitch, int64_t v0,
                                                int64_t vn, int64_t k_part, bool add, float* part,
                                                int64_t part_stride) {
@@ -340,8 +328,8 @@ __global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int
   if (m0 >= *c.n_rows) return;
   const int64_t k0 = blockIdx.z * k_part, k1 = k0 + k_part < vn ? k0 + k_part : vn;
   float acc[8][8];
-  product<float, T, true, false>({p, p_pitch, c.n_pad, p_pitch},
-                                 {static_cast<const T*>(c.w) + v0 * c.w_pitch, c.w_pitch, c.pitch, vn}, m0, n0,
+  product<true, false>({p, p_pitch, c.n_pad, p_pitch},
+                                 {static_cast<const float*>(c.w) + v0 * c.w_pitch, c.w_pitch, c.pitch, vn}, m0, n0,
                                  k0, k1, acc);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   float* o = part + blockIdx.z * part_stride;
@@ -357,13 +345,12 @@ __global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int
   }
 }
 
-template <typename T>
 __global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int64_t p_pitch, int64_t v0,
-                                               int64_t vn, const float* scale, T* dw) {
+                                               int64_t vn, const float* scale, float* dw) {
   const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
   const int64_t rows = up(*c.n_rows, kTile);
   float acc[8][8];
-  product<float, T, false, false>({p, p_pitch, p_pitch, rows}, {static_cast<const T*>(c.x), c.pitch, c.pitch, rows},
+  product<false, false>({p, p_pitch, p_pitch, rows}, {static_cast<const float*>(c.x), c.pitch, c.pitch, rows},
                                   m0, n0, 0, rows, acc);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const float s = *scale;
@@ -374,7 +361,7 @@ __global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int64_t d = n0 + at8(tx, j);
-      if (d < c.width) dw[(v0 + v) * c.width + d] = T(acc[i][j] * s);
+      if (d < c.width) dw[(v0 + v) * c.width + d] = acc[i][j] * s;
     }
   }
 }
@@ -386,9 +373,12 @@ struct Plan {
   Call c;
   bool copy_w;             // weight rows that cannot be read 16 bytes at a time are copied first
   int es;                  // bytes of an element of x and W
-  int tiles_v, tiles_m;    // 128 x 128 tiles
+  bool tc;                 // tensor cores (16-bit inputs)
+  int pes;                 // bytes of an element of P
+  int tiles_v, tiles_m;    // tiles of z
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
   int parts;               // parts of dx
+  int64_t k_part;          // vocabulary entries of a part
   // saved
   int64_t s_rows, s_label, s_lse, s_bytes;
   // scratch
@@ -420,14 +410,35 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->copy_w = a->width % unit || a->weight_stride % unit || (reinterpret_cast<uintptr_t>(a->weight) & 15);
   c.w = a->weight;
   c.w_pitch = p->copy_w ? c.pitch : a->vocab > 1 ? a->weight_stride : c.pitch;
-  p->tiles_v = (int)((c.vocab + kB - 1) / kB);
-  p->tiles_m = (int)(c.n_pad / kB);
-  const int64_t most = std::max<int64_t>(kTile, kPieceBytes / (c.n_pad * 4) / kTile * kTile);
-  p->piece = std::min(up(c.vocab, kTile), most);
-  const int tiles_d = (c.pitch + kB - 1) / kB;
-  // enough parts of at least 512 entries to give every SM two tiles
-  const int64_t want = (2 * 148 + (int64_t)tiles_d * p->tiles_m - 1) / ((int64_t)tiles_d * p->tiles_m);
-  p->parts = (int)std::max<int64_t>(1, std::min(want, p->piece / 512));
+  p->tc = a->dtype != GPA_B200_F32;
+  p->pes = p->tc ? 2 : 4;
+  const int tile = p->tc ? kTile : kB, at_once = p->tc ? tc_pairs() : 2 * 148;
+  p->tiles_v = (int)((c.vocab + tile - 1) / tile);
+  p->tiles_m = (int)(c.n_pad / tile);
+  const int64_t tiles_d = (c.pitch + tile - 1) / tile;
+  // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
+  // come out in fewer turns of the whole GPU (the pieces' turns added up).
+  const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * p->pes) / kTile);
+  const int64_t all = up(c.vocab, kTile) / kTile;
+  int64_t best = std::min(all, most), turns = INT64_MAX;
+  auto turns_of = [&](int64_t t) {
+    auto one = [&](int64_t v) { return (v * (kTile / tile) * tiles_d + at_once - 1) / at_once; };
+    return all / t * one(t) + (all % t ? one(all % t) : 0);
+  };
+  for (int64_t t = std::min(all, most); t >= 1 && t >= std::min(all, most) / 2; --t)
+    if (turns_of(t) < turns) turns = turns_of(t), best = t;
+  p->piece = best * kTile;
+  // dx: the reduction is cut into parts of at least 512 entries where that fills the GPU's turns
+  // better; every part costs another pass over dx in fp32, so a gain of 10 % is asked for.
+  p->parts = 1;
+  const int64_t tiles_x = tiles_d * p->tiles_m;
+  double cost = (double)((tiles_x + at_once - 1) / at_once);
+  for (int n = 2; n <= 2 * at_once && n <= p->piece / 512; ++n) {
+    const double now = (double)((tiles_x * n + at_once - 1) / at_once) / n;
+    if (now < 0.9 * cost) cost = now, p->parts = n;
+  }
+  p->k_part = up((p->piece + p->parts - 1) / p->parts, 64);
+  p->parts = (int)((p->piece + p->k_part - 1) / p->k_part);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -448,7 +459,7 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->loss = take(4 * c.n);
   p->fwd_bytes = at;
   at = common;
-  p->p = take(c.n_pad * p->piece * 4);
+  p->p = take(c.n_pad * p->piece * p->pes);
   p->dxp = take((int64_t)p->parts * c.n_pad * c.pitch * 4);
   p->r = take(4 * c.n);
   p->scale = take(4);
@@ -492,12 +503,14 @@ void bind(Plan* p, const void* saved, char* scratch) {
     else { using T = __half; CALL; }                       \
   } while (0)
 
+#define FAIL(MSG)                     \
+  do {                                \
+    *why = MSG;                       \
+    return GPA_B200_LAUNCH_FAILURE;   \
+  } while (0)
 #define OK_OR(MSG)                                   \
   do {                                               \
-    if (cudaGetLastError() != cudaSuccess) {         \
-      *why = MSG;                                    \
-      return GPA_B200_LAUNCH_FAILURE;                \
-    }                                                \
+    if (cudaGetLastError() != cudaSuccess) FAIL(MSG); \
   } while (0)
 
 }  // namespace
@@ -550,9 +563,13 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
     BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
     OK_OR("loss_gather launch failed");
     {
-      Launch scope("loss_stats", st);
-      BY_TYPE(a->dtype, (k_stats<T><<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label)));
-      OK_OR("loss_stats launch failed");
+      if (p.tc) {
+        if (!tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
+      } else {
+        Launch scope("loss_stats", st);
+        k_stats<<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label);
+        OK_OR("loss_stats launch failed");
+      }
     }
     Launch scope("loss_join", st);
     k_join<<<(unsigned)((c.n + 31) / 32), dim3(32, 8), 0, st>>>(part, p.tiles_v, c.n_pad, c.n_rows, row, c.label,
@@ -601,7 +618,7 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   const float* lse = reinterpret_cast<const float*>(sv + p.s_lse);
   float* r = reinterpret_cast<float*>(sc + p.r);
   float* scale = reinterpret_cast<float*>(sc + p.scale);
-  float* pr = reinterpret_cast<float*>(sc + p.p);
+  void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
   BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
   OK_OR("loss_gather launch failed");
@@ -612,32 +629,38 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   }
   const int64_t part_stride = c.n_pad * c.pitch;
   const unsigned tiles_d = (unsigned)((c.pitch + kB - 1) / kB);
-  const int64_t k_part = up((p.piece + p.parts - 1) / p.parts, kBK);
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
+    if (p.tc) {
+      if (!tc_probs(c, v0, vn, lse, r, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
+      if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.parts, (int)(p.k_part / 64), v0 > 0, dxp, part_stride, st))
+        FAIL("loss_dx_tc5 launch failed");
+      if (dweight && !tc_dw(c, pr, p.piece, v0, vn, scale, dweight, st)) FAIL("loss_dw_tc5 launch failed");
+      continue;
+    }
     const unsigned tv = (unsigned)(up(vn, kTile) / kB);
+    float* pf = static_cast<float*>(pr);
     {
       Launch scope("loss_probs", st);
-      BY_TYPE(a->dtype, (k_probs<T><<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, r, pr, p.piece)));
+      k_probs<<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, r, pf, p.piece);
       OK_OR("loss_probs launch failed");
     }
     if (dhidden) {
       Launch scope("loss_dx", st);
-      BY_TYPE(a->dtype, (k_dx<T><<<dim3(tiles_d, p.tiles_m, p.parts), 256, 0, st>>>(
-                            c, pr, p.piece, v0, vn, k_part, v0 > 0, dxp, part_stride)));
+      k_dx<<<dim3(tiles_d, p.tiles_m, p.parts), 256, 0, st>>>(c, pf, p.piece, v0, vn, p.k_part, v0 > 0, dxp,
+                                                              part_stride);
       OK_OR("loss_dx launch failed");
     }
     if (dweight) {
       Launch scope("loss_dw", st);
-      BY_TYPE(a->dtype, (k_dw<T><<<dim3(tiles_d, tv), 256, 0, st>>>(c, pr, p.piece, v0, vn, scale,
-                                                                  static_cast<T*>(dweight))));
+      k_dw<<<dim3(tiles_d, tv), 256, 0, st>>>(c, pf, p.piece, v0, vn, scale, static_cast<float*>(dweight));
       OK_OR("loss_dw launch failed");
     }
   }
   if (dhidden) {
     Launch scope("loss_finish", st);
     BY_TYPE(a->dtype, (k_finish<T><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, part_stride, c.pitch, c.n_rows, row,
-                                                                scale, c.width, static_cast<T*>(dhidden))));
+                                                                scale, 1.f / tc_p_scale(a->dtype), c.width, static_cast<T*>(dhidden))));
     OK_OR("loss_finish launch failed");
   }
   return GPA_B200_OK;

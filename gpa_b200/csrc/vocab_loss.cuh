@@ -26,8 +26,21 @@ struct Call {
 
 __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
+// The products of 16-bit inputs on tensor cores (vocab_loss_tc5.cu); false when a launch failed.
+// They tile by kTile x kTile and pair up the SMs: tc_pairs() tiles run at a time.
+int tc_pairs();
+float tc_p_scale(int dtype);  // P is stored times this
+bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st);
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const float* r, void* p, int64_t p_pitch,
+              cudaStream_t st);
+bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
+           float* dx, int64_t dx_part, cudaStream_t st);
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const float* scale, void* dw,
+           cudaStream_t st);
+
 }  // namespace vloss
 
+int loss_device_status(bool clear);
 int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_bytes, void* scratch,
                  size_t scratch_bytes, cudaStream_t st, const char** why);
 int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, const float* dloss,

@@ -1,0 +1,630 @@
+// The products of the vocabulary loss on the 5th-generation tensor cores, for 16-bit inputs
+// (formulas in vocab_loss.cu): z = x W^T with the softmax statistics or with P in its epilogue,
+// dx += P W, and dW = P^T x.
+//
+// One kernel shape serves all four: a pair of CTAs (cta_group::2) owns 256 x 256 tiles of the
+// product, each CTA 128 of the rows.  A pair shares its operands: each CTA brings in its own 128
+// rows of A and half of B's 256 columns (TMA, 128-byte swizzle, 64 of the reduction at a time, 6
+// stages), so an SM's shared memory takes 64 bytes a cycle in and gives 64 out, which its 128
+// allow; one CTA alone with the same tile would need 192.  K-major operands (x, W, P) come as
+// boxes of 64 k x 128 rows, MN-major ones (W in dx, P and x in dW) as two boxes of 64 columns x
+// 64 k: nothing is transposed in memory.  Two 256-column accumulators fill tensor memory: the
+// epilogue warps empty one while the next tile's products go to the other.
+//
+//   warp 0: copies     warp 1: products (first CTA of the pair)     warp 2: tensor memory
+//   warps 4-7: epilogue, a thread for each row of the tile
+//
+// Every wait is bounded (tc5.cuh); a wait that gives up sets the device status and the kernel
+// drains and returns.
+#include <cuda.h>
+
+#include "tc5.cuh"
+#include "vocab_loss.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+namespace gpa {
+
+__device__ int g_loss_status = 0;
+
+namespace vloss {
+namespace {
+
+constexpr int kStages = 6, kBK = 64;
+constexpr int kHalf = 128;                        // rows of an operand that one CTA holds
+constexpr uint32_t kOperand = kHalf * kBK * 2;    // bytes of one operand in one stage
+constexpr uint32_t kStage = 2 * kOperand;
+constexpr size_t kSmem = kStages * kStage + 1024 + 256;  // operands on 1024 bytes, barriers
+constexpr int kThreads = 256;
+constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Mode { kStats, kProbs, kDx, kDw };
+
+struct Args {
+  const int* n_rows;
+  const int* label;
+  int64_t vocab, v0, vn, n_pad;
+  int tiles_n;             // tiles across the product's columns
+  int k_blocks;            // reduction blocks of 64 (kDw: from the rows)
+  // kStats
+  float2* part;
+  float* z_label;
+  // kProbs
+  const float *lse, *r;
+  void* p;
+  int64_t p_pitch;
+  float p_scale;
+  // kDx
+  float* dx;
+  int64_t dx_part;
+  int parts, k_part, pitch;
+  bool add;
+  // kDw
+  void* dw;
+  const float* scale;
+  int width;
+  bool wide;               // dW rows start on 16-byte boundaries
+  uint32_t idesc;
+  bool f16;
+};
+
+// ------------------------------------------------------------------ pair primitives
+GPA_DEV uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+GPA_DEV void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// shared::cluster address of `p` in the first CTA of the pair
+GPA_DEV uint32_t in_first(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(tc5::saddr(p)));
+  return a;
+}
+GPA_DEV void tma_load(void* dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+      "%4}], [%2];" ::"r"(tc5::saddr(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+GPA_DEV void mma2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate));
+}
+// arrive on `bar` of both CTAs once the products issued so far are done
+GPA_DEV void commit2(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          tc5::saddr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+GPA_DEV void arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+GPA_DEV bool try_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(tc5::saddr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+GPA_DEV bool wait_cluster(uint64_t* bar, uint32_t parity) {
+  if (try_cluster(bar, parity)) return true;
+  const uint64_t t0 = tc5::gtime_ns();
+  for (;;) {
+    if (try_cluster(bar, parity)) return true;
+    if (tc5::gtime_ns() - t0 > tc5::kWaitNs) return false;
+  }
+}
+
+// Shared-memory descriptor of a 128-byte-swizzled operand.  K-major: rows of 128 bytes, 8-row
+// groups 1024 bytes apart, a 16-wide step of k 32 bytes further.  MN-major: 128-byte rows of 64
+// columns, one per k; 8-k groups 1024 bytes apart (stride), the next 64 columns 8192 bytes
+// further (leading), a 16-wide step of k 2048 bytes further.
+template <bool MN>
+GPA_DEV uint64_t operand(uint32_t addr, int step) {
+  const uint32_t a = addr + (uint32_t)step * (MN ? 2048u : 32u);
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | (uint64_t)(MN ? 8192u >> 4 : 1u) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+GPA_DEV void ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  __syncwarp();  // the load is the whole warp's; rows may have parted before it
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  tc5::tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+GPA_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+GPA_DEV uint32_t pack2(float a, float b, bool f16) {
+  if (f16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ------------------------------------------------------------------ tiles
+struct Tile {
+  int m, n, part, k0, k1;
+};
+
+template <Mode M>
+struct Walk {
+  int mt, nt, total, n_rows, k_blocks;
+  const Args& a;
+  GPA_DEV Walk(const Args& args) : a(args) {
+    n_rows = *args.n_rows;
+    nt = args.tiles_n;
+    if (M == kDw) {
+      mt = (int)((args.vn + kTile - 1) / kTile);
+      k_blocks = (n_rows + kBK - 1) / kBK;
+    } else {
+      mt = (n_rows + kTile - 1) / kTile;
+      k_blocks = args.k_blocks;
+    }
+    total = mt * nt * (M == kDx ? args.parts : 1);
+  }
+  GPA_DEV Tile at(int t) const {
+    Tile x;
+    x.part = 0;
+    x.k0 = 0;
+    x.k1 = k_blocks;
+    if (M == kStats || M == kProbs) {
+      // kGroup row tiles side by side walk over the vocabulary, so that the tiles in flight
+      // share a few tiles of x and of W in L2
+      const int per = kGroup * nt, g = t / per, in = t - g * per;
+      const int rows = mt - g * kGroup < kGroup ? mt - g * kGroup : kGroup;
+      x.n = in / rows;
+      x.m = g * kGroup + in - x.n * rows;
+    } else {
+      x.n = t % nt;
+      x.m = t / nt;
+      if (M == kDx) {
+        x.part = x.m / mt;
+        x.m -= x.part * mt;
+        x.k0 = x.part * a.k_part;
+        x.k1 = x.k0 + a.k_part < k_blocks ? x.k0 + a.k_part : k_blocks;
+      }
+    }
+    return x;
+  }
+};
+
+template <Mode M>
+GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, int rank, bool empty) {
+  const int in_tile = rank * kHalf + (threadIdx.x & 127);  // warps 4-7: one thread per row
+  const int64_t row = (int64_t)t.m * kTile + in_tile;
+  const int64_t col0 = (int64_t)t.n * kTile;
+  float v[32];
+  if (M == kStats) {
+    const bool live = row < n_rows;
+    const int64_t y = live ? (int64_t)a.label[row] - col0 : -1;
+    float big = -INFINITY, sum = 0.f;
+    for (int c = 0; c < kTile; c += 32) {
+      ld32(tc5::tmem_at(tmem, c), v);
+      if (y >= c && y < c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (y == c + i) a.z_label[row] = v[i];
+      }
+      const int64_t left = a.vocab - col0 - c;
+      if (left < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i >= left) v[i] = -INFINITY;
+      }
+      float m = big;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+      const float off = m == -INFINITY ? 0.f : m * kLog2e;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        s0 += ex2(fmaf(v[i], kLog2e, -off));
+        s1 += ex2(fmaf(v[i + 1], kLog2e, -off));
+      }
+      sum = fmaf(sum, ex2(fmaf(big, kLog2e, -off)), s0 + s1);
+      big = m;
+    }
+    if (live) a.part[(int64_t)t.n * a.n_pad + row] = make_float2(big, sum);
+  } else if (M == kProbs) {
+    const bool live = row < n_rows;
+    const float off = live ? a.lse[row] * kLog2e : 0.f, r = live ? a.r[row] * a.p_scale : 0.f;
+    const int64_t y = live ? (int64_t)a.label[row] - a.v0 - col0 : -1;
+    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p) + row * a.p_pitch + col0);
+    for (int c = 0; c < kTile; c += 32) {
+      ld32(tc5::tmem_at(tmem, c), v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -off));
+      if (y >= c && y < c + 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (y == c + i) v[i] -= 1.f;
+      }
+      const int64_t left = live ? a.vn - col0 - c : 0;
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        w[i] = pack2(2 * i < left ? v[2 * i] * r : 0.f, 2 * i + 1 < left ? v[2 * i + 1] * r : 0.f, a.f16);
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<uint4*>(out + c / 2 + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+  } else if (M == kDx) {
+    const bool live = row < n_rows;
+    float* out = a.dx + t.part * a.dx_part + row * a.pitch + col0;
+    for (int c = 0; c < kTile; c += 32) {
+      ld32(tc5::tmem_at(tmem, c), v);
+      if (!live) continue;
+      const int64_t left = a.pitch - col0 - c;  // a multiple of 8
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        if (i >= left) continue;
+        float4* o = reinterpret_cast<float4*>(out + c + i);
+        float4 f = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        if (a.add) {
+          const float4 g = *o;
+          f.x += g.x, f.y += g.y, f.z += g.z, f.w += g.w;
+        }
+        *o = f;
+      }
+    }
+  } else {
+    const bool live = row < a.vn;
+    const float s = *a.scale / a.p_scale;
+    uint16_t* out = static_cast<uint16_t*>(a.dw) + (a.v0 + row) * a.width + col0;
+    for (int c = 0; c < kTile; c += 32) {
+      if (!empty) {
+        ld32(tc5::tmem_at(tmem, c), v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.f;
+      }
+      if (!live) continue;
+      const int64_t left = a.width - col0 - c;
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i] * s, v[2 * i + 1] * s, a.f16);
+      if (a.wide) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          if (2 * i < left) *reinterpret_cast<uint4*>(out + c + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < left) out[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+
+template <Mode M>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
+  constexpr bool kAMn = M == kDw, kBMn = M == kDx || M == kDw;
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * kStage);
+  uint64_t *full = bars, *empty = bars + kStages, *acc_full = bars + 2 * kStages, *acc_empty = acc_full + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      tc5::mbar_init(&full[i], 1);
+      tc5::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc5::mbar_init(&acc_full[i], 1);
+      tc5::mbar_init(&acc_empty[i], 8);  // the four epilogue warps of both CTAs
+    }
+    tc5::mbar_fence_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc5::saddr(slot))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc5::fence_before_sync();
+  __syncthreads();
+  pair_sync();
+  tc5::fence_after_sync();
+  const uint32_t tmem = *slot;
+  const Walk<M> walk(a);
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int t = pair; t < walk.total && ok; t += pairs) {
+        const Tile x = walk.at(t);
+        const int ra = x.m * kTile + rank * kHalf, rb = x.n * kTile + rank * kHalf;
+        for (int k = x.k0; k < x.k1; ++k, ++it) {
+          const uint32_t s = it % kStages, turn = it / kStages;
+          if (turn && !(ok = tc5::mbar_wait(&empty[s], (turn - 1) & 1))) break;
+          unsigned char* sa = sm + s * kStage;
+          unsigned char* sb = sa + kOperand;
+          const uint32_t bar = in_first(&full[s]);
+          if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
+          const int kk = k * kBK;
+          if (kAMn) {
+            tma_load(sa, &map_a, ra, kk, bar);
+            tma_load(sa + kOperand / 2, &map_a, ra + 64, kk, bar);
+          } else {
+            tma_load(sa, &map_a, kk, ra, bar);
+          }
+          if (M == kDx) {  // the reduction runs over the piece's vocabulary entries
+            tma_load(sb, &map_b, rb, (int)a.v0 + kk, bar);
+            tma_load(sb + kOperand / 2, &map_b, rb + 64, (int)a.v0 + kk, bar);
+          } else if (kBMn) {
+            tma_load(sb, &map_b, rb, kk, bar);
+            tma_load(sb + kOperand / 2, &map_b, rb + 64, kk, bar);
+          } else {
+            tma_load(sb, &map_b, kk, (int)a.v0 + rb, bar);
+          }
+        }
+      }
+      // no copy is in flight when the pair leaves (after a wait that gave up, too)
+      if (rank == 0)
+        for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j)
+          ok = tc5::mbar_wait(&full[j % kStages], (j / kStages) & 1) && ok;
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      uint32_t it = 0, count = 0;
+      for (int t = pair; t < walk.total && ok; t += pairs) {
+        const Tile x = walk.at(t);
+        if (x.k0 >= x.k1) continue;
+        const uint32_t buf = count & 1, use = count >> 1;
+        ++count;
+        if (use && !(ok = wait_cluster(&acc_empty[buf], (use - 1) & 1))) break;
+        tc5::fence_after_sync();
+        for (int k = x.k0; k < x.k1; ++k, ++it) {
+          const uint32_t s = it % kStages;
+          if (!(ok = tc5::mbar_wait(&full[s], (it / kStages) & 1))) break;
+          tc5::fence_after_sync();
+          const uint32_t sa = tc5::saddr(sm + s * kStage), sb = sa + kOperand;
+#pragma unroll
+          for (int ks = 0; ks < kBK / 16; ++ks)
+            mma2(tmem + buf * kTile, operand<kAMn>(sa, ks), operand<kBMn>(sb, ks), a.idesc, k > x.k0 || ks > 0);
+          commit2(&empty[s]);
+        }
+        if (!ok) break;
+        commit2(&acc_full[buf]);
+      }
+    }
+  } else if (warp >= 4) {
+    uint32_t count = 0;
+    for (int t = pair; t < walk.total && ok; t += pairs) {
+      const Tile x = walk.at(t);
+      if (x.k0 >= x.k1) {
+        if (M == kDw) epilogue<M>(a, x, walk.n_rows, tmem, rank, true);
+        continue;
+      }
+      const uint32_t buf = count & 1, use = count >> 1;
+      ++count;
+      if (!(ok = __all_sync(0xffffffffu, tc5::mbar_wait(&acc_full[buf], use & 1)))) break;
+      tc5::fence_after_sync();
+      epilogue<M>(a, x, walk.n_rows, tmem + buf * kTile, rank, false);
+      tc5::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) arrive_first(in_first(&acc_empty[buf]));
+    }
+  }
+  if (!ok) g_loss_status = GPA_B200_DEVICE_TIMEOUT;
+  tc5::fence_before_sync();
+  __syncthreads();
+  pair_sync();
+  tc5::fence_after_sync();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ------------------------------------------------------------------ host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+  static std::atomic<EncodeFn> fn{nullptr};
+  EncodeFn f = fn.load(std::memory_order_relaxed);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return nullptr;
+    f = reinterpret_cast<EncodeFn>(p);
+    fn.store(f, std::memory_order_relaxed);
+  }
+  return f;
+}
+
+// [outer][inner] of 16-bit values, rows `pitch` elements apart, in boxes of 64 x `rows`
+bool make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int64_t pitch, int rows, bool f16) {
+  EncodeFn f = encoder();
+  if (!f) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)rows}, one[2] = {1, 1};
+  return f(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint32_t idesc_of(const Call& c, bool a_mn, bool b_mn) {
+  uint32_t d = tc5::idesc_bf16(2 * kHalf, kTile, a_mn, b_mn);
+  if (c.dtype == GPA_B200_F16) d &= ~((1u << 7) | (1u << 10));  // both operands fp16
+  return d;
+}
+
+Args base_args(const Call& c) {
+  Args a;
+  std::memset(&a, 0, sizeof(a));
+  a.n_rows = c.n_rows;
+  a.label = c.label;
+  a.vocab = c.vocab;
+  a.n_pad = c.n_pad;
+  a.pitch = c.pitch;
+  a.width = c.width;
+  a.f16 = c.dtype == GPA_B200_F16;
+  a.p_scale = tc_p_scale(c.dtype);
+  a.k_blocks = (c.pitch + kBK - 1) / kBK;
+  return a;
+}
+
+template <Mode M>
+bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
+            cudaStream_t st) {
+  if (cudaFuncSetAttribute(k_product<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+    return false;
+  const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
+  Launch scope(name, st);
+  k_product<M><<<2 * pairs, kThreads, kSmem, st>>>(ma, mb, a);
+  return cudaGetLastError() == cudaSuccess;
+}
+
+}  // namespace
+
+float tc_p_scale(int dtype) { return dtype == GPA_B200_F16 ? 16384.f : 1.f; }
+
+int tc_pairs() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 74;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    int sms = 0;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (sms / 2));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(k_product<kStats>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_product<kStats>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = std::max(1, sms / 2);
+    }
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
+  const bool f16 = c.dtype == GPA_B200_F16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, c.x, c.pitch, c.n, c.pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kHalf, f16))
+    return false;
+  Args a = base_args(c);
+  a.part = part;
+  a.z_label = z_label;
+  a.tiles_n = (int)((c.vocab + kTile - 1) / kTile);
+  a.idesc = idesc_of(c, false, false);
+  return launch<kStats>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
+}
+
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const float* r, void* p, int64_t p_pitch,
+              cudaStream_t st) {
+  const bool f16 = c.dtype == GPA_B200_F16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, c.x, c.pitch, c.n, c.pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kHalf, f16))
+    return false;
+  Args a = base_args(c);
+  a.v0 = v0;
+  a.vn = vn;
+  a.lse = lse;
+  a.r = r;
+  a.p = p;
+  a.p_pitch = p_pitch;
+  a.tiles_n = (int)((vn + kTile - 1) / kTile);
+  a.idesc = idesc_of(c, false, false);
+  return launch<kProbs>("loss_probs_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
+}
+
+bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
+           float* dx, int64_t dx_part, cudaStream_t st) {
+  const bool f16 = c.dtype == GPA_B200_F16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, p, p_pitch, c.n_pad, p_pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kBK, f16))
+    return false;
+  Args a = base_args(c);
+  a.v0 = v0;
+  a.vn = vn;
+  a.k_blocks = (int)((vn + kBK - 1) / kBK);
+  a.dx = dx;
+  a.dx_part = dx_part;
+  a.parts = parts;
+  a.k_part = k_part;
+  a.add = add;
+  a.tiles_n = (c.pitch + kTile - 1) / kTile;
+  a.idesc = idesc_of(c, false, true);
+  return launch<kDx>("loss_dx_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile) * parts, st);
+}
+
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const float* scale, void* dw,
+           cudaStream_t st) {
+  const bool f16 = c.dtype == GPA_B200_F16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, p, p_pitch, c.n_pad, p_pitch, kBK, f16) ||
+      !make_map(&mb, c.x, c.pitch, c.n_pad, c.pitch, kBK, f16))
+    return false;
+  Args a = base_args(c);
+  a.v0 = v0;
+  a.vn = vn;
+  a.scale = scale;
+  a.dw = dw;
+  a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
+  a.tiles_n = (c.pitch + kTile - 1) / kTile;
+  a.idesc = idesc_of(c, true, true);
+  return launch<kDw>("loss_dw_tc5", ma, mb, a, (int64_t)a.tiles_n * ((vn + kTile - 1) / kTile), st);
+}
+
+}  // namespace vloss
+
+int loss_device_status(bool clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_loss_status, sizeof(int)) != cudaSuccess) return -1;
+  if (clear && v) {
+    const int z = 0;
+    if (cudaMemcpyToSymbol(g_loss_status, &z, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return v;
+}
+
+}  // namespace gpa

@@ -12,6 +12,8 @@ graph and have first-order gradients.  They raise ``ValueError`` for arguments t
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
@@ -22,14 +24,14 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_NORM_WIDTH = 16384
 
 
+def _on(device):
+    """`device` made current: the library sizes its workspaces and launches for that one."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def _call(fn, device, *args):
-    """`fn(*args, stream)` on the current stream of `device`, made current for the call."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream)
+    """`fn(*args, stream)` on the current stream of `device`, which is current."""
+    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
     if rc:
         _lib.check(rc, fn.__name__)
 
@@ -119,18 +121,20 @@ def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, s
 
 def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
     lib = _lib.load()
-    nbytes = lib.gpa_b200_norm_scratch_bytes(a)
-    scratch = _scratch(nbytes, device)
     g = _lib.GpaNormGrads(*[None if t is None else t.data_ptr() for t in grads])
-    _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
-          _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
+    with _on(device):
+        nbytes = lib.gpa_b200_norm_scratch_bytes(a)
+        scratch = _scratch(nbytes, device)
+        _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
+              _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
 
 
 def _rms_forward(x, weight, eps, out_dtype):
     out = torch.empty(x.shape, device=x.device, dtype=out_dtype)
     if out.numel():
         a, keep = _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, out_dtype, x.shape)
-        _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
+        with _on(x.device):
+            _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
     return out
 
 
@@ -182,8 +186,9 @@ def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, c
     if stream.numel():
         a, keep = _norm_args(residual, update, weight, post_weight, gate, scale, eps, const,
                              residual.dtype, out_dtype, residual.shape)
-        _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
-              normed.data_ptr())
+        with _on(residual.device):
+            _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
+                  normed.data_ptr())
     return stream, normed
 
 
@@ -316,10 +321,11 @@ def _loss_forward(hidden, weight, labels, ignore_index, reduction):
     dev = hidden.device
     a, keep = _loss_args(hidden, weight, labels, ignore_index, reduction)
     loss = torch.empty(labels.shape if reduction == 2 else (), device=dev, dtype=torch.float32)
-    sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
-    saved, scratch = (_scratch(n, dev) for n in sizes)
-    _call(lib.gpa_b200_loss_forward, dev, a, loss.data_ptr(), saved.data_ptr(), sizes[0],
-          scratch.data_ptr(), sizes[1])
+    with _on(dev):
+        sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
+        saved, scratch = (_scratch(n, dev) for n in sizes)
+        _call(lib.gpa_b200_loss_forward, dev, a, loss.data_ptr(), saved.data_ptr(), sizes[0],
+              scratch.data_ptr(), sizes[1])
     return loss, saved
 
 
@@ -341,10 +347,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         dx, dw = (torch.empty(t.shape, device=dev, dtype=t.dtype) if need else None
                   for t, need in zip((hidden, weight), ctx.needs_input_grad))
         dloss = dloss.contiguous()
-        nbytes = lib.gpa_b200_loss_scratch_bytes(a, 1)
-        scratch = _scratch(nbytes, dev)
-        _call(lib.gpa_b200_loss_backward, dev, a, ctx.saved_ws.data_ptr(), ctx.saved_ws.numel(),
-              dloss.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), scratch.data_ptr(), nbytes)
+        with _on(dev):
+            nbytes = lib.gpa_b200_loss_scratch_bytes(a, 1)
+            scratch = _scratch(nbytes, dev)
+            _call(lib.gpa_b200_loss_backward, dev, a, ctx.saved_ws.data_ptr(), ctx.saved_ws.numel(),
+                  dloss.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), scratch.data_ptr(), nbytes)
         return dx, dw, None, None, None
 
 
