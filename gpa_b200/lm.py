@@ -11,10 +11,14 @@ without Hugging Face Transformers, with the same data flow per layer:
   of q and k, key/value heads repeated to the query heads (:183), the DenseGPA core, and
   the output projection (:192);
 * pre-norm residual blocks with a SwiGLU MLP and RMSNorm, a final RMSNorm and a head tied
-  to the embedding;
-* the training loss summed over 512-token chunks of next-token cross entropy, each chunk
-  recomputed in the backward (:388-401), and per-layer activation checkpointing
-  (:379-381), which keeps one layer's core workspace alive at a time;
+  to the embedding; on CUDA each residual addition and the norm after it are one kernel
+  (``gpa_b200.residual_norm``), which also takes the options of ``GPALMConfig`` that the
+  wrapper does not have: a norm after each block, a gate and a learned scale of its output;
+* the training loss, next-token cross entropy: on CUDA ``gpa_b200.linear_cross_entropy``, which
+  never stores the logits; elsewhere summed over chunks of ``loss_chunk_size`` tokens, each
+  recomputed in the backward (:388-401);
+* per-layer activation checkpointing (:379-381), which keeps one layer's core workspace alive
+  at a time;
 * a cache of per-layer ``GPAState`` plus convolution tails that reorders along the batch
   for beam search (``reorder_cache``, ``batch_repeat_interleave``: :92-115).
 
@@ -34,6 +38,7 @@ from torch.utils.checkpoint import checkpoint
 
 from .config import GPAConfig
 from .core import DenseGPA
+from .ops import _DTYPES, MAX_NORM_WIDTH, linear_cross_entropy, residual_norm, rms_norm
 from .state import GPAState, _map
 
 
@@ -48,17 +53,33 @@ class GPALMConfig:
     intermediate_size: int = 3072
     rms_eps: float = 1e-6
     conv_width: int = 4
-    loss_chunk_size: int = 512
+    loss_chunk_size: int = 512  # tokens of a chunk of the loss off CUDA
     slots: tuple = (64, 64, 64, 128)
     chunk_size: int = 64
     initializer_range: float = 0.02
     tie_embeddings: bool = True
+    post_norms: bool = False              # a norm of each block's output, before it is added
+    block_gate: str = "none"              # sigmoid gate of it, from the block's normed input:
+                                          # "token" (one value), "channel" (one per channel)
+    residual_scale: float | None = None   # initial value of its learned per-channel scale
 
     def __post_init__(self):
+        if self.block_gate not in ("none", "token", "channel"):
+            raise ValueError("block_gate must be none, token or channel")
         if self.num_heads % self.num_kv_heads:
             raise ValueError("query heads must be divisible by key/value heads")
         if self.conv_width < 1 or self.loss_chunk_size < 1:
             raise ValueError("conv_width and loss_chunk_size must be positive")
+
+
+def _kernels(x: Tensor) -> bool:
+    """Whether the norm kernels take rows like x's (else the plain torch form runs)."""
+    return x.is_cuda and x.dtype in _DTYPES and x.shape[-1] <= MAX_NORM_WIDTH
+
+
+def _projection_dtype(x: Tensor) -> torch.dtype:
+    """The dtype a linear layer reads x in: autocast's where it is on."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
 class RMSNorm(nn.Module):
@@ -67,7 +88,9 @@ class RMSNorm(nn.Module):
         self.weight = nn.Parameter(torch.ones(dim))
         self.eps = eps
 
-    def forward(self, x: Tensor) -> Tensor:
+    def forward(self, x: Tensor, out_dtype: torch.dtype | None = None) -> Tensor:
+        if _kernels(x):
+            return rms_norm(x, self.weight, self.eps, out_dtype=out_dtype)
         w = x.float()
         w = w * torch.rsqrt(w.square().mean(-1, keepdim=True) + self.eps)
         return (w * self.weight.float()).to(x.dtype)
@@ -163,18 +186,68 @@ class SwiGLU(nn.Module):
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
+class BlockOutput(nn.Module):
+    """What happens to a block's output on its way into the residual stream: by default nothing;
+    with the options of GPALMConfig a norm, a gate from the block's input and a scale."""
+
+    def __init__(self, cfg: GPALMConfig):
+        super().__init__()
+        dim = cfg.hidden_size
+        self.post = RMSNorm(dim, cfg.rms_eps) if cfg.post_norms else None
+        self.gate = (None if cfg.block_gate == "none" else
+                     nn.Linear(dim, 1 if cfg.block_gate == "token" else dim))
+        self.scale = (None if cfg.residual_scale is None else
+                      nn.Parameter(torch.full((dim,), float(cfg.residual_scale))))
+
+    def gate_of(self, normed: Tensor) -> Tensor | None:
+        return None if self.gate is None else self.gate(normed)
+
+    def add(self, x: Tensor, update: Tensor, gate: Tensor | None) -> Tensor:
+        if self.post is not None:
+            update = self.post(update)
+        if gate is not None:
+            update = torch.sigmoid(gate) * update
+        if self.scale is not None:
+            update = self.scale * update
+        return x + update
+
+    def add_and_norm(self, x: Tensor, update: Tensor, gate: Tensor | None, norm: RMSNorm):
+        """(x + the update's share, its norm for the next projections)."""
+        if _kernels(x):
+            return residual_norm(x, update, norm.weight, norm.eps, gate=gate, scale=self.scale,
+                                 post_weight=None if self.post is None else self.post.weight,
+                                 out_dtype=_projection_dtype(x))
+        x = self.add(x, update, gate)
+        return x, norm(x)
+
+
 class GPABlock(nn.Module):
     def __init__(self, cfg: GPALMConfig):
         super().__init__()
         self.input_norm = RMSNorm(cfg.hidden_size, cfg.rms_eps)
         self.attn = GPAAttention(cfg)
+        self.attn_out = BlockOutput(cfg)
         self.post_norm = RMSNorm(cfg.hidden_size, cfg.rms_eps)
         self.mlp = SwiGLU(cfg)
+        self.mlp_out = BlockOutput(cfg)
+
+    def step(self, x: Tensor, update: Tensor | None = None, gate: Tensor | None = None,
+             before: BlockOutput | None = None, memory: LayerMemory | None = None, attend=None):
+        """The block on a stream x whose last addition is still to be made: ``update`` and
+        ``gate`` are the previous block's, ``before`` its output stage (None for the first
+        block).  Returns (x, update, gate, memory) of this block, for the next one.  ``attend``
+        stands in for the attention (decoding sessions)."""
+        if update is None:
+            n = self.input_norm(x, _projection_dtype(x))
+        else:
+            x, n = before.add_and_norm(x, update, gate, self.input_norm)
+        y, memory = self.attn(n, memory) if attend is None else (attend(n), memory)
+        x, m = self.attn_out.add_and_norm(x, y, self.attn_out.gate_of(n), self.post_norm)
+        return x, self.mlp(m), self.mlp_out.gate_of(m), memory
 
     def forward(self, x: Tensor, memory: LayerMemory | None = None):
-        y, memory = self.attn(self.input_norm(x), memory)
-        x = x + y
-        return x + self.mlp(self.post_norm(x)), memory
+        x, update, gate, memory = self.step(x, memory=memory)
+        return self.mlp_out.add(x, update, gate), memory
 
 
 class GPALM(nn.Module):
@@ -212,18 +285,23 @@ class GPALM(nn.Module):
         if use_cache and cache is None:
             cache = GPALMCache([None] * cfg.num_layers)
         x = self.embed(ids)
+        update = gate = before = None  # the last block's output, not yet added to x
         with torch.autocast("cuda", dtype=torch.bfloat16, enabled=x.is_cuda and self.autocast):
             for i, blk in enumerate(self.blocks):
                 old = None if cache is None else cache.layers[i]
                 if self.training and self.gradient_checkpointing:
                     # reentrant: the layer's forward runs without a graph, so the core's
                     # forward workspace is freed at once and rebuilt in the backward
-                    x = checkpoint(lambda y, blk=blk: blk(y)[0], x, use_reentrant=True)
+                    x, update, gate = checkpoint(
+                        lambda y, u, g, blk=blk, before=before: blk.step(y, u, g, before)[:3],
+                        x, update, gate, use_reentrant=True)
                 else:
-                    x, mem = blk(x, old)
+                    x, update, gate, mem = blk.step(x, update, gate, before, old)
                     if cache is not None:
                         cache.layers[i] = mem
-            x = self.norm(x)
+                before = blk.mlp_out
+            x = (self.norm(x, _projection_dtype(x)) if update is None else
+                 before.add_and_norm(x, update, gate, self.norm)[1])
             if cache is not None:
                 cache.seen_tokens += ids.shape[1]
             if labels is None:
@@ -233,8 +311,12 @@ class GPALM(nn.Module):
             return self._loss(x, labels), cache
 
     def _loss(self, x: Tensor, labels: Tensor) -> Tensor:
-        """Mean next-token cross entropy over labels[:, 1:] != -100, in recomputed chunks."""
+        """Mean next-token cross entropy over labels[:, 1:] != -100."""
         t = x.shape[1]
+        if x.is_cuda and x.dtype in _DTYPES:
+            # position i predicts token i + 1; the last position predicts nothing
+            shifted = F.pad(labels[:, 1:], (0, 1), value=-100)
+            return linear_cross_entropy(x, self.lm_head.weight.to(x.dtype), shifted)
         count = (labels[:, 1:] != -100).sum().clamp_min(1)
         step = self.cfg.loss_chunk_size
 
@@ -282,21 +364,23 @@ class GPALM(nn.Module):
             b = tok.shape[0]
             x = self.embed(tok[:, None])
             with torch.autocast("cuda", dtype=torch.bfloat16):
+                update = gate = before = None
                 for i, (blk, sess) in enumerate(zip(self.blocks, sessions)):
-                    a = blk.attn
-                    y = blk.input_norm(x)
-                    proj = torch.cat((a.q_proj(y), a.k_proj(y), a.v_proj(y)), -1)
-                    proj, tail = causal_conv(proj, a.conv, tails[i])
-                    tails[i].copy_(tail)
-                    q, k, v = proj.split((h * d, kv * d, kv * d), -1)
-                    q = a.q_norm(q.reshape(b, 1, h, d))
-                    k = a.k_norm(k.reshape(b, 1, kv, d))
-                    v = v.reshape(b, 1, kv, d)
-                    k, v = (z.repeat_interleave(h // kv, dim=2) for z in (k, v))
-                    o = sess.step(*(z.to(torch.bfloat16).contiguous() for z in (q, k, v)))
-                    x = x + a.o_proj(o.reshape(b, 1, h * d).to(x.dtype))
-                    x = x + blk.mlp(blk.post_norm(x))
-                x = self.norm(x)
+                    def attend(y, a=blk.attn, sess=sess, held=tails[i]):
+                        proj = torch.cat((a.q_proj(y), a.k_proj(y), a.v_proj(y)), -1)
+                        proj, tail = causal_conv(proj, a.conv, held)
+                        held.copy_(tail)
+                        q, k, v = proj.split((h * d, kv * d, kv * d), -1)
+                        q = a.q_norm(q.reshape(b, 1, h, d))
+                        k = a.k_norm(k.reshape(b, 1, kv, d))
+                        v = v.reshape(b, 1, kv, d)
+                        k, v = (z.repeat_interleave(h // kv, dim=2) for z in (k, v))
+                        o = sess.step(*(z.to(torch.bfloat16).contiguous() for z in (q, k, v)))
+                        return a.o_proj(o.reshape(b, 1, h * d).to(y.dtype))
+
+                    x, update, gate, _ = blk.step(x, update, gate, before, attend=attend)
+                    before = blk.mlp_out
+                x = before.add_and_norm(x, update, gate, self.norm)[1]
                 tok.copy_(self.lm_head(x[:, -1]).float().argmax(-1))
 
         # every decode step is the same sequence of launches on fixed buffers: record one in a

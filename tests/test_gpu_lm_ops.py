@@ -1,0 +1,125 @@
+"""The norms and the vocabulary loss inside the LM, together as a training step uses them.
+
+A two-layer model runs with the operators on the GPU; its twin has the CPU oracle as its cores
+and the plain torch form of everything else, in float64.  fp32 end to end, with and without the
+block options (norm after a block, gates, learned scale), checkpointed and not: loss within 1e-5
+and every gradient within 1e-3 relative L2, the criteria of the model's other parity tests.
+"""
+from __future__ import annotations
+
+import dataclasses
+
+import pytest
+import torch
+
+from gpa_b200 import _lib
+from gpa_b200.lm import GPALM, GPALMConfig
+from gpa_b200.training_graph import GradientGraph
+from lm_oracle import oracle_lm
+from parity_util import rel
+
+pytestmark = pytest.mark.gpu
+
+CFG = GPALMConfig(vocab_size=500, hidden_size=128, num_layers=2, num_heads=4, num_kv_heads=2,
+                  head_dim=32, intermediate_size=256, slots=(16, 16, 32), chunk_size=64,
+                  loss_chunk_size=48)
+OPTIONS = [dict(post_norms=True), dict(block_gate="token"), dict(residual_scale=0.5),
+           dict(post_norms=True, block_gate="channel", residual_scale=0.5)]
+
+
+def _model(cfg, seed=0):
+    torch.manual_seed(seed)
+    m = GPALM(cfg)
+    with torch.no_grad():
+        for blk in m.blocks:
+            blk.attn.conv.normal_(0., .3)
+            for out in (blk.attn_out, blk.mlp_out):
+                for p in out.parameters():
+                    p.add_(torch.randn_like(p) * 0.1)
+            for w in blk.attn.gpa.query_weight:
+                w.normal_(0., .2)
+    return m
+
+
+@pytest.mark.parametrize("checkpointing", [False, True])
+@pytest.mark.parametrize("options", OPTIONS)
+def test_block_options_match_the_plain_form(options, checkpointing, cpu_threads):
+    m = _model(dataclasses.replace(CFG, **options))
+    twin = oracle_lm(m)
+    ids = torch.randint(0, CFG.vocab_size, (2, 70), generator=torch.Generator().manual_seed(1))
+    labels = ids.clone()
+    labels[0, 3:9] = -100
+    twin.train()
+    ref, _ = twin(ids, labels=labels)
+    ref.backward()
+    gpu = m.cuda().train()
+    gpu.gradient_checkpointing, gpu.autocast = checkpointing, False
+    loss, _ = gpu(ids.cuda(), labels=labels.cuda())
+    loss.backward()
+    assert rel(loss, ref) <= 1e-5
+    want = {n.replace("gpa.inner.", "gpa."): p.grad for n, p in twin.named_parameters() if p.grad is not None}
+    got = {n: p.grad for n, p in gpu.named_parameters() if p.grad is not None}
+    assert set(got) <= set(want)
+    bad = {n: rel(g, want[n]) for n, g in got.items() if not rel(g, want[n]) <= 1e-3}
+    assert not bad, bad
+
+
+def test_state_dict_names_are_those_without_the_options():
+    names = set(GPALM(CFG).state_dict())
+    assert not any("attn_out" in n or "mlp_out" in n for n in names)
+    assert {n.split("blocks.0.")[1] for n in set(_model(dataclasses.replace(CFG, **OPTIONS[3])).state_dict())
+            - names if "blocks.0." in n} == {
+        f"{b}_out.{p}" for b in ("attn", "mlp") for p in ("post.weight", "gate.weight", "gate.bias", "scale")}
+
+
+@pytest.mark.parametrize("options", [{}, OPTIONS[3]])
+def test_generation_paths_agree_and_use_the_kernels(options):
+    m = _model(dataclasses.replace(CFG, **options), seed=2).cuda().eval()
+    ids = torch.randint(0, CFG.vocab_size, (3, 70), generator=torch.Generator().manual_seed(3)).cuda()
+    a = m.generate(ids, 6, fused_decode=True)
+    _lib.profile_start()
+    b = m.generate(ids, 6, fused_decode=False)
+    counts = _lib.profile_stop()
+    # Both paths compute in bf16 with kernels of their own, whose results are within 2e-2 relative
+    # L2 of one another (the criterion of the bf16 parity tests).  A logit is n . w with |n| =
+    # sqrt(hidden) after the final norm (weights 1), so two candidates may change places only if
+    # their logits differ by at most 2e-2 |n| |w_a - w_b|; after that the sequences part.
+    head = m.lm_head.weight.detach().float()
+    for i in range(3):
+        part = (a[i] != b[i]).nonzero()
+        if len(part):
+            k = int(part[0])
+            with torch.no_grad():
+                logits, _ = m(torch.cat((ids[i], a[i, :k]))[None])
+            u, v = int(a[i, k]), int(b[i, k])
+            margin = float((logits[0, -1, u] - logits[0, -1, v]).abs())
+            assert margin <= 2e-2 * CFG.hidden_size ** .5 * float((head[u] - head[v]).norm()), (i, k, margin)
+    # per call: the first norm, a q and a k norm a layer, a join after each of its two blocks
+    assert counts["norm_fwd"][0] == 6 * (1 + 2 * (2 + 2))
+
+
+def test_training_step_runs_the_kernels_under_autocast_and_in_a_graph():
+    m = _model(CFG, seed=4).cuda().train()
+    ids = torch.randint(0, CFG.vocab_size, (2, 64), generator=torch.Generator().manual_seed(5)).cuda()
+    _lib.profile_start()
+    loss, _ = m(ids, labels=ids)
+    loss.backward()
+    counts = _lib.profile_stop()
+    assert {"norm_fwd", "norm_bwd", "loss_stats_tc5", "loss_probs_tc5", "loss_dx_tc5", "loss_dw_tc5"} <= set(counts)
+    want = {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+    value = loss.detach().clone()
+    del loss  # the eager graph is gone before the capture
+    graph = GradientGraph(m, (torch.zeros(1, device="cuda"),), lambda _: (m(ids, labels=ids)[0], ids))
+    got, _ = graph.replay(torch.zeros(1, device="cuda"))
+    assert torch.equal(got, value)
+    bad = {n: rel(p.grad, want[n]) for n, p in m.named_parameters()
+           if p.grad is not None and not rel(p.grad, want[n]) <= 1e-2}
+    assert not bad, bad
+
+
+def test_no_label_at_all_gives_zero_loss_and_gradients():
+    m = _model(CFG, seed=6).cuda().train()
+    ids = torch.zeros(2, 5, dtype=torch.long, device="cuda")
+    loss, _ = m(ids, labels=torch.full_like(ids, -100))
+    loss.backward()
+    assert float(loss) == 0 and not m.embed.weight.grad.any()
