@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int
 }
 
 // ------------------------------------------------------------------ plan of a call
-constexpr int64_t kPieceBytes = int64_t(1) << 30;  // of P at a time
+constexpr int64_t kPieceBytes = int64_t(3) << 29;  // of P at a time
 
 struct Plan {
   Call c;

@@ -170,6 +170,20 @@ GPA_DEV uint32_t pack2(float a, float b, bool f16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 32 bytes at a time, a whole sector: an epilogue thread owns a row, so neighbouring threads do
+// not share sectors and narrower accesses would move each one twice
+GPA_DEV void st8(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+GPA_DEV void ld8(const void* p, float* f) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7])
+               : "l"(p)
+               : "memory");
+}
+
 // ------------------------------------------------------------------ tiles
 struct Tile {
   int m, n, part, k0, k1;
@@ -274,8 +288,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
       for (int i = 0; i < 16; ++i)
         w[i] = pack2(2 * i < left ? v[2 * i] * r : 0.f, 2 * i + 1 < left ? v[2 * i + 1] * r : 0.f, a.f16);
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<uint4*>(out + c / 2 + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      for (int i = 0; i < 16; i += 8) st8(out + c / 2 + i, w + i);
     }
   } else if (M == kDx) {
     const bool live = row < n_rows;
@@ -284,17 +297,17 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
       ld32(tc5::tmem_at(tmem, c), v);
       if (!live) continue;
       const int64_t left = a.pitch - col0 - c;  // a multiple of 8
+      if (a.add) {
+        float g[32];
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        if (i >= left) continue;
-        float4* o = reinterpret_cast<float4*>(out + c + i);
-        float4 f = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        if (a.add) {
-          const float4 g = *o;
-          f.x += g.x, f.y += g.y, f.z += g.z, f.w += g.w;
-        }
-        *o = f;
+        for (int i = 0; i < 32; i += 8)
+          if (i < left) ld8(out + c + i, g + i);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] += g[i];
       }
+#pragma unroll
+      for (int i = 0; i < 32; i += 8)
+        if (i < left) st8(out + c + i, reinterpret_cast<const uint32_t*>(v + i));
     }
   } else {
     const bool live = row < a.vn;
