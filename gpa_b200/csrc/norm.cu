@@ -46,27 +46,43 @@ struct Bwd {
   int sum_w, sum_p, sum_c, sums;  // slot of dw / dwp / dc in a partial row, or -1
 };
 
-template <int VEC>
-GPA_DEV void ldv(const void* p, int64_t i, int dt, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = load_in(p, i, dt);
+// 8 values as they lie in memory (one or two 16-byte loads), so that a load in flight holds few
+// registers, and their conversion
+struct Raw8 {
+  uint4 a, b;
+};
+GPA_DEV Raw8 ldraw(const void* p, int64_t i, int dt) {
+  Raw8 r;
+  r.b = make_uint4(0, 0, 0, 0);
+  if (dt == kF32) {
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
+    r.a = q[0];
+    r.b = q[1];
   } else {
-    if (dt == kF32) {
-      const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-      const float4 a = q[0], b = q[1];
-      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
-      const uint32_t s[4] = {u.x, u.y, u.z, u.w};
+    r.a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+  }
+  return r;
+}
+GPA_DEV void unraw(const Raw8& r, int dt, float (&v)[8]) {
+  const uint32_t s[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+  if (dt == kF32) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float2 f;
-        if (dt == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&s[k]));
-        else f = __half22float2(*reinterpret_cast<const __half2*>(&s[k]));
-        v[2 * k] = f.x, v[2 * k + 1] = f.y;
-      }
+    for (int k = 0; k < 8; ++k) v[k] = __uint_as_float(s[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float2 f;
+      if (dt == kBF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&s[k]));
+      else f = __half22float2(*reinterpret_cast<const __half2*>(&s[k]));
+      v[2 * k] = f.x, v[2 * k + 1] = f.y;
     }
   }
+}
+
+template <int VEC>
+GPA_DEV void ldv(const void* p, int64_t i, int dt, float (&v)[VEC]) {
+  if constexpr (VEC == 1) v[0] = load_in(p, i, dt);
+  else unraw(ldraw(p, i, dt), dt, v);
 }
 
 template <int VEC>
@@ -222,6 +238,35 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
   }
 }
 
+// Column sums of a block's rows into its partial row: registers of one group, or of the block's
+// groups added through shared memory.
+template <int G, int VEC, int ITER>
+GPA_DEV void emit_sums(float* dst, const float (&a)[ITER][VEC], int width, int g, int t, uint32_t mine,
+                       uint32_t per, float* fold) {
+  if constexpr (G == 0) {
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const int c = (i * g + t) * VEC + k;
+        if (c < width) dst[c] = a[i][k];
+      }
+  } else {
+    constexpr int kCols = G * VEC * ITER;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITER; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) fold[mine * kCols + (i * G + t) * VEC + k] = a[i][k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < width; c += blockDim.x) {
+      float s = 0.f;
+      for (uint32_t j = 0; j < per; ++j) s += fold[j * kCols + c];
+      dst[c] = s;
+    }
+  }
+}
+
 template <int G, int VEC, int ITER, int MT>
 __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
   const Fwd& p = b.f;
@@ -342,51 +387,126 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
   }
   float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
   auto emit = [&](int slot, const float (&a)[ITER][VEC]) {
-    if (slot < 0) return;
-    float* dst = part + (int64_t)slot * p.width;
-    if constexpr (G == 0) {
-#pragma unroll
-      for (int i = 0; i < ITER; ++i)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const int c = (i * g + t) * VEC + k;
-          if (c < p.width) dst[c] = a[i][k];
-        }
-    } else {
-      constexpr int kCols = G * VEC * ITER;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < ITER; ++i)
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) fold[mine * kCols + (i * G + t) * VEC + k] = a[i][k];
-      __syncthreads();
-      for (int c = threadIdx.x; c < p.width; c += blockDim.x) {
-        float s = 0.f;
-        for (uint32_t j = 0; j < per; ++j) s += fold[j * kCols + c];
-        dst[c] = s;
-      }
-    }
+    if (slot >= 0) emit_sums<G, VEC, ITER>(part + (int64_t)slot * p.width, a, p.width, g, t, mine, per, fold);
   };
   emit(b.sum_w, aw);
   emit(b.sum_p, ap);
   emit(b.sum_c, ac);
 }
 
-// out[c] = sum over blocks of part[block][c], always in the same order: 8 lanes for 32 columns,
-// each adding every eighth block, then the lanes one after another.
-__global__ void k_norm_fold(const float* part, int blocks, int64_t pitch, int cols, float* out) {
-  __shared__ float sm[8][33];
+// The plain norm over narrow rows: each group takes kNarrow rows at once, all their loads in
+// flight together.
+constexpr int kNarrow = 4;
+template <int G>
+__global__ void __launch_bounds__(128) k_norm_narrow(const Fwd p) {
+  const int t = threadIdx.x % G, c = t * 8;
+  const uint32_t row0 = (blockIdx.x * (128 / G) + threadIdx.x / G) * kNarrow;
+  Raw8 raw[kNarrow];
+#pragma unroll
+  for (int u = 0; u < kNarrow; ++u) {
+    raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
+    if (row0 + u < p.rows && c < p.width) raw[u] = ldraw(p.y, row_at(p.ry, row0 + u, p.inner) + c, p.y_dt);
+  }
+  float w[8] = {};
+  if (c < p.width) ldv<8>(p.w, c, kF32, w);
+  const float inv = 1.f / (float)p.width;
+#pragma unroll
+  for (int u = 0; u < kNarrow; ++u) {
+    float x[8], s = 0.f;
+    unraw(raw[u], p.y_dt, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += x[k] * x[k];
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    const float r = rsqrtf(s * inv + p.eps);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] *= r * w[k];
+    if (row0 + u < p.rows && c < p.width) stv<8>(p.out, (int64_t)(row0 + u) * p.width + c, p.out_dt, x);
+  }
+}
+
+// Backward where the update's share is the update times a constant (or the plain norm): no more
+// than the stream and the two gradients are read.  A block's next row is loaded while the
+// current one is reduced and written.
+template <int G, int MT>
+__global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
+  const Fwd& p = b.f;
+  __shared__ float sm[2][3][32];
+  extern __shared__ float fold[];
+  int buf = 0;
+  const int g = G == 0 ? (int)blockDim.x : G;
+  const int t = G == 0 ? (int)threadIdx.x : (int)(threadIdx.x % G);
+  const uint32_t per = G == 0 ? 1u : blockDim.x / G;
+  const uint32_t mine = G == 0 ? 0u : threadIdx.x / G;
+  const bool plain = p.h_dt < 0;
+  const int x_dt = plain ? p.y_dt : p.h_dt;
+  const int c = t * 8;
+  const bool in = c < p.width;
+  const float inv = 1.f / (float)p.width;
+  float w[8] = {}, aw[1][8] = {};
+  if (in) ldv<8>(p.w, c, kF32, w);
+  const uint32_t step = gridDim.x * per;
+  Raw8 rx, rd, rs;
+  auto load = [&](uint32_t row) {
+    rx.a = rx.b = rd.a = rd.b = rs.a = rs.b = make_uint4(0, 0, 0, 0);
+    if (row >= p.rows || !in) return;
+    const int64_t at = (int64_t)row * p.width + c;
+    rx = plain ? ldraw(p.y, row_at(p.ry, row, p.inner) + c, x_dt) : ldraw(p.stream, at, x_dt);
+    if (b.dn) rd = ldraw(b.dn, at, p.out_dt);
+    if (b.ds) rs = ldraw(b.ds, at, p.h_dt);
+  };
+  load(blockIdx.x * per + mine);
+  for (uint32_t base = blockIdx.x * per; base < p.rows; base += step) {
+    const uint32_t row = base + mine;
+    float x[8], d[8], e[8];
+    unraw(rx, x_dt, x);
+    unraw(rd, p.out_dt, d);
+    if (b.ds) unraw(rs, p.h_dt, e);
+    load(row + step < row ? 0xffffffffu : row + step);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      s[0] += x[k] * x[k];
+      s[1] += w[k] * d[k] * x[k];
+    }
+    group_sum<G, 2>(s, sm, buf);
+    const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
+    if (row >= p.rows || !in) continue;
+    const int64_t at = (int64_t)row * p.width + c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      aw[0][k] += d[k] * x[k] * r;
+      d[k] = r * (w[k] * d[k] - x[k] * q);
+      if (b.ds) d[k] += e[k];
+    }
+    if (b.dh) stv<8>(b.dh, at, p.h_dt, d);
+    if (b.dy) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] *= p.c;
+      stv<8>(b.dy, at, p.y_dt, d);
+    }
+  }
+  if (b.sum_w >= 0) emit_sums<G, 8, 1>(b.part + (int64_t)blockIdx.x * p.width, aw, p.width, g, t, mine, per, fold);
+}
+
+// out[k][c] = sum over blocks of part[block][k][c] (k: blockIdx.y), always in the same order: 32
+// lanes for 32 columns, each adding every 32nd block, then the lanes in a tree.
+struct Sums {
+  float* out[3];
+};
+__global__ void __launch_bounds__(1024) k_norm_fold(const float* part, int blocks, int sums, int cols, Sums out) {
+  __shared__ float sm[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
+  const int64_t pitch = (int64_t)sums * cols;
+  const float* p = part + (int64_t)blockIdx.y * cols + c;
   float s = 0.f;
   if (c < cols)
-    for (int b = threadIdx.y; b < blocks; b += 8) s += part[b * pitch + c];
+    for (int b = threadIdx.y; b < blocks; b += 32) s += p[b * pitch];
   sm[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
-  if (threadIdx.y == 0 && c < cols) {
-#pragma unroll
-    for (int j = 1; j < 8; ++j) s += sm[j][threadIdx.x];
-    out[c] = s;
-  }
+  s = warp_sum(sm[threadIdx.x][threadIdx.y]);  // column blockIdx.x * 32 + threadIdx.y
+  const int mine = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && mine < cols) out.out[blockIdx.y][mine] = s;
 }
 
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -409,8 +529,9 @@ Shape shape_of(const Fwd& f, bool vec) {
     s.iter = 1;
     s.threads = 128;
   } else {
+    // single channels: four a thread, so that a block is not all barrier
     s.group = 0;
-    s.iter = 1;
+    s.iter = vec ? 1 : 4;
     while ((n + s.iter - 1) / s.iter > 1024) s.iter *= 2;
     s.threads = ((n + s.iter - 1) / s.iter + 31) / 32 * 32;
   }
@@ -430,6 +551,7 @@ constexpr int kMaxWidth = 16384;
       else if ((S).group == 16) { CALL(16, 8, 1, 128); }            \
       else if ((S).group == 32) { CALL(32, 8, 1, 128); }            \
       else if ((S).iter == 1 && (S).threads <= 256) { CALL(0, 8, 1, 256); } \
+      else if ((S).iter == 1 && (S).threads <= 512) { CALL(0, 8, 1, 512); } \
       else if ((S).iter == 1) { CALL(0, 8, 1, 1024); }              \
       else { CALL(0, 8, 2, 1024); }                                 \
     } else {                                                        \
@@ -437,8 +559,7 @@ constexpr int kMaxWidth = 16384;
       else if ((S).group == 8) { CALL(8, 1, 1, 128); }              \
       else if ((S).group == 16) { CALL(16, 1, 1, 128); }            \
       else if ((S).group == 32) { CALL(32, 1, 1, 128); }            \
-      else if ((S).iter == 1) { CALL(0, 1, 1, 1024); }              \
-      else if ((S).iter == 2) { CALL(0, 1, 2, 1024); }              \
+      else if ((S).iter == 4 && (S).threads <= 256) { CALL(0, 1, 4, 256); } \
       else if ((S).iter == 4) { CALL(0, 1, 4, 1024); }              \
       else if ((S).iter == 8) { CALL(0, 1, 8, 1024); }              \
       else { CALL(0, 1, 16, 1024); }                                \
@@ -493,13 +614,16 @@ bool vec_ok(const Fwd& f) {
          (!f.gate_full || (aligned8(f.gate) && strides8(f.rg)));
 }
 
-// Blocks of the backward: a few per SM, each with many rows, so that its column sums are added
-// in registers and few partial rows are left.
-int bwd_blocks(const Shape& s, uint32_t rows) {
+// Blocks of the backward: as many as run at once, each with many rows, so that its column sums
+// are added in registers and few partial rows are left.  At most 8 blocks of 128 threads an SM.
+int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
+int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem) {
   const uint32_t per = s.group ? s.threads / s.group : 1;
+  int at_once = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kernel, s.threads, smem) != cudaSuccess || at_once < 1)
+    at_once = 1;
   const uint32_t need = (rows + per - 1) / per;
-  const uint32_t most = 148u * (s.threads <= 128 ? 8u : s.threads <= 256 ? 4u : s.threads <= 512 ? 2u : 1u);
-  return (int)std::max(1u, std::min(need, most));
+  return (int)std::max(1u, std::min(need, (uint32_t)std::min(148 * at_once, most_blocks(s))));
 }
 
 }  // namespace
@@ -519,9 +643,20 @@ int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStrea
   f.stream = stream_out;
   f.out = normed;
   const Shape s = shape_of(f, vec_ok(f));
-  const uint32_t per = s.group ? s.threads / s.group : 1;
-  const uint32_t grid = (f.rows + per - 1) / per;
+  uint32_t per = s.group ? s.threads / s.group : 1;
   Launch scope("norm_fwd", st);
+  if (!f.h && s.vec == 8 && s.group) {
+    per *= kNarrow;
+    const uint32_t grid = (f.rows + per - 1) / per;
+    if (s.group == 4) k_norm_narrow<4><<<grid, 128, 0, st>>>(f);
+    else if (s.group == 8) k_norm_narrow<8><<<grid, 128, 0, st>>>(f);
+    else if (s.group == 16) k_norm_narrow<16><<<grid, 128, 0, st>>>(f);
+    else k_norm_narrow<32><<<grid, 128, 0, st>>>(f);
+    if (cudaGetLastError() == cudaSuccess) return GPA_B200_OK;
+    *why = "norm_fwd launch failed";
+    return GPA_B200_LAUNCH_FAILURE;
+  }
+  const uint32_t grid = (f.rows + per - 1) / per;
 #define CALL(G, V, I, M) k_norm_fwd<G, V, I, M><<<grid, s.threads, 0, st>>>(f)
   NORM_DISPATCH(s, CALL);
 #undef CALL
@@ -531,10 +666,10 @@ int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStrea
 }
 
 namespace {
-// whichever variant runs, its partial rows fit: the larger grid of the two
+// whichever variant runs, its partial rows fit
 size_t partial_floats(const Fwd& f) {
-  const int b = std::max(bwd_blocks(shape_of(f, true), f.rows), bwd_blocks(shape_of(f, false), f.rows));
-  return (size_t)b * 3 * f.width;
+  const int b = std::max(most_blocks(shape_of(f, true)), most_blocks(shape_of(f, false)));
+  return (size_t)std::min<int64_t>(b, f.rows) * 3 * f.width;
 }
 }  // namespace
 
@@ -588,30 +723,46 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
   const bool vec = vec_ok(f) && aligned8(dnormed) && aligned8(dstream) && aligned8(g->dresidual) &&
                    aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate));
   const Shape s = shape_of(f, vec);
-  const int blocks = bwd_blocks(s, f.rows);
+  const size_t smem = s.group ? sizeof(float) * s.threads * s.vec * s.iter : 0;
+  const bool light = s.vec == 8 && s.iter == 1 && !f.wp && !f.scale && !f.gate;
+  int blocks = 0;
   {
     Launch scope("norm_bwd", st);
-    const size_t smem = s.group ? sizeof(float) * s.threads * s.vec * s.iter : 0;
-#define CALL(G, V, I, M) k_norm_bwd<G, V, I, M><<<blocks, s.threads, smem, st>>>(b)
-    NORM_DISPATCH(s, CALL);
+#define RUN(K)                                                                   \
+  do {                                                                           \
+    blocks = bwd_blocks(s, f.rows, reinterpret_cast<const void*>(&K), smem);     \
+    K<<<blocks, s.threads, smem, st>>>(b);                                       \
+  } while (0)
+#define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>))
+#define CALL(G, V, I, M) RUN((k_norm_bwd<G, V, I, M>))
+    if (light) {
+      if (s.group == 4) LIGHT(4, 128);
+      else if (s.group == 8) LIGHT(8, 128);
+      else if (s.group == 16) LIGHT(16, 128);
+      else if (s.group == 32) LIGHT(32, 128);
+      else if (s.threads <= 256) LIGHT(0, 256);
+      else if (s.threads <= 512) LIGHT(0, 512);
+      else LIGHT(0, 1024);
+    } else {
+      NORM_DISPATCH(s, CALL);
+    }
 #undef CALL
+#undef LIGHT
+#undef RUN
     if (cudaGetLastError() != cudaSuccess) {
       *why = "norm_bwd launch failed";
       return GPA_B200_LAUNCH_FAILURE;
     }
   }
   if (!b.sums) return GPA_B200_OK;
-  // the sums of all wanted weights lie next to one another in a partial row
-  for (int k = 0, slot = 0; k < 3; ++k) {
-    if (!out[k]) continue;
-    Launch scope("norm_fold", st);
-    k_norm_fold<<<(f.width + 31) / 32, dim3(32, 8), 0, st>>>(b.part + (int64_t)slot * f.width, blocks,
-                                                           (int64_t)b.sums * f.width, f.width, out[k]);
-    ++slot;
-    if (cudaGetLastError() != cudaSuccess) {
-      *why = "norm_fold launch failed";
-      return GPA_B200_LAUNCH_FAILURE;
-    }
+  Sums sums = {};
+  for (int k = 0, slot = 0; k < 3; ++k)
+    if (out[k]) sums.out[slot++] = out[k];
+  Launch scope("norm_fold", st);
+  k_norm_fold<<<dim3((f.width + 31) / 32, b.sums), dim3(32, 32), 0, st>>>(b.part, blocks, b.sums, f.width, sums);
+  if (cudaGetLastError() != cudaSuccess) {
+    *why = "norm_fold launch failed";
+    return GPA_B200_LAUNCH_FAILURE;
   }
   return GPA_B200_OK;
 }

@@ -31,7 +31,7 @@ def _on(device):
 
 def _call(fn, device, *args):
     """`fn(*args, stream)` on the current stream of `device`, which is current."""
-    rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     if rc:
         _lib.check(rc, fn.__name__)
 
