@@ -85,6 +85,20 @@ GPA_DEV void ldv(const void* p, int64_t i, int dt, float (&v)[VEC]) {
   else unraw(ldraw(p, i, dt), dt, v);
 }
 
+// a value or 8 of them on their way from memory
+template <int VEC>
+struct Held {
+  Raw8 r;
+  GPA_DEV void load(const void* p, int64_t i, int dt) { r = ldraw(p, i, dt); }
+  GPA_DEV void get(int dt, float (&v)[8]) const { unraw(r, dt, v); }
+};
+template <>
+struct Held<1> {
+  float r;
+  GPA_DEV void load(const void* p, int64_t i, int dt) { r = load_in(p, i, dt); }
+  GPA_DEV void get(int, float (&v)[1]) const { v[0] = r; }
+};
+
 template <int VEC>
 GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
   if constexpr (VEC == 1) {
@@ -110,6 +124,9 @@ GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
     }
   }
 }
+
+// 1 / (1 + e^-a) to a few units of 2^-22: exp2 and reciprocal units instead of the full functions
+GPA_DEV float gate_of(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 
 GPA_DEV float round_to(float x, int dt) {
   if (dt == kBF16) return __bfloat162float(__float2bfloat16(x));
@@ -152,8 +169,19 @@ GPA_DEV int64_t row_at(const Rows& r, uint32_t row, uint32_t inner) {
   return (int64_t)o * r.so + (int64_t)(row - o * inner) * r.si;
 }
 
-template <int G, int VEC, int ITER, int MT>
+// The types of a kernel's tensors: known where it is built (DT), or read from its arguments
+// (DT < 0).  Built in, a load and its conversions are half the instructions of a row.
+constexpr int kAny = -1;
+constexpr int types_of(int stream, int update, int out) { return stream | update << 2 | out << 4; }
+#define NORM_TYPES(DT)                                                   \
+  const int h_dt = (DT) < 0 ? p.h_dt : (DT) & 3;                         \
+  const int y_dt = (DT) < 0 ? p.y_dt : (DT) >> 2 & 3;                    \
+  const int g_dt = (DT) < 0 ? p.g_dt : y_dt;                             \
+  const int out_dt = (DT) < 0 ? p.out_dt : (DT) >> 4 & 3
+
+template <int G, int VEC, int ITER, int MT, int DT>
 __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
+  NORM_TYPES(DT);
   __shared__ float sm[2][3][32];
   int buf = 0;
   const int g = G == 0 ? (int)blockDim.x : G;
@@ -164,14 +192,24 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
   const bool plain = p.h == nullptr;
   const float inv = 1.f / (float)p.width;
   float x[ITER][VEC];
+  Held<VEC> held_h[ITER], held_g[ITER];  // every load of the row in flight before its first sum
   const int64_t oy = live ? row_at(p.ry, row, p.inner) : 0;
+  const int64_t oh = live && !plain ? row_at(p.rh, row, p.inner) : 0;
+  const int64_t og = live && p.gate ? row_at(p.rg, row, p.inner) : 0;
   float s1[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < ITER; ++i) {
+    const int c = (i * g + t) * VEC;
+    if (!live || c >= p.width) continue;
+    if (!plain) held_h[i].load(p.h, oh + c, h_dt);
+    if (p.gate && p.gate_full) held_g[i].load(p.gate, og + c, g_dt);
+  }
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int c = (i * g + t) * VEC;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) x[i][k] = 0.f;
-    if (live && c < p.width) ldv<VEC>(p.y, oy + c, p.y_dt, x[i]);
+    if (live && c < p.width) ldv<VEC>(p.y, oy + c, y_dt, x[i]);
   }
   const int64_t at = (int64_t)row * p.width;
   if (!plain) {
@@ -184,23 +222,21 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
       group_sum<G, 1>(s1, sm, buf);
       ry = rsqrtf(s1[0] * inv + p.eps);
     }
-    const int64_t oh = live ? row_at(p.rh, row, p.inner) : 0;
-    const int64_t og = live && p.gate ? row_at(p.rg, row, p.inner) : 0;
     float gr = p.c;
-    if (live && p.gate && !p.gate_full) gr *= sigmoid(load_in(p.gate, og, p.g_dt));
+    if (live && p.gate && !p.gate_full) gr *= gate_of(load_in(p.gate, og, g_dt));
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
       if (!live || c >= p.width) continue;
       float h[VEC], m[VEC];
-      ldv<VEC>(p.h, oh + c, p.h_dt, h);
+      held_h[i].get(h_dt, h);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) m[k] = gr;
       if (p.gate && p.gate_full) {
         float a[VEC];
-        ldv<VEC>(p.gate, og + c, p.g_dt, a);
+        held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m[k] *= sigmoid(a[k]);
+        for (int k = 0; k < VEC; ++k) m[k] *= gate_of(a[k]);
       }
       if (p.scale) {
         float a[VEC];
@@ -215,8 +251,8 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
         for (int k = 0; k < VEC; ++k) x[i][k] *= ry * a[k];
       }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[i][k] = round_to(fmaf(m[k], x[i][k], h[k]), p.h_dt);
-      stv<VEC>(p.stream, at + c, p.h_dt, x[i]);
+      for (int k = 0; k < VEC; ++k) x[i][k] = round_to(fmaf(m[k], x[i][k], h[k]), h_dt);
+      stv<VEC>(p.stream, at + c, h_dt, x[i]);
     }
   }
   float s2[1] = {0.f};
@@ -234,7 +270,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
     ldv<VEC>(p.w, c, kF32, w);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) w[k] *= x[i][k] * r;
-    stv<VEC>(p.out, at + c, p.out_dt, w);
+    stv<VEC>(p.out, at + c, out_dt, w);
   }
 }
 
@@ -267,9 +303,10 @@ GPA_DEV void emit_sums(float* dst, const float (&a)[ITER][VEC], int width, int g
   }
 }
 
-template <int G, int VEC, int ITER, int MT>
+template <int G, int VEC, int ITER, int MT, int DT>
 __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
   const Fwd& p = b.f;
+  NORM_TYPES(DT);
   __shared__ float sm[2][3][32];
   extern __shared__ float fold[];  // sub-warp groups: [blockDim / G][G * VEC * ITER]
   int buf = 0;
@@ -294,16 +331,24 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
     const bool use_y = !plain && p.y != nullptr;
     float x[ITER][VEC], d[ITER][VEC], y[ITER][VEC];
     float s[3] = {0.f, 0.f, 0.f};  // x^2, w dn x, y^2
+    Held<VEC> held_s[ITER], held_g[ITER];  // read after the sums, on their way before them
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+      const int c = (i * g + t) * VEC;
+      if (!live || c >= p.width) continue;
+      if (b.ds) held_s[i].load(b.ds, at + c, h_dt);
+      if (p.gate && p.gate_full) held_g[i].load(p.gate, og + c, g_dt);
+    }
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) x[i][k] = d[i][k] = y[i][k] = 0.f;
       if (!live || c >= p.width) continue;
-      if (plain) ldv<VEC>(p.y, oy + c, p.y_dt, x[i]);
-      else ldv<VEC>(p.stream, at + c, p.h_dt, x[i]);
-      if (b.dn) ldv<VEC>(b.dn, at + c, p.out_dt, d[i]);
-      if (use_y) ldv<VEC>(p.y, oy + c, p.y_dt, y[i]);
+      if (plain) ldv<VEC>(p.y, oy + c, y_dt, x[i]);
+      else ldv<VEC>(p.stream, at + c, h_dt, x[i]);
+      if (b.dn) ldv<VEC>(b.dn, at + c, out_dt, d[i]);
+      if (use_y) ldv<VEC>(p.y, oy + c, y_dt, y[i]);
       float w[VEC];
       ldv<VEC>(p.w, c, kF32, w);
 #pragma unroll
@@ -317,7 +362,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
     const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
     const float ry = p.wp ? rsqrtf(s[2] * inv + p.eps) : 1.f;
     float gr = 1.f;
-    if (live && p.gate && !p.gate_full) gr = sigmoid(load_in(p.gate, og, p.g_dt));
+    if (live && p.gate && !p.gate_full) gr = gate_of(load_in(p.gate, og, g_dt));
     float s2[2] = {0.f, 0.f};  // wp du y, row-gate gradient
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -331,15 +376,15 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
         d[i][k] = r * (w[k] * d[i][k] - x[i][k] * q);
       }
       if (b.ds) {
-        ldv<VEC>(b.ds, at + c, p.h_dt, a);
+        held_s[i].get(h_dt, a);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[i][k] += a[k];
       }
       if (plain) {
-        stv<VEC>(b.dy, at + c, p.y_dt, d[i]);
+        stv<VEC>(b.dy, at + c, y_dt, d[i]);
         continue;
       }
-      if (b.dh) stv<VEC>(b.dh, at + c, p.h_dt, d[i]);
+      if (b.dh) stv<VEC>(b.dh, at + c, h_dt, d[i]);
       float wp[VEC], cs[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) wp[k] = 1.f, cs[k] = p.c;
@@ -352,9 +397,9 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) a[k] = gr;
       if (p.gate && p.gate_full) {
-        ldv<VEC>(p.gate, og + c, p.g_dt, a);
+        held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a[k] = sigmoid(a[k]);
+        for (int k = 0; k < VEC; ++k) a[k] = gate_of(a[k]);
       }
       float dg[VEC];
 #pragma unroll
@@ -368,12 +413,12 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
         d[i][k] = du * wp[k];
         s2[0] += d[i][k] * y[i][k];
       }
-      if (p.gate && p.gate_full && b.dgate) stv<VEC>(b.dgate, at + c, p.g_dt, dg);
+      if (p.gate && p.gate_full && b.dgate) stv<VEC>(b.dgate, at + c, g_dt, dg);
     }
     if (plain) continue;
     const bool row_gate = p.gate && !p.gate_full && b.dgate;
     if (p.wp || row_gate) group_sum<G, 2>(s2, sm, buf);
-    if (row_gate && live && t == 0) store_out(b.dgate, row, s2[1], p.g_dt);
+    if (row_gate && live && t == 0) store_out(b.dgate, row, s2[1], g_dt);
     if (!b.dy) continue;
     const float qy = p.wp ? s2[0] * inv * ry * ry : 0.f;
 #pragma unroll
@@ -382,7 +427,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
       if (!live || c >= p.width) continue;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) d[i][k] = ry * (d[i][k] - y[i][k] * qy);
-      stv<VEC>(b.dy, at + c, p.y_dt, d[i]);
+      stv<VEC>(b.dy, at + c, y_dt, d[i]);
     }
   }
   float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
@@ -531,7 +576,8 @@ Shape shape_of(const Fwd& f, bool vec) {
   } else {
     // single channels: four a thread, so that a block is not all barrier
     s.group = 0;
-    s.iter = vec ? 1 : 4;
+    // and two turns of a smaller block where one of more than 512 threads would run out of registers
+    s.iter = vec ? (n > 512 ? 2 : 1) : 4;
     while ((n + s.iter - 1) / s.iter > 1024) s.iter *= 2;
     s.threads = ((n + s.iter - 1) / s.iter + 31) / 32 * 32;
   }
@@ -540,31 +586,44 @@ Shape shape_of(const Fwd& f, bool vec) {
 
 constexpr int kMaxWidth = 16384;
 
-}  // namespace
-
-// (group, vec, iter, most threads) of every shape that shape_of can return
-#define NORM_DISPATCH(S, CALL)                                      \
+// Runs CALL(group, vec, iter, most threads, types) for the shape: the types are built in for blocks
+// over aligned rows with the mixes that models train in, and read from the arguments elsewhere.
+// 640 threads at most leave 96 registers a thread, so that two blocks of 320 fit an SM.
+#define NORM_TYPED(DT, CALL, I, M)                                                            \
+  do {                                                                                        \
+    if ((DT) == types_of(kF32, kBF16, kBF16)) { CALL(0, 8, I, M, types_of(kF32, kBF16, kBF16)); } \
+    else if ((DT) == types_of(kBF16, kBF16, kBF16)) { CALL(0, 8, I, M, types_of(kBF16, kBF16, kBF16)); } \
+    else if ((DT) == types_of(kF32, kF32, kF32)) { CALL(0, 8, I, M, types_of(kF32, kF32, kF32)); } \
+    else { CALL(0, 8, I, M, kAny); }                                                          \
+  } while (0)
+#define NORM_DISPATCH(S, DT, CALL)                                  \
   do {                                                              \
     if ((S).vec == 8) {                                             \
-      if ((S).group == 4) { CALL(4, 8, 1, 128); }                   \
-      else if ((S).group == 8) { CALL(8, 8, 1, 128); }              \
-      else if ((S).group == 16) { CALL(16, 8, 1, 128); }            \
-      else if ((S).group == 32) { CALL(32, 8, 1, 128); }            \
-      else if ((S).iter == 1 && (S).threads <= 256) { CALL(0, 8, 1, 256); } \
-      else if ((S).iter == 1 && (S).threads <= 512) { CALL(0, 8, 1, 512); } \
-      else if ((S).iter == 1) { CALL(0, 8, 1, 1024); }              \
-      else { CALL(0, 8, 2, 1024); }                                 \
+      if ((S).group == 4) { CALL(4, 8, 1, 128, kAny); }             \
+      else if ((S).group == 8) { CALL(8, 8, 1, 128, kAny); }        \
+      else if ((S).group == 16) { CALL(16, 8, 1, 128, kAny); }      \
+      else if ((S).group == 32) { CALL(32, 8, 1, 128, kAny); }      \
+      else if ((S).iter == 1 && (S).threads <= 256) { NORM_TYPED(DT, CALL, 1, 256); } \
+      else if ((S).iter == 1) { NORM_TYPED(DT, CALL, 1, 640); }     \
+      else if ((S).threads <= 512) { CALL(0, 8, 2, 512, kAny); }    \
+      else { CALL(0, 8, 2, 1024, kAny); }                           \
     } else {                                                        \
-      if ((S).group == 4) { CALL(4, 1, 1, 128); }                   \
-      else if ((S).group == 8) { CALL(8, 1, 1, 128); }              \
-      else if ((S).group == 16) { CALL(16, 1, 1, 128); }            \
-      else if ((S).group == 32) { CALL(32, 1, 1, 128); }            \
-      else if ((S).iter == 4 && (S).threads <= 256) { CALL(0, 1, 4, 256); } \
-      else if ((S).iter == 4) { CALL(0, 1, 4, 1024); }              \
-      else if ((S).iter == 8) { CALL(0, 1, 8, 1024); }              \
-      else { CALL(0, 1, 16, 1024); }                                \
+      if ((S).group == 4) { CALL(4, 1, 1, 128, kAny); }             \
+      else if ((S).group == 8) { CALL(8, 1, 1, 128, kAny); }        \
+      else if ((S).group == 16) { CALL(16, 1, 1, 128, kAny); }      \
+      else if ((S).group == 32) { CALL(32, 1, 1, 128, kAny); }      \
+      else if ((S).iter == 4 && (S).threads <= 256) { CALL(0, 1, 4, 256, kAny); } \
+      else if ((S).iter == 4) { CALL(0, 1, 4, 1024, kAny); }        \
+      else if ((S).iter == 8) { CALL(0, 1, 8, 1024, kAny); }        \
+      else { CALL(0, 1, 16, 1024, kAny); }                          \
     }                                                               \
   } while (0)
+
+int built_types(const Fwd& f, int stream_dt) {
+  return f.gate && f.g_dt != f.y_dt ? kAny : types_of(stream_dt, f.y_dt, f.out_dt);
+}
+
+}  // namespace
 
 namespace {
 
@@ -657,8 +716,9 @@ int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStrea
     return GPA_B200_LAUNCH_FAILURE;
   }
   const uint32_t grid = (f.rows + per - 1) / per;
-#define CALL(G, V, I, M) k_norm_fwd<G, V, I, M><<<grid, s.threads, 0, st>>>(f)
-  NORM_DISPATCH(s, CALL);
+  const int types = f.h ? built_types(f, f.h_dt) : kAny;
+#define CALL(G, V, I, M, T) k_norm_fwd<G, V, I, M, T><<<grid, s.threads, 0, st>>>(f)
+  NORM_DISPATCH(s, types, CALL);
 #undef CALL
   if (cudaGetLastError() == cudaSuccess) return GPA_B200_OK;
   *why = "norm_fwd launch failed";
@@ -734,17 +794,17 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     K<<<blocks, s.threads, smem, st>>>(b);                                       \
   } while (0)
 #define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>))
-#define CALL(G, V, I, M) RUN((k_norm_bwd<G, V, I, M>))
+#define CALL(G, V, I, M, T) RUN((k_norm_bwd<G, V, I, M, T>))
+    const int types = plain ? kAny : built_types(f, f.h_dt);
     if (light) {
       if (s.group == 4) LIGHT(4, 128);
       else if (s.group == 8) LIGHT(8, 128);
       else if (s.group == 16) LIGHT(16, 128);
       else if (s.group == 32) LIGHT(32, 128);
       else if (s.threads <= 256) LIGHT(0, 256);
-      else if (s.threads <= 512) LIGHT(0, 512);
-      else LIGHT(0, 1024);
+      else LIGHT(0, 512);
     } else {
-      NORM_DISPATCH(s, CALL);
+      NORM_DISPATCH(s, types, CALL);
     }
 #undef CALL
 #undef LIGHT
