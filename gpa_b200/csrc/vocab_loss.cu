@@ -1,11 +1,10 @@
 // Softmax cross entropy of z = x W^T over a large vocabulary, in pieces of it, without keeping z:
 //   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_{i, y_i}
 //   P_iv = (exp(z_iv - lse_i) - [v = y_i]) r_i        dx = s P W        dW = s P^T x
-// with the upstream gradient of row i written as s r_i, |r_i| <= 1 (s carries the scalar of a
-// mean or sum, or the largest of a vector).
+// with the upstream gradient of row i written as s r_i (see Upstream).
 //
-// Rows without a label are dropped first: the labelled ones are packed (k_rows, k_gather), so
-// masked tokens cost nothing and whatever they hold (NaN included) reaches no product.
+// Rows without a label are dropped first: the labelled ones are packed (k_pack), so masked
+// tokens cost nothing and whatever they hold (NaN included) reaches no product.
 //   forward:  each tile of z leaves (max, sum of exp) per row, k_join puts the tiles together
 //   backward: the vocabulary goes by in pieces; z of a piece is formed again and turned into P
 //             (in the piece's buffer), then dx += P W over the piece and dW of the piece = P^T x.
@@ -21,164 +20,222 @@ namespace vloss {
 namespace {
 
 // ------------------------------------------------------------------ rows
-// Packs the labelled rows: row[j] = index of the j-th row with a label, label[j] its label (-1
-// outside the vocabulary).  One block; each thread owns a run of rows.
-__global__ void __launch_bounds__(1024) k_rows(const int64_t* labels, int n, int64_t ignore,
-                                               int64_t vocab, int* row, int* label, int* n_rows,
-                                               float* loss_each) {
-  __shared__ int sums[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int run = (n + 1023) / 1024;
-  const int64_t b = (int64_t)threadIdx.x * run;
-  const int begin = (int)(b < n ? b : n), end = begin + (run < n - begin ? run : n - begin);
-  int mine = 0;
-  for (int i = begin; i < end; ++i) mine += labels[i] != ignore;
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    int s = sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += v;
-    }
-    sums[lane] = s;
-  }
-  __syncthreads();
-  int at = incl - mine + (warp ? sums[warp - 1] : 0);
-  for (int i = begin; i < end; ++i) {
-    const int64_t y = labels[i];
-    if (y != ignore) {
-      row[at] = i;
-      label[at++] = y >= 0 && y < vocab ? (int)y : -1;
-    } else if (loss_each) {
-      loss_each[i] = 0.f;
-    }
-  }
-  if (threadIdx.x == 0) *n_rows = sums[31];
+constexpr int kRun = 32;              // caller's rows per block of k_pack
+constexpr int kCountDirectly = 4096;  // up to here each block counts the labels before its own
+
+__global__ void k_count(const int64_t* labels, int n, int64_t ignore, int* count) {
+  const int i = blockIdx.x * kRun + threadIdx.x;
+  const unsigned b = __ballot_sync(0xffffffffu, i < n && labels[i] != ignore);
+  if (threadIdx.x == 0) count[blockIdx.x] = __popc(b);
 }
 
-// Packed copy of the labelled rows (row == NULL: of all rows), zero in the padding channels and
-// behind the last row up to the end of its tile.
+struct Pack {
+  const int64_t* labels;
+  int n;
+  int64_t ignore, vocab;
+  const int* count;        // labelled rows of each run before, or NULL: counted here
+  int runs;
+  int *info, *row, *label, *pos;  // info: [packed rows, counter of k_join]
+  int64_t so, si, inner;   // the caller's rows
+  int width, pitch;
+  bool vec;
+};
+
+// Packs the labelled rows: row[j], label[j] (-1 outside the vocabulary) and the channels of the
+// j-th of them, pos[i] its place or -1.  A block takes kRun rows; two more fill the places behind
+// the last row with zeros up to a multiple of 64, the reduction block of dW.  Four blocks share a
+// run's copies (blockIdx.y), a row for each of their warps.  In n <= 4096 rows
+// one launch is cheaper than k_count before it (a block reads 32 KB of labels at most); beyond,
+// the labels before a block are counted once.
 template <typename T>
-__global__ void k_gather(const T* src, int64_t so, int64_t si, int64_t inner, const int* row,
-                         const int* n_rows, int64_t n, int width, int pitch, T* dst, bool vec) {
+__global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, T* dst) {
   constexpr int kV = 16 / sizeof(T);
-  const int64_t j = blockIdx.x;
-  const int64_t rows = n_rows ? *n_rows : n;
-  if (j >= up(rows, kTile)) return;
-  T* d = dst + j * pitch;
-  if (j >= rows) {
-    for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = T(0.f);
+  __shared__ int part[8];
+  __shared__ int place[kRun];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int run = min((int)blockIdx.x, p.runs);
+  int before = 0;
+  if (p.count) {
+    for (int i = threadIdx.x; i < run; i += 256) before += p.count[i];
+  } else {
+    const int stop = min(run * kRun, p.n);
+    for (int i = threadIdx.x; i < stop; i += 256) before += p.labels[i] != p.ignore;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) part[warp] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) before += part[k];
+  if ((int)blockIdx.x >= p.runs) {  // `before` is the number of packed rows
+    const int extra = blockIdx.x - p.runs;
+    if (extra == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.info[0] = before, p.info[1] = 0;
+    const int end = (before + 63) / 64 * 64;
+    for (int j = before + extra * kRun + blockIdx.y; j < min(end, before + (extra + 1) * kRun); j += 4)
+      for (int c = threadIdx.x; c < p.pitch; c += 256) dst[(int64_t)j * p.pitch + c] = T(0.f);
     return;
   }
-  const int64_t i = row ? row[j] : j;
-  const T* s = src + (i / inner) * so + (i % inner) * si;
-  if (vec) {
-    for (int c = threadIdx.x * kV; c < width; c += blockDim.x * kV)
+  if (warp == 0) {
+    const int i = blockIdx.x * kRun + lane;
+    const int64_t y = i < p.n ? p.labels[i] : p.ignore;
+    const bool has = i < p.n && y != p.ignore;
+    const unsigned b = __ballot_sync(0xffffffffu, has);
+    const int at = before + __popc(b & ((1u << lane) - 1));
+    place[lane] = has ? at : -1;
+    if (has && blockIdx.y == 0) {
+      p.row[at] = i;
+      p.label[at] = y >= 0 && y < p.vocab ? (int)y : -1;
+    }
+    if (i < p.n && blockIdx.y == 0) p.pos[i] = has ? at : -1;
+  }
+  __syncthreads();
+  const int k = blockIdx.y * 8 + warp;
+  if (place[k] < 0) return;
+  const int64_t i = (int64_t)blockIdx.x * kRun + k;
+  const T* s = src + (i / p.inner) * p.so + (i % p.inner) * p.si;
+  T* d = dst + (int64_t)place[k] * p.pitch;
+  if (p.vec) {
+#pragma unroll 4
+    for (int c = lane * kV; c < p.width; c += 32 * kV)
       *reinterpret_cast<uint4*>(d + c) = *reinterpret_cast<const uint4*>(s + c);
   } else {
-    for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = c < width ? s[c] : T(0.f);
+    for (int c = lane; c < p.pitch; c += 32) d[c] = c < p.width ? s[c] : T(0.f);
   }
+}
+
+// Weight rows that cannot be read 16 bytes at a time: a copy with padded rows.
+template <typename T>
+__global__ void k_pad(const T* src, int64_t stride, int width, int pitch, T* dst) {
+  const T* s = src + blockIdx.x * stride;
+  T* d = dst + (int64_t)blockIdx.x * pitch;
+  for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = c < width ? s[c] : T(0.f);
 }
 
 // ------------------------------------------------------------------ joins
-// lse and loss of each packed row from the (max, sum) pairs of its tiles: 32 rows a block, 8
-// lanes of tiles.
-__global__ void k_join(const float2* part, int tiles, int64_t n_pad, const int* n_rows, const int* row,
-                       const int* label, const float* z_label, float* lse, float* loss_each,
-                       float* loss_packed) {
-  __shared__ float sm[8][33], ss[8][33];
-  const int64_t j = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  const bool live = j < *n_rows;
+GPA_DEV void merge(float& m, float& s, float m2, float s2) {
+  const float big = fmaxf(m, m2), safe = big == -INFINITY ? 0.f : big;
+  s = s * expf(m - safe) + s2 * expf(m2 - safe);
+  m = big;
+}
+
+// lse and loss of each packed row from the (max, sum) pairs of its tiles: blockDim.x rows a block,
+// blockDim.y lanes of tiles each (256 threads).  The block that finishes last adds the losses of
+// a mean or sum in double, in a fixed order.
+__global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, int tiles, const float* z_label,
+                                              float* lse, float* each, const int* pos, float* packed,
+                                              float* total, bool mean, int* counter) {
+  __shared__ float2 sm[256];
+  __shared__ bool last;
+  const int rows = *c.n_rows, lanes = blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
+  const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const bool live = j < rows;
   float m = -INFINITY, s = 0.f;
   if (live) {
-    for (int t = threadIdx.y; t < tiles; t += 8) {
-      const float2 p = part[t * n_pad + j];
-      const float big = fmaxf(m, p.x), safe = big == -INFINITY ? 0.f : big;
-      s = s * expf(m - safe) + p.y * expf(p.x - safe);
-      m = big;
+    int t = threadIdx.y;
+    for (; t + 3 * lanes < tiles; t += 4 * lanes) {
+      float2 p[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) p[k] = part[(t + k * lanes) * c.n_pad + j];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) merge(m, s, p[k].x, p[k].y);
+    }
+    for (; t < tiles; t += lanes) {
+      const float2 p = part[t * c.n_pad + j];
+      merge(m, s, p.x, p.y);
     }
   }
-  sm[threadIdx.y][threadIdx.x] = m;
-  ss[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y || !live) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) {
-    const float m2 = sm[k][threadIdx.x], s2 = ss[k][threadIdx.x];
-    const float big = fmaxf(m, m2), safe = big == -INFINITY ? 0.f : big;
-    s = s * expf(m - safe) + s2 * expf(m2 - safe);
-    m = big;
-  }
-  const float log_s = logf(s);
-  lse[j] = m + log_s;
-  const float l = label[j] < 0 ? NAN : (m - z_label[j]) + log_s;
-  if (loss_each) loss_each[row[j]] = l;
-  if (loss_packed) loss_packed[j] = l;
-}
-
-// mean / sum of the packed losses, added in double by one block in a fixed order
-__global__ void __launch_bounds__(1024) k_total(const float* loss, const int* n_rows, bool mean, float* out) {
-  __shared__ double sm[32];
-  const int n = *n_rows;
-  double s = 0.;
-  for (int i = threadIdx.x; i < n; i += 1024) s += (double)loss[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    s = sm[threadIdx.x];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) *out = (float)(mean ? s / (double)(n > 0 ? n : 1) : s);
-  }
-}
-
-// Row factors of the gradient: s in *scale, r_i per packed row (see the file comment).  A label
-// outside the vocabulary makes its row NaN.
-__global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, int reduction, const int* n_rows,
-                                                    const int* row, const int* label, float* r,
-                                                    float* scale) {
-  __shared__ float sm[32];
-  const int n = *n_rows;
-  float s = 1.f;
-  if (reduction == GPA_B200_LOSS_NONE) {
-    float big = 0.f;
-    for (int j = threadIdx.x; j < n; j += 1024) big = fmaxf(big, fabsf(dloss[row[j]]));
-    big = warp_max(big);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = big;
+  sm[tid] = make_float2(m, s);
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
     __syncthreads();
-    big = warp_max(sm[threadIdx.x & 31]);
-    s = big > 0.f && big < INFINITY ? big : 1.f;
+    if (threadIdx.y < o) {
+      const float2 p = sm[tid + o * blockDim.x];
+      merge(m, s, p.x, p.y);
+      sm[tid] = make_float2(m, s);
+    }
   }
-  for (int j = threadIdx.x; j < n; j += 1024)
-    r[j] = label[j] < 0 ? NAN : reduction == GPA_B200_LOSS_NONE ? dloss[row[j]] / s : 1.f;
-  if (threadIdx.x == 0)
-    *scale = reduction == GPA_B200_LOSS_NONE ? s
-             : reduction == GPA_B200_LOSS_MEAN ? *dloss / (float)(n > 0 ? n : 1) : *dloss;
+  if (threadIdx.y == 0 && live) {
+    const float log_s = logf(s);
+    lse[j] = m + log_s;
+    const float l = c.label[j] < 0 ? NAN : (m - z_label[j]) + log_s;
+    if (each) each[c.row[j]] = l;
+    else packed[j] = l;
+  }
+  if (each) {  // rows without a label, by the caller's numbering
+    if (threadIdx.y == 0 && j < c.n && pos[j] < 0) each[j] = 0.f;
+    return;
+  }
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(counter, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  __shared__ double sums[8];
+  double v = 0.;
+  for (int i = tid; i < rows; i += 256) v += (double)__ldcg(packed + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((tid & 31) == 0) sums[tid >> 5] = v;
+  __syncthreads();
+  if (tid == 0) {
+    for (int k = 1; k < 8; ++k) v += sums[k];
+    *total = (float)(mean ? v / (double)(rows > 0 ? rows : 1) : v);
+    *counter = 0;
+  }
 }
 
-// dx of the caller's rows: the parts added in order, scaled, rounded and put back in place.
-template <typename T>
-__global__ void k_finish(const float* part, int parts, int64_t part_stride, int pitch, const int* n_rows,
-                         const int* row, const float* scale, float unit, int width, T* dx) {
-  const int64_t j = blockIdx.x;
-  if (j >= *n_rows) return;
-  const float s = *scale * unit;
-  T* out = dx + (int64_t)row[j] * width;
-  const float* p = part + j * pitch;
-  for (int c = threadIdx.x; c < width; c += blockDim.x) {
-    float v = p[c];
-    for (int k = 1; k < parts; ++k) v += p[k * part_stride + c];
-    out[c] = T(v * s);
+// fp16, a gradient for each row: s = the largest magnitude, r = its share (fp16's range would lose
+// the products otherwise).
+__global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Call c, float* r, float* scale) {
+  __shared__ float sm[32];
+  const int n = *c.n_rows;
+  float big = 0.f;
+  for (int j = threadIdx.x; j < n; j += 1024) big = fmaxf(big, fabsf(dloss[c.row[j]]));
+  big = warp_max(big);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = big;
+  __syncthreads();
+  big = warp_max(sm[threadIdx.x & 31]);
+  const float s = big > 0.f && big < INFINITY ? big : 1.f;
+  for (int j = threadIdx.x; j < n; j += 1024) r[j] = dloss[c.row[j]] / s;
+  if (threadIdx.x == 0) *scale = s;
+}
+
+// dx of the caller's rows: the parts added in order, scaled, rounded; zero for rows without a
+// label.  kV channels a thread at a time.
+template <typename T, int kV>
+__global__ void k_finish(const float* part, int parts, int64_t part_stride, const Call c, const int* pos,
+                         const Upstream up, float unit, T* dx) {
+  const int64_t i = blockIdx.x;
+  const int j = pos[i];
+  const float s = up.scale(*c.n_rows) * unit;
+  T* out = dx + i * c.width;
+  const float* p = part + (int64_t)j * c.pitch;
+  for (int k = threadIdx.x * kV; k < c.width; k += blockDim.x * kV) {
+    float v[kV];
+    T o[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) v[e] = 0.f;
+    if (j >= 0) {
+      for (int q = 0; q < parts; ++q) {
+        if constexpr (kV > 1) {  // rows of the parts start on 16 bytes
+#pragma unroll
+          for (int e = 0; e < kV; e += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(p + q * part_stride + k + e);
+            v[e] += f.x, v[e + 1] += f.y, v[e + 2] += f.z, v[e + 3] += f.w;
+          }
+        } else {
+          v[0] += p[q * part_stride + k];
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kV; ++e) o[e] = T(j >= 0 ? v[e] * s : 0.f);
+    if constexpr (kV > 1) {
+      *reinterpret_cast<uint4*>(out + k) = *reinterpret_cast<const uint4*>(o);
+    } else {
+      out[k] = o[0];
+    }
   }
 }
 
@@ -298,9 +355,9 @@ __global__ void __launch_bounds__(256, 2) k_stats(const Call c, float2* part, fl
 }
 
 __global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int64_t vn, const float* lse,
-                                                  const float* r, float* p, int64_t p_pitch) {
+                                                  const Upstream up, float* p, int64_t p_pitch) {
   const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  if (m0 >= up(*c.n_rows, kTile)) return;
+  if (m0 >= *c.n_rows) return;
   float acc[8][8];
   product<true, true>({static_cast<const float*>(c.x), c.pitch, c.n_pad, c.pitch},
                             {static_cast<const float*>(c.w) + v0 * c.w_pitch, c.w_pitch, vn, c.pitch}, m0, n0, 0,
@@ -310,7 +367,7 @@ __global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int6
   for (int i = 0; i < 8; ++i) {
     const int64_t m = m0 + at8(ty, i);
     const bool live = m < *c.n_rows;
-    const float l = live ? lse[m] : 0.f, ri = live ? r[m] : 0.f;
+    const float l = live ? lse[m] : 0.f, ri = live ? up.r(c, m) : 0.f;
     const int64_t y = live ? c.label[m] - v0 : -1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -346,14 +403,14 @@ __global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int
 }
 
 __global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int64_t p_pitch, int64_t v0,
-                                               int64_t vn, const float* scale, float* dw) {
+                                               int64_t vn, const Upstream up, float* dw) {
   const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  const int64_t rows = up(*c.n_rows, kTile);
+  const int64_t rows = *c.n_rows;
   float acc[8][8];
   product<false, false>({p, p_pitch, p_pitch, rows}, {static_cast<const float*>(c.x), c.pitch, c.pitch, rows},
                                   m0, n0, 0, rows, acc);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const float s = *scale;
+  const float s = up.scale(*c.n_rows);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t v = m0 + at8(ty, i);
@@ -380,9 +437,9 @@ struct Plan {
   int parts;               // parts of dx
   int64_t k_part;          // vocabulary entries of a part
   // saved
-  int64_t s_rows, s_label, s_lse, s_bytes;
+  int64_t s_row, s_label, s_pos, s_lse, s_x, s_bytes;
   // scratch
-  int64_t x, w, part, z_label, loss, fwd_bytes;
+  int64_t w, count, part, z_label, loss, fwd_bytes;
   int64_t p, dxp, r, scale, bwd_bytes;
 };
 
@@ -445,15 +502,17 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
     at += up(bytes, 256);
     return here;
   };
-  take(256);  // n_rows
-  p->s_rows = take(4 * c.n);
+  take(256);  // packed rows, counter
+  p->s_row = take(4 * c.n);
   p->s_label = take(4 * c.n);
+  p->s_pos = take(4 * c.n);
   p->s_lse = take(4 * c.n);
+  p->s_x = take(c.n_pad * c.pitch * p->es);
   p->s_bytes = at;
   at = 0;
-  p->x = take(c.n_pad * c.pitch * p->es);
   p->w = take(p->copy_w ? c.vocab * c.pitch * p->es : 0);
   const int64_t common = at;
+  p->count = take(4 * up(c.n, kRun) / kRun);
   p->part = take((int64_t)p->tiles_v * c.n_pad * 8);
   p->z_label = take(4 * c.n);
   p->loss = take(4 * c.n);
@@ -468,31 +527,63 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
 }
 
 template <typename T>
-cudaError_t gather(const GpaLossArgs* a, const Plan& p, const int* row, char* scratch, cudaStream_t st) {
+void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaStream_t st) {
   const Call& c = p.c;
   constexpr int kV = 16 / sizeof(T);
-  {
-    const bool vec = a->width % kV == 0 && a->hidden_stride[0] % kV == 0 && a->hidden_stride[1] % kV == 0 &&
-                     (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
-    Launch scope("loss_gather", st);
-    k_gather<T><<<(unsigned)c.n_pad, 128, 0, st>>>(
-        static_cast<const T*>(a->hidden), a->hidden_stride[0], a->hidden_stride[1], a->inner, row, c.n_rows, c.n,
-        c.width, c.pitch, reinterpret_cast<T*>(scratch + p.x), vec);
+  Pack k;
+  k.labels = a->labels;
+  k.n = (int)c.n;
+  k.ignore = a->ignore_index;
+  k.vocab = c.vocab;
+  k.count = nullptr;
+  k.runs = (int)(up(c.n, kRun) / kRun);
+  k.info = reinterpret_cast<int*>(saved);
+  k.row = reinterpret_cast<int*>(saved + p.s_row);
+  k.label = reinterpret_cast<int*>(saved + p.s_label);
+  k.pos = reinterpret_cast<int*>(saved + p.s_pos);
+  k.so = a->hidden_stride[0];
+  k.si = a->hidden_stride[1];
+  k.inner = std::max<int64_t>(a->inner, 1);
+  k.width = c.width;
+  k.pitch = c.pitch;
+  k.vec = a->width % kV == 0 && k.so % kV == 0 && k.si % kV == 0 &&
+          (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
+  if (c.n > kCountDirectly) {
+    int* count = reinterpret_cast<int*>(scratch + p.count);
+    k.count = count;
+    Launch scope("loss_count", st);
+    k_count<<<k.runs, kRun, 0, st>>>(a->labels, k.n, k.ignore, count);
   }
-  if (p.copy_w) {
-    Launch scope("loss_gather", st);
-    k_gather<T><<<(unsigned)c.vocab, 128, 0, st>>>(static_cast<const T*>(a->weight), 0, a->weight_stride, c.vocab,
-                                                   nullptr, nullptr, c.vocab, c.width, c.pitch,
-                                                   reinterpret_cast<T*>(scratch + p.w), false);
-  }
-  return cudaGetLastError();
+  Launch scope("loss_pack", st);
+  k_pack<T><<<dim3(k.runs + 2, 4), 256, 0, st>>>(k, static_cast<const T*>(a->hidden), reinterpret_cast<T*>(saved + p.s_x));
+}
+
+template <typename T>
+void pad_weight(const GpaLossArgs* a, const Plan& p, char* scratch, cudaStream_t st) {
+  Launch scope("loss_pad", st);
+  k_pad<T><<<(unsigned)p.c.vocab, 128, 0, st>>>(static_cast<const T*>(a->weight), a->weight_stride, p.c.width,
+                                                p.c.pitch, reinterpret_cast<T*>(scratch + p.w));
+}
+
+template <typename T>
+void finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, const Upstream& up, void* dx,
+            cudaStream_t st) {
+  constexpr int kV = 16 / sizeof(T);
+  const Call& c = p.c;
+  const float unit = 1.f / (p.tc ? tc_p_scale(c.dtype) : 1.f);
+  Launch scope("loss_finish", st);
+  if (c.width % kV == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0)
+    k_finish<T, kV><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, stride, c, pos, up, unit, static_cast<T*>(dx));
+  else
+    k_finish<T, 1><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, stride, c, pos, up, unit, static_cast<T*>(dx));
 }
 
 void bind(Plan* p, const void* saved, char* scratch) {
   const char* s = static_cast<const char*>(saved);
   p->c.n_rows = reinterpret_cast<const int*>(s);
+  p->c.row = reinterpret_cast<const int*>(s + p->s_row);
   p->c.label = reinterpret_cast<const int*>(s + p->s_label);
-  p->c.x = scratch + p->x;
+  p->c.x = s + p->s_x;
   if (p->copy_w) p->c.w = scratch + p->w;
 }
 
@@ -548,39 +639,33 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
   char* sv = static_cast<char*>(saved);
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved, sc);
-  int* row = reinterpret_cast<int*>(sv + p.s_rows);
   float* each = none ? loss : nullptr;
-  float* packed = none ? nullptr : reinterpret_cast<float*>(sc + p.loss);
   float* z_label = reinterpret_cast<float*>(sc + p.z_label);
   float2* part = reinterpret_cast<float2*>(sc + p.part);
-  {
-    Launch scope("loss_rows", st);
-    k_rows<<<1, 1024, 0, st>>>(a->labels, (int)c.n, a->ignore_index, c.vocab, row,
-                               reinterpret_cast<int*>(sv + p.s_label), reinterpret_cast<int*>(sv), each);
-    OK_OR("loss_rows launch failed");
+  BY_TYPE(a->dtype, pack<T>(a, p, sv, sc, st));
+  OK_OR("loss_pack launch failed");
+  if (p.copy_w && c.n) {
+    BY_TYPE(a->dtype, pad_weight<T>(a, p, sc, st));
+    OK_OR("loss_pad launch failed");
   }
   if (c.n) {
-    BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
-    OK_OR("loss_gather launch failed");
-    {
-      if (p.tc) {
-        if (!tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
-      } else {
-        Launch scope("loss_stats", st);
-        k_stats<<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label);
-        OK_OR("loss_stats launch failed");
-      }
+    if (p.tc) {
+      if (!tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
+    } else {
+      Launch scope("loss_stats", st);
+      k_stats<<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label);
+      OK_OR("loss_stats launch failed");
     }
-    Launch scope("loss_join", st);
-    k_join<<<(unsigned)((c.n + 31) / 32), dim3(32, 8), 0, st>>>(part, p.tiles_v, c.n_pad, c.n_rows, row, c.label,
-                                                               z_label, reinterpret_cast<float*>(sv + p.s_lse),
-                                                               each, packed);
-    OK_OR("loss_join launch failed");
   }
-  if (!none) {
-    Launch scope("loss_total", st);
-    k_total<<<1, 1024, 0, st>>>(packed, c.n_rows, a->reduction == GPA_B200_LOSS_MEAN, loss);
-    OK_OR("loss_total launch failed");
+  if (c.n || !none) {
+    // few rows: more lanes for the tiles of each
+    const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;
+    Launch scope("loss_join", st);
+    k_join<<<(unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st>>>(
+        c, part, p.tiles_v, z_label, reinterpret_cast<float*>(sv + p.s_lse), each,
+        reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
+        a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1);
+    OK_OR("loss_join launch failed");
   }
   return GPA_B200_OK;
 }
@@ -592,17 +677,13 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   int code;
   if ((*why = plan_of(a, &p, &code))) return code;
   const Call& c = p.c;
-  if (!a->weight || !saved || !scratch || (c.n && (!a->hidden || !dloss)) || (!dhidden && !dweight)) {
+  if (!a->weight || !saved || !scratch || (c.n && !dloss) || (!dhidden && !dweight)) {
     *why = "a tensor is NULL";
     return GPA_B200_BAD_ARGUMENT;
   }
   if (saved_bytes < (size_t)p.s_bytes || scratch_bytes < (size_t)p.bwd_bytes) {
     *why = "saved or scratch is smaller than its size query";
     return GPA_B200_BAD_ARGUMENT;
-  }
-  if (dhidden && cudaMemsetAsync(dhidden, 0, (size_t)c.n * c.width * p.es, st) != cudaSuccess) {
-    *why = "clearing dhidden failed";
-    return GPA_B200_LAUNCH_FAILURE;
   }
   if (!c.n) {
     if (dweight && cudaMemsetAsync(dweight, 0, (size_t)c.vocab * c.width * p.es, st) != cudaSuccess) {
@@ -614,35 +695,39 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   const char* sv = static_cast<const char*>(saved);
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved, sc);
-  const int* row = reinterpret_cast<const int*>(sv + p.s_rows);
   const float* lse = reinterpret_cast<const float*>(sv + p.s_lse);
-  float* r = reinterpret_cast<float*>(sc + p.r);
-  float* scale = reinterpret_cast<float*>(sc + p.scale);
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
-  BY_TYPE(a->dtype, gather<T>(a, p, row, sc, st));
-  OK_OR("loss_gather launch failed");
-  {
+  if (p.copy_w) {
+    BY_TYPE(a->dtype, pad_weight<T>(a, p, sc, st));
+    OK_OR("loss_pad launch failed");
+  }
+  const bool none = a->reduction == GPA_B200_LOSS_NONE;
+  Upstream up = {none ? dloss : nullptr, true, none ? nullptr : dloss, a->reduction == GPA_B200_LOSS_MEAN};
+  if (none && a->dtype == GPA_B200_F16) {
+    float* r = reinterpret_cast<float*>(sc + p.r);
+    float* s = reinterpret_cast<float*>(sc + p.scale);
     Launch scope("loss_row_scale", st);
-    k_row_scale<<<1, 1024, 0, st>>>(dloss, a->reduction, c.n_rows, row, c.label, r, scale);
+    k_row_scale<<<1, 1024, 0, st>>>(dloss, c, r, s);
     OK_OR("loss_row_scale launch failed");
+    up = {r, false, s, false};
   }
   const int64_t part_stride = c.n_pad * c.pitch;
   const unsigned tiles_d = (unsigned)((c.pitch + kB - 1) / kB);
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
     if (p.tc) {
-      if (!tc_probs(c, v0, vn, lse, r, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
+      if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
       if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.parts, (int)(p.k_part / 64), v0 > 0, dxp, part_stride, st))
         FAIL("loss_dx_tc5 launch failed");
-      if (dweight && !tc_dw(c, pr, p.piece, v0, vn, scale, dweight, st)) FAIL("loss_dw_tc5 launch failed");
+      if (dweight && !tc_dw(c, pr, p.piece, v0, vn, up, dweight, st)) FAIL("loss_dw_tc5 launch failed");
       continue;
     }
-    const unsigned tv = (unsigned)(up(vn, kTile) / kB);
+    const unsigned tv = (unsigned)(vloss::up(vn, kTile) / kB);
     float* pf = static_cast<float*>(pr);
     {
       Launch scope("loss_probs", st);
-      k_probs<<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, r, pf, p.piece);
+      k_probs<<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, up, pf, p.piece);
       OK_OR("loss_probs launch failed");
     }
     if (dhidden) {
@@ -653,14 +738,12 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
     }
     if (dweight) {
       Launch scope("loss_dw", st);
-      k_dw<<<dim3(tiles_d, tv), 256, 0, st>>>(c, pf, p.piece, v0, vn, scale, static_cast<float*>(dweight));
+      k_dw<<<dim3(tiles_d, tv), 256, 0, st>>>(c, pf, p.piece, v0, vn, up, static_cast<float*>(dweight));
       OK_OR("loss_dw launch failed");
     }
   }
   if (dhidden) {
-    Launch scope("loss_finish", st);
-    BY_TYPE(a->dtype, (k_finish<T><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, part_stride, c.pitch, c.n_rows, row,
-                                                                scale, 1.f / tc_p_scale(a->dtype), c.width, static_cast<T*>(dhidden))));
+    BY_TYPE(a->dtype, finish<T>(p, dxp, part_stride, reinterpret_cast<const int*>(sv + p.s_pos), up, dhidden, st));
     OK_OR("loss_finish launch failed");
   }
   return GPA_B200_OK;

@@ -18,10 +18,28 @@ struct Call {
   int dtype;
   const int* n_rows;  // device: packed rows
   const int* label;   // [n] label of a packed row, -1 when outside the vocabulary
-  const void* x;      // packed rows [pad(n)][pitch], zero behind the last one's tile
+  const int* row;     // [n] the caller's row of a packed row
+  const void* x;      // packed rows [n_pad][pitch], zero behind the last one up to a multiple of 64
   const void* w;      // weight [vocab][w_pitch]
   int64_t w_pitch;
   int64_t n_pad;      // n rounded up to tiles
+};
+
+// The gradient of a packed row's loss, as s r with |r| <= 1 where fp16 needs it:
+//   r: 1 (each == NULL), each[row] (by_row) or each[packed row];  NaN for a label outside the vocabulary
+//   s: *s (1 if NULL), over the number of labelled rows for a mean
+struct Upstream {
+  const float* each;
+  bool by_row;
+  const float* s;
+  bool mean;
+  __device__ __forceinline__ float r(const Call& c, int64_t j) const {
+    if (c.label[j] < 0) return NAN;
+    return !each ? 1.f : each[by_row ? c.row[j] : j];
+  }
+  __device__ __forceinline__ float scale(int n_rows) const {
+    return (s ? *s : 1.f) / (mean ? (float)(n_rows > 0 ? n_rows : 1) : 1.f);
+  }
 };
 
 __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -31,11 +49,11 @@ __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1)
 int tc_pairs();
 float tc_p_scale(int dtype);  // P is stored times this
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st);
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const float* r, void* p, int64_t p_pitch,
-              cudaStream_t st);
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const Upstream& up, void* p,
+              int64_t p_pitch, cudaStream_t st);
 bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
            float* dx, int64_t dx_part, cudaStream_t st);
-bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const float* scale, void* dw,
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
            cudaStream_t st);
 
 }  // namespace vloss

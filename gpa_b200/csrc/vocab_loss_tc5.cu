@@ -44,28 +44,26 @@ constexpr float kLog2e = 1.4426950408889634f;
 enum Mode { kStats, kProbs, kDx, kDw };
 
 struct Args {
-  const int* n_rows;
-  const int* label;
-  int64_t vocab, v0, vn, n_pad;
+  Call c;
+  Upstream up;
+  int64_t v0, vn;
   int tiles_n;             // tiles across the product's columns
   int k_blocks;            // reduction blocks of 64 (kDw: from the rows)
   // kStats
   float2* part;
   float* z_label;
   // kProbs
-  const float *lse, *r;
+  const float* lse;
   void* p;
   int64_t p_pitch;
   float p_scale;
   // kDx
   float* dx;
   int64_t dx_part;
-  int parts, k_part, pitch;
+  int parts, k_part;
   bool add;
   // kDw
   void* dw;
-  const float* scale;
-  int width;
   bool wide;               // dW rows start on 16-byte boundaries
   uint32_t idesc;
   bool f16;
@@ -194,7 +192,7 @@ struct Walk {
   int mt, nt, total, n_rows, k_blocks;
   const Args& a;
   GPA_DEV Walk(const Args& args) : a(args) {
-    n_rows = *args.n_rows;
+    n_rows = *args.c.n_rows;
     nt = args.tiles_n;
     if (M == kDw) {
       mt = (int)((args.vn + kTile - 1) / kTile);
@@ -239,7 +237,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
   float v[32];
   if (M == kStats) {
     const bool live = row < n_rows;
-    const int64_t y = live ? (int64_t)a.label[row] - col0 : -1;
+    const int64_t y = live ? (int64_t)a.c.label[row] - col0 : -1;
     float big = -INFINITY, sum = 0.f;
     for (int c = 0; c < kTile; c += 32) {
       ld32(tc5::tmem_at(tmem, c), v);
@@ -248,7 +246,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
         for (int i = 0; i < 32; ++i)
           if (y == c + i) a.z_label[row] = v[i];
       }
-      const int64_t left = a.vocab - col0 - c;
+      const int64_t left = a.c.vocab - col0 - c;
       if (left < 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -267,11 +265,11 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
       sum = fmaf(sum, ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
     }
-    if (live) a.part[(int64_t)t.n * a.n_pad + row] = make_float2(big, sum);
+    if (live) a.part[(int64_t)t.n * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
     const bool live = row < n_rows;
-    const float off = live ? a.lse[row] * kLog2e : 0.f, r = live ? a.r[row] * a.p_scale : 0.f;
-    const int64_t y = live ? (int64_t)a.label[row] - a.v0 - col0 : -1;
+    const float off = live ? a.lse[row] * kLog2e : 0.f, r = live ? a.up.r(a.c, row) * a.p_scale : 0.f;
+    const int64_t y = live ? (int64_t)a.c.label[row] - a.v0 - col0 : -1;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p) + row * a.p_pitch + col0);
     for (int c = 0; c < kTile; c += 32) {
       ld32(tc5::tmem_at(tmem, c), v);
@@ -292,11 +290,11 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
     }
   } else if (M == kDx) {
     const bool live = row < n_rows;
-    float* out = a.dx + t.part * a.dx_part + row * a.pitch + col0;
+    float* out = a.dx + t.part * a.dx_part + row * a.c.pitch + col0;
     for (int c = 0; c < kTile; c += 32) {
       ld32(tc5::tmem_at(tmem, c), v);
       if (!live) continue;
-      const int64_t left = a.pitch - col0 - c;  // a multiple of 8
+      const int64_t left = a.c.pitch - col0 - c;  // a multiple of 8
       if (a.add) {
         float g[32];
 #pragma unroll
@@ -311,8 +309,8 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
     }
   } else {
     const bool live = row < a.vn;
-    const float s = *a.scale / a.p_scale;
-    uint16_t* out = static_cast<uint16_t*>(a.dw) + (a.v0 + row) * a.width + col0;
+    const float s = a.up.scale(n_rows) / a.p_scale;
+    uint16_t* out = static_cast<uint16_t*>(a.dw) + (a.v0 + row) * a.c.width + col0;
     for (int c = 0; c < kTile; c += 32) {
       if (!empty) {
         ld32(tc5::tmem_at(tmem, c), v);
@@ -321,7 +319,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
       }
       if (!live) continue;
-      const int64_t left = a.width - col0 - c;
+      const int64_t left = a.c.width - col0 - c;
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i] * s, v[2 * i + 1] * s, a.f16);
@@ -483,7 +481,10 @@ EncodeFn encoder() {
 // [outer][inner] of 16-bit values, rows `pitch` elements apart, in boxes of 64 x `rows`
 bool make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int64_t pitch, int rows, bool f16) {
   EncodeFn f = encoder();
-  if (!f) return false;
+  int dev = 0;
+  // the encoder is a driver call and wants a current context, which a thread's first runtime call
+  // on the device makes (a backward runs on a thread of its own)
+  if (!f || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   const cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
   const cuuint32_t box[2] = {64, (cuuint32_t)rows}, one[2] = {1, 1};
@@ -501,12 +502,7 @@ uint32_t idesc_of(const Call& c, bool a_mn, bool b_mn) {
 Args base_args(const Call& c) {
   Args a;
   std::memset(&a, 0, sizeof(a));
-  a.n_rows = c.n_rows;
-  a.label = c.label;
-  a.vocab = c.vocab;
-  a.n_pad = c.n_pad;
-  a.pitch = c.pitch;
-  a.width = c.width;
+  a.c = c;
   a.f16 = c.dtype == GPA_B200_F16;
   a.p_scale = tc_p_scale(c.dtype);
   a.k_blocks = (c.pitch + kBK - 1) / kBK;
@@ -516,8 +512,15 @@ Args base_args(const Call& c) {
 template <Mode M>
 bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
             cudaStream_t st) {
-  if (cudaFuncSetAttribute(k_product<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
-    return false;
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(k_product<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+      return false;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
   Launch scope(name, st);
   k_product<M><<<2 * pairs, kThreads, kSmem, st>>>(ma, mb, a);
@@ -570,8 +573,8 @@ bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   return launch<kStats>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
 }
 
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const float* r, void* p, int64_t p_pitch,
-              cudaStream_t st) {
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const Upstream& up, void* p,
+              int64_t p_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
   if (!make_map(&ma, c.x, c.pitch, c.n, c.pitch, kHalf, f16) ||
@@ -581,7 +584,7 @@ bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const flo
   a.v0 = v0;
   a.vn = vn;
   a.lse = lse;
-  a.r = r;
+  a.up = up;
   a.p = p;
   a.p_pitch = p_pitch;
   a.tiles_n = (int)((vn + kTile - 1) / kTile);
@@ -610,7 +613,7 @@ bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   return launch<kDx>("loss_dx_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile) * parts, st);
 }
 
-bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const float* scale, void* dw,
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
            cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
@@ -620,7 +623,7 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   Args a = base_args(c);
   a.v0 = v0;
   a.vn = vn;
-  a.scale = scale;
+  a.up = up;
   a.dw = dw;
   a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
   a.tiles_n = (c.pitch + kTile - 1) / kTile;

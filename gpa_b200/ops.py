@@ -298,18 +298,20 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _loss_args(hidden, weight, labels, ignore_index, reduction):
+def _loss_args(weight, shape, dtype, ignore_index, reduction):
+    """GpaLossArgs without the caller's rows, which only the forward reads, and the weight it points to."""
     a = _lib.GpaLossArgs()
-    x, so, si = _rows(hidden)
     w = weight if weight.stride(-1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
-    a.hidden, a.weight, a.labels = x.data_ptr(), w.data_ptr(), labels.data_ptr()
-    a.width, a.vocab = hidden.shape[-1], weight.shape[0]
-    a.inner = hidden.shape[-2] if hidden.ndim > 1 else 1
-    a.outer = labels.numel() // a.inner if a.inner else 0
-    a.hidden_stride[0], a.hidden_stride[1] = so, si
+    a.weight = w.data_ptr()
+    a.vocab, a.width = weight.shape
+    a.inner = shape[-2] if len(shape) > 1 else 1
+    rows = 1
+    for n in shape[:-1]:
+        rows *= n
+    a.outer = rows // a.inner if a.inner else 0
     a.weight_stride = w.stride(0)
-    a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[hidden.dtype], reduction
-    return a, (x, w)
+    a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[dtype], reduction
+    return a, w
 
 
 def _scratch(nbytes, device):
@@ -319,7 +321,9 @@ def _scratch(nbytes, device):
 def _loss_forward(hidden, weight, labels, ignore_index, reduction):
     lib = _lib.load()
     dev = hidden.device
-    a, keep = _loss_args(hidden, weight, labels, ignore_index, reduction)
+    a, keep = _loss_args(weight, hidden.shape, hidden.dtype, ignore_index, reduction)
+    x, a.hidden_stride[0], a.hidden_stride[1] = _rows(hidden)
+    a.hidden, a.labels = x.data_ptr(), labels.data_ptr()
     loss = torch.empty(labels.shape if reduction == 2 else (), device=dev, dtype=torch.float32)
     with _on(dev):
         sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
@@ -333,24 +337,27 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
         loss, saved = _loss_forward(hidden, weight, labels, ignore_index, reduction)
-        ctx.save_for_backward(hidden, weight, labels)
-        ctx.saved_ws, ctx.ignore_index, ctx.reduction = saved, ignore_index, reduction
+        # the labelled rows are packed into `saved`: hidden and labels are not needed again
+        ctx.save_for_backward(weight, saved)
+        ctx.hidden = hidden.shape, hidden.dtype
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        hidden, weight, labels = ctx.saved_tensors
+        weight, saved = ctx.saved_tensors
+        shape, dtype = ctx.hidden
         lib = _lib.load()
-        dev = hidden.device
-        a, keep = _loss_args(hidden, weight, labels, ctx.ignore_index, ctx.reduction)
-        dx, dw = (torch.empty(t.shape, device=dev, dtype=t.dtype) if need else None
-                  for t, need in zip((hidden, weight), ctx.needs_input_grad))
+        dev = weight.device
+        a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
+        dx, dw = (torch.empty(s, device=dev, dtype=dtype) if need else None
+                  for s, need in zip((shape, weight.shape), ctx.needs_input_grad))
         dloss = dloss.contiguous()
         with _on(dev):
             nbytes = lib.gpa_b200_loss_scratch_bytes(a, 1)
             scratch = _scratch(nbytes, dev)
-            _call(lib.gpa_b200_loss_backward, dev, a, ctx.saved_ws.data_ptr(), ctx.saved_ws.numel(),
+            _call(lib.gpa_b200_loss_backward, dev, a, saved.data_ptr(), saved.numel(),
                   dloss.data_ptr(), _lib.ptr(dx), _lib.ptr(dw), scratch.data_ptr(), nbytes)
         return dx, dw, None, None, None
 

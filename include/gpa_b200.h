@@ -274,7 +274,8 @@ size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward);
 /* loss: one fp32, or one per row for GPA_B200_LOSS_NONE (0 for rows without a label). */
 int gpa_b200_loss_forward(const GpaLossArgs* args, float* loss, void* saved, size_t saved_bytes,
                           void* scratch, size_t scratch_bytes, void* stream);
-/* dloss: fp32, loss's shape.  dhidden [rows, width], dweight [vocab, width]: contiguous, dtype,
+/* args as in the forward, whose hidden and labels the backward does not read (saved holds the
+ * labelled rows); dloss: fp32, loss's shape.  dhidden [rows, width], dweight [vocab, width]: contiguous, dtype,
  * overwritten; either may be NULL. */
 int gpa_b200_loss_backward(const GpaLossArgs* args, const void* saved, size_t saved_bytes,
                            const float* dloss, void* dhidden, void* dweight, void* scratch,
