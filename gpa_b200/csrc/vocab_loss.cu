@@ -1,6 +1,6 @@
 // Softmax cross entropy of z = x W^T over a large vocabulary, in pieces of it, without keeping z:
-//   lse_i = log sum_v exp z_iv        loss_i = lse_i - z_{i, y_i}
-//   P_iv = (exp(z_iv - lse_i) - [v = y_i]) r_i        dx = s P W        dW = s P^T x
+//   m_i = max_v z_iv    s_i = sum_v exp(z_iv - m_i)    loss_i = m_i - z_{i, y_i} + log s_i
+//   P_iv = (exp(z_iv - m_i) / s_i - [v = y_i]) r_i        dx = s P W        dW = s P^T x
 // with the upstream gradient of row i written as s r_i (see Upstream).
 //
 // Rows without a label are dropped first: the labelled ones are packed (k_pack), so masked
@@ -38,8 +38,61 @@ struct Pack {
   int *info, *row, *label, *pos;  // info: [packed rows, counter of k_join]
   int64_t so, si, inner;   // the caller's rows
   int width, pitch;
+  int64_t plane;
   bool vec;
 };
+
+// A value as it goes to the tensor cores: itself, or for fp32 three bf16 parts of 8 bits each, in
+// planes `plane` elements apart.
+GPA_DEV void put(__nv_bfloat16* d, int64_t, __nv_bfloat16 v) { *d = v; }
+GPA_DEV void put(__half* d, int64_t, __half v) { *d = v; }
+GPA_DEV void put(__nv_bfloat16* d, int64_t plane, float v) {
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    const __nv_bfloat16 b = __float2bfloat16(v);
+    d[q * plane] = b;
+    v -= __bfloat162float(b);
+  }
+}
+template <typename T>
+struct Part {
+  using type = T;
+};
+template <>
+struct Part<float> {
+  using type = __nv_bfloat16;
+};
+
+// One row of `width` values to `pitch` places, by one warp; 8 at a time where both ends allow it.
+template <typename T>
+GPA_DEV void put_row(const T* s, typename Part<T>::type* d, int64_t plane, int width, int pitch, bool vec, int lane) {
+  if (vec) {
+#pragma unroll 4
+    for (int c = lane * 8; c < width; c += 256) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(d + c) = *reinterpret_cast<const uint4*>(s + c);
+      } else {
+        float v[8];
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(s + c);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(s + c + 4);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            const float2 f = __bfloat1622float2(b);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+            v[2 * i] -= f.x, v[2 * i + 1] -= f.y;
+          }
+          *reinterpret_cast<uint4*>(d + q * plane + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  } else {
+    for (int c = lane; c < pitch; c += 32) put(d + c, plane, c < width ? s[c] : T(0.f));
+  }
+}
 
 // Packs the labelled rows: row[j], label[j] (-1 outside the vocabulary) and the channels of the
 // j-th of them, pos[i] its place or -1.  A block takes kRun rows; two more fill the places behind
@@ -48,8 +101,7 @@ struct Pack {
 // one launch is cheaper than k_count before it (a block reads 32 KB of labels at most); beyond,
 // the labels before a block are counted once.
 template <typename T>
-__global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, T* dst) {
-  constexpr int kV = 16 / sizeof(T);
+__global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, typename Part<T>::type* dst) {
   __shared__ int part[8];
   __shared__ int place[kRun];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -73,7 +125,7 @@ __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, T* dst
     if (extra == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.info[0] = before, p.info[1] = 0;
     const int end = (before + 63) / 64 * 64;
     for (int j = before + extra * kRun + blockIdx.y; j < min(end, before + (extra + 1) * kRun); j += 4)
-      for (int c = threadIdx.x; c < p.pitch; c += 256) dst[(int64_t)j * p.pitch + c] = T(0.f);
+      for (int c = threadIdx.x; c < p.pitch; c += 256) put(dst + (int64_t)j * p.pitch + c, p.plane, T(0.f));
     return;
   }
   if (warp == 0) {
@@ -93,23 +145,22 @@ __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, T* dst
   const int k = blockIdx.y * 8 + warp;
   if (place[k] < 0) return;
   const int64_t i = (int64_t)blockIdx.x * kRun + k;
-  const T* s = src + (i / p.inner) * p.so + (i % p.inner) * p.si;
-  T* d = dst + (int64_t)place[k] * p.pitch;
-  if (p.vec) {
-#pragma unroll 4
-    for (int c = lane * kV; c < p.width; c += 32 * kV)
-      *reinterpret_cast<uint4*>(d + c) = *reinterpret_cast<const uint4*>(s + c);
-  } else {
-    for (int c = lane; c < p.pitch; c += 32) d[c] = c < p.width ? s[c] : T(0.f);
-  }
+  put_row(src + (i / p.inner) * p.so + (i % p.inner) * p.si, dst + (int64_t)place[k] * p.pitch, p.plane, p.width,
+          p.pitch, p.vec, lane);
 }
 
-// Weight rows that cannot be read 16 bytes at a time: a copy with padded rows.
+// The weight where the tensor cores cannot read the caller's: rows that do not start on 16 bytes,
+// or fp32.  A warp a row; rows behind the last (of a plane) become zero.
 template <typename T>
-__global__ void k_pad(const T* src, int64_t stride, int width, int pitch, T* dst) {
-  const T* s = src + blockIdx.x * stride;
-  T* d = dst + (int64_t)blockIdx.x * pitch;
-  for (int c = threadIdx.x; c < pitch; c += blockDim.x) d[c] = c < width ? s[c] : T(0.f);
+__global__ void __launch_bounds__(256) k_weight(const T* src, int64_t stride, int64_t vocab, int64_t rows, int width,
+                                                int pitch, int64_t plane, bool vec, typename Part<T>::type* dst) {
+  const int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (v >= rows) return;
+  auto* d = dst + v * pitch;
+  if (v < vocab) put_row(src + v * stride, d, plane, width, pitch, vec, lane);
+  else
+    for (int c = lane; c < pitch; c += 32) put(d + c, plane, T(0.f));
 }
 
 // ------------------------------------------------------------------ joins
@@ -119,11 +170,11 @@ GPA_DEV void merge(float& m, float& s, float m2, float s2) {
   m = big;
 }
 
-// lse and loss of each packed row from the (max, sum) pairs of its tiles: blockDim.x rows a block,
+// Maximum and 1 / sum of exp, and loss, of each packed row from the (max, sum) pairs of its tiles: blockDim.x rows a block,
 // blockDim.y lanes of tiles each (256 threads).  The block that finishes last adds the losses of
 // a mean or sum in double, in a fixed order.
 __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, int tiles, const float* z_label,
-                                              float* lse, float* each, const int* pos, float* packed,
+                                              float2* lse, float* each, const int* pos, float* packed,
                                               float* total, bool mean, int* counter) {
   __shared__ float2 sm[256];
   __shared__ bool last;
@@ -156,7 +207,7 @@ __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, 
   }
   if (threadIdx.y == 0 && live) {
     const float log_s = logf(s);
-    lse[j] = m + log_s;
+    lse[j] = make_float2(m, 1.f / s);
     const float l = c.label[j] < 0 ? NAN : (m - z_label[j]) + log_s;
     if (each) each[c.row[j]] = l;
     else packed[j] = l;
@@ -239,200 +290,14 @@ __global__ void k_finish(const float* part, int parts, int64_t part_stride, cons
   }
 }
 
-// ------------------------------------------------------------------ products without tensor cores
-// fp32 inputs: C (128 x 128 per block, 8 x 8 per thread) = A B over k, fp32 multiply-adds.  An
-// operand is K-major (k contiguous) or MN-major; both are read 4 elements at a time.  Tensor cores
-// would take three bf16 parts of each operand and six products for the same precision, and lose
-// it again over reductions as long as the vocabulary.
-constexpr int kB = 128, kBK = 16;
-
-struct Operand {
-  const float* p;
-  int64_t pitch;
-  int64_t mn, k;  // extents: reads outside give zero (whole groups of 4 along the contiguous axis)
-};
-
-template <bool KMAJOR>
-GPA_DEV void fetch(const Operand& o, int64_t mn0, int64_t k0, float (&v)[2][4]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * 256;  // 512 groups of 4 of a 128 x 16 tile
-    const int64_t mn = mn0 + (KMAJOR ? i >> 2 : (i & 31) * 4), k = k0 + (KMAJOR ? (i & 3) * 4 : i >> 5);
-    v[h][0] = v[h][1] = v[h][2] = v[h][3] = 0.f;
-    if (mn < o.mn && k < o.k) {
-      const float4 f = *reinterpret_cast<const float4*>(o.p + (KMAJOR ? mn * o.pitch + k : k * o.pitch + mn));
-      v[h][0] = f.x, v[h][1] = f.y, v[h][2] = f.z, v[h][3] = f.w;
-    }
-  }
-}
-
-template <bool KMAJOR>
-GPA_DEV void put(float (*s)[kB + 4], const float (&v)[2][4]) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = threadIdx.x + h * 256;
-    if (KMAJOR) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[(i & 3) * 4 + e][i >> 2] = v[h][e];
-    } else {
-      *reinterpret_cast<float4*>(&s[i >> 5][(i & 31) * 4]) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
-    }
-  }
-}
-
-// acc[i][j]: row m0 + (ty * 4 + i % 4) + 64 * (i / 4), column n0 + (tx * 4 + j % 4) + 64 * (j / 4)
-template <bool AK, bool BK_>
-GPA_DEV void product(const Operand& a, const Operand& b, int64_t m0, int64_t n0, int64_t k0,
-                     int64_t k1, float (&acc)[8][8]) {
-  __shared__ float sa[2][kBK][kB + 4], sb[2][kBK][kB + 4];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
-  float va[2][4], vb[2][4];
-  if (k0 < k1) {
-    fetch<AK>(a, m0, k0, va);
-    fetch<BK_>(b, n0, k0, vb);
-  }
-  int s = 0;
-  for (int64_t k = k0; k < k1; k += kBK, s ^= 1) {
-    put<AK>(sa[s], va);
-    put<BK_>(sb[s], vb);
-    __syncthreads();
-    if (k + kBK < k1) {
-      fetch<AK>(a, m0, k + kBK, va);
-      fetch<BK_>(b, n0, k + kBK, vb);
-    }
-#pragma unroll
-    for (int kk = 0; kk < kBK; ++kk) {
-      float fa[8], fb[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        *reinterpret_cast<float4*>(fa + 4 * h) = *reinterpret_cast<const float4*>(&sa[s][kk][ty * 4 + 64 * h]);
-        *reinterpret_cast<float4*>(fb + 4 * h) = *reinterpret_cast<const float4*>(&sb[s][kk][tx * 4 + 64 * h]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
-    }
-  }
-}
-
-GPA_DEV int at8(int t, int i) { return t * 4 + (i & 3) + 64 * (i >> 2); }
-
-__global__ void __launch_bounds__(256, 2) k_stats(const Call c, float2* part, float* z_label) {
-  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  if (m0 >= *c.n_rows) return;
-  float acc[8][8];
-  product<true, true>({static_cast<const float*>(c.x), c.pitch, c.n_pad, c.pitch},
-                            {static_cast<const float*>(c.w), c.w_pitch, c.vocab, c.pitch}, m0, n0, 0, c.pitch, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + at8(ty, i);
-    const bool live = m < *c.n_rows;
-    const int y = live ? c.label[m] : -1;
-    float big = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t v = n0 + at8(tx, j);
-      if (v >= c.vocab) acc[i][j] = -INFINITY;
-      else if (v == y) z_label[m] = acc[i][j];
-      big = fmaxf(big, acc[i][j]);
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-    const float safe = big == -INFINITY ? 0.f : big;
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += expf(acc[i][j] - safe);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (tx == 0 && live) part[blockIdx.x * c.n_pad + m] = make_float2(big, s);
-  }
-}
-
-__global__ void __launch_bounds__(256, 2) k_probs(const Call c, int64_t v0, int64_t vn, const float* lse,
-                                                  const Upstream up, float* p, int64_t p_pitch) {
-  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  if (m0 >= *c.n_rows) return;
-  float acc[8][8];
-  product<true, true>({static_cast<const float*>(c.x), c.pitch, c.n_pad, c.pitch},
-                            {static_cast<const float*>(c.w) + v0 * c.w_pitch, c.w_pitch, vn, c.pitch}, m0, n0, 0,
-                            c.pitch, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + at8(ty, i);
-    const bool live = m < *c.n_rows;
-    const float l = live ? lse[m] : 0.f, ri = live ? up.r(c, m) : 0.f;
-    const int64_t y = live ? c.label[m] - v0 : -1;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t v = n0 + at8(tx, j);
-      p[m * p_pitch + v] = live && v < vn ? (expf(acc[i][j] - l) - (v == y ? 1.f : 0.f)) * ri : 0.f;
-    }
-  }
-}
-
-// part[z] (+)= P[:, k of part z] W
-__global__ void __launch_bounds__(256, 2) k_dx(const Call c, const float* p, int64_t p_pitch, int64_t v0,
-                                               int64_t vn, int64_t k_part, bool add, float* part,
-                                               int64_t part_stride) {
-  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  if (m0 >= *c.n_rows) return;
-  const int64_t k0 = blockIdx.z * k_part, k1 = k0 + k_part < vn ? k0 + k_part : vn;
-  float acc[8][8];
-  product<true, false>({p, p_pitch, c.n_pad, p_pitch},
-                                 {static_cast<const float*>(c.w) + v0 * c.w_pitch, c.w_pitch, c.pitch, vn}, m0, n0,
-                                 k0, k1, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float* o = part + blockIdx.z * part_stride;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + at8(ty, i);
-    if (m >= *c.n_rows) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t d = n0 + at8(tx, j);
-      if (d < c.pitch) o[m * c.pitch + d] = add ? o[m * c.pitch + d] + acc[i][j] : acc[i][j];
-    }
-  }
-}
-
-__global__ void __launch_bounds__(256, 2) k_dw(const Call c, const float* p, int64_t p_pitch, int64_t v0,
-                                               int64_t vn, const Upstream up, float* dw) {
-  const int64_t m0 = (int64_t)blockIdx.y * kB, n0 = (int64_t)blockIdx.x * kB;
-  const int64_t rows = *c.n_rows;
-  float acc[8][8];
-  product<false, false>({p, p_pitch, p_pitch, rows}, {static_cast<const float*>(c.x), c.pitch, c.pitch, rows},
-                                  m0, n0, 0, rows, acc);
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const float s = up.scale(*c.n_rows);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t v = m0 + at8(ty, i);
-    if (v >= vn) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t d = n0 + at8(tx, j);
-      if (d < c.width) dw[(v0 + v) * c.width + d] = acc[i][j] * s;
-    }
-  }
-}
-
 // ------------------------------------------------------------------ plan of a call
 constexpr int64_t kPieceBytes = int64_t(3) << 29;  // of P at a time
 
 struct Plan {
   Call c;
-  bool copy_w;             // weight rows that cannot be read 16 bytes at a time are copied first
-  int es;                  // bytes of an element of x and W
-  bool tc;                 // tensor cores (16-bit inputs)
-  int pes;                 // bytes of an element of P
-  int tiles_v, tiles_m;    // tiles of z
+  bool copy_w;             // the weight is copied first (k_weight)
+  int es;                  // bytes of an element of the caller's tensors
+  int parts_v;             // (max, sum) pairs of a row
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
   int parts;               // parts of dx
   int64_t k_part;          // vocabulary entries of a part
@@ -453,46 +318,47 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   if (a->weight_stride < a->width && a->vocab > 1) return "weight rows must not overlap";
   *code = GPA_B200_UNSUPPORTED;
   if (a->width > 65536) return "at most 65536 channels";
-  if (a->vocab > (int64_t(1) << 30)) return "at most 2^30 vocabulary entries";
+  if (a->vocab > (int64_t(1) << 29)) return "at most 2^29 vocabulary entries";
   if (a->inner && a->outer > (int64_t(1) << 22) / a->inner) return "at most 2^22 rows in a call";
   Call& c = p->c;
   c.n = a->outer * a->inner;
   c.vocab = a->vocab;
   c.width = a->width;
   c.dtype = a->dtype;
-  p->es = a->dtype == GPA_B200_F32 ? 4 : 2;
-  const int unit = 16 / p->es;
-  c.pitch = (int)up(a->width, unit);
+  const bool f32 = a->dtype == GPA_B200_F32;
+  p->es = f32 ? 4 : 2;
+  c.planes = f32 ? 3 : 1;
+  c.pitch = (int)up(a->width, 8);
   c.n_pad = up(std::max<int64_t>(c.n, 1), kTile);
-  p->copy_w = a->width % unit || a->weight_stride % unit || (reinterpret_cast<uintptr_t>(a->weight) & 15);
+  p->copy_w = f32 || a->width % 8 || a->weight_stride % 8 || (reinterpret_cast<uintptr_t>(a->weight) & 15);
   c.w = a->weight;
-  c.w_pitch = p->copy_w ? c.pitch : a->vocab > 1 ? a->weight_stride : c.pitch;
-  p->tc = a->dtype != GPA_B200_F32;
-  p->pes = p->tc ? 2 : 4;
-  const int tile = p->tc ? kTile : kB, at_once = p->tc ? tc_pairs() : 2 * 148;
-  p->tiles_v = (int)((c.vocab + tile - 1) / tile);
-  p->tiles_m = (int)(c.n_pad / tile);
-  const int64_t tiles_d = (c.pitch + tile - 1) / tile;
+  c.w_pitch = p->copy_w || a->vocab == 1 ? c.pitch : a->weight_stride;
+  const int at_once = tc_pairs();
+  const int64_t tiles_v = up(c.vocab, kTile) / kTile, tiles_m = c.n_pad / kTile;
+  const int64_t tiles_d = (c.pitch + kTile - 1) / kTile;
+  p->parts_v = (int)(f32 ? 2 * tiles_v : tiles_v);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
   // come out in fewer turns of the whole GPU (the pieces' turns added up).
-  const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * p->pes) / kTile);
-  const int64_t all = up(c.vocab, kTile) / kTile;
-  int64_t best = std::min(all, most), turns = INT64_MAX;
+  const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * 2 * c.planes) / kTile);
+  int64_t best = std::min(tiles_v, most), turns = INT64_MAX;
   auto turns_of = [&](int64_t t) {
-    auto one = [&](int64_t v) { return (v * (kTile / tile) * tiles_d + at_once - 1) / at_once; };
-    return all / t * one(t) + (all % t ? one(all % t) : 0);
+    auto one = [&](int64_t v) { return (v * tiles_d + at_once - 1) / at_once; };
+    return tiles_v / t * one(t) + (tiles_v % t ? one(tiles_v % t) : 0);
   };
-  for (int64_t t = std::min(all, most); t >= 1 && t >= std::min(all, most) / 2; --t)
+  for (int64_t t = best; t >= 1 && t >= std::min(tiles_v, most) / 2; --t)
     if (turns_of(t) < turns) turns = turns_of(t), best = t;
   p->piece = best * kTile;
   // dx: the reduction is cut into parts of at least 512 entries where that fills the GPU's turns
-  // better; every part costs another pass over dx in fp32, so a gain of 10 % is asked for.
+  // better.  A turn over a piece goes at about 1.4 PFLOP/s; each part is written and read again in
+  // fp32, at about 5 TB/s.
+  const int64_t tiles_x = tiles_d * tiles_m;
+  const double turn = 2.0 * kTile * kTile * at_once * (double)p->piece * (f32 ? 6 : 1) / 1.4e15;
+  const double pass = (double)c.n_pad * c.pitch * 8 / 5e12;
   p->parts = 1;
-  const int64_t tiles_x = tiles_d * p->tiles_m;
-  double cost = (double)((tiles_x + at_once - 1) / at_once);
-  for (int n = 2; n <= 2 * at_once && n <= p->piece / 512; ++n) {
-    const double now = (double)((tiles_x * n + at_once - 1) / at_once) / n;
-    if (now < 0.9 * cost) cost = now, p->parts = n;
+  double cost = 1e30;
+  for (int n = 1; n == 1 || (n <= 2 * at_once && n <= p->piece / 512); ++n) {
+    const double now = (double)((tiles_x * n + at_once - 1) / at_once) / n * turn + n * pass;
+    if (now < cost) cost = now, p->parts = n;
   }
   p->k_part = up((p->piece + p->parts - 1) / p->parts, 64);
   p->parts = (int)((p->piece + p->k_part - 1) / p->k_part);
@@ -506,19 +372,19 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->s_row = take(4 * c.n);
   p->s_label = take(4 * c.n);
   p->s_pos = take(4 * c.n);
-  p->s_lse = take(4 * c.n);
-  p->s_x = take(c.n_pad * c.pitch * p->es);
+  p->s_lse = take(8 * c.n);
+  p->s_x = take(c.planes * c.n_pad * c.pitch * 2);
   p->s_bytes = at;
   at = 0;
-  p->w = take(p->copy_w ? c.vocab * c.pitch * p->es : 0);
+  p->w = take(p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0);
   const int64_t common = at;
   p->count = take(4 * up(c.n, kRun) / kRun);
-  p->part = take((int64_t)p->tiles_v * c.n_pad * 8);
+  p->part = take((int64_t)p->parts_v * c.n_pad * 8);
   p->z_label = take(4 * c.n);
   p->loss = take(4 * c.n);
   p->fwd_bytes = at;
   at = common;
-  p->p = take(c.n_pad * p->piece * p->pes);
+  p->p = take(c.planes * c.n_pad * p->piece * 2);
   p->dxp = take((int64_t)p->parts * c.n_pad * c.pitch * 4);
   p->r = take(4 * c.n);
   p->scale = take(4);
@@ -529,7 +395,6 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
 template <typename T>
 void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaStream_t st) {
   const Call& c = p.c;
-  constexpr int kV = 16 / sizeof(T);
   Pack k;
   k.labels = a->labels;
   k.n = (int)c.n;
@@ -546,8 +411,8 @@ void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaS
   k.inner = std::max<int64_t>(a->inner, 1);
   k.width = c.width;
   k.pitch = c.pitch;
-  k.vec = a->width % kV == 0 && k.so % kV == 0 && k.si % kV == 0 &&
-          (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
+  k.plane = c.n_pad * c.pitch;
+  k.vec = a->width % 8 == 0 && k.so % 8 == 0 && k.si % 8 == 0 && (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
   if (c.n > kCountDirectly) {
     int* count = reinterpret_cast<int*>(scratch + p.count);
     k.count = count;
@@ -555,14 +420,19 @@ void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaS
     k_count<<<k.runs, kRun, 0, st>>>(a->labels, k.n, k.ignore, count);
   }
   Launch scope("loss_pack", st);
-  k_pack<T><<<dim3(k.runs + 2, 4), 256, 0, st>>>(k, static_cast<const T*>(a->hidden), reinterpret_cast<T*>(saved + p.s_x));
+  k_pack<T><<<dim3(k.runs + 2, 4), 256, 0, st>>>(
+      k, static_cast<const T*>(a->hidden), reinterpret_cast<typename Part<T>::type*>(saved + p.s_x));
 }
 
 template <typename T>
-void pad_weight(const GpaLossArgs* a, const Plan& p, char* scratch, cudaStream_t st) {
-  Launch scope("loss_pad", st);
-  k_pad<T><<<(unsigned)p.c.vocab, 128, 0, st>>>(static_cast<const T*>(a->weight), a->weight_stride, p.c.width,
-                                                p.c.pitch, reinterpret_cast<T*>(scratch + p.w));
+void copy_weight(const GpaLossArgs* a, const Plan& p, char* scratch, cudaStream_t st) {
+  const Call& c = p.c;
+  const int64_t rows = c.planes > 1 ? up(c.vocab, kTile) : c.vocab;
+  const bool vec = c.width % 8 == 0 && a->weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a->weight) & 15) == 0;
+  Launch scope("loss_weight", st);
+  k_weight<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
+      static_cast<const T*>(a->weight), a->weight_stride, c.vocab, rows, c.width, c.pitch, rows * c.pitch, vec,
+      reinterpret_cast<typename Part<T>::type*>(scratch + p.w));
 }
 
 template <typename T>
@@ -570,7 +440,7 @@ void finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, con
             cudaStream_t st) {
   constexpr int kV = 16 / sizeof(T);
   const Call& c = p.c;
-  const float unit = 1.f / (p.tc ? tc_p_scale(c.dtype) : 1.f);
+  const float unit = 1.f / tc_p_scale(c.dtype);
   Launch scope("loss_finish", st);
   if (c.width % kV == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0)
     k_finish<T, kV><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, stride, c, pos, up, unit, static_cast<T*>(dx));
@@ -645,24 +515,16 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
   BY_TYPE(a->dtype, pack<T>(a, p, sv, sc, st));
   OK_OR("loss_pack launch failed");
   if (p.copy_w && c.n) {
-    BY_TYPE(a->dtype, pad_weight<T>(a, p, sc, st));
-    OK_OR("loss_pad launch failed");
+    BY_TYPE(a->dtype, copy_weight<T>(a, p, sc, st));
+    OK_OR("loss_weight launch failed");
   }
-  if (c.n) {
-    if (p.tc) {
-      if (!tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
-    } else {
-      Launch scope("loss_stats", st);
-      k_stats<<<dim3(p.tiles_v, p.tiles_m), 256, 0, st>>>(c, part, z_label);
-      OK_OR("loss_stats launch failed");
-    }
-  }
+  if (c.n && !tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
   if (c.n || !none) {
     // few rows: more lanes for the tiles of each
     const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;
     Launch scope("loss_join", st);
     k_join<<<(unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st>>>(
-        c, part, p.tiles_v, z_label, reinterpret_cast<float*>(sv + p.s_lse), each,
+        c, part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
         reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
         a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1);
     OK_OR("loss_join launch failed");
@@ -695,12 +557,12 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   const char* sv = static_cast<const char*>(saved);
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved, sc);
-  const float* lse = reinterpret_cast<const float*>(sv + p.s_lse);
+  const float2* lse = reinterpret_cast<const float2*>(sv + p.s_lse);
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
   if (p.copy_w) {
-    BY_TYPE(a->dtype, pad_weight<T>(a, p, sc, st));
-    OK_OR("loss_pad launch failed");
+    BY_TYPE(a->dtype, copy_weight<T>(a, p, sc, st));
+    OK_OR("loss_weight launch failed");
   }
   const bool none = a->reduction == GPA_B200_LOSS_NONE;
   Upstream up = {none ? dloss : nullptr, true, none ? nullptr : dloss, a->reduction == GPA_B200_LOSS_MEAN};
@@ -713,34 +575,12 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
     up = {r, false, s, false};
   }
   const int64_t part_stride = c.n_pad * c.pitch;
-  const unsigned tiles_d = (unsigned)((c.pitch + kB - 1) / kB);
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
-    if (p.tc) {
-      if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
-      if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.parts, (int)(p.k_part / 64), v0 > 0, dxp, part_stride, st))
-        FAIL("loss_dx_tc5 launch failed");
-      if (dweight && !tc_dw(c, pr, p.piece, v0, vn, up, dweight, st)) FAIL("loss_dw_tc5 launch failed");
-      continue;
-    }
-    const unsigned tv = (unsigned)(vloss::up(vn, kTile) / kB);
-    float* pf = static_cast<float*>(pr);
-    {
-      Launch scope("loss_probs", st);
-      k_probs<<<dim3(tv, p.tiles_m), 256, 0, st>>>(c, v0, vn, lse, up, pf, p.piece);
-      OK_OR("loss_probs launch failed");
-    }
-    if (dhidden) {
-      Launch scope("loss_dx", st);
-      k_dx<<<dim3(tiles_d, p.tiles_m, p.parts), 256, 0, st>>>(c, pf, p.piece, v0, vn, p.k_part, v0 > 0, dxp,
-                                                              part_stride);
-      OK_OR("loss_dx launch failed");
-    }
-    if (dweight) {
-      Launch scope("loss_dw", st);
-      k_dw<<<dim3(tiles_d, tv), 256, 0, st>>>(c, pf, p.piece, v0, vn, up, static_cast<float*>(dweight));
-      OK_OR("loss_dw launch failed");
-    }
+    if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
+    if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.parts, (int)(p.k_part / 64), v0 > 0, dxp, part_stride, st))
+      FAIL("loss_dx_tc5 launch failed");
+    if (dweight && !tc_dw(c, pr, p.piece, v0, vn, up, dweight, st)) FAIL("loss_dw_tc5 launch failed");
   }
   if (dhidden) {
     BY_TYPE(a->dtype, finish<T>(p, dxp, part_stride, reinterpret_cast<const int*>(sv + p.s_pos), up, dhidden, st));

@@ -1,5 +1,5 @@
 // Softmax cross entropy over a vocabulary: shapes and buffers shared by its kernels
-// (vocab_loss.cu: rows, joins and the fp32 products; see there for the formulas).
+// (vocab_loss.cu: rows and joins; see there for the formulas).
 #pragma once
 #include "../../include/gpa_b200.h"
 #include "common.cuh"
@@ -16,11 +16,13 @@ struct Call {
   int64_t vocab;
   int width, pitch;   // channels, and the element pitch of the packed rows
   int dtype;
+  int planes;         // parts of each value: 1, or the 3 bf16 parts of fp32 (x, W and P in planes of n_pad rows,
+                      // of vocab rounded up to tiles, and of n_pad rows)
   const int* n_rows;  // device: packed rows
   const int* label;   // [n] label of a packed row, -1 when outside the vocabulary
   const int* row;     // [n] the caller's row of a packed row
   const void* x;      // packed rows [n_pad][pitch], zero behind the last one up to a multiple of 64
-  const void* w;      // weight [vocab][w_pitch]
+  const void* w;      // weight [vocab][w_pitch], 16-bit elements
   int64_t w_pitch;
   int64_t n_pad;      // n rounded up to tiles
 };
@@ -44,12 +46,12 @@ struct Upstream {
 
 __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
-// The products of 16-bit inputs on tensor cores (vocab_loss_tc5.cu); false when a launch failed.
+// The products, on tensor cores (vocab_loss_tc5.cu); false when a launch failed.
 // They tile by kTile x kTile and pair up the SMs: tc_pairs() tiles run at a time.
 int tc_pairs();
 float tc_p_scale(int dtype);  // P is stored times this
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st);
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const Upstream& up, void* p,
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
               int64_t p_pitch, cudaStream_t st);
 bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
            float* dx, int64_t dx_part, cudaStream_t st);

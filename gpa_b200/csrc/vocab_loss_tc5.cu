@@ -1,6 +1,6 @@
-// The products of the vocabulary loss on the 5th-generation tensor cores, for 16-bit inputs
-// (formulas in vocab_loss.cu): z = x W^T with the softmax statistics or with P in its epilogue,
-// dx += P W, and dW = P^T x.
+// The products of the vocabulary loss on the 5th-generation tensor cores (formulas in
+// vocab_loss.cu): z = x W^T with the softmax statistics or with P in its epilogue, dx += P W, and
+// dW = P^T x.
 //
 // One kernel shape serves all four: a pair of CTAs (cta_group::2) owns 256 x 256 tiles of the
 // product, each CTA 128 of the rows.  A pair shares its operands: each CTA brings in its own 128
@@ -13,6 +13,13 @@
 //
 //   warp 0: copies     warp 1: products (first CTA of the pair)     warp 2: tensor memory
 //   warps 4-7: epilogue, a thread for each row of the tile
+//
+// fp32 inputs come as three bf16 parts, x = x0 + x1 + x2 (24 bits), in planes one behind the
+// other, and each product is the six of them that matter, the smallest first: x2 y0, x1 y1, x0 y2,
+// x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
+// step of 16, so a long reduction would lose what the parts gained: the accumulator is emptied
+// after kSegment of it and the segments are added in registers, in round-to-nearest fp32, by
+// eight epilogue warps (two threads a row).
 //
 // Every wait is bounded (tc5.cuh); a wait that gives up sets the device status and the kernel
 // drains and returns.
@@ -37,7 +44,8 @@ constexpr int kHalf = 128;                        // rows of an operand that one
 constexpr uint32_t kOperand = kHalf * kBK * 2;    // bytes of one operand in one stage
 constexpr uint32_t kStage = 2 * kOperand;
 constexpr size_t kSmem = kStages * kStage + 1024 + 256;  // operands on 1024 bytes, barriers
-constexpr int kThreads = 256;
+constexpr int kSegment = 8;  // reduction blocks between two additions in registers (fp32)
+constexpr int threads_of(bool f32) { return f32 ? 384 : 256; }
 constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -47,13 +55,14 @@ struct Args {
   Call c;
   Upstream up;
   int64_t v0, vn;
+  int a_plane, b_plane;    // fp32: rows of a plane of the operands
   int tiles_n;             // tiles across the product's columns
   int k_blocks;            // reduction blocks of 64 (kDw: from the rows)
   // kStats
   float2* part;
   float* z_label;
   // kProbs
-  const float* lse;
+  const float2* lse;       // (max, 1 / sum of exp) of each row
   void* p;
   int64_t p_pitch;
   float p_scale;
@@ -64,7 +73,7 @@ struct Args {
   bool add;
   // kDw
   void* dw;
-  bool wide;               // dW rows start on 16-byte boundaries
+  bool wide;               // dW rows start on the boundaries that its stores need
   uint32_t idesc;
   bool f16;
 };
@@ -154,6 +163,11 @@ GPA_DEV void ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+GPA_DEV void ld16(uint32_t taddr, float (&v)[16]) {
+  tc5::tmem_ld16(taddr, v);
+  tc5::tmem_wait_ld();
+}
+
 GPA_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -229,18 +243,38 @@ struct Walk {
   }
 };
 
-template <Mode M>
-GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, int rank, bool empty) {
-  const int in_tile = rank * kHalf + (threadIdx.x & 127);  // warps 4-7: one thread per row
+// What a thread holds of its row when the tile is done: 256 columns in tensor memory (16-bit
+// inputs), or the half of them that it has added up in registers (fp32).
+template <bool F32>
+struct Row {
+  uint32_t tmem;
+  GPA_DEV void get(int chunk, float (&v)[32]) const { ld32(tc5::tmem_at(tmem, 32 * chunk), v); }
+};
+template <>
+struct Row<true> {
+  float acc[128];
+  GPA_DEV void get(int chunk, float (&v)[32]) const {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = acc[32 * chunk + i];
+  }
+};
+
+template <Mode M, bool F32>
+GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32>& held, int rank, bool empty) {
+  constexpr int kChunks = F32 ? 4 : 8, kUnroll = F32 ? 4 : 1;
+  const int half = F32 ? (threadIdx.x - 128) >> 7 : 0;  // of the tile's columns
+  const int in_tile = rank * kHalf + (threadIdx.x & 127);
   const int64_t row = (int64_t)t.m * kTile + in_tile;
-  const int64_t col0 = (int64_t)t.n * kTile;
+  const int64_t col0 = (int64_t)t.n * kTile + half * 128;
   float v[32];
   if (M == kStats) {
     const bool live = row < n_rows;
     const int64_t y = live ? (int64_t)a.c.label[row] - col0 : -1;
     float big = -INFINITY, sum = 0.f;
-    for (int c = 0; c < kTile; c += 32) {
-      ld32(tc5::tmem_at(tmem, c), v);
+#pragma unroll kUnroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = 32 * k;
+      held.get(k, v);
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -255,44 +289,61 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
       float m = big;
 #pragma unroll
       for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
-      const float off = m == -INFINITY ? 0.f : m * kLog2e;
+      const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        s0 += ex2(fmaf(v[i], kLog2e, -off));
-        s1 += ex2(fmaf(v[i + 1], kLog2e, -off));
+        s0 += F32 ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
+        s1 += F32 ? expf(v[i + 1] - safe) : ex2(fmaf(v[i + 1], kLog2e, -off));
       }
-      sum = fmaf(sum, ex2(fmaf(big, kLog2e, -off)), s0 + s1);
+      sum = fmaf(sum, F32 ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
     }
-    if (live) a.part[(int64_t)t.n * a.c.n_pad + row] = make_float2(big, sum);
+    if (live) a.part[(int64_t)(F32 ? 2 * t.n + half : t.n) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
     const bool live = row < n_rows;
-    const float off = live ? a.lse[row] * kLog2e : 0.f, r = live ? a.up.r(a.c, row) * a.p_scale : 0.f;
+    const float2 l = live ? a.lse[row] : make_float2(0.f, 0.f);
+    const float r = live ? a.up.r(a.c, row) * a.p_scale : 0.f, f = l.y * r, off = l.x * kLog2e;
     const int64_t y = live ? (int64_t)a.c.label[row] - a.v0 - col0 : -1;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p) + row * a.p_pitch + col0);
-    for (int c = 0; c < kTile; c += 32) {
-      ld32(tc5::tmem_at(tmem, c), v);
+    const int64_t plane = a.c.n_pad * a.p_pitch / 2;
+#pragma unroll kUnroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = 32 * k;
+      held.get(k, v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], kLog2e, -off));
+      for (int i = 0; i < 32; ++i) v[i] = (F32 ? expf(v[i] - l.x) : ex2(fmaf(v[i], kLog2e, -off))) * f;
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (y == c + i) v[i] -= 1.f;
+          if (y == c + i) v[i] -= r;
       }
       const int64_t left = live ? a.vn - col0 - c : 0;
-      uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        w[i] = pack2(2 * i < left ? v[2 * i] * r : 0.f, 2 * i + 1 < left ? v[2 * i + 1] * r : 0.f, a.f16);
+      for (int i = 0; i < 32; ++i)
+        if (i >= left) v[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; i += 8) st8(out + c / 2 + i, w + i);
+      for (int q = 0; q < (F32 ? 3 : 1); ++q) {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          w[i] = pack2(v[2 * i], v[2 * i + 1], !F32 && a.f16);
+          if (F32) {  // what this part leaves
+            const float2 g = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+            v[2 * i] -= g.x, v[2 * i + 1] -= g.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 8) st8(out + q * plane + c / 2 + i, w + i);
+      }
     }
   } else if (M == kDx) {
     const bool live = row < n_rows;
     float* out = a.dx + t.part * a.dx_part + row * a.c.pitch + col0;
-    for (int c = 0; c < kTile; c += 32) {
-      ld32(tc5::tmem_at(tmem, c), v);
+#pragma unroll kUnroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = 32 * k;
+      held.get(k, v);
       if (!live) continue;
       const int64_t left = a.c.pitch - col0 - c;  // a multiple of 8
       if (a.add) {
@@ -310,36 +361,59 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, uint32_t tmem, i
   } else {
     const bool live = row < a.vn;
     const float s = a.up.scale(n_rows) / a.p_scale;
-    uint16_t* out = static_cast<uint16_t*>(a.dw) + (a.v0 + row) * a.c.width + col0;
-    for (int c = 0; c < kTile; c += 32) {
+    const int64_t at = (a.v0 + row) * a.c.width + col0;
+#pragma unroll kUnroll
+    for (int k = 0; k < kChunks; ++k) {
+      const int c = 32 * k;
       if (!empty) {
-        ld32(tc5::tmem_at(tmem, c), v);
+        held.get(k, v);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0.f;
       }
       if (!live) continue;
       const int64_t left = a.c.width - col0 - c;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= s;
+      if (F32) {
+        float* out = static_cast<float*>(a.dw) + at + c;
+        if (a.wide) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (i < left) st8(out + i, reinterpret_cast<const uint32_t*>(v + i));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < left) out[i] = v[i];
+        }
+        continue;
+      }
+      uint16_t* out = static_cast<uint16_t*>(a.dw) + at + c;
       uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i] * s, v[2 * i + 1] * s, a.f16);
+      for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], a.f16);
       if (a.wide) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-          if (2 * i < left) *reinterpret_cast<uint4*>(out + c + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+          if (2 * i < left) *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (i < left) out[c + i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+          if (i < left) out[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
       }
     }
   }
 }
 
-template <Mode M>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+// Planes of the products of a pair of operands, the smallest first.
+GPA_DEV int plane_a(int q) { return q == 0 ? 2 : q == 1 || q == 3 ? 1 : 0; }
+GPA_DEV int plane_b(int q) { return q == 2 ? 2 : q == 1 || q == 4 ? 1 : 0; }
+
+template <Mode M, bool F32>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
     k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
   constexpr bool kAMn = M == kDw, kBMn = M == kDx || M == kDw;
+  constexpr int kProducts = F32 ? 6 : 1;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * kStage);
@@ -354,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       tc5::mbar_init(&acc_full[i], 1);
-      tc5::mbar_init(&acc_empty[i], 8);  // the four epilogue warps of both CTAs
+      tc5::mbar_init(&acc_empty[i], F32 ? 16 : 8);  // the epilogue warps of both CTAs
     }
     tc5::mbar_fence_init();
   }
@@ -371,34 +445,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const Walk<M> walk(a);
   bool ok = true;
 
+  // The reduction of a tile goes by in segments, each into an accumulator of its own: all of it at
+  // once for 16-bit inputs, kSegment blocks times the products of the parts for fp32.
+  auto segment_end = [](int k, int k1) { return F32 && k + kSegment < k1 ? k + kSegment : k1; };
+
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
       for (int t = pair; t < walk.total && ok; t += pairs) {
         const Tile x = walk.at(t);
         const int ra = x.m * kTile + rank * kHalf, rb = x.n * kTile + rank * kHalf;
-        for (int k = x.k0; k < x.k1; ++k, ++it) {
-          const uint32_t s = it % kStages, turn = it / kStages;
-          if (turn && !(ok = tc5::mbar_wait(&empty[s], (turn - 1) & 1))) break;
-          unsigned char* sa = sm + s * kStage;
-          unsigned char* sb = sa + kOperand;
-          const uint32_t bar = in_first(&full[s]);
-          if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
-          const int kk = k * kBK;
-          if (kAMn) {
-            tma_load(sa, &map_a, ra, kk, bar);
-            tma_load(sa + kOperand / 2, &map_a, ra + 64, kk, bar);
-          } else {
-            tma_load(sa, &map_a, kk, ra, bar);
-          }
-          if (M == kDx) {  // the reduction runs over the piece's vocabulary entries
-            tma_load(sb, &map_b, rb, (int)a.v0 + kk, bar);
-            tma_load(sb + kOperand / 2, &map_b, rb + 64, (int)a.v0 + kk, bar);
-          } else if (kBMn) {
-            tma_load(sb, &map_b, rb, kk, bar);
-            tma_load(sb + kOperand / 2, &map_b, rb + 64, kk, bar);
-          } else {
-            tma_load(sb, &map_b, kk, (int)a.v0 + rb, bar);
+        for (int k0 = x.k0; k0 < x.k1 && ok; k0 = segment_end(k0, x.k1)) {
+          const int blocks = segment_end(k0, x.k1) - k0;
+          for (int j = 0; j < blocks * kProducts; ++j, ++it) {
+            const int q = F32 ? j / blocks : 0, k = k0 + j - q * blocks;
+            const uint32_t s = it % kStages, turn = it / kStages;
+            if (turn && !(ok = tc5::mbar_wait(&empty[s], (turn - 1) & 1))) break;
+            unsigned char* sa = sm + s * kStage;
+            unsigned char* sb = sa + kOperand;
+            const uint32_t bar = in_first(&full[s]);
+            if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
+            const int kk = k * kBK, pa = F32 ? plane_a(q) * a.a_plane : 0, pb = F32 ? plane_b(q) * a.b_plane : 0;
+            if (kAMn) {
+              tma_load(sa, &map_a, ra, pa + kk, bar);
+              tma_load(sa + kOperand / 2, &map_a, ra + 64, pa + kk, bar);
+            } else {
+              tma_load(sa, &map_a, kk, pa + ra, bar);
+            }
+            if (kBMn) {  // in dx the reduction runs over the piece's vocabulary entries
+              const int kb = pb + (M == kDx ? (int)a.v0 : 0) + kk;
+              tma_load(sb, &map_b, rb, kb, bar);
+              tma_load(sb + kOperand / 2, &map_b, rb + 64, kb, bar);
+            } else {
+              tma_load(sb, &map_b, kk, pb + (int)a.v0 + rb, bar);
+            }
           }
         }
       }
@@ -412,41 +492,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint32_t it = 0, count = 0;
       for (int t = pair; t < walk.total && ok; t += pairs) {
         const Tile x = walk.at(t);
-        if (x.k0 >= x.k1) continue;
-        const uint32_t buf = count & 1, use = count >> 1;
-        ++count;
-        if (use && !(ok = wait_cluster(&acc_empty[buf], (use - 1) & 1))) break;
-        tc5::fence_after_sync();
-        for (int k = x.k0; k < x.k1; ++k, ++it) {
-          const uint32_t s = it % kStages;
-          if (!(ok = tc5::mbar_wait(&full[s], (it / kStages) & 1))) break;
+        for (int k0 = x.k0; k0 < x.k1 && ok; k0 = segment_end(k0, x.k1), ++count) {
+          const uint32_t buf = count & 1, use = count >> 1;
+          if (use && !(ok = wait_cluster(&acc_empty[buf], (use - 1) & 1))) break;
           tc5::fence_after_sync();
-          const uint32_t sa = tc5::saddr(sm + s * kStage), sb = sa + kOperand;
+          const int steps = (segment_end(k0, x.k1) - k0) * kProducts;
+          for (int j = 0; j < steps; ++j, ++it) {
+            const uint32_t s = it % kStages;
+            if (!(ok = tc5::mbar_wait(&full[s], (it / kStages) & 1))) break;
+            tc5::fence_after_sync();
+            const uint32_t sa = tc5::saddr(sm + s * kStage), sb = sa + kOperand;
 #pragma unroll
-          for (int ks = 0; ks < kBK / 16; ++ks)
-            mma2(tmem + buf * kTile, operand<kAMn>(sa, ks), operand<kBMn>(sb, ks), a.idesc, k > x.k0 || ks > 0);
-          commit2(&empty[s]);
+            for (int ks = 0; ks < kBK / 16; ++ks)
+              mma2(tmem + buf * kTile, operand<kAMn>(sa, ks), operand<kBMn>(sb, ks), a.idesc, j > 0 || ks > 0);
+            commit2(&empty[s]);
+          }
+          if (ok) commit2(&acc_full[buf]);
         }
-        if (!ok) break;
-        commit2(&acc_full[buf]);
       }
     }
   } else if (warp >= 4) {
     uint32_t count = 0;
+    const int half = (warp - 4) >> 2;
     for (int t = pair; t < walk.total && ok; t += pairs) {
       const Tile x = walk.at(t);
-      if (x.k0 >= x.k1) {
-        if (M == kDw) epilogue<M>(a, x, walk.n_rows, tmem, rank, true);
-        continue;
+      Row<F32> held;
+      const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (kDx)
+      if (none && M != kDw) continue;
+      for (int k0 = x.k0; k0 < x.k1; k0 = segment_end(k0, x.k1), ++count) {
+        const uint32_t buf = count & 1, use = count >> 1;
+        if (!(ok = __all_sync(0xffffffffu, tc5::mbar_wait(&acc_full[buf], use & 1)))) break;
+        tc5::fence_after_sync();
+        if constexpr (F32) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 16) {
+            float v[16];
+            ld16(tc5::tmem_at(tmem, buf * kTile + half * 128 + c), v);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) held.acc[c + i] = k0 == x.k0 ? v[i] : held.acc[c + i] + v[i];
+          }
+        } else {
+          held.tmem = tmem + buf * kTile;
+          epilogue<M, F32>(a, x, walk.n_rows, held, rank, false);
+        }
+        tc5::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_first(in_first(&acc_empty[buf]));
       }
-      const uint32_t buf = count & 1, use = count >> 1;
-      ++count;
-      if (!(ok = __all_sync(0xffffffffu, tc5::mbar_wait(&acc_full[buf], use & 1)))) break;
-      tc5::fence_after_sync();
-      epilogue<M>(a, x, walk.n_rows, tmem + buf * kTile, rank, false);
-      tc5::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) arrive_first(in_first(&acc_empty[buf]));
+      if (ok && (F32 || none)) epilogue<M, F32>(a, x, walk.n_rows, held, rank, none);
     }
   }
   if (!ok) g_loss_status = GPA_B200_DEVICE_TIMEOUT;
@@ -499,6 +592,8 @@ uint32_t idesc_of(const Call& c, bool a_mn, bool b_mn) {
   return d;
 }
 
+int64_t w_rows(const Call& c) { return c.planes > 1 ? c.planes * up(c.vocab, kTile) : c.vocab; }
+
 Args base_args(const Call& c) {
   Args a;
   std::memset(&a, 0, sizeof(a));
@@ -506,25 +601,34 @@ Args base_args(const Call& c) {
   a.f16 = c.dtype == GPA_B200_F16;
   a.p_scale = tc_p_scale(c.dtype);
   a.k_blocks = (c.pitch + kBK - 1) / kBK;
+  a.a_plane = (int)c.n_pad;
+  a.b_plane = (int)up(c.vocab, kTile);
   return a;
 }
 
-template <Mode M>
-bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
+template <Mode M, bool F32>
+bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
             cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k_product<M>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_product<M, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
       return false;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
   Launch scope(name, st);
-  k_product<M><<<2 * pairs, kThreads, kSmem, st>>>(ma, mb, a);
+  k_product<M, F32><<<2 * pairs, threads_of(F32), kSmem, st>>>(ma, mb, a);
   return cudaGetLastError() == cudaSuccess;
+}
+
+template <Mode M>
+bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
+            cudaStream_t st) {
+  return a.c.dtype == GPA_B200_F32 ? launch_as<M, true>(name, ma, mb, a, tiles, st)
+                                   : launch_as<M, false>(name, ma, mb, a, tiles, st);
 }
 
 }  // namespace
@@ -541,7 +645,7 @@ int tc_pairs() {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(threads_of(false));
     cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -549,8 +653,8 @@ int tc_pairs() {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(k_product<kStats>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_product<kStats>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaFuncSetAttribute(k_product<kStats, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = std::max(1, sms / 2);
     }
@@ -562,8 +666,8 @@ int tc_pairs() {
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, c.x, c.pitch, c.n, c.pitch, kHalf, f16) ||
-      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kHalf, f16))
+  if (!make_map(&ma, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16))
     return false;
   Args a = base_args(c);
   a.part = part;
@@ -573,12 +677,12 @@ bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   return launch<kStats>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
 }
 
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float* lse, const Upstream& up, void* p,
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
               int64_t p_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, c.x, c.pitch, c.n, c.pitch, kHalf, f16) ||
-      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kHalf, f16))
+  if (!make_map(&ma, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16))
     return false;
   Args a = base_args(c);
   a.v0 = v0;
@@ -596,8 +700,8 @@ bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
            float* dx, int64_t dx_part, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, p, p_pitch, c.n_pad, p_pitch, kHalf, f16) ||
-      !make_map(&mb, c.w, c.pitch, c.vocab, c.w_pitch, kBK, f16))
+  if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kBK, f16))
     return false;
   Args a = base_args(c);
   a.v0 = v0;
@@ -617,15 +721,16 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
            cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, p, p_pitch, c.n_pad, p_pitch, kBK, f16) ||
-      !make_map(&mb, c.x, c.pitch, c.n_pad, c.pitch, kBK, f16))
+  if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kBK, f16) ||
+      !make_map(&mb, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kBK, f16))
     return false;
   Args a = base_args(c);
   a.v0 = v0;
   a.vn = vn;
   a.up = up;
   a.dw = dw;
-  a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0;
+  a.b_plane = (int)c.n_pad;
+  a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0;
   a.tiles_n = (c.pitch + kTile - 1) / kTile;
   a.idesc = idesc_of(c, true, true);
   return launch<kDw>("loss_dw_tc5", ma, mb, a, (int64_t)a.tiles_n * ((vn + kTile - 1) / kTile), st);

@@ -367,7 +367,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
     """Softmax cross entropy of the logits ``hidden @ weight.T`` against ``labels``, in fp32.
 
     hidden [..., D] and weight [V, D] of one dtype (float32, bfloat16, float16), labels [...]
-    integers; D up to 65536, V up to 2^30, 2^22 tokens.  The logits are formed tile by tile and
+    integers; D up to 65536, V up to 2^29, 2^22 tokens.  The logits are formed tile by tile and
     never stored; the backward forms them again.  Tokens labelled ``ignore_index`` have no loss
     and zero gradients, cost nothing and are not read.  A label outside [0, V) makes its loss,
     and every gradient it reaches, NaN.
@@ -393,8 +393,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
         raise ValueError(f"labels is on {labels.device}, the other tensors are on {dev}")
     if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
         raise ValueError(f"labels must be integers, not {labels.dtype}")
-    if not 1 <= hidden.shape[-1] <= 65536 or not 1 <= weight.shape[0] <= 1 << 30:
-        raise ValueError(f"1 to 65536 channels and 1 to 2^30 vocabulary entries, not {weight.shape[1]} "
+    if not 1 <= hidden.shape[-1] <= 65536 or not 1 <= weight.shape[0] <= 1 << 29:
+        raise ValueError(f"1 to 65536 channels and 1 to 2^29 vocabulary entries, not {weight.shape[1]} "
                          f"and {weight.shape[0]}")
     if labels.numel() > 1 << 22:
         raise ValueError(f"at most 2^22 tokens in a call, not {labels.numel()}")

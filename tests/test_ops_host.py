@@ -92,7 +92,7 @@ def test_loss_refuses_cpu_tensors():
 @pytest.mark.parametrize("change,code,word", [
     (dict(dtype=3), 1, "dtype"), (dict(reduction=3), 1, "reduction"), (dict(width=0), 1, "width"),
     (dict(vocab=0), 1, "vocab"), (dict(outer=-1), 1, "outer"), (dict(weight_stride=7), 1, "overlap"),
-    (dict(width=65537, weight_stride=65537), 2, "channels"), (dict(vocab=(1 << 30) + 1), 2, "vocabulary"),
+    (dict(width=65537, weight_stride=65537), 2, "channels"), (dict(vocab=(1 << 29) + 1), 2, "vocabulary"),
     (dict(outer=1 << 21), 2, "rows"), (dict(weight=None), 1, "NULL"),
 ])
 def test_loss_entry_points_refuse_bad_arguments(change, code, word):
