@@ -35,11 +35,12 @@ struct Pack {
   int64_t ignore, vocab;
   const int* count;        // labelled rows of each run before, or NULL: counted here
   int runs;
-  int *info, *row, *label, *pos;  // info: [packed rows, counter of k_join]
+  int *info, *row, *label, *pos;  // info: see Call::n_rows
   int64_t so, si, inner;   // the caller's rows
   int width, pitch;
   int64_t plane;
   bool vec;
+  Split split;
 };
 
 // A value as it goes to the tensor cores: itself, or for fp32 three bf16 parts of 8 bits each, in
@@ -122,7 +123,12 @@ __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, typena
   for (int k = 0; k < 8; ++k) before += part[k];
   if ((int)blockIdx.x >= p.runs) {  // `before` is the number of packed rows
     const int extra = blockIdx.x - p.runs;
-    if (extra == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.info[0] = before, p.info[1] = 0;
+    if (extra == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+      p.info[0] = before;
+      p.info[1] = 0;
+      p.info[2] = p.split.parts ? p.split.parts : parts_of(p.split, (before + kTile - 1) / kTile, &p.info[3]);
+      if (p.split.parts) p.info[3] = p.split.k_part;
+    }
     const int end = (before + 63) / 64 * 64;
     for (int j = before + extra * kRun + blockIdx.y; j < min(end, before + (extra + 1) * kRun); j += 4)
       for (int c = threadIdx.x; c < p.pitch; c += 256) put(dst + (int64_t)j * p.pitch + c, p.plane, T(0.f));
@@ -255,10 +261,10 @@ __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Ca
 // dx of the caller's rows: the parts added in order, scaled, rounded; zero for rows without a
 // label.  kV channels a thread at a time.
 template <typename T, int kV>
-__global__ void k_finish(const float* part, int parts, int64_t part_stride, const Call c, const int* pos,
+__global__ void k_finish(const float* part, int64_t part_stride, const Call c, const int* pos,
                          const Upstream up, float unit, T* dx) {
   const int64_t i = blockIdx.x;
-  const int j = pos[i];
+  const int j = pos[i], parts = c.n_rows[2];
   const float s = up.scale(*c.n_rows) * unit;
   T* out = dx + i * c.width;
   const float* p = part + (int64_t)j * c.pitch;
@@ -299,12 +305,11 @@ struct Plan {
   int es;                  // bytes of an element of the caller's tensors
   int parts_v;             // (max, sum) pairs of a row
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
-  int parts;               // parts of dx
-  int64_t k_part;          // vocabulary entries of a part
+  Split split;             // of the reduction of dx
   // saved
-  int64_t s_row, s_label, s_pos, s_lse, s_x, s_bytes;
+  int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
   // scratch
-  int64_t w, count, part, z_label, loss, fwd_bytes;
+  int64_t count, part, z_label, loss, fwd_bytes;
   int64_t p, dxp, r, scale, bwd_bytes;
 };
 
@@ -336,7 +341,8 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   const int at_once = tc_pairs();
   const int64_t tiles_v = up(c.vocab, kTile) / kTile, tiles_m = c.n_pad / kTile;
   const int64_t tiles_d = (c.pitch + kTile - 1) / kTile;
-  p->parts_v = (int)(f32 ? 2 * tiles_v : tiles_v);
+  c.few = c.n <= 32 ? 32 : c.n <= 128 ? 128 : 0;
+  p->parts_v = tc_stats_parts(c);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
   // come out in fewer turns of the whole GPU (the pieces' turns added up).
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * 2 * c.planes) / kTile);
@@ -348,20 +354,19 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   for (int64_t t = best; t >= 1 && t >= std::min(tiles_v, most) / 2; --t)
     if (turns_of(t) < turns) turns = turns_of(t), best = t;
   p->piece = best * kTile;
-  // dx: the reduction is cut into parts of at least 512 entries where that fills the GPU's turns
-  // better.  A turn over a piece goes at about 1.4 PFLOP/s; each part is written and read again in
-  // fp32, at about 5 TB/s.
-  const int64_t tiles_x = tiles_d * tiles_m;
-  const double turn = 2.0 * kTile * kTile * at_once * (double)p->piece * (f32 ? 6 : 1) / 1.4e15;
-  const double pass = (double)c.n_pad * c.pitch * 8 / 5e12;
-  p->parts = 1;
-  double cost = 1e30;
-  for (int n = 1; n == 1 || (n <= 2 * at_once && n <= p->piece / 512); ++n) {
-    const double now = (double)((tiles_x * n + at_once - 1) / at_once) / n * turn + n * pass;
-    if (now < cost) cost = now, p->parts = n;
-  }
-  p->k_part = up((p->piece + p->parts - 1) / p->parts, 64);
-  p->parts = (int)((p->piece + p->k_part - 1) / p->k_part);
+  // dx: parts of at least 512 entries, and of 256 MB in all beside the first.  A turn over a piece
+  // goes at about 1.4 PFLOP/s, the parts in fp32 at about 5 TB/s.
+  Split& d = p->split;
+  d.tiles_d = (int)tiles_d;
+  d.at_once = at_once;
+  d.blocks = (int)(p->piece / 64);
+  const int64_t one = c.n_pad * c.pitch * 4;
+  d.most = (int)std::max<int64_t>(1, std::min<int64_t>({tiles_m == 1 ? 2 * at_once : 16, p->piece / 512,
+                                                        1 + (int64_t(1) << 28) / one}));
+  d.turn = (float)(2.0 * kTile * kTile * at_once * (double)p->piece * (f32 ? 6 : 1) / 1.4e15);
+  d.pass = (float)((double)kTile * c.pitch * 8 / 5e12);
+  d.parts = d.k_part = 0;
+  if (tiles_m == 1) d.parts = parts_of(d, 1, &d.k_part);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -374,18 +379,17 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->s_pos = take(4 * c.n);
   p->s_lse = take(8 * c.n);
   p->s_x = take(c.planes * c.n_pad * c.pitch * 2);
+  p->s_w = take(p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0);
   p->s_bytes = at;
   at = 0;
-  p->w = take(p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0);
-  const int64_t common = at;
-  p->count = take(4 * up(c.n, kRun) / kRun);
+    p->count = take(4 * up(c.n, kRun) / kRun);
   p->part = take((int64_t)p->parts_v * c.n_pad * 8);
   p->z_label = take(4 * c.n);
   p->loss = take(4 * c.n);
   p->fwd_bytes = at;
-  at = common;
+  at = 0;
   p->p = take(c.planes * c.n_pad * p->piece * 2);
-  p->dxp = take((int64_t)p->parts * c.n_pad * c.pitch * 4);
+  p->dxp = take((int64_t)p->split.most * c.n_pad * c.pitch * 4);
   p->r = take(4 * c.n);
   p->scale = take(4);
   p->bwd_bytes = at;
@@ -411,6 +415,7 @@ void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaS
   k.inner = std::max<int64_t>(a->inner, 1);
   k.width = c.width;
   k.pitch = c.pitch;
+  k.split = p.split;
   k.plane = c.n_pad * c.pitch;
   k.vec = a->width % 8 == 0 && k.so % 8 == 0 && k.si % 8 == 0 && (reinterpret_cast<uintptr_t>(a->hidden) & 15) == 0;
   if (c.n > kCountDirectly) {
@@ -425,14 +430,14 @@ void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaS
 }
 
 template <typename T>
-void copy_weight(const GpaLossArgs* a, const Plan& p, char* scratch, cudaStream_t st) {
+void copy_weight(const GpaLossArgs* a, const Plan& p, char* saved, cudaStream_t st) {
   const Call& c = p.c;
   const int64_t rows = c.planes > 1 ? up(c.vocab, kTile) : c.vocab;
   const bool vec = c.width % 8 == 0 && a->weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a->weight) & 15) == 0;
   Launch scope("loss_weight", st);
   k_weight<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
       static_cast<const T*>(a->weight), a->weight_stride, c.vocab, rows, c.width, c.pitch, rows * c.pitch, vec,
-      reinterpret_cast<typename Part<T>::type*>(scratch + p.w));
+      reinterpret_cast<typename Part<T>::type*>(saved + p.s_w));
 }
 
 template <typename T>
@@ -443,18 +448,18 @@ void finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, con
   const float unit = 1.f / tc_p_scale(c.dtype);
   Launch scope("loss_finish", st);
   if (c.width % kV == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0)
-    k_finish<T, kV><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, stride, c, pos, up, unit, static_cast<T*>(dx));
+    k_finish<T, kV><<<(unsigned)c.n, 128, 0, st>>>(dxp, stride, c, pos, up, unit, static_cast<T*>(dx));
   else
-    k_finish<T, 1><<<(unsigned)c.n, 128, 0, st>>>(dxp, p.parts, stride, c, pos, up, unit, static_cast<T*>(dx));
+    k_finish<T, 1><<<(unsigned)c.n, 128, 0, st>>>(dxp, stride, c, pos, up, unit, static_cast<T*>(dx));
 }
 
-void bind(Plan* p, const void* saved, char* scratch) {
+void bind(Plan* p, const void* saved) {
   const char* s = static_cast<const char*>(saved);
   p->c.n_rows = reinterpret_cast<const int*>(s);
   p->c.row = reinterpret_cast<const int*>(s + p->s_row);
   p->c.label = reinterpret_cast<const int*>(s + p->s_label);
   p->c.x = s + p->s_x;
-  if (p->copy_w) p->c.w = scratch + p->w;
+  if (p->copy_w) p->c.w = s + p->s_w;
 }
 
 #define BY_TYPE(DT, CALL)                                  \
@@ -508,14 +513,14 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
   }
   char* sv = static_cast<char*>(saved);
   char* sc = static_cast<char*>(scratch);
-  bind(&p, saved, sc);
+  bind(&p, saved);
   float* each = none ? loss : nullptr;
   float* z_label = reinterpret_cast<float*>(sc + p.z_label);
   float2* part = reinterpret_cast<float2*>(sc + p.part);
   BY_TYPE(a->dtype, pack<T>(a, p, sv, sc, st));
   OK_OR("loss_pack launch failed");
   if (p.copy_w && c.n) {
-    BY_TYPE(a->dtype, copy_weight<T>(a, p, sc, st));
+    BY_TYPE(a->dtype, copy_weight<T>(a, p, sv, st));
     OK_OR("loss_weight launch failed");
   }
   if (c.n && !tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
@@ -556,14 +561,10 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   }
   const char* sv = static_cast<const char*>(saved);
   char* sc = static_cast<char*>(scratch);
-  bind(&p, saved, sc);
+  bind(&p, saved);
   const float2* lse = reinterpret_cast<const float2*>(sv + p.s_lse);
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
-  if (p.copy_w) {
-    BY_TYPE(a->dtype, copy_weight<T>(a, p, sc, st));
-    OK_OR("loss_weight launch failed");
-  }
   const bool none = a->reduction == GPA_B200_LOSS_NONE;
   Upstream up = {none ? dloss : nullptr, true, none ? nullptr : dloss, a->reduction == GPA_B200_LOSS_MEAN};
   if (none && a->dtype == GPA_B200_F16) {
@@ -578,7 +579,7 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
     if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
-    if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.parts, (int)(p.k_part / 64), v0 > 0, dxp, part_stride, st))
+    if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.split.most, v0 > 0, dxp, part_stride, st))
       FAIL("loss_dx_tc5 launch failed");
     if (dweight && !tc_dw(c, pr, p.piece, v0, vn, up, dweight, st)) FAIL("loss_dw_tc5 launch failed");
   }

@@ -18,13 +18,14 @@ struct Call {
   int dtype;
   int planes;         // parts of each value: 1, or the 3 bf16 parts of fp32 (x, W and P in planes of n_pad rows,
                       // of vocab rounded up to tiles, and of n_pad rows)
-  const int* n_rows;  // device: packed rows
+  const int* n_rows;  // device: packed rows, counter of k_join, parts of dx, reduction blocks of a part
   const int* label;   // [n] label of a packed row, -1 when outside the vocabulary
   const int* row;     // [n] the caller's row of a packed row
   const void* x;      // packed rows [n_pad][pitch], zero behind the last one up to a multiple of 64
   const void* w;      // weight [vocab][w_pitch], 16-bit elements
   int64_t w_pitch;
   int64_t n_pad;      // n rounded up to tiles
+  int few;            // 32 or 128: at least n, and z and dx are formed transposed; 0: more rows
 };
 
 // The gradient of a packed row's loss, as s r with |r| <= 1 where fp16 needs it:
@@ -46,14 +47,36 @@ struct Upstream {
 
 __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
+// How the reduction of dx is cut: into the parts whose turns of the whole GPU, and passes over dx in
+// fp32 to add them up, take least.  Decided on the device, where the number of packed rows is
+// known; n_rows[2] holds the parts and n_rows[3] the reduction blocks (of 64) of each.
+struct Split {
+  int tiles_d, at_once;  // tiles across dx, tiles that run at a time
+  int blocks;            // reduction blocks of a piece
+  int most;              // parts that the buffer holds
+  float turn, pass;      // seconds of a turn over a piece, and of writing and reading one part's tile row
+  int parts, k_part;     // decided on the host where one row of tiles is all there can be (parts > 0)
+};
+__host__ __device__ inline int parts_of(const Split& s, int tiles_m, int* k_part) {
+  int parts = 1;
+  float cost = 3e38f;
+  for (int n = 1; n <= s.most; ++n) {
+    const float now = (float)((s.tiles_d * tiles_m * n + s.at_once - 1) / s.at_once) / n * s.turn + n * tiles_m * s.pass;
+    if (now < cost) cost = now, parts = n;
+  }
+  *k_part = (s.blocks + parts - 1) / parts;
+  return (s.blocks + *k_part - 1) / *k_part;
+}
+
 // The products, on tensor cores (vocab_loss_tc5.cu); false when a launch failed.
 // They tile by kTile x kTile and pair up the SMs: tc_pairs() tiles run at a time.
 int tc_pairs();
+int tc_stats_parts(const Call& c);  // (max, sum) pairs of a row that tc_stats leaves
 float tc_p_scale(int dtype);  // P is stored times this
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st);
 bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
               int64_t p_pitch, cudaStream_t st);
-bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
+bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int most_parts, bool add,
            float* dx, int64_t dx_part, cudaStream_t st);
 bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
            cudaStream_t st);

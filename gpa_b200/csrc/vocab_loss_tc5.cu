@@ -14,6 +14,11 @@
 //   warp 0: copies     warp 1: products (first CTA of the pair)     warp 2: tensor memory
 //   warps 4-7: epilogue, a thread for each row of the tile
 //
+// Up to 128 rows of x would leave most of such a tile empty, and what counts then is how fast W
+// comes by.  There z and dx are formed the other way round (kStatsT, kProbsT, kDxT): 256 vocabulary
+// entries or channels by the 32 or 128 rows, so that a step of the products costs an eighth or
+// half as much and more copies of W are on their way at a time.
+//
 // fp32 inputs come as three bf16 parts, x = x0 + x1 + x2 (24 bits), in planes one behind the
 // other, and each product is the six of them that matter, the smallest first: x2 y0, x1 y1, x0 y2,
 // x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
@@ -39,17 +44,26 @@ __device__ int g_loss_status = 0;
 namespace vloss {
 namespace {
 
-constexpr int kStages = 6, kBK = 64;
-constexpr int kHalf = 128;                        // rows of an operand that one CTA holds
-constexpr uint32_t kOperand = kHalf * kBK * 2;    // bytes of one operand in one stage
-constexpr uint32_t kStage = 2 * kOperand;
-constexpr size_t kSmem = kStages * kStage + 1024 + 256;  // operands on 1024 bytes, barriers
+constexpr int kBK = 64;
+constexpr int kHalf = 128;                        // rows of A that one CTA holds
+constexpr uint32_t kOperand = kHalf * kBK * 2;    // their bytes in one stage
+// Shared memory of a pair of tiles with BN columns: the stages, barriers, and for the transposed
+// products a table of the rows and the square of one chunk of columns for either half.
+constexpr int kSquare = 129;                      // pitch of its columns: no bank conflicts either way
+template <int BN>
+struct Smem {
+  static constexpr int kStages = BN == 256 ? 6 : BN == 128 ? 7 : 9;
+  static constexpr uint32_t kColumns = BN / 2 * kBK * 2;
+  static constexpr uint32_t kStage = kOperand + kColumns;
+  static constexpr uint32_t kBars = kStages * kStage, kTable = kBars + 256, kSquares = kTable + BN * 16;
+  static constexpr size_t kBytes = 1024 + (BN == 256 ? kTable : kSquares + 2 * 32 * kSquare * 4);
+};
 constexpr int kSegment = 8;  // reduction blocks between two additions in registers (fp32)
-constexpr int threads_of(bool f32) { return f32 ? 384 : 256; }
+__host__ __device__ constexpr int threads_of(bool f32) { return f32 ? 384 : 256; }
 constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum Mode { kStats, kProbs, kDx, kDw };
+enum Mode { kStats, kProbs, kDx, kDw, kStatsT, kProbsT, kDxT };
 
 struct Args {
   Call c;
@@ -69,7 +83,6 @@ struct Args {
   // kDx
   float* dx;
   int64_t dx_part;
-  int parts, k_part;
   bool add;
   // kDw
   void* dw;
@@ -203,19 +216,25 @@ struct Tile {
 
 template <Mode M>
 struct Walk {
-  int mt, nt, total, n_rows, k_blocks;
+  int mt, nt, total, n_rows, k_blocks, k_part;
   const Args& a;
   GPA_DEV Walk(const Args& args) : a(args) {
     n_rows = *args.c.n_rows;
     nt = args.tiles_n;
-    if (M == kDw) {
+    if (M == kStatsT || M == kProbsT || M == kDxT) {
+      mt = n_rows == 0 ? 0 : (int)(((M == kDxT ? args.c.pitch : args.vn) + kTile - 1) / kTile);
+      nt = 1;
+      k_blocks = args.k_blocks;
+    } else if (M == kDw) {
       mt = (int)((args.vn + kTile - 1) / kTile);
       k_blocks = (n_rows + kBK - 1) / kBK;
     } else {
       mt = (n_rows + kTile - 1) / kTile;
       k_blocks = args.k_blocks;
     }
-    total = mt * nt * (M == kDx ? args.parts : 1);
+    constexpr bool kParts = M == kDx || M == kDxT;
+    total = mt * nt * (kParts ? args.c.n_rows[2] : 1);
+    k_part = kParts ? args.c.n_rows[3] : 0;
   }
   GPA_DEV Tile at(int t) const {
     Tile x;
@@ -232,35 +251,36 @@ struct Walk {
     } else {
       x.n = t % nt;
       x.m = t / nt;
-      if (M == kDx) {
+      if (M == kDx || M == kDxT) {
         x.part = x.m / mt;
         x.m -= x.part * mt;
-        x.k0 = x.part * a.k_part;
-        x.k1 = x.k0 + a.k_part < k_blocks ? x.k0 + a.k_part : k_blocks;
+        x.k0 = x.part * k_part;
+        x.k1 = x.k0 + k_part < k_blocks ? x.k0 + k_part : k_blocks;
       }
     }
     return x;
   }
 };
 
-// What a thread holds of its row when the tile is done: 256 columns in tensor memory (16-bit
-// inputs), or the half of them that it has added up in registers (fp32).
-template <bool F32>
+// What a thread holds of its row of the tile when it is done: the columns in tensor memory (16-bit
+// inputs), or the CW of them that it has added up in registers (fp32: half the tile's).
+template <bool F32, int CW>
 struct Row {
   uint32_t tmem;
   GPA_DEV void get(int chunk, float (&v)[32]) const { ld32(tc5::tmem_at(tmem, 32 * chunk), v); }
 };
-template <>
-struct Row<true> {
-  float acc[128];
-  GPA_DEV void get(int chunk, float (&v)[32]) const {
+template <int CW>
+struct Row<true, CW> {
+  float acc[CW];
+  template <int CH>
+  GPA_DEV void get(int chunk, float (&v)[CH]) const {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = acc[32 * chunk + i];
+    for (int i = 0; i < CH; ++i) v[i] = acc[CH * chunk + i];
   }
 };
 
 template <Mode M, bool F32>
-GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32>& held, int rank, bool empty) {
+GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 128>& held, int rank, bool empty) {
   constexpr int kChunks = F32 ? 4 : 8, kUnroll = F32 ? 4 : 1;
   const int half = F32 ? (threadIdx.x - 128) >> 7 : 0;  // of the tile's columns
   const int in_tile = rank * kHalf + (threadIdx.x & 127);
@@ -405,20 +425,161 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32>& 
   }
 }
 
+// ---- transposed tiles: a thread's row is a vocabulary entry (or a channel), its columns are rows of x
+template <bool F32, int BN>
+struct Cols {
+  static constexpr int kCw = F32 ? BN / 2 : BN;        // columns of a thread
+  static constexpr int kCh = kCw < 32 ? kCw : 32;      // of a chunk
+  static constexpr int kChunks = kCw / kCh;
+  static constexpr int kLanes = 128 / kCh;             // threads that share a column of the square
+};
+
+GPA_DEV void half_sync(int half) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+// whether every warp of the half got its accumulator (they all wait for it, each for a limited time)
+GPA_DEV bool half_all(int half, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.b32 p, %1, 0;\nbarrier.cta.red.and.pred q, %2, 128, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"((uint32_t)ok), "r"(1 + half)
+      : "memory");
+  return r != 0;
+}
+
+// (max, sum of exp) of the columns over every tile of the CTA.  A chunk of columns goes through
+// shared memory, so that a thread meets kCh entries of one column at a time.
+template <bool F32, int BN>
+struct Stats {
+  using C = Cols<F32, BN>;
+  float big[C::kChunks], sum[C::kChunks];
+  int64_t label[C::kChunks];
+  int half, col, lane;  // this thread's column of a chunk, and its share of the rows
+
+  GPA_DEV void start(const Args& a, int n_rows) {
+    half = F32 ? (threadIdx.x - 128) >> 7 : 0;
+    const int i = threadIdx.x & 127;
+    col = i % C::kCh;
+    lane = i / C::kCh;
+#pragma unroll
+    for (int k = 0; k < C::kChunks; ++k) {
+      const int j = column(k);
+      big[k] = -INFINITY, sum[k] = 0.f;
+      label[k] = j < n_rows ? a.c.label[j] : -1;
+    }
+  }
+  GPA_DEV int column(int k) const { return half * C::kCw + k * C::kCh + col; }
+  GPA_DEV void tile(const Args& a, const Tile& t, const Row<F32, C::kCw>& held, int rank, float* square) {
+    const int r = threadIdx.x & 127;
+    const int64_t base = (int64_t)t.m * kTile + rank * kHalf;
+    const bool in = base + r < a.vn;
+#pragma unroll
+    for (int k = 0; k < C::kChunks; ++k) {
+      float v[C::kCh];
+      held.get(k, v);
+#pragma unroll
+      for (int i = 0; i < C::kCh; ++i) square[i * kSquare + r] = in ? v[i] : -INFINITY;
+      half_sync(half);
+      const float* s = square + col * kSquare + lane * C::kCh;
+      float m = big[k];
+#pragma unroll
+      for (int i = 0; i < C::kCh; ++i) {
+        v[i] = s[i];
+        m = fmaxf(m, v[i]);
+      }
+      const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
+      float more = 0.f;
+#pragma unroll
+      for (int i = 0; i < C::kCh; ++i) more += F32 ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
+      sum[k] = fmaf(sum[k], F32 ? expf(big[k] - safe) : ex2(fmaf(big[k], kLog2e, -off)), more);
+      big[k] = m;
+      const int64_t y = label[k] - base - lane * C::kCh;
+      if (label[k] >= 0 && y >= 0 && y < C::kCh) a.z_label[column(k)] = s[y];
+      half_sync(half);
+    }
+  }
+  GPA_DEV void finish(const Args& a, int n_rows) const {
+#pragma unroll
+    for (int k = 0; k < C::kChunks; ++k)
+      if (column(k) < n_rows)
+        a.part[((int64_t)blockIdx.x * C::kLanes + lane) * a.c.n_pad + column(k)] = make_float2(big[k], sum[k]);
+  }
+};
+
+// {max (times log2 e for 16-bit inputs), factor of the exp, r, label within the piece} of row j of x
+template <bool F32>
+GPA_DEV float4 row_of(const Args& a, int j, int n_rows) {
+  if (j >= n_rows) return make_float4(0.f, 0.f, 0.f, __int_as_float(-2));  // no row
+  const float2 l = a.lse[j];
+  const float r = a.up.r(a.c, j) * a.p_scale;
+  const int64_t y = (int64_t)a.c.label[j] - a.v0;
+  return make_float4(F32 ? l.x : l.x * kLog2e, l.y * r, r, __int_as_float(y >= 0 && y < a.vn ? (int)y : -1));
+}
+
+template <Mode M, bool F32, int BN>
+GPA_DEV void epilogue_t(const Args& a, const Tile& t, int n_rows, const Row<F32, Cols<F32, BN>::kCw>& held, int rank,
+                        const float4* table) {
+  using C = Cols<F32, BN>;
+  const int half = F32 ? (threadIdx.x - 128) >> 7 : 0;
+  const int64_t at = (int64_t)t.m * kTile + rank * kHalf + (threadIdx.x & 127);
+#pragma unroll
+  for (int k = 0; k < C::kChunks; ++k) {
+    float v[C::kCh];
+    held.get(k, v);
+    const int j0 = half * C::kCw + k * C::kCh;
+    if (M == kProbsT) {
+      uint16_t* out = static_cast<uint16_t*>(a.p) + at;
+      const int64_t plane = a.c.n_pad * a.p_pitch;
+#pragma unroll
+      for (int i = 0; i < C::kCh; ++i) {
+        const float4 x = table[j0 + i];
+        const int y = __float_as_int(x.w);
+        float p = (F32 ? expf(v[i] - x.x) : ex2(fmaf(v[i], kLog2e, -x.x))) * x.y - (y == at ? x.z : 0.f);
+        if (y == -2 || at >= a.vn) p = 0.f;
+        uint16_t* o = out + (j0 + i) * a.p_pitch;
+#pragma unroll
+        for (int q = 0; q < (F32 ? 3 : 1); ++q) {
+          const uint32_t b = pack2(p, 0.f, !F32 && a.f16) & 0xffffu;
+          o[q * plane] = (uint16_t)b;
+          if (F32) p -= __uint_as_float(b << 16);
+        }
+      }
+      if (BN < kBK) {  // dW reduces over whole blocks of rows
+#pragma unroll
+        for (int i = 0; i < C::kCh; ++i)
+#pragma unroll
+          for (int q = 0; q < (F32 ? 3 : 1); ++q) out[(j0 + BN + i) * a.p_pitch + q * plane] = 0;
+      }
+    } else if (at < a.c.pitch) {
+      float* out = a.dx + t.part * a.dx_part + at;
+#pragma unroll
+      for (int i = 0; i < C::kCh; ++i) {
+        if (j0 + i >= n_rows) continue;
+        float* o = out + (int64_t)(j0 + i) * a.c.pitch;
+        *o = a.add ? *o + v[i] : v[i];
+      }
+    }
+  }
+}
+
 // Planes of the products of a pair of operands, the smallest first.
 GPA_DEV int plane_a(int q) { return q == 0 ? 2 : q == 1 || q == 3 ? 1 : 0; }
 GPA_DEV int plane_b(int q) { return q == 2 ? 2 : q == 1 || q == 4 ? 1 : 0; }
 
-template <Mode M, bool F32>
+template <Mode M, bool F32, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
     k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
-  constexpr bool kAMn = M == kDw, kBMn = M == kDx || M == kDw;
+  constexpr bool kT = M == kStatsT || M == kProbsT || M == kDxT;
+  constexpr bool kAMn = M == kDw || M == kDxT, kBMn = M == kDx || M == kDw;
   constexpr int kProducts = F32 ? 6 : 1;
+  using S = Smem<BN>;
+  constexpr int kStages = S::kStages;
+  constexpr uint32_t kStage = S::kStage;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + kStages * kStage);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
   uint64_t *full = bars, *empty = bars + kStages, *acc_full = bars + 2 * kStages, *acc_empty = acc_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float4* table = reinterpret_cast<float4*>(sm + S::kTable);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cta_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
@@ -432,6 +593,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
     }
     tc5::mbar_fence_init();
   }
+  if (M == kProbsT)
+    for (int j = threadIdx.x; j < BN; j += threads_of(F32)) table[j] = row_of<F32>(a, j, *a.c.n_rows);
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc5::saddr(slot))
                  : "memory");
@@ -454,7 +617,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
       uint32_t it = 0;
       for (int t = pair; t < walk.total && ok; t += pairs) {
         const Tile x = walk.at(t);
-        const int ra = x.m * kTile + rank * kHalf, rb = x.n * kTile + rank * kHalf;
+        const int ra = x.m * kTile + rank * kHalf, rb = x.n * BN + rank * (BN / 2);
+        // the piece's vocabulary entries are rows of W, whichever operand it is
+        const int va = kT ? (int)a.v0 : 0, vb = M == kStats || M == kProbs || M == kDx ? (int)a.v0 : 0;
         for (int k0 = x.k0; k0 < x.k1 && ok; k0 = segment_end(k0, x.k1)) {
           const int blocks = segment_end(k0, x.k1) - k0;
           for (int j = 0; j < blocks * kProducts; ++j, ++it) {
@@ -465,19 +630,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
             unsigned char* sb = sa + kOperand;
             const uint32_t bar = in_first(&full[s]);
             if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
-            const int kk = k * kBK, pa = F32 ? plane_a(q) * a.a_plane : 0, pb = F32 ? plane_b(q) * a.b_plane : 0;
+            const int kk = k * kBK, pa = va + (F32 ? plane_a(q) * a.a_plane : 0);
+            const int pb = vb + (F32 ? plane_b(q) * a.b_plane : 0);
             if (kAMn) {
               tma_load(sa, &map_a, ra, pa + kk, bar);
               tma_load(sa + kOperand / 2, &map_a, ra + 64, pa + kk, bar);
             } else {
               tma_load(sa, &map_a, kk, pa + ra, bar);
             }
-            if (kBMn) {  // in dx the reduction runs over the piece's vocabulary entries
-              const int kb = pb + (M == kDx ? (int)a.v0 : 0) + kk;
-              tma_load(sb, &map_b, rb, kb, bar);
-              tma_load(sb + kOperand / 2, &map_b, rb + 64, kb, bar);
+            if (kBMn) {
+              tma_load(sb, &map_b, rb, pb + kk, bar);
+              tma_load(sb + kOperand / 2, &map_b, rb + 64, pb + kk, bar);
             } else {
-              tma_load(sb, &map_b, kk, pb + (int)a.v0 + rb, bar);
+              tma_load(sb, &map_b, kk, pb + rb, bar);
             }
           }
         }
@@ -512,35 +677,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
       }
     }
   } else if (warp >= 4) {
+    using C = Cols<F32, BN>;
+    constexpr int kCw = F32 ? BN / 2 : 128;  // columns that a thread adds up
     uint32_t count = 0;
     const int half = (warp - 4) >> 2;
+    Stats<F32, BN> stats;
+    float* square = reinterpret_cast<float*>(sm + S::kSquares) + half * 32 * kSquare;
+    if constexpr (M == kStatsT) stats.start(a, walk.n_rows);
     for (int t = pair; t < walk.total && ok; t += pairs) {
       const Tile x = walk.at(t);
-      Row<F32> held;
-      const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (kDx)
+      Row<F32, kT ? C::kCw : kCw> held;
+      const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (dx)
       if (none && M != kDw) continue;
+      auto done = [&](bool empty) {
+        if constexpr (M == kStatsT) stats.tile(a, x, held, rank, square);
+        else if constexpr (kT) epilogue_t<M, F32, BN>(a, x, walk.n_rows, held, rank, table);
+        else epilogue<M, F32>(a, x, walk.n_rows, held, rank, empty);
+      };
       for (int k0 = x.k0; k0 < x.k1; k0 = segment_end(k0, x.k1), ++count) {
         const uint32_t buf = count & 1, use = count >> 1;
-        if (!(ok = __all_sync(0xffffffffu, tc5::mbar_wait(&acc_full[buf], use & 1)))) break;
+        ok = __all_sync(0xffffffffu, tc5::mbar_wait(&acc_full[buf], use & 1));
+        if (M == kStatsT) ok = half_all(half, ok);
+        if (!ok) break;
         tc5::fence_after_sync();
         if constexpr (F32) {
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) {
+          for (int c = 0; c < kCw; c += 16) {
             float v[16];
-            ld16(tc5::tmem_at(tmem, buf * kTile + half * 128 + c), v);
+            ld16(tc5::tmem_at(tmem, buf * kTile + half * kCw + c), v);
 #pragma unroll
             for (int i = 0; i < 16; ++i) held.acc[c + i] = k0 == x.k0 ? v[i] : held.acc[c + i] + v[i];
           }
         } else {
           held.tmem = tmem + buf * kTile;
-          epilogue<M, F32>(a, x, walk.n_rows, held, rank, false);
+          done(false);
         }
         tc5::fence_before_sync();
         __syncwarp();
         if (lane == 0) arrive_first(in_first(&acc_empty[buf]));
       }
-      if (ok && (F32 || none)) epilogue<M, F32>(a, x, walk.n_rows, held, rank, none);
+      if (ok && (F32 || none)) done(none);
     }
+    if constexpr (M == kStatsT) stats.finish(a, walk.n_rows);
   }
   if (!ok) g_loss_status = GPA_B200_DEVICE_TIMEOUT;
   tc5::fence_before_sync();
@@ -586,8 +764,8 @@ bool make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, in
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-uint32_t idesc_of(const Call& c, bool a_mn, bool b_mn) {
-  uint32_t d = tc5::idesc_bf16(2 * kHalf, kTile, a_mn, b_mn);
+uint32_t idesc_of(const Call& c, int columns, bool a_mn, bool b_mn) {
+  uint32_t d = tc5::idesc_bf16(2 * kHalf, columns, a_mn, b_mn);
   if (c.dtype == GPA_B200_F16) d &= ~((1u << 7) | (1u << 10));  // both operands fp16
   return d;
 }
@@ -606,29 +784,46 @@ Args base_args(const Call& c) {
   return a;
 }
 
-template <Mode M, bool F32>
+template <Mode M, bool F32, int BN>
 bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
-            cudaStream_t st) {
+               cudaStream_t st) {
+  constexpr int kSmem = (int)Smem<BN>::kBytes;
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k_product<M, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_product<M, F32, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
       return false;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
   Launch scope(name, st);
-  k_product<M, F32><<<2 * pairs, threads_of(F32), kSmem, st>>>(ma, mb, a);
+  k_product<M, F32, BN><<<2 * pairs, threads_of(F32), kSmem, st>>>(ma, mb, a);
   return cudaGetLastError() == cudaSuccess;
 }
 
-template <Mode M>
+template <Mode M, int BN>
 bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
             cudaStream_t st) {
-  return a.c.dtype == GPA_B200_F32 ? launch_as<M, true>(name, ma, mb, a, tiles, st)
-                                   : launch_as<M, false>(name, ma, mb, a, tiles, st);
+  return a.c.dtype == GPA_B200_F32 ? launch_as<M, true, BN>(name, ma, mb, a, tiles, st)
+                                   : launch_as<M, false, BN>(name, ma, mb, a, tiles, st);
+}
+
+// z as W x^T for few rows: the map of W in boxes of 128 rows, of x in boxes of half the columns
+template <Mode M>
+bool launch_z_t(const char* name, Args a, cudaStream_t st) {
+  const Call& c = a.c;
+  const bool f16 = c.dtype == GPA_B200_F16;
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16) ||
+      !make_map(&mb, c.x, c.pitch, c.planes * c.n_pad, c.pitch, c.few / 2, f16))
+    return false;
+  std::swap(a.a_plane, a.b_plane);
+  a.idesc = idesc_of(c, c.few, false, false);
+  const int64_t tiles = (a.vn + kTile - 1) / kTile;
+  return c.few == 32 ? launch<M, 32>(name, ma, mb, a, tiles, st) : launch<M, 128>(name, ma, mb, a, tiles, st);
 }
 
 }  // namespace
@@ -645,6 +840,7 @@ int tc_pairs() {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2));
+    constexpr int kSmem = (int)Smem<256>::kBytes;
     cfg.blockDim = dim3(threads_of(false));
     cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute at;
@@ -653,8 +849,8 @@ int tc_pairs() {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(k_product<kStats, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaFuncSetAttribute(k_product<kStats, false, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false, 256>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = std::max(1, sms / 2);
     }
@@ -663,8 +859,22 @@ int tc_pairs() {
   return n;
 }
 
+int tc_stats_parts(const Call& c) {
+  const int64_t tiles = (c.vocab + kTile - 1) / kTile;
+  const bool f32 = c.dtype == GPA_B200_F32;
+  if (!c.few) return (int)(f32 ? 2 * tiles : tiles);
+  return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * (f32 && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes);
+}
+
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
+  if (c.few) {
+    Args a = base_args(c);
+    a.part = part;
+    a.z_label = z_label;
+    a.vn = c.vocab;
+    return launch_z_t<kStatsT>("loss_stats_tc5", a, st);
+  }
   CUtensorMap ma, mb;
   if (!make_map(&ma, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kHalf, f16) ||
       !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16))
@@ -673,17 +883,13 @@ bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   a.part = part;
   a.z_label = z_label;
   a.tiles_n = (int)((c.vocab + kTile - 1) / kTile);
-  a.idesc = idesc_of(c, false, false);
-  return launch<kStats>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
+  a.idesc = idesc_of(c, kTile, false, false);
+  return launch<kStats, 256>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
 }
 
 bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
               int64_t p_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
-  CUtensorMap ma, mb;
-  if (!make_map(&ma, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kHalf, f16) ||
-      !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16))
-    return false;
   Args a = base_args(c);
   a.v0 = v0;
   a.vn = vn;
@@ -691,16 +897,21 @@ bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Up
   a.up = up;
   a.p = p;
   a.p_pitch = p_pitch;
+  if (c.few) return launch_z_t<kProbsT>("loss_probs_tc5", a, st);
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kHalf, f16) ||
+      !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kHalf, f16))
+    return false;
   a.tiles_n = (int)((vn + kTile - 1) / kTile);
-  a.idesc = idesc_of(c, false, false);
-  return launch<kProbs>("loss_probs_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
+  a.idesc = idesc_of(c, kTile, false, false);
+  return launch<kProbs, 256>("loss_probs_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
 }
 
-bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int parts, int k_part, bool add,
+bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int most_parts, bool add,
            float* dx, int64_t dx_part, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kHalf, f16) ||
+  if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, c.few ? c.few / 2 : kHalf, f16) ||
       !make_map(&mb, c.w, c.pitch, w_rows(c), c.w_pitch, kBK, f16))
     return false;
   Args a = base_args(c);
@@ -709,12 +920,17 @@ bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   a.k_blocks = (int)((vn + kBK - 1) / kBK);
   a.dx = dx;
   a.dx_part = dx_part;
-  a.parts = parts;
-  a.k_part = k_part;
   a.add = add;
   a.tiles_n = (c.pitch + kTile - 1) / kTile;
-  a.idesc = idesc_of(c, false, true);
-  return launch<kDx>("loss_dx_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile) * parts, st);
+  if (c.few) {  // dx^T = W^T P^T: the operands change places
+    std::swap(a.a_plane, a.b_plane);
+    a.idesc = idesc_of(c, c.few, true, false);
+    const int64_t tiles = (int64_t)a.tiles_n * most_parts;
+    return c.few == 32 ? launch<kDxT, 32>("loss_dx_tc5", mb, ma, a, tiles, st)
+                       : launch<kDxT, 128>("loss_dx_tc5", mb, ma, a, tiles, st);
+  }
+  a.idesc = idesc_of(c, kTile, false, true);
+  return launch<kDx, 256>("loss_dx_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile) * most_parts, st);
 }
 
 bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
@@ -732,8 +948,8 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   a.b_plane = (int)c.n_pad;
   a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0;
   a.tiles_n = (c.pitch + kTile - 1) / kTile;
-  a.idesc = idesc_of(c, true, true);
-  return launch<kDw>("loss_dw_tc5", ma, mb, a, (int64_t)a.tiles_n * ((vn + kTile - 1) / kTile), st);
+  a.idesc = idesc_of(c, kTile, true, true);
+  return launch<kDw, 256>("loss_dw_tc5", ma, mb, a, (int64_t)a.tiles_n * ((vn + kTile - 1) / kTile), st);
 }
 
 }  // namespace vloss

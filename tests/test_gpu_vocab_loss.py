@@ -122,8 +122,15 @@ def test_sizes(dtype, lead, width, vocab):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("masked", [0.0, 0.3, 0.97])
-def test_reductions_and_masks(dtype, reduction, masked):
-    _case(11, (4, 150), 136, 900, dtype, reduction, masked)
+@pytest.mark.parametrize("lead", [(4, 150), (3, 40), (2, 13)])  # the three forms of the products
+def test_reductions_and_masks(dtype, reduction, masked, lead):
+    _case(11, lead, 136, 900, dtype, reduction, masked)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 127, 128, 129, 256, 257])
+def test_rows_round_the_tiles(dtype, rows):
+    _case(rows, (rows,), 200, 1290, dtype, "mean")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
