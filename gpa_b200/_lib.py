@@ -56,8 +56,10 @@ class GpaStateRef(ctypes.Structure):
 class GpaNormArgs(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in ("residual", "update", "gate", "weight", "post_weight",
                                         "scale")] + [
-        ("outer", c_int64), ("inner", c_int64), ("residual_stride", c_int64 * 2),
-        ("update_stride", c_int64 * 2), ("gate_stride", c_int64 * 2), ("width", c_int32),
+        # the header's stride pairs, flat: cheaper to fill
+        ("outer", c_int64), ("inner", c_int64), ("residual_outer", c_int64),
+        ("residual_inner", c_int64), ("update_outer", c_int64), ("update_inner", c_int64),
+        ("gate_outer", c_int64), ("gate_inner", c_int64), ("width", c_int32),
         ("stream_dtype", c_int32), ("update_dtype", c_int32), ("gate_dtype", c_int32),
         ("out_dtype", c_int32), ("gate_mode", c_int32), ("eps", c_float),
         ("scale_const", c_float)]
@@ -70,8 +72,8 @@ class GpaNormGrads(ctypes.Structure):
 
 class GpaLossArgs(ctypes.Structure):
     _fields_ = [("hidden", c_void_p), ("weight", c_void_p), ("labels", c_void_p),
-                ("outer", c_int64), ("inner", c_int64), ("hidden_stride", c_int64 * 2),
-                ("weight_stride", c_int64), ("vocab", c_int64), ("ignore_index", c_int64),
+                ("outer", c_int64), ("inner", c_int64), ("hidden_outer", c_int64),
+                ("hidden_inner", c_int64), ("weight_stride", c_int64), ("vocab", c_int64), ("ignore_index", c_int64),
                 ("width", c_int32), ("dtype", c_int32), ("reduction", c_int32)]
 
 

@@ -20,6 +20,7 @@
 #include "norm.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace gpa {
 namespace {
@@ -676,11 +677,15 @@ bool vec_ok(const Fwd& f) {
 // Blocks of the backward: as many as run at once, each with many rows, so that its column sums
 // are added in registers and few partial rows are left.  At most 8 blocks of 128 threads an SM.
 int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
-int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem) {
+using Known = std::atomic<int>[33];  // a kernel's blocks per SM, by warps of a block (0: not asked yet)
+int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, Known& known) {
   const uint32_t per = s.group ? s.threads / s.group : 1;
-  int at_once = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kernel, s.threads, smem) != cudaSuccess || at_once < 1)
-    at_once = 1;
+  int at_once = known[s.threads / 32].load(std::memory_order_relaxed);
+  if (!at_once) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kernel, s.threads, smem) != cudaSuccess || at_once < 1)
+      at_once = 1;
+    known[s.threads / 32].store(at_once, std::memory_order_relaxed);
+  }
   const uint32_t need = (rows + per - 1) / per;
   return (int)std::max(1u, std::min(need, (uint32_t)std::min(148 * at_once, most_blocks(s))));
 }
@@ -790,7 +795,8 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     Launch scope("norm_bwd", st);
 #define RUN(K)                                                                   \
   do {                                                                           \
-    blocks = bwd_blocks(s, f.rows, reinterpret_cast<const void*>(&K), smem);     \
+    static Known known;                                                          \
+    blocks = bwd_blocks(s, f.rows, reinterpret_cast<const void*>(&K), smem, known); \
     K<<<blocks, s.threads, smem, st>>>(b);                                       \
   } while (0)
 #define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>))

@@ -13,6 +13,7 @@ graph and have first-order gradients.  They raise ``ValueError`` for arguments t
 from __future__ import annotations
 
 import contextlib
+import math
 
 import torch
 from torch import Tensor
@@ -25,8 +26,11 @@ MAX_NORM_WIDTH = 16384
 
 
 def _on(device):
-    """`device` made current: the library sizes its workspaces and launches for that one."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """`device` as the current one: the library sizes its workspaces and launches for that."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _call(fn, device, *args):
@@ -80,43 +84,22 @@ def _check_width(width: int):
         raise ValueError(f"the norms take 1 to {MAX_NORM_WIDTH} channels, not {width}")
 
 
+_NONE = (None, 0, 0)  # no tensor, no strides
+
+
 def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, stream_dtype,
-               out_dtype, shape):
+               update_dtype, out_dtype, shape):
     """(GpaNormArgs, tensors that must outlive the launch)."""
-    a = _lib.GpaNormArgs()
-    keep = []
     width = shape[-1]
-    a.width = width
-    a.inner = shape[-2] if len(shape) > 1 else 1
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    a.outer = rows // a.inner if a.inner else 0
-    a.stream_dtype = _DTYPES[stream_dtype]
-    a.out_dtype = _DTYPES[out_dtype]
-    a.eps, a.scale_const = eps, const
-    if residual is not None:
-        t, so, si = _rows(residual)
-        keep.append(t)
-        a.residual = t.data_ptr()
-        a.residual_stride[0], a.residual_stride[1] = so, si
-    if update is not None:
-        t, so, si = _rows(update)
-        keep.append(t)
-        a.update, a.update_dtype = t.data_ptr(), _DTYPES[update.dtype]
-        a.update_stride[0], a.update_stride[1] = so, si
-    if gate is not None:
-        t, so, si = _rows(gate)
-        keep.append(t)
-        a.gate, a.gate_dtype = t.data_ptr(), _DTYPES[gate.dtype]
-        a.gate_stride[0], a.gate_stride[1] = so, si
-        a.gate_mode = 2 if gate.shape[-1] == width else 1
-    a.weight = weight.data_ptr()
-    if post_weight is not None:
-        a.post_weight = post_weight.data_ptr()
-    if scale is not None:
-        a.scale = scale.data_ptr()
-    return a, keep
+    inner = shape[-2] if len(shape) > 1 else 1
+    h, h0, h1 = _NONE if residual is None else _rows(residual)
+    y, y0, y1 = _NONE if update is None else _rows(update)
+    g, g0, g1 = _NONE if gate is None else _rows(gate)
+    a = _lib.GpaNormArgs(
+        _lib.ptr(h), _lib.ptr(y), _lib.ptr(g), weight.data_ptr(), _lib.ptr(post_weight),
+        _lib.ptr(scale), math.prod(shape[:-2]) if inner else 0, inner, h0, h1, y0, y1, g0, g1, width, _DTYPES[stream_dtype], _DTYPES[update_dtype], 0 if g is None else _DTYPES[g.dtype],
+        _DTYPES[out_dtype], 0 if g is None else 2 if g.shape[-1] == width else 1, eps, const)
+    return a, (h, y, g)
 
 
 def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
@@ -132,7 +115,8 @@ def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
 def _rms_forward(x, weight, eps, out_dtype):
     out = torch.empty(x.shape, device=x.device, dtype=out_dtype)
     if out.numel():
-        a, keep = _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, out_dtype, x.shape)
+        a, keep = _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, x.dtype, out_dtype,
+                             x.shape)
         with _on(x.device):
             _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
     return out
@@ -154,7 +138,7 @@ class _RMSNorm(torch.autograd.Function):
             return dx, torch.zeros_like(weight), None, None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         a, keep = _norm_args(None, x, weight, None, None, None, ctx.eps, 1., x.dtype,
-                             ctx.out_dtype, x.shape)
+                             x.dtype, ctx.out_dtype, x.shape)
         _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
         return dx, dw, None, None
 
@@ -185,7 +169,7 @@ def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, c
     normed = torch.empty(residual.shape, device=residual.device, dtype=out_dtype)
     if stream.numel():
         a, keep = _norm_args(residual, update, weight, post_weight, gate, scale, eps, const,
-                             residual.dtype, out_dtype, residual.shape)
+                             residual.dtype, update.dtype, out_dtype, residual.shape)
         with _on(residual.device):
             _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
                   normed.data_ptr())
@@ -231,9 +215,7 @@ class _ResidualNorm(torch.autograd.Function):
         dstream = None if dstream is None else dstream.contiguous()
         dnormed = None if dnormed is None else dnormed.contiguous()
         a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
-                             stream.dtype, ctx.out_dtype, shape)
-        if update is None:
-            a.update_dtype = _DTYPES[ctx.update_dtype]
+                             stream.dtype, ctx.update_dtype, ctx.out_dtype, shape)
         _norm_backward(a, dev, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
         return dres, dupd, dw, dpw, dgate, dscale, None, None, None
 
@@ -298,20 +280,14 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def _loss_args(weight, shape, dtype, ignore_index, reduction):
-    """GpaLossArgs without the caller's rows, which only the forward reads, and the weight it points to."""
-    a = _lib.GpaLossArgs()
+def _loss_args(weight, shape, dtype, ignore_index, reduction, hidden=_NONE, labels=None):
+    """(GpaLossArgs, the weight it points to); only the forward gives hidden and labels."""
     w = weight if weight.stride(-1) == 1 and weight.stride(0) >= weight.shape[1] else weight.contiguous()
-    a.weight = w.data_ptr()
-    a.vocab, a.width = weight.shape
-    a.inner = shape[-2] if len(shape) > 1 else 1
-    rows = 1
-    for n in shape[:-1]:
-        rows *= n
-    a.outer = rows // a.inner if a.inner else 0
-    a.weight_stride = w.stride(0)
-    a.ignore_index, a.dtype, a.reduction = ignore_index, _DTYPES[dtype], reduction
-    return a, w
+    inner = shape[-2] if len(shape) > 1 else 1
+    vocab, width = weight.shape
+    return _lib.GpaLossArgs(
+        _lib.ptr(hidden[0]), w.data_ptr(), labels, math.prod(shape[:-2]) if inner else 0, inner,
+        hidden[1], hidden[2], w.stride(0), vocab, ignore_index, width, _DTYPES[dtype], reduction), w
 
 
 def _scratch(nbytes, device):
@@ -321,9 +297,9 @@ def _scratch(nbytes, device):
 def _loss_forward(hidden, weight, labels, ignore_index, reduction):
     lib = _lib.load()
     dev = hidden.device
-    a, keep = _loss_args(weight, hidden.shape, hidden.dtype, ignore_index, reduction)
-    x, a.hidden_stride[0], a.hidden_stride[1] = _rows(hidden)
-    a.hidden, a.labels = x.data_ptr(), labels.data_ptr()
+    rows = _rows(hidden)
+    a, keep = _loss_args(weight, hidden.shape, hidden.dtype, ignore_index, reduction, rows,
+                         labels.data_ptr())
     loss = torch.empty(labels.shape if reduction == 2 else (), device=dev, dtype=torch.float32)
     with _on(dev):
         sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)

@@ -19,7 +19,7 @@ def _args(**kw):
     a = _lib.GpaNormArgs()
     a.update = a.weight = 16
     a.outer, a.inner, a.width = 2, 3, 8
-    a.update_stride[0], a.update_stride[1] = 24, 8
+    a.update_outer, a.update_inner = 24, 8
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -77,7 +77,7 @@ def _loss_args(**kw):
     a = _lib.GpaLossArgs()
     a.hidden = a.weight = a.labels = 16
     a.outer, a.inner, a.width, a.vocab, a.weight_stride, a.dtype = 1, 3, 8, 10, 8, 1
-    a.hidden_stride[0], a.hidden_stride[1] = 24, 8
+    a.hidden_outer, a.hidden_inner = 24, 8
     for k, v in kw.items():
         setattr(a, k, v)
     return a
