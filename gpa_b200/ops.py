@@ -13,11 +13,11 @@ graph and have first-order gradients.  They raise ``ValueError`` for arguments t
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -31,6 +31,37 @@ def _on(device):
 
 
 _HERE = contextlib.nullcontext()
+
+
+class _Refuse(torch.autograd.Function):
+    """Passes gradients on; whoever differentiates them again is told that there is no more."""
+
+    @staticmethod
+    def forward(ctx, token, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("second derivatives of this operator are not implemented")
+
+
+def _first_order(backward):
+    """A backward without a graph of its own.  With ``create_graph`` its results carry a node that
+    refuses to be differentiated, so that a missing second derivative is an error, not a zero."""
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        held = [g for g in out if g is not None]
+        if not held:
+            return out
+        marked = iter(_Refuse.apply(torch.zeros((), device=held[0].device, requires_grad=True), *held))
+        return tuple(None if g is None else next(marked) for g in out)
+
+    return run
 
 
 def _call(fn, device, *args):
@@ -130,7 +161,7 @@ class _RMSNorm(torch.autograd.Function):
         return _rms_forward(x, weight, eps, out_dtype)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         x, weight = ctx.saved_tensors
         dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
@@ -190,7 +221,7 @@ class _ResidualNorm(torch.autograd.Function):
         return stream, normed
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dstream, dnormed):
         if dstream is None and dnormed is None:
             return (None,) * 9
@@ -320,7 +351,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dloss):
         weight, saved = ctx.saved_tensors
         shape, dtype = ctx.hidden

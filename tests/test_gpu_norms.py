@@ -311,3 +311,40 @@ def test_launches_are_counted():
     n = _lib.launch_count()
     rms_norm(torch.ones(2, 8, device="cuda"), torch.ones(8, device="cuda"))
     assert _lib.launch_count() == n + 1
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(rms_norm(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        g.sum().backward()
+
+
+def test_one_tensor_in_two_places_gets_both_gradients():
+    g = _gen(20)
+    x, w = _randn(g, (5, 72)).requires_grad_(), (1 + 0.1 * _randn(g, (72,))).requires_grad_()
+    up = _randn(g, (5, 72))
+    s, n = residual_norm(x, x, w, EPS, post_weight=w)
+    dx, dw = torch.autograd.grad((s, n), (x, w), (up, up))
+    a, b, u, v = (t.detach().clone().requires_grad_() for t in (x, x, w, w))
+    parts = torch.autograd.grad(residual_norm(a, b, u, EPS, post_weight=v), (a, b, u, v), (up, up))
+    assert torch.equal(dx, parts[0] + parts[1]) and torch.equal(dw, parts[2] + parts[3])
+
+
+def test_offsets_beyond_32_bits():
+    """2^31 values and more: the last rows equal those of a call with these rows alone."""
+    rows, width = (1 << 21) + 3, 1024
+    x = torch.empty(rows, width, device="cuda", dtype=BF16)
+    x[-5:] = _randn(_gen(21), (5, width), BF16)
+    x[:-5] = 1
+    w = 1 + 0.1 * _randn(_gen(22), (width,))
+    assert torch.equal(rms_norm(x, w)[-5:], rms_norm(x[-5:].clone(), w))
+    leaf = x.requires_grad_()
+    y = rms_norm(leaf, w)
+    up = torch.zeros_like(y)
+    up[-5:] = x[-5:].detach()
+    (dx,) = torch.autograd.grad(y, leaf, up)
+    small = x[-5:].detach().clone().requires_grad_()
+    (ds,) = torch.autograd.grad(rms_norm(small, w), small, up[-5:])
+    assert torch.equal(dx[-5:], ds) and not dx[:-5].any()

@@ -306,5 +306,104 @@ def test_other_stream_repeats_and_replays(dtype):
                 assert torch.equal(a, b)
 
 
+def test_second_derivatives_are_refused():
+    x, w, y = _inputs(17, (9,), 32, 50, F32)
+    x.requires_grad_()
+    (g,) = torch.autograd.grad(linear_cross_entropy(x, w, y), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("lead", [(300,), (20,)])
+def test_two_streams_at_once(lead):
+    cases = [_inputs(30 + i, lead, 256, 5000, BF16, 0.1) for i in range(2)]
+    want = [_run(*c, "mean") for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, (s, c) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                x, w = (t.detach().requires_grad_() for t in c[:2])
+                loss = linear_cross_entropy(x, w, c[2])
+                got[i].append((loss.detach(), *torch.autograd.grad(loss, (x, w), want[i][3])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 values of hidden, and of the weight: the tokens and entries at the far end."""
+    n, d, v = (1 << 21) + 70, 1024, 300
+    x = torch.zeros(n, d, device="cuda", dtype=BF16)
+    xs, w, ys = _inputs(40, (70,), d, v, BF16)
+    x[-70:] = xs
+    y = torch.full((n,), -100, device="cuda")
+    y[-70:] = ys
+    y[0] = 1
+    loss = linear_cross_entropy(x, w, y, reduction="none")
+    want = linear_cross_entropy(xs, w, ys, reduction="none")
+    # the same logits through differently cut sums: two fp32 results of the same exact value
+    bound = 2 * _reference(xs, w, ys, torch.zeros(70), "none")["loss"][1]
+    assert ((loss[-70:] - want).abs().double().cpu() <= bound).all() and not loss[1:-70].any()
+    del x
+    v = (1 << 21) + 300
+    w = torch.zeros(v, d, device="cuda", dtype=BF16)
+    xs, end, ys = _inputs(41, (9,), d, 300, BF16)
+    w[-300:] = end
+    wr = w.requires_grad_()
+    ys = ys + (v - 300)
+    loss = linear_cross_entropy(xs, wr, ys, reduction="none")
+    z = xs.double() @ end.detach().double().T
+    z = torch.cat((z, z.new_zeros(9, 1)), 1)  # every other entry has the logit 0
+    z[:, -1] += torch.log(torch.tensor(float(v - 300), dtype=torch.float64))
+    ref = torch.nn.functional.cross_entropy(z, ys - (v - 300), reduction="none")
+    ez = 2 * (d + 2) * U * (xs.double().abs() @ end.double().abs().T).amax(-1)
+    # beside the logits' errors: 2^21 equal terms, each within 64 U, added in any order
+    assert ((loss.double() - ref).abs() <= 2 * ez + 200 * U + 8 * U * ref.abs()).all()
+    (dw,) = torch.autograd.grad(loss.sum(), wr)
+    p = torch.softmax(z, -1)[:, :300] - torch.nn.functional.one_hot(ys - (v - 300), 300)
+    want = p.T @ xs.double()
+    off = HALF[BF16] * (p.abs().T @ xs.double().abs()) * 1.1 + HALF[BF16] * want.abs()
+    assert ((dw[-300:].double() - want).abs() <= off).all()
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from gpa_b200 import linear_cross_entropy, residual_norm
+g = torch.Generator().manual_seed(0)
+x = torch.randn(300, 128, generator=g).bfloat16().cuda().requires_grad_()
+h = torch.randn(300, 128, generator=g).cuda().requires_grad_()
+w = torch.randn(700, 128, generator=g).bfloat16().cuda().requires_grad_()
+n = torch.ones(128, device="cuda", requires_grad=True)
+y = torch.randint(0, 700, (300,), generator=g).cuda()
+def step():
+    s, m = residual_norm(h, x, n)
+    loss = linear_cross_entropy(m, w, y) + s.float().mean()
+    return (loss.detach(), *torch.autograd.grad(loss, (x, h, w, n)))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+for a, b in zip(got, step()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], cwd=root, capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_no_tensor_core_kernel_timed_out():
     assert _lib.device_status() == 0
