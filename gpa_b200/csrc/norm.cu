@@ -304,10 +304,10 @@ GPA_DEV void emit_sums(float* dst, const float (&a)[ITER][VEC], int width, int g
   }
 }
 
-template <int G, int VEC, int ITER, int MT, int DT>
+template <int G, int VEC, int ITER, int MT>
 __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
   const Fwd& p = b.f;
-  NORM_TYPES(DT);
+  NORM_TYPES(kAny);
   __shared__ float sm[2][3][32];
   extern __shared__ float fold[];  // sub-warp groups: [blockDim / G][G * VEC * ITER]
   int buf = 0;
@@ -535,6 +535,157 @@ __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
   if (b.sum_w >= 0) emit_sums<G, 8, 1>(b.part + (int64_t)blockIdx.x * p.width, aw, p.width, g, t, mine, per, fold);
 }
 
+// Backward with a post weight, a gate or a scale, over rows of whole blocks with 8 channels a
+// thread.  Five tensors are read and a row is met three times (before the first sums, after them,
+// and after the second), so each thread copies its share of the next row into shared memory
+// (cp.async, two stages, 16 bytes a thread and slot: no other thread reads it, so no barrier) and
+// reads the current row from there whenever it needs it, instead of holding it in registers.
+GPA_DEV void copy16(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+
+template <int MT, int DT>
+__global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const Bwd b) {
+  const Fwd& p = b.f;
+  NORM_TYPES(DT);
+  __shared__ float sm[2][3][32];
+  extern __shared__ uint4 slots[];  // [stage][slot][thread]
+  int buf = 0;
+  const int n = blockDim.x, t = threadIdx.x, c = t * 8;
+  const bool in = c < p.width, full = p.gate && p.gate_full;
+  const float inv = 1.f / (float)p.width;
+  const auto wide = [](int dt) { return dt == kF32 ? 2 : 1; };  // slots of 8 values
+  const int sx = 0, sd = sx + wide(h_dt), ss = sd + wide(out_dt), sy = ss + wide(h_dt), sg = sy + wide(y_dt);
+  const int stage = (sg + wide(g_dt)) * n;
+  uint4* mine = slots + t;
+  auto fetch = [&](int slot, const void* src, int64_t i, int dt) {
+    const char* q = static_cast<const char*>(src) + i * (dt == kF32 ? 4 : 2);
+    copy16(mine + slot, q);
+    if (dt == kF32) copy16(mine + slot + n, q + 16);
+  };
+  auto fetch_row = [&](uint32_t row, int s) {
+    if (row < p.rows && in) {
+      const int64_t at = (int64_t)row * p.width + c;
+      fetch(s + sx * n, p.stream, at, h_dt);
+      if (b.dn) fetch(s + sd * n, b.dn, at, out_dt);
+      if (b.ds) fetch(s + ss * n, b.ds, at, h_dt);
+      fetch(s + sy * n, p.y, row_at(p.ry, row, p.inner) + c, y_dt);
+      if (full) fetch(s + sg * n, p.gate, row_at(p.rg, row, p.inner) + c, g_dt);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto read = [&](int slot, int dt, float (&v)[8]) {
+    Raw8 r;
+    r.a = mine[slot];
+    if (dt == kF32) r.b = mine[slot + n];
+    else r.b = make_uint4(0, 0, 0, 0);
+    unraw(r, dt, v);
+  };
+  float aw[1][8] = {}, ap[1][8] = {}, ac[1][8] = {};
+  int s = 0;
+  fetch_row(blockIdx.x, s);
+  for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, s = stage - s) {
+    fetch_row(row + gridDim.x < row ? 0xffffffffu : row + gridDim.x, stage - s);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const int64_t at = (int64_t)row * p.width + c;
+    float sums[3] = {0.f, 0.f, 0.f};  // x^2, w dn x, y^2
+    if (in) {
+      float x[8], v[8], w[8];
+      read(s + sx * n, h_dt, x);
+      if (b.dn) {
+        read(s + sd * n, out_dt, v);
+        ldv<8>(p.w, c, kF32, w);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sums[0] += x[k] * x[k];
+        if (b.dn) sums[1] += w[k] * v[k] * x[k];
+      }
+      if (p.wp) {
+        read(s + sy * n, y_dt, v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sums[2] += v[k] * v[k];
+      }
+    }
+    group_sum<0, 3>(sums, sm, buf);
+    const float r = rsqrtf(sums[0] * inv + p.eps), q = sums[1] * inv * r * r;
+    const float ry = p.wp ? rsqrtf(sums[2] * inv + p.eps) : 1.f;
+    float gr = 1.f;
+    if (p.gate && !full) gr = gate_of(load_in(p.gate, row_at(p.rg, row, p.inner), g_dt));
+    float two[2] = {0.f, 0.f};  // wp du y, row-gate gradient
+    float d[8];
+    if (in) {
+      float x[8], a[8];
+      read(s + sx * n, h_dt, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = 0.f;
+      if (b.dn) {
+        float w[8];
+        read(s + sd * n, out_dt, d);
+        ldv<8>(p.w, c, kF32, w);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          aw[0][k] += d[k] * x[k] * r;
+          d[k] = r * (w[k] * d[k] - x[k] * q);
+        }
+      }
+      if (b.ds) {
+        read(s + ss * n, h_dt, a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k] += a[k];
+      }
+      if (b.dh) stv<8>(b.dh, at, h_dt, d);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) a[k] = gr;
+      if (full) {
+        read(s + sg * n, g_dt, a);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] = gate_of(a[k]);
+      }
+      float cs[8], wp[8], y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) wp[k] = 1.f, cs[k] = p.c;
+      if (p.scale) {
+        ldv<8>(p.scale, c, kF32, cs);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) cs[k] *= p.c;
+      }
+      if (p.wp) ldv<8>(p.wp, c, kF32, wp);
+      read(s + sy * n, y_dt, y);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float u = y[k] * ry * wp[k], ga = d[k] * a[k];
+        ac[0][k] += ga * u * p.c;
+        const float du = ga * cs[k];
+        ap[0][k] += du * y[k] * ry;
+        a[k] = du * u * (1.f - a[k]);  // the gate's gradient
+        two[1] += a[k];
+        d[k] = du * wp[k];
+        two[0] += d[k] * y[k];
+      }
+      if (full && b.dgate) stv<8>(b.dgate, at, g_dt, a);
+    }
+    const bool row_gate = p.gate && !full && b.dgate;
+    if (p.wp || row_gate) group_sum<0, 2>(two, sm, buf);
+    if (row_gate && t == 0) store_out(b.dgate, row, two[1], g_dt);
+    if (!b.dy || !in) continue;
+    if (p.wp) {
+      float y[8];
+      read(s + sy * n, y_dt, y);
+      const float qy = two[0] * inv * ry * ry;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = ry * (d[k] - y[k] * qy);
+    }
+    stv<8>(b.dy, at, y_dt, d);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
+  if (b.sum_w >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_w * p.width, aw, p.width, n, t, 0, 1, nullptr);
+  if (b.sum_p >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_p * p.width, ap, p.width, n, t, 0, 1, nullptr);
+  if (b.sum_c >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_c * p.width, ac, p.width, n, t, 0, 1, nullptr);
+}
+
 // out[k][c] = sum over blocks of part[block][k][c] (k: blockIdx.y), always in the same order: 32
 // lanes for 32 columns, each adding every 32nd block, then the lanes in a tree.
 struct Sums {
@@ -587,36 +738,34 @@ Shape shape_of(const Fwd& f, bool vec) {
 
 constexpr int kMaxWidth = 16384;
 
-// Runs CALL(group, vec, iter, most threads, types) for the shape: the types are built in for blocks
+// Runs CALL(group, vec, iter, most threads, types) for the shape.  The types are built in for blocks
 // over aligned rows with the mixes that models train in, and read from the arguments elsewhere.
-// 640 threads at most leave 96 registers a thread, so that two blocks of 320 fit an SM.
-#define NORM_TYPED(DT, CALL, I, M)                                                            \
-  do {                                                                                        \
-    if ((DT) == types_of(kF32, kBF16, kBF16)) { CALL(0, 8, I, M, types_of(kF32, kBF16, kBF16)); } \
-    else if ((DT) == types_of(kBF16, kBF16, kBF16)) { CALL(0, 8, I, M, types_of(kBF16, kBF16, kBF16)); } \
-    else if ((DT) == types_of(kF32, kF32, kF32)) { CALL(0, 8, I, M, types_of(kF32, kF32, kF32)); } \
-    else { CALL(0, 8, I, M, kAny); }                                                          \
+#define NORM_TYPED(DT, CALL, M)                                                             \
+  do {                                                                                      \
+    if ((DT) == types_of(kF32, kBF16, kBF16)) { CALL(M, types_of(kF32, kBF16, kBF16)); }    \
+    else if ((DT) == types_of(kBF16, kBF16, kBF16)) { CALL(M, types_of(kBF16, kBF16, kBF16)); } \
+    else if ((DT) == types_of(kF32, kF32, kF32)) { CALL(M, types_of(kF32, kF32, kF32)); }   \
+    else { CALL(M, kAny); }                                                                 \
   } while (0)
-#define NORM_DISPATCH(S, DT, CALL)                                  \
+#define NORM_DISPATCH(S, CALL, BLOCK)                               \
   do {                                                              \
     if ((S).vec == 8) {                                             \
-      if ((S).group == 4) { CALL(4, 8, 1, 128, kAny); }             \
-      else if ((S).group == 8) { CALL(8, 8, 1, 128, kAny); }        \
-      else if ((S).group == 16) { CALL(16, 8, 1, 128, kAny); }      \
-      else if ((S).group == 32) { CALL(32, 8, 1, 128, kAny); }      \
-      else if ((S).iter == 1 && (S).threads <= 256) { NORM_TYPED(DT, CALL, 1, 256); } \
-      else if ((S).iter == 1) { NORM_TYPED(DT, CALL, 1, 640); }     \
-      else if ((S).threads <= 512) { CALL(0, 8, 2, 512, kAny); }    \
-      else { CALL(0, 8, 2, 1024, kAny); }                           \
+      if ((S).group == 4) { CALL(4, 8, 1, 128); }                   \
+      else if ((S).group == 8) { CALL(8, 8, 1, 128); }              \
+      else if ((S).group == 16) { CALL(16, 8, 1, 128); }            \
+      else if ((S).group == 32) { CALL(32, 8, 1, 128); }            \
+      else if ((S).iter == 1) { BLOCK; }                            \
+      else if ((S).threads <= 512) { CALL(0, 8, 2, 512); }          \
+      else { CALL(0, 8, 2, 1024); }                                 \
     } else {                                                        \
-      if ((S).group == 4) { CALL(4, 1, 1, 128, kAny); }             \
-      else if ((S).group == 8) { CALL(8, 1, 1, 128, kAny); }        \
-      else if ((S).group == 16) { CALL(16, 1, 1, 128, kAny); }      \
-      else if ((S).group == 32) { CALL(32, 1, 1, 128, kAny); }      \
-      else if ((S).iter == 4 && (S).threads <= 256) { CALL(0, 1, 4, 256, kAny); } \
-      else if ((S).iter == 4) { CALL(0, 1, 4, 1024, kAny); }        \
-      else if ((S).iter == 8) { CALL(0, 1, 8, 1024, kAny); }        \
-      else { CALL(0, 1, 16, 1024, kAny); }                          \
+      if ((S).group == 4) { CALL(4, 1, 1, 128); }                   \
+      else if ((S).group == 8) { CALL(8, 1, 1, 128); }              \
+      else if ((S).group == 16) { CALL(16, 1, 1, 128); }            \
+      else if ((S).group == 32) { CALL(32, 1, 1, 128); }            \
+      else if ((S).iter == 4 && (S).threads <= 256) { CALL(0, 1, 4, 256); } \
+      else if ((S).iter == 4) { CALL(0, 1, 4, 1024); }              \
+      else if ((S).iter == 8) { CALL(0, 1, 8, 1024); }              \
+      else { CALL(0, 1, 16, 1024); }                                \
     }                                                               \
   } while (0)
 
@@ -677,14 +826,21 @@ bool vec_ok(const Fwd& f) {
 // Blocks of the backward: as many as run at once, each with many rows, so that its column sums
 // are added in registers and few partial rows are left.  At most 8 blocks of 128 threads an SM.
 int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
-using Known = std::atomic<int>[33];  // a kernel's blocks per SM, by warps of a block (0: not asked yet)
+// 0: the kernel cannot have its shared memory.
+using Known = std::atomic<int>[8][33];  // a kernel's blocks per SM by device and warps of a block (0: not asked yet)
 int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, Known& known) {
   const uint32_t per = s.group ? s.threads / s.group : 1;
-  int at_once = known[s.threads / 32].load(std::memory_order_relaxed);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  int at_once = dev < 8 ? known[dev][s.threads / 32].load(std::memory_order_relaxed) : 0;
   if (!at_once) {
+    // rows of whole blocks: up to 2 x 10 slots of 16 bytes for 512 threads, whatever the types of this call
+    if (!s.group && smem &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
+      return 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kernel, s.threads, smem) != cudaSuccess || at_once < 1)
       at_once = 1;
-    known[s.threads / 32].store(at_once, std::memory_order_relaxed);
+    if (dev < 8) known[dev][s.threads / 32].store(at_once, std::memory_order_relaxed);
   }
   const uint32_t need = (rows + per - 1) / per;
   return (int)std::max(1u, std::min(need, (uint32_t)std::min(148 * at_once, most_blocks(s))));
@@ -722,8 +878,14 @@ int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStrea
   }
   const uint32_t grid = (f.rows + per - 1) / per;
   const int types = f.h ? built_types(f, f.h_dt) : kAny;
-#define CALL(G, V, I, M, T) k_norm_fwd<G, V, I, M, T><<<grid, s.threads, 0, st>>>(f)
-  NORM_DISPATCH(s, types, CALL);
+#define CALL(G, V, I, M) k_norm_fwd<G, V, I, M, kAny><<<grid, s.threads, 0, st>>>(f)
+#define TYPED(M, T) k_norm_fwd<0, 8, 1, M, T><<<grid, s.threads, 0, st>>>(f)
+#define BLOCK                                            \
+  if (s.threads <= 256) NORM_TYPED(types, TYPED, 256);   \
+  else NORM_TYPED(types, TYPED, 512)
+  NORM_DISPATCH(s, CALL, BLOCK);
+#undef BLOCK
+#undef TYPED
 #undef CALL
   if (cudaGetLastError() == cudaSuccess) return GPA_B200_OK;
   *why = "norm_fwd launch failed";
@@ -788,20 +950,28 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
   const bool vec = vec_ok(f) && aligned8(dnormed) && aligned8(dstream) && aligned8(g->dresidual) &&
                    aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate));
   const Shape s = shape_of(f, vec);
-  const size_t smem = s.group ? sizeof(float) * s.threads * s.vec * s.iter : 0;
   const bool light = s.vec == 8 && s.iter == 1 && !f.wp && !f.scale && !f.gate;
   int blocks = 0;
   {
     Launch scope("norm_bwd", st);
-#define RUN(K)                                                                   \
+#define RUN(K, SMEM)                                                             \
   do {                                                                           \
     static Known known;                                                          \
+    const size_t smem = (SMEM);                                                  \
     blocks = bwd_blocks(s, f.rows, reinterpret_cast<const void*>(&K), smem, known); \
-    K<<<blocks, s.threads, smem, st>>>(b);                                       \
+    if (blocks) K<<<blocks, s.threads, smem, st>>>(b);                           \
   } while (0)
-#define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>))
-#define CALL(G, V, I, M, T) RUN((k_norm_bwd<G, V, I, M, T>))
-    const int types = plain ? kAny : built_types(f, f.h_dt);
+#define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>), fold_smem)
+#define CALL(G, V, I, M) RUN((k_norm_bwd<G, V, I, M>), fold_smem)
+#define TYPED(M, T) RUN((k_norm_bwd_parts<M, T>), slot_smem)
+#define BLOCK                                            \
+  if (s.threads <= 320) NORM_TYPED(types, TYPED, 320);   \
+  else NORM_TYPED(types, TYPED, 512)
+    const int types = built_types(f, f.h_dt);
+    const size_t fold_smem = s.group ? sizeof(float) * s.threads * s.vec * s.iter : 0;
+    auto slots = [](int dt) { return dt == kF32 ? 2 : 1; };
+    const size_t slot_smem = (size_t)2 * s.threads * 16 *
+                             (2 * slots(f.h_dt) + slots(f.out_dt) + slots(f.y_dt) + slots(f.gate ? f.g_dt : f.y_dt));
     if (light) {
       if (s.group == 4) LIGHT(4, 128);
       else if (s.group == 8) LIGHT(8, 128);
@@ -810,8 +980,10 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
       else if (s.threads <= 256) LIGHT(0, 256);
       else LIGHT(0, 512);
     } else {
-      NORM_DISPATCH(s, types, CALL);
+      NORM_DISPATCH(s, CALL, BLOCK);
     }
+#undef BLOCK
+#undef TYPED
 #undef CALL
 #undef LIGHT
 #undef RUN
