@@ -143,11 +143,17 @@ def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
               _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
 
 
-def _rms_forward(x, weight, eps, out_dtype):
-    out = torch.empty(x.shape, device=x.device, dtype=out_dtype)
+_DENSE = torch.contiguous_format
+
+
+def _rms_args(x, weight, eps, out_dtype):
+    return _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, x.dtype, out_dtype, x.shape)
+
+
+def _rms_forward(x, weight, eps, out_dtype, args=None):
+    out = torch.empty_like(x, dtype=out_dtype, memory_format=_DENSE)
     if out.numel():
-        a, keep = _norm_args(None, x, weight, None, None, None, eps, 1., x.dtype, x.dtype, out_dtype,
-                             x.shape)
+        a, keep = _rms_args(x, weight, eps, out_dtype) if args is None else args
         with _on(x.device):
             _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
     return out
@@ -156,20 +162,22 @@ def _rms_forward(x, weight, eps, out_dtype):
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, eps, out_dtype):
+        args = _rms_args(x, weight, eps, out_dtype)
         ctx.save_for_backward(x, weight)
+        # the arguments serve the backward too, unless they point to a copy made for this call
+        ctx.args = args if args[1][1] is x else None
         ctx.eps, ctx.out_dtype = eps, out_dtype
-        return _rms_forward(x, weight, eps, out_dtype)
+        return _rms_forward(x, weight, eps, out_dtype, args)
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
         x, weight = ctx.saved_tensors
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        dx = torch.empty_like(x, memory_format=_DENSE)
         if not x.numel():
             return dx, torch.zeros_like(weight), None, None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        a, keep = _norm_args(None, x, weight, None, None, None, ctx.eps, 1., x.dtype,
-                             x.dtype, ctx.out_dtype, x.shape)
+        a, keep = ctx.args or _rms_args(x, weight, ctx.eps, ctx.out_dtype)
         _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
         return dx, dw, None, None
 
@@ -195,12 +203,18 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, *,
     return _rms_forward(x, weight, eps, out_dtype)
 
 
-def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, const, out_dtype):
-    stream = torch.empty(residual.shape, device=residual.device, dtype=residual.dtype)
-    normed = torch.empty(residual.shape, device=residual.device, dtype=out_dtype)
+def _residual_args(residual, update, weight, post_weight, gate, scale, eps, const, out_dtype):
+    return _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, residual.dtype,
+                      update.dtype, out_dtype, residual.shape)
+
+
+def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, const, out_dtype,
+                      args=None):
+    stream = torch.empty_like(residual, memory_format=_DENSE)
+    normed = torch.empty_like(residual, dtype=out_dtype, memory_format=_DENSE)
     if stream.numel():
-        a, keep = _norm_args(residual, update, weight, post_weight, gate, scale, eps, const,
-                             residual.dtype, update.dtype, out_dtype, residual.shape)
+        a, keep = args or _residual_args(residual, update, weight, post_weight, gate, scale, eps,
+                                         const, out_dtype)
         with _on(residual.device):
             _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
                   normed.data_ptr())
@@ -210,11 +224,16 @@ def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, c
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, residual, update, weight, post_weight, gate, scale, eps, const, out_dtype):
-        stream, normed = _residual_forward(residual, update, weight, post_weight, gate, scale, eps,
-                                           const, out_dtype)
+        given = (residual, update, weight, post_weight, gate, scale, eps, const, out_dtype)
+        args = _residual_args(*given)
+        stream, normed = _residual_forward(*given, args)
         # the update itself is needed only where the residual's share depends on it
         read = post_weight is not None or gate is not None or scale is not None
         ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
+        # the arguments serve the backward too, unless they point to a copy made for this call
+        ctx.args = args[0] if args[1][1] is update and args[1][2] is gate else None
+        if not read:
+            args[0].update = None
         ctx.update_dtype = update.dtype
         ctx.eps, ctx.const, ctx.out_dtype = eps, const, out_dtype
         ctx.set_materialize_grads(False)
@@ -227,17 +246,10 @@ class _ResidualNorm(torch.autograd.Function):
             return (None,) * 9
         stream, update, weight, post_weight, gate, scale = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dev, shape = stream.device, stream.shape
-
-        def new(i, like_shape, dtype):
-            return torch.empty(like_shape, device=dev, dtype=dtype) if need[i] else None
-
-        dres = new(0, shape, stream.dtype)
-        dupd = new(1, shape, ctx.update_dtype)
-        dw = new(2, weight.shape, torch.float32)
-        dpw = new(3, weight.shape, torch.float32)
-        dgate = None if gate is None else new(4, gate.shape, gate.dtype)
-        dscale = new(5, weight.shape, torch.float32)
+        dres = torch.empty_like(stream) if need[0] else None
+        dupd = torch.empty_like(stream, dtype=ctx.update_dtype) if need[1] else None
+        dw, dpw, dscale = (torch.empty_like(weight) if need[i] else None for i in (2, 3, 5))
+        dgate = torch.empty_like(gate, memory_format=_DENSE) if need[4] else None
         if not stream.numel():
             for t in (dw, dpw, dscale):
                 if t is not None:
@@ -245,9 +257,11 @@ class _ResidualNorm(torch.autograd.Function):
             return dres, dupd, dw, dpw, dgate, dscale, None, None, None
         dstream = None if dstream is None else dstream.contiguous()
         dnormed = None if dnormed is None else dnormed.contiguous()
-        a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
-                             stream.dtype, ctx.update_dtype, ctx.out_dtype, shape)
-        _norm_backward(a, dev, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
+        a, keep = ctx.args, None
+        if a is None:
+            a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
+                                 stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
+        _norm_backward(a, stream.device, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
         return dres, dupd, dw, dpw, dgate, dscale, None, None, None
 
 
@@ -325,25 +339,31 @@ def _scratch(nbytes, device):
     return torch.empty(nbytes, device=device, dtype=torch.uint8)
 
 
-def _loss_forward(hidden, weight, labels, ignore_index, reduction):
+def _loss_forward(hidden, weight, labels, ignore_index, reduction, keep_rows):
+    """(loss, what the backward reads or None, GpaLossArgs or None where it points to a copy)."""
     lib = _lib.load()
     dev = hidden.device
     rows = _rows(hidden)
-    a, keep = _loss_args(weight, hidden.shape, hidden.dtype, ignore_index, reduction, rows,
-                         labels.data_ptr())
-    loss = torch.empty(labels.shape if reduction == 2 else (), device=dev, dtype=torch.float32)
+    a, w = _loss_args(weight, hidden.shape, hidden.dtype, ignore_index, reduction, rows,
+                      labels.data_ptr())
+    if reduction == 2:
+        loss = torch.empty_like(labels, dtype=torch.float32)
+    else:
+        loss = torch.empty((), device=dev, dtype=torch.float32)
     with _on(dev):
-        sizes = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
-        saved, scratch = (_scratch(n, dev) for n in sizes)
-        _call(lib.gpa_b200_loss_forward, dev, a, loss.data_ptr(), saved.data_ptr(), sizes[0],
-              scratch.data_ptr(), sizes[1])
-    return loss, saved
+        kept, more = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 0)
+        saved = _scratch(kept if keep_rows else kept + more, dev)
+        scratch = _scratch(more, dev) if keep_rows else None  # else behind what the backward would read
+        at = saved.data_ptr()
+        _call(lib.gpa_b200_loss_forward, dev, a, loss.data_ptr(), at, kept,
+              scratch.data_ptr() if keep_rows else at + kept, more)
+    return loss, saved if keep_rows else None, a if w is weight else None
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, labels, ignore_index, reduction):
-        loss, saved = _loss_forward(hidden, weight, labels, ignore_index, reduction)
+        loss, saved, ctx.args = _loss_forward(hidden, weight, labels, ignore_index, reduction, True)
         # the labelled rows are packed into `saved`: hidden and labels are not needed again
         ctx.save_for_backward(weight, saved)
         ctx.hidden = hidden.shape, hidden.dtype
@@ -357,9 +377,11 @@ class _LinearCrossEntropy(torch.autograd.Function):
         shape, dtype = ctx.hidden
         lib = _lib.load()
         dev = weight.device
-        a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
-        dx, dw = (torch.empty(s, device=dev, dtype=dtype) if need else None
-                  for s, need in zip((shape, weight.shape), ctx.needs_input_grad))
+        a, keep = ctx.args, None
+        if a is None:
+            a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
+        dx = torch.empty(shape, device=dev, dtype=dtype) if ctx.needs_input_grad[0] else None
+        dw = torch.empty_like(weight, memory_format=_DENSE) if ctx.needs_input_grad[1] else None
         dloss = dloss.contiguous()
         with _on(dev):
             nbytes = lib.gpa_b200_loss_scratch_bytes(a, 1)
@@ -405,11 +427,12 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
                          f"and {weight.shape[0]}")
     if labels.numel() > 1 << 22:
         raise ValueError(f"at most 2^22 tokens in a call, not {labels.numel()}")
-    labels = labels.long().contiguous()
+    if labels.dtype != torch.int64 or not labels.is_contiguous():
+        labels = labels.long().contiguous()
     args = (hidden, weight, labels, int(ignore_index), _REDUCTIONS[reduction])
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         return _LinearCrossEntropy.apply(*args)
-    return _loss_forward(*args)[0]
+    return _loss_forward(*args, False)[0]
 
 
 __all__ = ["linear_cross_entropy", "rms_norm", "residual_norm"]
