@@ -922,6 +922,10 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     *why = "a tensor that the gradients need is NULL";
     return GPA_B200_BAD_ARGUMENT;
   }
+  if ((g->dpost_weight && !f.wp) || (g->dscale && !f.scale) || (g->dgate && !f.gate)) {
+    *why = "a gradient is asked for of a tensor that is not there";
+    return GPA_B200_BAD_ARGUMENT;
+  }
   b.sums = 0;
   b.sum_w = g->dweight ? b.sums++ : -1;
   b.sum_p = g->dpost_weight ? b.sums++ : -1;

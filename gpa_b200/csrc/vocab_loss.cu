@@ -98,9 +98,9 @@ GPA_DEV void put_row(const T* s, typename Part<T>::type* d, int64_t plane, int w
 // Packs the labelled rows: row[j], label[j] (-1 outside the vocabulary) and the channels of the
 // j-th of them, pos[i] its place or -1.  A block takes kRun rows; two more fill the places behind
 // the last row with zeros up to a multiple of 64, the reduction block of dW.  Four blocks share a
-// run's copies (blockIdx.y), a row for each of their warps.  In n <= 4096 rows
-// one launch is cheaper than k_count before it (a block reads 32 KB of labels at most); beyond,
-// the labels before a block are counted once.
+// run's copies (blockIdx.y), a row for each of their warps.  Up to 4096 rows a block counts the
+// labels before its own (at most 32 KB), which costs less than a launch of k_count; beyond, they
+// are counted once.
 template <typename T>
 __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, typename Part<T>::type* dst) {
   __shared__ int part[8];
@@ -176,8 +176,8 @@ GPA_DEV void merge(float& m, float& s, float m2, float s2) {
   m = big;
 }
 
-// Maximum and 1 / sum of exp, and loss, of each packed row from the (max, sum) pairs of its tiles: blockDim.x rows a block,
-// blockDim.y lanes of tiles each (256 threads).  The block that finishes last adds the losses of
+// Maximum and 1 / sum of exp, and loss, of each packed row from the (max, sum) pairs of its
+// tiles: blockDim.x rows a block, blockDim.y lanes of tiles each (256 threads).  The block that finishes last adds the losses of
 // a mean or sum in double, in a fixed order.
 __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, int tiles, const float* z_label,
                                               float2* lse, float* each, const int* pos, float* packed,
@@ -341,6 +341,7 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   const int at_once = tc_pairs();
   const int64_t tiles_v = up(c.vocab, kTile) / kTile, tiles_m = c.n_pad / kTile;
   const int64_t tiles_d = (c.pitch + kTile - 1) / kTile;
+  if (tiles_v * tiles_m > (int64_t(1) << 30)) return "at most 2^30 tiles of 256 x 256 logits in a call";
   c.few = c.n <= 32 ? 32 : c.n <= 128 ? 128 : 0;
   p->parts_v = tc_stats_parts(c);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
@@ -382,7 +383,7 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->s_w = take(p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0);
   p->s_bytes = at;
   at = 0;
-    p->count = take(4 * up(c.n, kRun) / kRun);
+  p->count = take(4 * (up(c.n, kRun) / kRun));
   p->part = take((int64_t)p->parts_v * c.n_pad * 8);
   p->z_label = take(4 * c.n);
   p->loss = take(4 * c.n);
@@ -453,6 +454,10 @@ void finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, con
     k_finish<T, 1><<<(unsigned)c.n, 128, 0, st>>>(dxp, stride, c, pos, up, unit, static_cast<T*>(dx));
 }
 
+// the kernels read and write the workspaces 32 bytes at a time
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
+const char* const kMisaligned = "saved and scratch must start on 32 bytes";
+
 void bind(Plan* p, const void* saved) {
   const char* s = static_cast<const char*>(saved);
   p->c.n_rows = reinterpret_cast<const int*>(s);
@@ -511,6 +516,10 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
     *why = "saved or scratch is smaller than its size query";
     return GPA_B200_BAD_ARGUMENT;
   }
+  if (!aligned(saved) || !aligned(scratch)) {
+    *why = kMisaligned;
+    return GPA_B200_BAD_ARGUMENT;
+  }
   char* sv = static_cast<char*>(saved);
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved);
@@ -550,6 +559,10 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   }
   if (saved_bytes < (size_t)p.s_bytes || scratch_bytes < (size_t)p.bwd_bytes) {
     *why = "saved or scratch is smaller than its size query";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  if (!aligned(saved) || !aligned(scratch)) {
+    *why = kMisaligned;
     return GPA_B200_BAD_ARGUMENT;
   }
   if (!c.n) {

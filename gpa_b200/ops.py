@@ -178,6 +178,8 @@ class _RMSNorm(torch.autograd.Function):
             return dx, torch.zeros_like(weight), None, None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
         a, keep = ctx.args or _rms_args(x, weight, ctx.eps, ctx.out_dtype)
+        if ctx.args:  # the tensors may have moved since (sharded parameters do)
+            a.update, a.weight = x.data_ptr(), weight.data_ptr()
         _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
         return dx, dw, None, None
 
@@ -232,8 +234,6 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args[0] if args[1][1] is update and args[1][2] is gate else None
-        if not read:
-            args[0].update = None
         ctx.update_dtype = update.dtype
         ctx.eps, ctx.const, ctx.out_dtype = eps, const, out_dtype
         ctx.set_materialize_grads(False)
@@ -261,6 +261,9 @@ class _ResidualNorm(torch.autograd.Function):
         if a is None:
             a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
                                  stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
+        else:  # the tensors may have moved since (sharded parameters do)
+            a.update, a.weight, a.gate = _lib.ptr(update), weight.data_ptr(), _lib.ptr(gate)
+            a.post_weight, a.scale = _lib.ptr(post_weight), _lib.ptr(scale)
         _norm_backward(a, stream.device, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
         return dres, dupd, dw, dpw, dgate, dscale, None, None, None
 
@@ -380,6 +383,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         a, keep = ctx.args, None
         if a is None:
             a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
+        else:
+            a.weight = weight.data_ptr()  # which may have moved since (sharded parameters do)
         dx = torch.empty(shape, device=dev, dtype=dtype) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(weight, memory_format=_DENSE) if ctx.needs_input_grad[1] else None
         dloss = dloss.contiguous()

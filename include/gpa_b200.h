@@ -268,7 +268,9 @@ typedef struct GpaLossArgs {
 } GpaLossArgs;
 
 /* Bytes of the buffer that the forward leaves for the backward, and of either call's scratch
- * (0 for arguments the entry points refuse). */
+ * (0 for arguments the entry points refuse); both start on 32 bytes.  saved holds the labelled
+ * rows, and a copy of a weight that the tensor cores cannot read in place (fp32, or rows that do
+ * not start on 16 bytes). */
 size_t gpa_b200_loss_saved_bytes(const GpaLossArgs* args);
 size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward);
 /* loss: one fp32, or one per row for GPA_B200_LOSS_NONE (0 for rows without a label). */

@@ -348,3 +348,22 @@ def test_offsets_beyond_32_bits():
     small = x[-5:].detach().clone().requires_grad_()
     (ds,) = torch.autograd.grad(rms_norm(small, w), small, up[-5:])
     assert torch.equal(dx[-5:], ds) and not dx[:-5].any()
+
+
+def test_tensors_that_move_between_forward_and_backward():
+    """As sharded parameters do: the values come back at another address before the backward."""
+    g = _gen(30)
+    x, w = _randn(g, (6, 80)).requires_grad_(), (1 + 0.1 * _randn(g, (80,))).requires_grad_()
+    up = _randn(g, (6, 80))
+    want = torch.autograd.grad(rms_norm(x, w), (x, w), up)
+    y = rms_norm(x, w)
+    s, n = residual_norm(x, x.detach().clone(), w, post_weight=w)  # not the memory spoilt below
+    old = x.data, w.data
+    with torch.no_grad():
+        x.data, w.data = old[0].clone(), old[1].clone()
+        for t in old:
+            t.fill_(float("nan"))
+    for a, b in zip(want, torch.autograd.grad(y, (x, w), up)):
+        assert torch.equal(a, b)
+    (dw,) = torch.autograd.grad(n, (w,), up)
+    assert dw.isfinite().all()

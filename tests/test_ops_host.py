@@ -73,6 +73,16 @@ def test_norm_entry_points_refuse_missing_tensors():
     assert lib.gpa_b200_norm_scratch_bytes(a) >= 2 * 8 * 4
 
 
+@pytest.mark.parametrize("name", ["dpost_weight", "dscale", "dgate"])
+def test_norm_backward_refuses_gradients_of_tensors_that_are_not_there(name):
+    lib = _lib.load()
+    g = _lib.GpaNormGrads()
+    g.dresidual = 16
+    setattr(g, name, 16)
+    assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, 16, 1 << 30, None) == 1
+    assert "not there" in _message()
+
+
 def _loss_args(**kw):
     a = _lib.GpaLossArgs()
     a.hidden = a.weight = a.labels = 16
@@ -93,7 +103,8 @@ def test_loss_refuses_cpu_tensors():
     (dict(dtype=3), 1, "dtype"), (dict(reduction=3), 1, "reduction"), (dict(width=0), 1, "width"),
     (dict(vocab=0), 1, "vocab"), (dict(outer=-1), 1, "outer"), (dict(weight_stride=7), 1, "overlap"),
     (dict(width=65537, weight_stride=65537), 2, "channels"), (dict(vocab=(1 << 29) + 1), 2, "vocabulary"),
-    (dict(outer=1 << 21), 2, "rows"), (dict(weight=None), 1, "NULL"),
+    (dict(outer=1 << 21), 2, "rows"),
+    (dict(outer=1 << 20, vocab=1 << 29), 2, "tiles"), (dict(weight=None), 1, "NULL"),
 ])
 def test_loss_entry_points_refuse_bad_arguments(change, code, word):
     lib = _lib.load()
@@ -121,6 +132,9 @@ def test_loss_entry_points_refuse_small_workspaces():
     assert lib.gpa_b200_loss_forward(a, None, 16, saved, 16, fwd, None) == 1
     assert lib.gpa_b200_loss_backward(a, 16, saved, 16, 16, 16, 16, bwd - 1, None) == 1
     assert lib.gpa_b200_loss_backward(a, 16, saved, 16, None, None, 16, bwd, None) == 1
+    # the workspaces are read 32 bytes at a time
+    assert lib.gpa_b200_loss_forward(a, 16, 16, saved, 32, fwd, None) == 1 and "32 bytes" in _message()
+    assert lib.gpa_b200_loss_backward(a, 32, saved, 16, 16, 16, 48, bwd, None) == 1 and "32 bytes" in _message()
 
 
 def test_loss_workspace_of_a_training_step_stays_small():
