@@ -126,7 +126,9 @@ GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
   }
 }
 
-// 1 / (1 + e^-a) to a few units of 2^-22: exp2 and reciprocal units instead of the full functions
+// The gate in the backward, 1 / (1 + e^-a) to a few units of 2^-22: exp2 and reciprocal units
+// instead of the full functions, which the forward takes (its bound is the bytes, and its results
+// lie next to rounding borders).
 GPA_DEV float gate_of(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 
 GPA_DEV float round_to(float x, int dt) {
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
       ry = rsqrtf(s1[0] * inv + p.eps);
     }
     float gr = p.c;
-    if (live && p.gate && !p.gate_full) gr *= gate_of(load_in(p.gate, og, g_dt));
+    if (live && p.gate && !p.gate_full) gr *= sigmoid(load_in(p.gate, og, g_dt));
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
         float a[VEC];
         held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m[k] *= gate_of(a[k]);
+        for (int k = 0; k < VEC; ++k) m[k] *= sigmoid(a[k]);
       }
       if (p.scale) {
         float a[VEC];

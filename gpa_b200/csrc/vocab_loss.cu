@@ -66,7 +66,8 @@ struct Part<float> {
 
 // One row of `width` values to `pitch` places, by one warp; 8 at a time where both ends allow it.
 template <typename T>
-GPA_DEV void put_row(const T* s, typename Part<T>::type* d, int64_t plane, int width, int pitch, bool vec, int lane) {
+GPA_DEV void put_row(const T* __restrict__ s, typename Part<T>::type* __restrict__ d, int64_t plane, int width,
+                     int pitch, bool vec, int lane) {
   if (vec) {
 #pragma unroll 4
     for (int c = lane * 8; c < width; c += 256) {
@@ -91,6 +92,7 @@ GPA_DEV void put_row(const T* s, typename Part<T>::type* d, int64_t plane, int w
       }
     }
   } else {
+#pragma unroll 8
     for (int c = lane; c < pitch; c += 32) put(d + c, plane, c < width ? s[c] : T(0.f));
   }
 }
@@ -167,6 +169,18 @@ __global__ void __launch_bounds__(256) k_weight(const T* src, int64_t stride, in
   if (v < vocab) put_row(src + v * stride, d, plane, width, pitch, vec, lane);
   else
     for (int c = lane; c < pitch; c += 32) put(d + c, plane, T(0.f));
+}
+
+// dW of a piece where the caller's rows do not start on 16 bytes: from padded rows, a warp each.
+// Stores of single values straight from the tile (a row a thread) measured four times as long as
+// the whole step (14 x 314 x 85437).
+template <typename T>
+__global__ void __launch_bounds__(256) k_unpad(const T* __restrict__ src, int pitch, int64_t rows, int width,
+                                               T* __restrict__ dst) {
+  const int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (v >= rows) return;
+#pragma unroll 8
+  for (int c = threadIdx.x & 31; c < width; c += 32) dst[v * width + c] = src[v * pitch + c];
 }
 
 // ------------------------------------------------------------------ joins
@@ -261,8 +275,8 @@ __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Ca
 // dx of the caller's rows: the parts added in order, scaled, rounded; zero for rows without a
 // label.  kV channels a thread at a time.
 template <typename T, int kV>
-__global__ void k_finish(const float* part, int64_t part_stride, const Call c, const int* pos,
-                         const Upstream up, float unit, T* dx) {
+__global__ void k_finish(const float* __restrict__ part, int64_t part_stride, const Call c, const int* pos,
+                         const Upstream up, float unit, T* __restrict__ dx) {
   const int64_t i = blockIdx.x;
   const int j = pos[i], parts = c.n_rows[2];
   const float s = up.scale(*c.n_rows) * unit;
@@ -274,6 +288,7 @@ __global__ void k_finish(const float* part, int64_t part_stride, const Call c, c
 #pragma unroll
     for (int e = 0; e < kV; ++e) v[e] = 0.f;
     if (j >= 0) {
+#pragma unroll 8
       for (int q = 0; q < parts; ++q) {
         if constexpr (kV > 1) {  // rows of the parts start on 16 bytes
 #pragma unroll
@@ -310,7 +325,7 @@ struct Plan {
   int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
   // scratch
   int64_t count, part, z_label, loss, fwd_bytes;
-  int64_t p, dxp, r, scale, bwd_bytes;
+  int64_t p, dxp, dwp, r, scale, bwd_bytes;
 };
 
 const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
@@ -391,6 +406,7 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   at = 0;
   p->p = take(c.planes * c.n_pad * p->piece * 2);
   p->dxp = take((int64_t)p->split.most * c.n_pad * c.pitch * 4);
+  p->dwp = take(p->piece * c.pitch * p->es);
   p->r = take(4 * c.n);
   p->scale = take(4);
   p->bwd_bytes = at;
@@ -589,12 +605,22 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
     up = {r, false, s, false};
   }
   const int64_t part_stride = c.n_pad * c.pitch;
+  // pieces start at multiples of 256 rows: every row of dW on 16 bytes (32 for fp32), or none
+  const bool in_place = c.width == c.pitch && (reinterpret_cast<uintptr_t>(dweight) & (p.es == 4 ? 31 : 15)) == 0;
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
     if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
     if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.split.most, v0 > 0, dxp, part_stride, st))
       FAIL("loss_dx_tc5 launch failed");
-    if (dweight && !tc_dw(c, pr, p.piece, v0, vn, up, dweight, st)) FAIL("loss_dw_tc5 launch failed");
+    if (!dweight) continue;
+    char* dw = static_cast<char*>(dweight) + v0 * c.width * p.es;
+    if (!tc_dw(c, pr, p.piece, v0, vn, up, in_place ? dw : sc + p.dwp, c.pitch, st)) FAIL("loss_dw_tc5 launch failed");
+    if (!in_place) {
+      Launch scope("loss_unpad", st);
+      BY_TYPE(a->dtype, (k_unpad<T><<<(unsigned)((vn + 7) / 8), 256, 0, st>>>(
+                            reinterpret_cast<const T*>(sc + p.dwp), c.pitch, vn, c.width, reinterpret_cast<T*>(dw))));
+      OK_OR("loss_unpad launch failed");
+    }
   }
   if (dhidden) {
     BY_TYPE(a->dtype, finish<T>(p, dxp, part_stride, reinterpret_cast<const int*>(sv + p.s_pos), up, dhidden, st));

@@ -78,8 +78,9 @@ bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Up
               int64_t p_pitch, cudaStream_t st);
 bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int most_parts, bool add,
            float* dx, int64_t dx_part, cudaStream_t st);
+// dW of a piece; its rows are a multiple of 8 values long and start on 16 bytes (fp32: 32)
 bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
-           cudaStream_t st);
+           int64_t dw_pitch, cudaStream_t st);
 
 }  // namespace vloss
 

@@ -23,8 +23,10 @@
 // other, and each product is the six of them that matter, the smallest first: x2 y0, x1 y1, x0 y2,
 // x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
 // step of 16, so a long reduction would lose what the parts gained: the accumulator is emptied
-// after kSegment of it and the segments are added in registers, in round-to-nearest fp32, by
-// eight epilogue warps (two threads a row).
+// after a segment of it and the segments are added in registers, in round-to-nearest fp32, by
+// more epilogue warps (four threads a row of 256 columns, 64 registers each).  The statistics of 16-bit inputs are formed the same
+// way beyond 1024 channels: the loss is an fp32 result, and its error would grow with the width
+// (2048 channels: 1.1e-6 of the loss in one accumulator, 0.5e-6 in two).
 //
 // Every wait is bounded (tc5.cuh); a wait that gives up sets the device status and the kernel
 // drains and returns.
@@ -58,12 +60,15 @@ struct Smem {
   static constexpr uint32_t kBars = kStages * kStage, kTable = kBars + 256, kSquares = kTable + BN * 16;
   static constexpr size_t kBytes = 1024 + (BN == 256 ? kTable : kSquares + 2 * 32 * kSquare * 4);
 };
-constexpr int kSegment = 8;  // reduction blocks between two additions in registers (fp32)
-__host__ __device__ constexpr int threads_of(bool f32) { return f32 ? 384 : 256; }
+// reduction blocks between two additions in registers: 512 for the six products of fp32 parts, 1024 for one
+constexpr int kSegmentF32 = 8, kSegment16 = 16;
 constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { kStats, kProbs, kDx, kDw, kStatsT, kProbsT, kDxT };
+// groups of four epilogue warps: threads that share a row of the tile
+__host__ __device__ constexpr int groups_of(Mode m, bool f32) { return !f32 ? 1 : m >= kStatsT ? 2 : 4; }
+__host__ __device__ constexpr int threads_of(Mode m, bool f32) { return 128 + 128 * groups_of(m, f32); }
 
 struct Args {
   Call c;
@@ -85,8 +90,8 @@ struct Args {
   int64_t dx_part;
   bool add;
   // kDw
-  void* dw;
-  bool wide;               // dW rows start on the boundaries that its stores need
+  void* dw;                // of the piece
+  int64_t dw_pitch;
   uint32_t idesc;
   bool f16;
 };
@@ -263,30 +268,35 @@ struct Walk {
 };
 
 // What a thread holds of its row of the tile when it is done: the columns in tensor memory (16-bit
-// inputs), or the CW of them that it has added up in registers (fp32: half the tile's).
+// inputs), or the CW of them that it has added up in registers.
 template <bool F32, int CW>
 struct Row {
   uint32_t tmem;
-  GPA_DEV void get(int chunk, float (&v)[32]) const { ld32(tc5::tmem_at(tmem, 32 * chunk), v); }
+  // chunk k of CH columns, to be used up: read into `buffer`, or the registers that hold it
+  template <int CH>
+  GPA_DEV float (&take(int k, float (&buffer)[CH]))[CH] {
+    ld32(tc5::tmem_at(tmem, CH * k), buffer);
+    return buffer;
+  }
 };
 template <int CW>
 struct Row<true, CW> {
-  float acc[CW];
+  static constexpr int kCh = CW < 32 ? CW : 32;
+  float acc[CW / kCh][kCh];
   template <int CH>
-  GPA_DEV void get(int chunk, float (&v)[CH]) const {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) v[i] = acc[CH * chunk + i];
+  GPA_DEV float (&take(int k, float (&)[CH]))[CH] {
+    return acc[k];
   }
 };
 
-template <Mode M, bool F32>
-GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 128>& held, int rank, bool empty) {
-  constexpr int kChunks = F32 ? 4 : 8, kUnroll = F32 ? 4 : 1;
-  const int half = F32 ? (threadIdx.x - 128) >> 7 : 0;  // of the tile's columns
+template <Mode M, bool F32, bool EXACT>
+GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& held, int rank, bool empty) {
+  constexpr int kChunks = F32 ? 2 : 8, kUnroll = F32 ? 2 : 1;
+  const int group = F32 ? (threadIdx.x - 128) >> 7 : 0;  // of the tile's columns
   const int in_tile = rank * kHalf + (threadIdx.x & 127);
   const int64_t row = (int64_t)t.m * kTile + in_tile;
-  const int64_t col0 = (int64_t)t.n * kTile + half * 128;
-  float v[32];
+  const int64_t col0 = (int64_t)t.n * kTile + group * 64;
+  float buffer[32];
   if (M == kStats) {
     const bool live = row < n_rows;
     const int64_t y = live ? (int64_t)a.c.label[row] - col0 : -1;
@@ -294,7 +304,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 1
 #pragma unroll kUnroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = 32 * k;
-      held.get(k, v);
+      float (&v)[32] = held.take(k, buffer);
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -313,13 +323,13 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 1
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        s0 += F32 ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
-        s1 += F32 ? expf(v[i + 1] - safe) : ex2(fmaf(v[i + 1], kLog2e, -off));
+        s0 += EXACT ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
+        s1 += EXACT ? expf(v[i + 1] - safe) : ex2(fmaf(v[i + 1], kLog2e, -off));
       }
-      sum = fmaf(sum, F32 ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
+      sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
     }
-    if (live) a.part[(int64_t)(F32 ? 2 * t.n + half : t.n) * a.c.n_pad + row] = make_float2(big, sum);
+    if (live) a.part[(int64_t)(F32 ? 4 * t.n + group : t.n) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
     const bool live = row < n_rows;
     const float2 l = live ? a.lse[row] : make_float2(0.f, 0.f);
@@ -330,9 +340,9 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 1
 #pragma unroll kUnroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = 32 * k;
-      held.get(k, v);
+      float (&v)[32] = held.take(k, buffer);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = (F32 ? expf(v[i] - l.x) : ex2(fmaf(v[i], kLog2e, -off))) * f;
+      for (int i = 0; i < 32; ++i) v[i] = (EXACT ? expf(v[i] - l.x) : ex2(fmaf(v[i], kLog2e, -off))) * f;
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -363,7 +373,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 1
 #pragma unroll kUnroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = 32 * k;
-      held.get(k, v);
+      float (&v)[32] = held.take(k, buffer);
       if (!live) continue;
       const int64_t left = a.c.pitch - col0 - c;  // a multiple of 8
       if (a.add) {
@@ -381,46 +391,29 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, const Row<F32, 1
   } else {
     const bool live = row < a.vn;
     const float s = a.up.scale(n_rows) / a.p_scale;
-    const int64_t at = (a.v0 + row) * a.c.width + col0;
+    const int64_t at = row * a.dw_pitch + col0;
 #pragma unroll kUnroll
     for (int k = 0; k < kChunks; ++k) {
       const int c = 32 * k;
-      if (!empty) {
-        held.get(k, v);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-      }
+      float (&v)[32] = !F32 && empty ? buffer : held.take(k, buffer);
       if (!live) continue;
-      const int64_t left = a.c.width - col0 - c;
+      const int64_t left = a.dw_pitch - col0 - c;  // a multiple of 8
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= s;
+      for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : v[i] * s;
       if (F32) {
         float* out = static_cast<float*>(a.dw) + at + c;
-        if (a.wide) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            if (i < left) st8(out + i, reinterpret_cast<const uint32_t*>(v + i));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < left) out[i] = v[i];
-        }
+        for (int i = 0; i < 32; i += 8)
+          if (i < left) st8(out + i, reinterpret_cast<const uint32_t*>(v + i));
         continue;
       }
       uint16_t* out = static_cast<uint16_t*>(a.dw) + at + c;
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) w[i] = pack2(v[2 * i], v[2 * i + 1], a.f16);
-      if (a.wide) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          if (2 * i < left) *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < left) out[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-      }
+      for (int i = 0; i < 16; i += 4)
+        if (2 * i < left) *reinterpret_cast<uint4*>(out + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
     }
   }
 }
@@ -448,7 +441,7 @@ GPA_DEV bool half_all(int half, bool ok) {
 
 // (max, sum of exp) of the columns over every tile of the CTA.  A chunk of columns goes through
 // shared memory, so that a thread meets kCh entries of one column at a time.
-template <bool F32, int BN>
+template <bool F32, int BN, bool EXACT>
 struct Stats {
   using C = Cols<F32, BN>;
   float big[C::kChunks], sum[C::kChunks];
@@ -468,14 +461,14 @@ struct Stats {
     }
   }
   GPA_DEV int column(int k) const { return half * C::kCw + k * C::kCh + col; }
-  GPA_DEV void tile(const Args& a, const Tile& t, const Row<F32, C::kCw>& held, int rank, float* square) {
+  GPA_DEV void tile(const Args& a, const Tile& t, Row<F32, C::kCw>& held, int rank, float* square) {
     const int r = threadIdx.x & 127;
     const int64_t base = (int64_t)t.m * kTile + rank * kHalf;
     const bool in = base + r < a.vn;
 #pragma unroll
     for (int k = 0; k < C::kChunks; ++k) {
-      float v[C::kCh];
-      held.get(k, v);
+      float buffer[C::kCh];
+      float (&v)[C::kCh] = held.take(k, buffer);
 #pragma unroll
       for (int i = 0; i < C::kCh; ++i) square[i * kSquare + r] = in ? v[i] : -INFINITY;
       half_sync(half);
@@ -489,8 +482,8 @@ struct Stats {
       const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
       float more = 0.f;
 #pragma unroll
-      for (int i = 0; i < C::kCh; ++i) more += F32 ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
-      sum[k] = fmaf(sum[k], F32 ? expf(big[k] - safe) : ex2(fmaf(big[k], kLog2e, -off)), more);
+      for (int i = 0; i < C::kCh; ++i) more += EXACT ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
+      sum[k] = fmaf(sum[k], EXACT ? expf(big[k] - safe) : ex2(fmaf(big[k], kLog2e, -off)), more);
       big[k] = m;
       const int64_t y = label[k] - base - lane * C::kCh;
       if (label[k] >= 0 && y >= 0 && y < C::kCh) a.z_label[column(k)] = s[y];
@@ -516,15 +509,15 @@ GPA_DEV float4 row_of(const Args& a, int j, int n_rows) {
 }
 
 template <Mode M, bool F32, int BN>
-GPA_DEV void epilogue_t(const Args& a, const Tile& t, int n_rows, const Row<F32, Cols<F32, BN>::kCw>& held, int rank,
+GPA_DEV void epilogue_t(const Args& a, const Tile& t, int n_rows, Row<F32, Cols<F32, BN>::kCw>& held, int rank,
                         const float4* table) {
   using C = Cols<F32, BN>;
   const int half = F32 ? (threadIdx.x - 128) >> 7 : 0;
   const int64_t at = (int64_t)t.m * kTile + rank * kHalf + (threadIdx.x & 127);
 #pragma unroll
   for (int k = 0; k < C::kChunks; ++k) {
-    float v[C::kCh];
-    held.get(k, v);
+    float buffer[C::kCh];
+    float (&v)[C::kCh] = held.take(k, buffer);
     const int j0 = half * C::kCw + k * C::kCh;
     if (M == kProbsT) {
       uint16_t* out = static_cast<uint16_t*>(a.p) + at;
@@ -565,12 +558,14 @@ GPA_DEV void epilogue_t(const Args& a, const Tile& t, int n_rows, const Row<F32,
 GPA_DEV int plane_a(int q) { return q == 0 ? 2 : q == 1 || q == 3 ? 1 : 0; }
 GPA_DEV int plane_b(int q) { return q == 2 ? 2 : q == 1 || q == 4 ? 1 : 0; }
 
-template <Mode M, bool F32, int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
+// F32: segments added in registers; PRODUCTS: 6 for fp32 inputs (which also take the full exp), else 1
+template <Mode M, bool F32, int BN, int PRODUCTS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 1)
     k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
   constexpr bool kT = M == kStatsT || M == kProbsT || M == kDxT;
   constexpr bool kAMn = M == kDw || M == kDxT, kBMn = M == kDx || M == kDw;
-  constexpr int kProducts = F32 ? 6 : 1;
+  constexpr int kProducts = PRODUCTS, kSegment = PRODUCTS > 1 ? kSegmentF32 : kSegment16;
+  constexpr bool kPlanes = PRODUCTS > 1;
   using S = Smem<BN>;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kStage = S::kStage;
@@ -589,12 +584,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
     }
     for (int i = 0; i < 2; ++i) {
       tc5::mbar_init(&acc_full[i], 1);
-      tc5::mbar_init(&acc_empty[i], F32 ? 16 : 8);  // the epilogue warps of both CTAs
+      tc5::mbar_init(&acc_empty[i], 8 * groups_of(M, F32));  // the epilogue warps of both CTAs
     }
     tc5::mbar_fence_init();
   }
   if (M == kProbsT)
-    for (int j = threadIdx.x; j < BN; j += threads_of(F32)) table[j] = row_of<F32>(a, j, *a.c.n_rows);
+    for (int j = threadIdx.x; j < BN; j += threads_of(M, F32)) table[j] = row_of<F32>(a, j, *a.c.n_rows);
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc5::saddr(slot))
                  : "memory");
@@ -609,7 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
   bool ok = true;
 
   // The reduction of a tile goes by in segments, each into an accumulator of its own: all of it at
-  // once for 16-bit inputs, kSegment blocks times the products of the parts for fp32.
+  // once (16-bit operands and results), or kSegment blocks times the products.
   auto segment_end = [](int k, int k1) { return F32 && k + kSegment < k1 ? k + kSegment : k1; };
 
   if (warp == 0) {
@@ -623,15 +618,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
         for (int k0 = x.k0; k0 < x.k1 && ok; k0 = segment_end(k0, x.k1)) {
           const int blocks = segment_end(k0, x.k1) - k0;
           for (int j = 0; j < blocks * kProducts; ++j, ++it) {
-            const int q = F32 ? j / blocks : 0, k = k0 + j - q * blocks;
+            const int q = kPlanes ? j / blocks : 0, k = k0 + j - q * blocks;
             const uint32_t s = it % kStages, turn = it / kStages;
             if (turn && !(ok = tc5::mbar_wait(&empty[s], (turn - 1) & 1))) break;
             unsigned char* sa = sm + s * kStage;
             unsigned char* sb = sa + kOperand;
             const uint32_t bar = in_first(&full[s]);
             if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
-            const int kk = k * kBK, pa = va + (F32 ? plane_a(q) * a.a_plane : 0);
-            const int pb = vb + (F32 ? plane_b(q) * a.b_plane : 0);
+            const int kk = k * kBK, pa = va + (kPlanes ? plane_a(q) * a.a_plane : 0);
+            const int pb = vb + (kPlanes ? plane_b(q) * a.b_plane : 0);
             if (kAMn) {
               tma_load(sa, &map_a, ra, pa + kk, bar);
               tma_load(sa + kOperand / 2, &map_a, ra + 64, pa + kk, bar);
@@ -678,21 +673,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
     }
   } else if (warp >= 4) {
     using C = Cols<F32, BN>;
-    constexpr int kCw = F32 ? BN / 2 : 128;  // columns that a thread adds up
+    constexpr int kCw = kT ? C::kCw : 64;  // columns that a thread adds up
     uint32_t count = 0;
     const int half = (warp - 4) >> 2;
-    Stats<F32, BN> stats;
+    Stats<F32, BN, kPlanes> stats;
     float* square = reinterpret_cast<float*>(sm + S::kSquares) + half * 32 * kSquare;
     if constexpr (M == kStatsT) stats.start(a, walk.n_rows);
     for (int t = pair; t < walk.total && ok; t += pairs) {
       const Tile x = walk.at(t);
-      Row<F32, kT ? C::kCw : kCw> held;
+      Row<F32, kCw> held;
       const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (dx)
       if (none && M != kDw) continue;
       auto done = [&](bool empty) {
         if constexpr (M == kStatsT) stats.tile(a, x, held, rank, square);
         else if constexpr (kT) epilogue_t<M, F32, BN>(a, x, walk.n_rows, held, rank, table);
-        else epilogue<M, F32>(a, x, walk.n_rows, held, rank, empty);
+        else epilogue<M, F32, kPlanes>(a, x, walk.n_rows, held, rank, empty);
       };
       for (int k0 = x.k0; k0 < x.k1; k0 = segment_end(k0, x.k1), ++count) {
         const uint32_t buf = count & 1, use = count >> 1;
@@ -706,7 +701,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(F32), 1)
             float v[16];
             ld16(tc5::tmem_at(tmem, buf * kTile + half * kCw + c), v);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) held.acc[c + i] = k0 == x.k0 ? v[i] : held.acc[c + i] + v[i];
+            for (int i = 0; i < 16; ++i) {
+              float& sum = held.acc[(c + i) / held.kCh][(c + i) % held.kCh];
+              sum = k0 == x.k0 ? v[i] : sum + v[i];
+            }
           }
         } else {
           held.tmem = tmem + buf * kTile;
@@ -784,7 +782,7 @@ Args base_args(const Call& c) {
   return a;
 }
 
-template <Mode M, bool F32, int BN>
+template <Mode M, bool F32, int BN, int PRODUCTS>
 bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
                cudaStream_t st) {
   constexpr int kSmem = (int)Smem<BN>::kBytes;
@@ -794,21 +792,26 @@ bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, c
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k_product<M, F32, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_product<M, F32, BN, PRODUCTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) !=
+        cudaSuccess)
       return false;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
   Launch scope(name, st);
-  k_product<M, F32, BN><<<2 * pairs, threads_of(F32), kSmem, st>>>(ma, mb, a);
+  k_product<M, F32, BN, PRODUCTS><<<2 * pairs, threads_of(M, F32), kSmem, st>>>(ma, mb, a);
   return cudaGetLastError() == cudaSuccess;
 }
+
+bool exact_stats(const Call& c) { return c.dtype == GPA_B200_F32 || c.pitch > kSegment16 * kBK; }
 
 template <Mode M, int BN>
 bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
             cudaStream_t st) {
-  return a.c.dtype == GPA_B200_F32 ? launch_as<M, true, BN>(name, ma, mb, a, tiles, st)
-                                   : launch_as<M, false, BN>(name, ma, mb, a, tiles, st);
+  if (a.c.dtype == GPA_B200_F32) return launch_as<M, true, BN, 6>(name, ma, mb, a, tiles, st);
+  if constexpr (M == kStats || M == kStatsT)
+    if (exact_stats(a.c)) return launch_as<M, true, BN, 1>(name, ma, mb, a, tiles, st);
+  return launch_as<M, false, BN, 1>(name, ma, mb, a, tiles, st);
 }
 
 // z as W x^T for few rows: the map of W in boxes of 128 rows, of x in boxes of half the columns
@@ -841,7 +844,7 @@ int tc_pairs() {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2));
     constexpr int kSmem = (int)Smem<256>::kBytes;
-    cfg.blockDim = dim3(threads_of(false));
+    cfg.blockDim = dim3(threads_of(kStats, false));
     cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -849,8 +852,8 @@ int tc_pairs() {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(k_product<kStats, false, 256>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false, 256>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaFuncSetAttribute(k_product<kStats, false, 256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false, 256, 1>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = std::max(1, sms / 2);
     }
@@ -861,9 +864,9 @@ int tc_pairs() {
 
 int tc_stats_parts(const Call& c) {
   const int64_t tiles = (c.vocab + kTile - 1) / kTile;
-  const bool f32 = c.dtype == GPA_B200_F32;
-  if (!c.few) return (int)(f32 ? 2 * tiles : tiles);
-  return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * (f32 && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes);
+  const bool exact = exact_stats(c);
+  if (!c.few) return (int)(exact ? 4 * tiles : tiles);
+  return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * (exact && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes);
 }
 
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
@@ -934,7 +937,7 @@ bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
 }
 
 bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
-           cudaStream_t st) {
+           int64_t dw_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
   if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kBK, f16) ||
@@ -946,7 +949,7 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   a.up = up;
   a.dw = dw;
   a.b_plane = (int)c.n_pad;
-  a.wide = c.width % 8 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0;
+  a.dw_pitch = dw_pitch;
   a.tiles_n = (c.pitch + kTile - 1) / kTile;
   a.idesc = idesc_of(c, kTile, true, true);
   return launch<kDw, 256>("loss_dw_tc5", ma, mb, a, (int64_t)a.tiles_n * ((vn + kTile - 1) / kTile), st);
