@@ -12,7 +12,11 @@
 //
 // A group of G threads owns a row, each thread VEC consecutive channels at a time: sub-warp
 // groups for narrow rows (several rows per warp), whole blocks for wide ones.  Rows are read
-// once; the bound is the bytes moved.  Column sums of the backward stay in registers over a
+// once; the bound is the bytes moved.  Measured (GPU time, B200, copy 6.54 TB/s):
+//   65536 x 1024, fp32 stream, bf16 update and result: forward 127 us = 6.3 TB/s, backward 163 us
+//   (6.6), fold of the weight gradient 7 us;  262144 x 128 bf16, plain: 27 us (5.0) and 55 us (3.7);
+//   8188 x 2560 bf16 with post weight, gate and scale: 55 us (3.8) and 103 us (3.3).
+// Column sums of the backward stay in registers over a
 // block's rows, go to one partial row per block and are added in block order by a second
 // kernel, so results do not depend on scheduling.
 #include "../../include/gpa_b200.h"
@@ -443,7 +447,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
 }
 
 // The plain norm over narrow rows: each group takes kNarrow rows at once, all their loads in
-// flight together.
+// flight together (262144 x 128 bf16: 39 -> 27 us).
 constexpr int kNarrow = 4;
 template <int G>
 __global__ void __launch_bounds__(128) k_norm_narrow(const Fwd p) {
@@ -475,7 +479,8 @@ __global__ void __launch_bounds__(128) k_norm_narrow(const Fwd p) {
 
 // Backward where the update's share is the update times a constant (or the plain norm): no more
 // than the stream and the two gradients are read.  A block's next row is loaded while the
-// current one is reduced and written.
+// current one is reduced and written (65536 x 1024: 346 -> 163 us).  Types built in, as in the other
+// block kernels, gave nothing here (163 -> 172 us).
 template <int G, int MT>
 __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
   const Fwd& p = b.f;
@@ -541,7 +546,10 @@ __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
 // thread.  Five tensors are read and a row is met three times (before the first sums, after them,
 // and after the second), so each thread copies its share of the next row into shared memory
 // (cp.async, two stages, 16 bytes a thread and slot: no other thread reads it, so no barrier) and
-// reads the current row from there whenever it needs it, instead of holding it in registers.
+// reads the current row from there whenever it needs it, instead of holding it in registers.  The
+// 96 registers of 320 threads let two blocks run on an SM.  What bounds it now is its own
+// instructions (62 % of the issue slots busy, DRAM 36 %): 103 us for 8188 x 2560 in bf16, against
+// 118 us with direct loads and 125 us with three blocks of 64 registers, which spill.
 GPA_DEV void copy16(uint4* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
                : "memory");

@@ -19,6 +19,9 @@
 // entries or channels by the 32 or 128 rows, so that a step of the products costs an eighth or
 // half as much and more copies of W are on their way at a time.
 //
+// For fp32 the parts of W are then read once each instead of once for each product: a stage holds a
+// part of W and every part of x that it meets (54 x 1024 x 86791: z 187 -> 173 us).
+//
 // fp32 inputs come as three bf16 parts, x = x0 + x1 + x2 (24 bits), in planes one behind the
 // other, and each product is the six of them that matter, the smallest first: x2 y0, x1 y1, x0 y2,
 // x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
@@ -27,6 +30,13 @@
 // more epilogue warps (four threads a row of 256 columns, 64 registers each).  The statistics of 16-bit inputs are formed the same
 // way beyond 1024 channels: the loss is an fp32 result, and its error would grow with the width
 // (2048 channels: 1.1e-6 of the loss in one accumulator, 0.5e-6 in two).
+//
+// Measured (GPU time of one launch, B200): 65536 rows x 1024 channels x 151936 entries, bf16:
+// statistics 16.3 ms = 1.25 PFLOP/s, P 18.4 ms, dx 15.7 ms, dW 15.4 ms (1.30 PFLOP/s; a library
+// product of 8192^3 sustains 1.38 under the power limit, which bounds all four).  2048 x 2048 x
+// 50000, fp16: dW 275 us = 1.53 PFLOP/s (1.65 in a burst).  1026 x 512 x 16001, fp32: dW 107 us =
+// 157 TFLOP/s of fp32 products, 940 of bf16 ones.  8 x 1024 x 151936, bf16: statistics 53 us =
+// 5.9 TB/s of W.  One CTA instead of the pair was not built: its shared memory would bound it.
 //
 // Every wait is bounded (tc5.cuh); a wait that gives up sets the device status and the kernel
 // drains and returns.
@@ -52,16 +62,18 @@ constexpr uint32_t kOperand = kHalf * kBK * 2;    // their bytes in one stage
 // Shared memory of a pair of tiles with BN columns: the stages, barriers, and for the transposed
 // products a table of the rows and the square of one chunk of columns for either half.
 constexpr int kSquare = 129;                      // pitch of its columns: no bank conflicts either way
-template <int BN>
+template <int BN, bool SHARE>
 struct Smem {
-  static constexpr int kStages = BN == 256 ? 6 : BN == 128 ? 7 : 9;
+  static constexpr int kStages = BN == 256 ? 6 : BN == 128 ? (SHARE ? 4 : 7) : (SHARE ? 7 : 9);
   static constexpr uint32_t kColumns = BN / 2 * kBK * 2;
-  static constexpr uint32_t kStage = kOperand + kColumns;
+  static constexpr uint32_t kStage = kOperand + kColumns * (SHARE ? 3 : 1);
   static constexpr uint32_t kBars = kStages * kStage, kTable = kBars + 256, kSquares = kTable + BN * 16;
   static constexpr size_t kBytes = 1024 + (BN == 256 ? kTable : kSquares + 2 * 32 * kSquare * 4);
 };
-// reduction blocks between two additions in registers: 512 for the six products of fp32 parts, 1024 for one
-constexpr int kSegmentF32 = 8, kSegment16 = 16;
+// Reduction blocks between two additions in registers: 512 for the six products of fp32 parts one
+// after the other, 128 where the products of a part follow one another in every block (few rows,
+// see below), 1024 for single products.
+constexpr int kSegmentF32 = 8, kSegmentShare = 2, kSegment16 = 16;
 constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -331,6 +343,10 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
     }
     if (live) a.part[(int64_t)(F32 ? 4 * t.n + group : t.n) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
+    // P is rounded once to the type of its product's other operand: the relative error of a logit's
+    // gradient is half a step of that type, the same as the caller's own rounding of dx and dW.
+    // (fp32: three parts, 24 bits.)  fp16 takes it times 2^14 (tc_p_scale): a probability of
+    // 2^-28 keeps its full precision, and the largest value is 2^14 |r|.
     const bool live = row < n_rows;
     const float2 l = live ? a.lse[row] : make_float2(0.f, 0.f);
     const float r = live ? a.up.r(a.c, row) * a.p_scale : 0.f, f = l.y * r, off = l.x * kLog2e;
@@ -564,9 +580,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
     k_product(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Args a) {
   constexpr bool kT = M == kStatsT || M == kProbsT || M == kDxT;
   constexpr bool kAMn = M == kDw || M == kDxT, kBMn = M == kDx || M == kDw;
-  constexpr int kProducts = PRODUCTS, kSegment = PRODUCTS > 1 ? kSegmentF32 : kSegment16;
-  constexpr bool kPlanes = PRODUCTS > 1;
-  using S = Smem<BN>;
+  constexpr bool kPlanes = PRODUCTS > 1, kShare = kPlanes && kT;
+  constexpr int kSegment = kShare ? kSegmentShare : kPlanes ? kSegmentF32 : kSegment16;
+  constexpr int kPasses = kShare ? 3 : PRODUCTS;  // over a segment
+  using S = Smem<BN, kShare>;
   constexpr int kStages = S::kStages;
   constexpr uint32_t kStage = S::kStage;
   extern __shared__ unsigned char raw[];
@@ -617,16 +634,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
         const int va = kT ? (int)a.v0 : 0, vb = M == kStats || M == kProbs || M == kDx ? (int)a.v0 : 0;
         for (int k0 = x.k0; k0 < x.k1 && ok; k0 = segment_end(k0, x.k1)) {
           const int blocks = segment_end(k0, x.k1) - k0;
-          for (int j = 0; j < blocks * kProducts; ++j, ++it) {
+          for (int j = 0; j < blocks * kPasses; ++j, ++it) {
             const int q = kPlanes ? j / blocks : 0, k = k0 + j - q * blocks;
             const uint32_t s = it % kStages, turn = it / kStages;
             if (turn && !(ok = tc5::mbar_wait(&empty[s], (turn - 1) & 1))) break;
             unsigned char* sa = sm + s * kStage;
             unsigned char* sb = sa + kOperand;
             const uint32_t bar = in_first(&full[s]);
-            if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * kStage);
-            const int kk = k * kBK, pa = va + (kPlanes ? plane_a(q) * a.a_plane : 0);
-            const int pb = vb + (kPlanes ? plane_b(q) * a.b_plane : 0);
+            const int parts_b = kShare ? q + 1 : 1;  // part 2 of W meets part 0 of x, part 1 two, part 0 all
+            if (rank == 0) tc5::mbar_expect_tx(&full[s], 2 * (kOperand + parts_b * S::kColumns));
+            const int kk = k * kBK, pa = va + (kShare ? 2 - q : kPlanes ? plane_a(q) : 0) * a.a_plane;
+            const int pb = vb + (kPlanes && !kShare ? plane_b(q) * a.b_plane : 0);
             if (kAMn) {
               tma_load(sa, &map_a, ra, pa + kk, bar);
               tma_load(sa + kOperand / 2, &map_a, ra + 64, pa + kk, bar);
@@ -637,7 +655,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
               tma_load(sb, &map_b, rb, pb + kk, bar);
               tma_load(sb + kOperand / 2, &map_b, rb + 64, pb + kk, bar);
             } else {
-              tma_load(sb, &map_b, kk, pb + rb, bar);
+              for (int b = 0; b < parts_b; ++b) tma_load(sb + b * S::kColumns, &map_b, kk, pb + b * a.b_plane + rb, bar);
             }
           }
         }
@@ -656,15 +674,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
           const uint32_t buf = count & 1, use = count >> 1;
           if (use && !(ok = wait_cluster(&acc_empty[buf], (use - 1) & 1))) break;
           tc5::fence_after_sync();
-          const int steps = (segment_end(k0, x.k1) - k0) * kProducts;
+          const int blocks = segment_end(k0, x.k1) - k0, steps = blocks * kPasses;
           for (int j = 0; j < steps; ++j, ++it) {
             const uint32_t s = it % kStages;
             if (!(ok = tc5::mbar_wait(&full[s], (it / kStages) & 1))) break;
             tc5::fence_after_sync();
             const uint32_t sa = tc5::saddr(sm + s * kStage), sb = sa + kOperand;
+            const int last = kShare ? j / blocks : 0;  // parts of x in the stage, the smallest product first
+            for (int b = last; b >= 0; --b)
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks)
-              mma2(tmem + buf * kTile, operand<kAMn>(sa, ks), operand<kBMn>(sb, ks), a.idesc, j > 0 || ks > 0);
+              for (int ks = 0; ks < kBK / 16; ++ks)
+                mma2(tmem + buf * kTile, operand<kAMn>(sa, ks), operand<kBMn>(sb + b * S::kColumns, ks), a.idesc,
+                     j > 0 || b < last || ks > 0);
             commit2(&empty[s]);
           }
           if (ok) commit2(&acc_full[buf]);
@@ -785,7 +806,7 @@ Args base_args(const Call& c) {
 template <Mode M, bool F32, int BN, int PRODUCTS>
 bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, const Args& a, int64_t tiles,
                cudaStream_t st) {
-  constexpr int kSmem = (int)Smem<BN>::kBytes;
+  constexpr int kSmem = (int)Smem<BN, (PRODUCTS > 1 && M >= kStatsT)>::kBytes;
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
   int dev = 0;
@@ -843,7 +864,7 @@ int tc_pairs() {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * (sms / 2));
-    constexpr int kSmem = (int)Smem<256>::kBytes;
+    constexpr int kSmem = (int)Smem<256, false>::kBytes;
     cfg.blockDim = dim3(threads_of(kStats, false));
     cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute at;
