@@ -94,12 +94,13 @@ def _rows(t: Tensor):
 
 
 def _check_tensor(name: str, t: Tensor, device=None):
+    if t.is_cuda and t.dtype in _DTYPES and (device is None or t.device == device):
+        return
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (B200, sm_100a)")
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+    raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
 
 
 def _vector(name: str, t: Tensor, width: int, device) -> Tensor:
@@ -320,7 +321,10 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
     elif scale is not None:
         const, scale = float(scale), None
     args = (residual, update, weight, post_weight, gate, scale, float(eps), const, out_dtype)
-    if torch.is_grad_enabled() and any(isinstance(t, Tensor) and t.requires_grad for t in args):
+    if torch.is_grad_enabled() and (
+            residual.requires_grad or update.requires_grad or weight.requires_grad or
+            (post_weight is not None and post_weight.requires_grad) or
+            (gate is not None and gate.requires_grad) or (scale is not None and scale.requires_grad)):
         return _ResidualNorm.apply(*args)
     return _residual_forward(*args)
 
