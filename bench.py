@@ -646,7 +646,7 @@ def run_lm(args, rank, world, local):
         "steps": args.steps, "warmup": args.warmup, "ms_per_step": round(ms, 1),
         "higher_is_better": True, "scaling": "weak", "vs_baseline": None, "dtype": "bf16",
         "data": "synthetic (uniform random token ids; random-init weights)",
-        "config": {"workload": "all-GPA LM train step (fwd+bwd, per-layer checkpointing, chunked CE)",
+        "config": {"workload": "all-GPA LM train step (fwd+bwd, per-layer checkpointing, vocabulary loss without logits)",
                    "model": "GPALM 28 x (hidden 1024, 16 heads x 128, 8 KV heads, SwiGLU 3072), "
                             "vocab 151936, DenseGPA slots 64/64/64/128",
                    "parameters": num_parameters(model), "global_batch": BATCH * world,

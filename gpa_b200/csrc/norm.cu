@@ -130,6 +130,11 @@ GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
   }
 }
 
+// 1 / rms of a row from its sum of squares.  The forward takes the correctly rounded division and
+// root (one each per row and thread): what it is off by shifts every value of the row, and the
+// stream is rounded to 16 bits next.
+GPA_DEV float inv_rms(float sum, int width, float eps) { return 1.f / sqrtf(sum / (float)width + eps); }
+
 // The gate in the backward, 1 / (1 + e^-a) to a few units of 2^-22: exp2 and reciprocal units
 // instead of the full functions, which the forward takes (its bound is the bytes, and its results
 // lie next to rounding borders).
@@ -197,7 +202,6 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
   const uint32_t row = blockIdx.x * per + (G == 0 ? 0u : threadIdx.x / G);
   const bool live = row < p.rows;  // idle groups of a warp still take part in its shuffles
   const bool plain = p.h == nullptr;
-  const float inv = 1.f / (float)p.width;
   float x[ITER][VEC];
   Held<VEC> held_h[ITER], held_g[ITER];  // every load of the row in flight before its first sum
   const int64_t oy = live ? row_at(p.ry, row, p.inner) : 0;
@@ -227,7 +231,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s1[0] += x[i][k] * x[i][k];
       group_sum<G, 1>(s1, sm, buf);
-      ry = rsqrtf(s1[0] * inv + p.eps);
+      ry = inv_rms(s1[0], p.width, p.eps);
     }
     float gr = p.c;
     if (live && p.gate && !p.gate_full) gr *= sigmoid(load_in(p.gate, og, g_dt));
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) s2[0] += x[i][k] * x[i][k];
   group_sum<G, 1>(s2, sm, buf);
-  const float r = rsqrtf(s2[0] * inv + p.eps);
+  const float r = inv_rms(s2[0], p.width, p.eps);
 #pragma unroll
   for (int i = 0; i < ITER; ++i) {
     const int c = (i * g + t) * VEC;
@@ -461,7 +465,6 @@ __global__ void __launch_bounds__(128) k_norm_narrow(const Fwd p) {
   }
   float w[8] = {};
   if (c < p.width) ldv<8>(p.w, c, kF32, w);
-  const float inv = 1.f / (float)p.width;
 #pragma unroll
   for (int u = 0; u < kNarrow; ++u) {
     float x[8], s = 0.f;
@@ -470,7 +473,7 @@ __global__ void __launch_bounds__(128) k_norm_narrow(const Fwd p) {
     for (int k = 0; k < 8; ++k) s += x[k] * x[k];
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float r = rsqrtf(s * inv + p.eps);
+    const float r = inv_rms(s, p.width, p.eps);
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] *= r * w[k];
     if (row0 + u < p.rows && c < p.width) stv<8>(p.out, (int64_t)(row0 + u) * p.width + c, p.out_dt, x);

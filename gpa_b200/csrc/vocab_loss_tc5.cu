@@ -694,6 +694,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
     }
   } else if (warp >= 4) {
     using C = Cols<F32, BN>;
+    static_assert(!kT || 128 % C::kLanes == 0, "a half's threads share the columns of a chunk evenly");
     constexpr int kCw = kT ? C::kCw : 64;  // columns that a thread adds up
     uint32_t count = 0;
     const int half = (warp - 4) >> 2;
