@@ -15,7 +15,7 @@
 // once; the bound is the bytes moved.  Measured (GPU time, B200, copy 6.54 TB/s):
 //   65536 x 1024, fp32 stream, bf16 update and result: forward 127 us = 6.3 TB/s, backward 163 us
 //   (6.6), fold of the weight gradient 7 us;  262144 x 128 bf16, plain: 27 us (5.0) and 55 us (3.7);
-//   8188 x 2560 bf16 with post weight, gate and scale: 55 us (3.8) and 103 us (3.3).
+//   8188 x 2560 bf16 with post weight, gate and scale: 61 us (3.4) and 96 us (3.5).
 // Column sums of the backward stay in registers over a
 // block's rows, go to one partial row per block and are added in block order by a second
 // kernel, so results do not depend on scheduling.
@@ -135,10 +135,25 @@ GPA_DEV void stv(void* p, int64_t i, int dt, const float (&v)[VEC]) {
 // stream is rounded to 16 bits next.
 GPA_DEV float inv_rms(float sum, int width, float eps) { return 1.f / sqrtf(sum / (float)width + eps); }
 
-// The gate in the backward, 1 / (1 + e^-a) to a few units of 2^-22: exp2 and reciprocal units
-// instead of the full functions, which the forward takes (its bound is the bytes, and its results
-// lie next to rounding borders).
-GPA_DEV float gate_of(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
+// 1 / (1 + e^-a), to about 2^-22.  The exponent a log2 e is split into its rounded value, which the
+// exp2 unit takes, and what the rounding left, which enters to first order; one Newton step
+// follows the reciprocal unit.  (Full exp and division: 10 us of 66 for 8188 x 2560.)
+GPA_DEV float gate_of(float a) {
+  constexpr float kLog2e = 1.44269502f, kRest = 1.92596303e-8f, kLn2 = 0.693147182f;  // log2 e = kLog2e + kRest
+  const float x = a < -87.f ? -87.f : a > 87.f ? 87.f : a;  // e^-x and the rests stay finite; NaN passes
+  const float t = -x * kLog2e;
+  const float rest = fmaf(-x, kRest, fmaf(-x, kLog2e, -t));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  const float d = 1.f + fmaf(e, rest * kLn2, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  r = r * fmaf(-d, r, 2.f);
+  return a < -87.f ? 0.f : r;
+}
+
+// The gate in the backward, whose results are not rounded next to a border of another tensor's:
+// exp2 and reciprocal units alone (7 us less there).
+GPA_DEV float gate_near(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
 
 GPA_DEV float round_to(float x, int dt) {
   if (dt == kBF16) return __bfloat162float(__float2bfloat16(x));
@@ -234,7 +249,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
       ry = inv_rms(s1[0], p.width, p.eps);
     }
     float gr = p.c;
-    if (live && p.gate && !p.gate_full) gr *= sigmoid(load_in(p.gate, og, g_dt));
+    if (live && p.gate && !p.gate_full) gr *= gate_of(load_in(p.gate, og, g_dt));
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
@@ -247,7 +262,7 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
         float a[VEC];
         held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) m[k] *= sigmoid(a[k]);
+        for (int k = 0; k < VEC; ++k) m[k] *= gate_of(a[k]);
       }
       if (p.scale) {
         float a[VEC];
@@ -373,7 +388,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
     const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
     const float ry = p.wp ? rsqrtf(s[2] * inv + p.eps) : 1.f;
     float gr = 1.f;
-    if (live && p.gate && !p.gate_full) gr = gate_of(load_in(p.gate, og, g_dt));
+    if (live && p.gate && !p.gate_full) gr = gate_near(load_in(p.gate, og, g_dt));
     float s2[2] = {0.f, 0.f};  // wp du y, row-gate gradient
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -410,7 +425,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
       if (p.gate && p.gate_full) {
         held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a[k] = gate_of(a[k]);
+        for (int k = 0; k < VEC; ++k) a[k] = gate_near(a[k]);
       }
       float dg[VEC];
 #pragma unroll
@@ -551,8 +566,9 @@ __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
 // (cp.async, two stages, 16 bytes a thread and slot: no other thread reads it, so no barrier) and
 // reads the current row from there whenever it needs it, instead of holding it in registers.  The
 // 96 registers of 320 threads let two blocks run on an SM.  What bounds it now is its own
-// instructions (62 % of the issue slots busy, DRAM 36 %): 103 us for 8188 x 2560 in bf16, against
-// 118 us with direct loads and 125 us with three blocks of 64 registers, which spill.
+// instructions (62 % of the issue slots busy, DRAM 36 % before the packed arithmetic): 96 us for
+// 8188 x 2560 in bf16, against 104 us one channel to an instruction, 118 us with direct loads and
+// 125 us with three blocks of 64 registers, which spill.
 GPA_DEV void copy16(uint4* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
                : "memory");
@@ -588,14 +604,27 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto read = [&](int slot, int dt, float (&v)[8]) {
+  // two channels to an instruction: the kernel is bound by its instructions
+  struct V8 {
+    float2 v[4];
+  };
+  auto read = [&](int slot, int dt) {
     Raw8 r;
     r.a = mine[slot];
     if (dt == kF32) r.b = mine[slot + n];
     else r.b = make_uint4(0, 0, 0, 0);
-    unraw(r, dt, v);
+    V8 o;
+    unraw(r, dt, reinterpret_cast<float(&)[8]>(o));
+    return o;
   };
-  float aw[1][8] = {}, ap[1][8] = {}, ac[1][8] = {};
+  auto load = [&](const float* q) {
+    V8 o;
+    ldv<8>(q, c, kF32, reinterpret_cast<float(&)[8]>(o));
+    return o;
+  };
+  auto store = [&](void* q, int64_t i, int dt, const V8& o) { stv<8>(q, i, dt, reinterpret_cast<const float(&)[8]>(o)); };
+  auto both = [](float f) { return make_float2(f, f); };
+  V8 aw = {}, ap = {}, ac = {};
   int s = 0;
   fetch_row(blockIdx.x, s);
   for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, s = stage - s) {
@@ -604,99 +633,101 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
     const int64_t at = (int64_t)row * p.width + c;
     float sums[3] = {0.f, 0.f, 0.f};  // x^2, w dn x, y^2
     if (in) {
-      float x[8], v[8], w[8];
-      read(s + sx * n, h_dt, x);
-      if (b.dn) {
-        read(s + sd * n, out_dt, v);
-        ldv<8>(p.w, c, kF32, w);
-      }
+      float2 xx = both(0.f), wx = both(0.f), yy = both(0.f);
+      const V8 x = read(s + sx * n, h_dt);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        sums[0] += x[k] * x[k];
-        if (b.dn) sums[1] += w[k] * v[k] * x[k];
+      for (int k = 0; k < 4; ++k) xx = __ffma2_rn(x.v[k], x.v[k], xx);
+      if (b.dn) {
+        const V8 d = read(s + sd * n, out_dt), w = load(p.w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) wx = __ffma2_rn(__fmul2_rn(w.v[k], d.v[k]), x.v[k], wx);
       }
       if (p.wp) {
-        read(s + sy * n, y_dt, v);
+        const V8 y = read(s + sy * n, y_dt);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sums[2] += v[k] * v[k];
+        for (int k = 0; k < 4; ++k) yy = __ffma2_rn(y.v[k], y.v[k], yy);
       }
+      sums[0] = xx.x + xx.y, sums[1] = wx.x + wx.y, sums[2] = yy.x + yy.y;
     }
     group_sum<0, 3>(sums, sm, buf);
     const float r = rsqrtf(sums[0] * inv + p.eps), q = sums[1] * inv * r * r;
     const float ry = p.wp ? rsqrtf(sums[2] * inv + p.eps) : 1.f;
     float gr = 1.f;
-    if (p.gate && !full) gr = gate_of(load_in(p.gate, row_at(p.rg, row, p.inner), g_dt));
+    if (p.gate && !full) gr = gate_near(load_in(p.gate, row_at(p.rg, row, p.inner), g_dt));
     float two[2] = {0.f, 0.f};  // wp du y, row-gate gradient
-    float d[8];
+    V8 d;
     if (in) {
-      float x[8], a[8];
-      read(s + sx * n, h_dt, x);
+      const V8 x = read(s + sx * n, h_dt);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = 0.f;
+      for (int k = 0; k < 4; ++k) d.v[k] = both(0.f);
       if (b.dn) {
-        float w[8];
-        read(s + sd * n, out_dt, d);
-        ldv<8>(p.w, c, kF32, w);
+        d = read(s + sd * n, out_dt);
+        const V8 w = load(p.w);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          aw[0][k] += d[k] * x[k] * r;
-          d[k] = r * (w[k] * d[k] - x[k] * q);
+        for (int k = 0; k < 4; ++k) {
+          aw.v[k] = __ffma2_rn(__fmul2_rn(d.v[k], x.v[k]), both(r), aw.v[k]);
+          d.v[k] = __fmul2_rn(both(r), __ffma2_rn(x.v[k], both(-q), __fmul2_rn(w.v[k], d.v[k])));
         }
       }
       if (b.ds) {
-        read(s + ss * n, h_dt, a);
+        const V8 e = read(s + ss * n, h_dt);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) d[k] += a[k];
+        for (int k = 0; k < 4; ++k) d.v[k] = __fadd2_rn(d.v[k], e.v[k]);
       }
-      if (b.dh) stv<8>(b.dh, at, h_dt, d);
+      if (b.dh) store(b.dh, at, h_dt, d);
+      V8 a;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) a[k] = gr;
+      for (int k = 0; k < 4; ++k) a.v[k] = both(gr);
       if (full) {
-        read(s + sg * n, g_dt, a);
+        a = read(s + sg * n, g_dt);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] = gate_of(a[k]);
+        for (int k = 0; k < 4; ++k) a.v[k] = make_float2(gate_near(a.v[k].x), gate_near(a.v[k].y));
       }
-      float cs[8], wp[8], y[8];
+      V8 cs, wp;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) wp[k] = 1.f, cs[k] = p.c;
+      for (int k = 0; k < 4; ++k) wp.v[k] = both(1.f), cs.v[k] = both(p.c);
       if (p.scale) {
-        ldv<8>(p.scale, c, kF32, cs);
+        cs = load(p.scale);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) cs[k] *= p.c;
+        for (int k = 0; k < 4; ++k) cs.v[k] = __fmul2_rn(cs.v[k], both(p.c));
       }
-      if (p.wp) ldv<8>(p.wp, c, kF32, wp);
-      read(s + sy * n, y_dt, y);
+      if (p.wp) wp = load(p.wp);
+      const V8 y = read(s + sy * n, y_dt);
+      float2 wy = both(0.f), gg = both(0.f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float u = y[k] * ry * wp[k], ga = d[k] * a[k];
-        ac[0][k] += ga * u * p.c;
-        const float du = ga * cs[k];
-        ap[0][k] += du * y[k] * ry;
-        a[k] = du * u * (1.f - a[k]);  // the gate's gradient
-        two[1] += a[k];
-        d[k] = du * wp[k];
-        two[0] += d[k] * y[k];
+      for (int k = 0; k < 4; ++k) {
+        const float2 yr = __fmul2_rn(y.v[k], both(ry)), u = __fmul2_rn(yr, wp.v[k]);
+        const float2 ga = __fmul2_rn(d.v[k], a.v[k]);
+        ac.v[k] = __ffma2_rn(__fmul2_rn(ga, u), both(p.c), ac.v[k]);
+        const float2 du = __fmul2_rn(ga, cs.v[k]);
+        ap.v[k] = __ffma2_rn(du, yr, ap.v[k]);
+        // the gate's gradient, du u (1 - a)
+        a.v[k] = __fmul2_rn(__fmul2_rn(du, u), __ffma2_rn(a.v[k], both(-1.f), both(1.f)));
+        gg = __fadd2_rn(gg, a.v[k]);
+        d.v[k] = __fmul2_rn(du, wp.v[k]);
+        wy = __ffma2_rn(d.v[k], y.v[k], wy);
       }
-      if (full && b.dgate) stv<8>(b.dgate, at, g_dt, a);
+      two[0] = wy.x + wy.y, two[1] = gg.x + gg.y;
+      if (full && b.dgate) store(b.dgate, at, g_dt, a);
     }
     const bool row_gate = p.gate && !full && b.dgate;
     if (p.wp || row_gate) group_sum<0, 2>(two, sm, buf);
     if (row_gate && t == 0) store_out(b.dgate, row, two[1], g_dt);
     if (!b.dy || !in) continue;
     if (p.wp) {
-      float y[8];
-      read(s + sy * n, y_dt, y);
+      const V8 y = read(s + sy * n, y_dt);
       const float qy = two[0] * inv * ry * ry;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = ry * (d[k] - y[k] * qy);
+      for (int k = 0; k < 4; ++k) d.v[k] = __fmul2_rn(both(ry), __ffma2_rn(y.v[k], both(-qy), d.v[k]));
     }
-    stv<8>(b.dy, at, y_dt, d);
+    store(b.dy, at, y_dt, d);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
-  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
-  if (b.sum_w >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_w * p.width, aw, p.width, n, t, 0, 1, nullptr);
-  if (b.sum_p >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_p * p.width, ap, p.width, n, t, 0, 1, nullptr);
-  if (b.sum_c >= 0) emit_sums<0, 8, 1>(part + (int64_t)b.sum_c * p.width, ac, p.width, n, t, 0, 1, nullptr);
+  if (!in) return;
+  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width + c;
+  if (b.sum_w >= 0) stv<8>(part + (int64_t)b.sum_w * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(aw));
+  if (b.sum_p >= 0) stv<8>(part + (int64_t)b.sum_p * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(ap));
+  if (b.sum_c >= 0) stv<8>(part + (int64_t)b.sum_c * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(ac));
 }
 
 // out[k][c] = sum over blocks of part[block][k][c] (k: blockIdx.y), always in the same order: 32

@@ -367,3 +367,22 @@ def test_tensors_that_move_between_forward_and_backward():
         assert torch.equal(a, b)
     (dw,) = torch.autograd.grad(n, (w,), up)
     assert dw.isfinite().all()
+
+
+def test_gates_at_the_ends_of_their_range():
+    """Closed, open and saturated gates: 0, 1 and the values between, and no NaN from infinities."""
+    a = torch.tensor([-float("inf"), -1e30, -200., -88., -87.5, -86., -20., -1., -0., 1e-30, 1., 20., 86., 200.,
+                      1e30, float("inf")], device="cuda")
+    width = 64
+    g = _gen(31)
+    h, u = _randn(g, (16, width)), _randn(g, (16, width))
+    w = torch.ones(width, device="cuda")
+    for gate in (a[:, None].contiguous(), a[:, None].expand(16, width).contiguous()):
+        gate.requires_grad_()
+        s, n = residual_norm(h, u, w, EPS, gate=gate)
+        ref.check("stream", s, ref.stream_of(h, u, None, gate, None, 1.0, EPS))
+        assert torch.equal(s[0], h[0]) and torch.equal(s[-1], h[-1] + u[-1])
+        (da,) = torch.autograd.grad((s, n), (gate,), (u, u))
+        assert da.isfinite().all() and not da[:3].any() and not da[-3:].any()
+    nan = torch.full((16, 1), float("nan"), device="cuda")
+    assert residual_norm(h, u, w, EPS, gate=nan)[0].isnan().all()
