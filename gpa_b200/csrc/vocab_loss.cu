@@ -107,6 +107,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, typename Part<T>::type* dst) {
   __shared__ int part[8];
   __shared__ int place[kRun];
+  let_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int run = min((int)blockIdx.x, p.runs);
   int before = 0;
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, 
                                               float* total, bool mean, int* counter) {
   __shared__ float2 sm[256];
   __shared__ bool last;
+  after_previous();
   const int rows = *c.n_rows, lanes = blockDim.y, tid = threadIdx.y * blockDim.x + threadIdx.x;
   const int64_t j = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const bool live = j < rows;
@@ -277,6 +279,7 @@ __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Ca
 template <typename T, int kV>
 __global__ void k_finish(const float* __restrict__ part, int64_t part_stride, const Call c, const int* pos,
                          const Upstream up, float unit, T* __restrict__ dx) {
+  after_previous();
   const int64_t i = blockIdx.x;
   const int j = pos[i], parts = c.n_rows[2];
   const float s = up.scale(*c.n_rows) * unit;
@@ -458,16 +461,15 @@ void copy_weight(const GpaLossArgs* a, const Plan& p, char* saved, cudaStream_t 
 }
 
 template <typename T>
-void finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, const Upstream& up, void* dx,
+bool finish(const Plan& p, const float* dxp, int64_t stride, const int* pos, const Upstream& up, void* dx,
             cudaStream_t st) {
   constexpr int kV = 16 / sizeof(T);
   const Call& c = p.c;
   const float unit = 1.f / tc_p_scale(c.dtype);
   Launch scope("loss_finish", st);
-  if (c.width % kV == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0)
-    k_finish<T, kV><<<(unsigned)c.n, 128, 0, st>>>(dxp, stride, c, pos, up, unit, static_cast<T*>(dx));
-  else
-    k_finish<T, 1><<<(unsigned)c.n, 128, 0, st>>>(dxp, stride, c, pos, up, unit, static_cast<T*>(dx));
+  const bool vec = c.width % kV == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0;
+  return launch_next(vec ? k_finish<T, kV> : k_finish<T, 1>, (unsigned)c.n, 128, 0, st, dxp, stride, c, pos, up, unit,
+                     static_cast<T*>(dx));
 }
 
 // the kernels read and write the workspaces 32 bytes at a time
@@ -553,11 +555,11 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
     // few rows: more lanes for the tiles of each
     const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;
     Launch scope("loss_join", st);
-    k_join<<<(unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st>>>(
-        c, part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
-        reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
-        a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1);
-    OK_OR("loss_join launch failed");
+    if (!launch_next(k_join, (unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st, c,
+                     part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
+                     reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
+                     a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1))
+      FAIL("loss_join launch failed");
   }
   return GPA_B200_OK;
 }
@@ -623,8 +625,9 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
     }
   }
   if (dhidden) {
-    BY_TYPE(a->dtype, finish<T>(p, dxp, part_stride, reinterpret_cast<const int*>(sv + p.s_pos), up, dhidden, st));
-    OK_OR("loss_finish launch failed");
+    bool ok = false;
+    BY_TYPE(a->dtype, ok = finish<T>(p, dxp, part_stride, reinterpret_cast<const int*>(sv + p.s_pos), up, dhidden, st));
+    if (!ok) FAIL("loss_finish launch failed");
   }
   return GPA_B200_OK;
 }

@@ -68,6 +68,29 @@ __host__ __device__ inline int parts_of(const Split& s, int tiles_m, int* k_part
   return (s.blocks + *k_part - 1) / *k_part;
 }
 
+// The kernels of a call follow one another closely: each lets the next one start its blocks
+// (let_next) and does what needs no results first, then waits until everything before it on the
+// stream is done (after_previous, by every thread, before its first access to global memory).
+// 8 x 1024 x 151936 scores: 67.3 -> 63.9 us; 2457 x 1000 x 32003 step: 663 -> 643 us.
+GPA_DEV void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+GPA_DEV void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that calls after_previous; any other kernel is launched the usual way.
+template <typename... P, typename... A>
+bool launch_next(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess;
+}
+
 // The products, on tensor cores (vocab_loss_tc5.cu); false when a launch failed.
 // They tile by kTile x kTile and pair up the SMs: tc_pairs() tiles run at a time.
 int tc_pairs();

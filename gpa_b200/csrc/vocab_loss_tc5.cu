@@ -605,13 +605,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
     }
     tc5::mbar_fence_init();
   }
-  if (M == kProbsT)
-    for (int j = threadIdx.x; j < BN; j += threads_of(M, F32)) table[j] = row_of<F32>(a, j, *a.c.n_rows);
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tc5::saddr(slot))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  let_next();
+  after_previous();
+  if (M == kProbsT)
+    for (int j = threadIdx.x; j < BN; j += threads_of(M, F32)) table[j] = row_of<F32>(a, j, *a.c.n_rows);
   tc5::fence_before_sync();
   __syncthreads();
   pair_sync();
@@ -821,8 +823,7 @@ bool launch_as(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, c
   }
   const int pairs = (int)std::min<int64_t>(tiles, tc_pairs());
   Launch scope(name, st);
-  k_product<M, F32, BN, PRODUCTS><<<2 * pairs, threads_of(M, F32), kSmem, st>>>(ma, mb, a);
-  return cudaGetLastError() == cudaSuccess;
+  return launch_next(k_product<M, F32, BN, PRODUCTS>, 2 * pairs, threads_of(M, F32), kSmem, st, ma, mb, a);
 }
 
 bool exact_stats(const Call& c) { return c.dtype == GPA_B200_F32 || c.pitch > kSegment16 * kBK; }
