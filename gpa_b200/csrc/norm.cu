@@ -16,9 +16,8 @@
 //   65536 x 1024, fp32 stream, bf16 update and result: forward 127 us = 6.3 TB/s, backward 163 us
 //   (6.6), fold of the weight gradient 7 us;  262144 x 128 bf16, plain: 27 us (5.0) and 55 us (3.7);
 //   8188 x 2560 bf16 with post weight, gate and scale: 61 us (3.4) and 96 us (3.5).
-// Column sums of the backward stay in registers over a
-// block's rows, go to one partial row per block and are added in block order by a second
-// kernel, so results do not depend on scheduling.
+// Column sums of the backward stay in registers over a block's rows, go to one partial row per
+// block and are added in block order by a second kernel, so results do not depend on scheduling.
 #include "../../include/gpa_b200.h"
 #include "common.cuh"
 #include "norm.cuh"
@@ -622,7 +621,9 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
     ldv<8>(q, c, kF32, reinterpret_cast<float(&)[8]>(o));
     return o;
   };
-  auto store = [&](void* q, int64_t i, int dt, const V8& o) { stv<8>(q, i, dt, reinterpret_cast<const float(&)[8]>(o)); };
+  auto store = [&](void* q, int64_t i, int dt, const V8& o) {
+    stv<8>(q, i, dt, reinterpret_cast<const float(&)[8]>(o));
+  };
   auto both = [](float f) { return make_float2(f, f); };
   V8 aw = {}, ap = {}, ac = {};
   int s = 0;
@@ -817,13 +818,10 @@ int built_types(const Fwd& f, int stream_dt) {
   return f.gate && f.g_dt != f.y_dt ? kAny : types_of(stream_dt, f.y_dt, f.out_dt);
 }
 
-}  // namespace
-
-namespace {
-
 const char* fill(const GpaNormArgs* a, Fwd* f) {
   if (!a) return "args is NULL";
-  if (a->outer < 0 || a->inner < 0 || a->width < 1) return "outer, inner and width must not be negative, width at least 1";
+  if (a->outer < 0 || a->inner < 0 || a->width < 1)
+    return "outer, inner and width must not be negative, width at least 1";
   for (int dt : {a->stream_dtype, a->update_dtype, a->gate_dtype, a->out_dtype})
     if (dt < 0 || dt > 2) return "dtypes must be F32, BF16 or F16";
   if (!a->update && !a->residual) return "update must not be NULL";
@@ -870,8 +868,9 @@ bool vec_ok(const Fwd& f) {
 // Blocks of the backward: as many as run at once, each with many rows, so that its column sums
 // are added in registers and few partial rows are left.  At most 8 blocks of 128 threads an SM.
 int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
-// 0: the kernel cannot have its shared memory.
-using Known = std::atomic<int>[8][33];  // a kernel's blocks per SM by device and warps of a block (0: not asked yet)
+// 0: the kernel cannot have its shared memory.  Known: a kernel's blocks per SM by device and warps
+// of a block, 0 where not asked yet.
+using Known = std::atomic<int>[8][33];
 int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, Known& known) {
   const uint32_t per = s.group ? s.threads / s.group : 1;
   int dev = 0;
@@ -987,6 +986,10 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     *why = "scratch is smaller than gpa_b200_norm_scratch_bytes";
     return GPA_B200_BAD_ARGUMENT;
   }
+  if (b.sums && !aligned8(scratch)) {
+    *why = "scratch must start on 16 bytes";
+    return GPA_B200_BAD_ARGUMENT;
+  }
   f.stream = const_cast<void*>(stream_in);
   f.h = nullptr;  // the backward reads the stream, not the residual that went in
   b.dn = dnormed;
@@ -1035,7 +1038,7 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
 #undef CALL
 #undef LIGHT
 #undef RUN
-    if (cudaGetLastError() != cudaSuccess) {
+    if (cudaGetLastError() != cudaSuccess || !blocks) {
       *why = "norm_bwd launch failed";
       return GPA_B200_LAUNCH_FAILURE;
     }

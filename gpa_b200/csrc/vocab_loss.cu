@@ -192,8 +192,8 @@ GPA_DEV void merge(float& m, float& s, float m2, float s2) {
 }
 
 // Maximum and 1 / sum of exp, and loss, of each packed row from the (max, sum) pairs of its
-// tiles: blockDim.x rows a block, blockDim.y lanes of tiles each (256 threads).  The block that finishes last adds the losses of
-// a mean or sum in double, in a fixed order.
+// tiles: blockDim.x rows a block, blockDim.y lanes of tiles each (256 threads).  The block that
+// finishes last adds the losses of a mean or sum in double, in a fixed order.
 __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, int tiles, const float* z_label,
                                               float2* lse, float* each, const int* pos, float* packed,
                                               float* total, bool mean, int* counter) {

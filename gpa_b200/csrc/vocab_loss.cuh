@@ -61,7 +61,8 @@ __host__ __device__ inline int parts_of(const Split& s, int tiles_m, int* k_part
   int parts = 1;
   float cost = 3e38f;
   for (int n = 1; n <= s.most; ++n) {
-    const float now = (float)((s.tiles_d * tiles_m * n + s.at_once - 1) / s.at_once) / n * s.turn + n * tiles_m * s.pass;
+    const int turns = (s.tiles_d * tiles_m * n + s.at_once - 1) / s.at_once;
+    const float now = (float)turns / n * s.turn + n * tiles_m * s.pass;
     if (now < cost) cost = now, parts = n;
   }
   *k_part = (s.blocks + parts - 1) / parts;

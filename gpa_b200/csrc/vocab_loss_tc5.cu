@@ -27,9 +27,10 @@
 // x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
 // step of 16, so a long reduction would lose what the parts gained: the accumulator is emptied
 // after a segment of it and the segments are added in registers, in round-to-nearest fp32, by
-// more epilogue warps (four threads a row of 256 columns, 64 registers each).  The statistics of 16-bit inputs are formed the same
-// way beyond 1024 channels: the loss is an fp32 result, and its error would grow with the width
-// (2048 channels: 1.1e-6 of the loss in one accumulator, 0.5e-6 in two).
+// more epilogue warps (four threads a row of 256 columns, 64 registers each).  The statistics of
+// 16-bit inputs are formed the same way beyond 1024 channels: the loss is an fp32 result, and its
+// error would grow with the width (2048 channels: 1.1e-6 of the loss in one accumulator, 0.5e-6
+// in two).
 //
 // Measured (GPU time of one launch, B200): 65536 rows x 1024 channels x 151936 entries, bf16:
 // statistics 16.3 ms = 1.25 PFLOP/s, P 18.4 ms, dx 15.7 ms, dW 15.4 ms (1.30 PFLOP/s; a library
@@ -657,7 +658,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
               tma_load(sb, &map_b, rb, pb + kk, bar);
               tma_load(sb + kOperand / 2, &map_b, rb + 64, pb + kk, bar);
             } else {
-              for (int b = 0; b < parts_b; ++b) tma_load(sb + b * S::kColumns, &map_b, kk, pb + b * a.b_plane + rb, bar);
+              for (int b = 0; b < parts_b; ++b)
+                tma_load(sb + b * S::kColumns, &map_b, kk, pb + b * a.b_plane + rb, bar);
             }
           }
         }
@@ -875,8 +877,9 @@ int tc_pairs() {
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(k_product<kStats, false, 256, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_product<kStats, false, 256, 1>, &cfg) != cudaSuccess || n < 1) {
+    auto* kernel = k_product<kStats, false, 256, 1>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = std::max(1, sms / 2);
     }
@@ -889,7 +892,8 @@ int tc_stats_parts(const Call& c) {
   const int64_t tiles = (c.vocab + kTile - 1) / kTile;
   const bool exact = exact_stats(c);
   if (!c.few) return (int)(exact ? 4 * tiles : tiles);
-  return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * (exact && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes);
+  const int lanes = exact && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes;
+  return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * lanes;
 }
 
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {

@@ -6,9 +6,12 @@
 * :func:`linear_cross_entropy` -- softmax cross entropy over a large vocabulary, in pieces of it
   and without keeping the logits.
 
-They take CUDA tensors in float32, bfloat16 or float16 (the norms any mix of them), sum in fp32, run on
-the current stream without synchronising, allocate through PyTorch, can be captured in a CUDA
-graph and have first-order gradients.  They raise ``ValueError`` for arguments they refuse.
+They take CUDA tensors in float32, bfloat16 or float16 (the norms any mix of them), sum in fp32,
+run on the current stream without synchronising, allocate through PyTorch, can be captured in a
+CUDA graph and have first-order gradients.  They raise ``ValueError`` for arguments they refuse.
+
+As for any PyTorch operator, a backward that is captured must find no eager graph of the same
+leaves alive: their gradient accumulators would belong to the eager stream.
 """
 from __future__ import annotations
 
@@ -129,7 +132,8 @@ def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, s
     g, g0, g1 = _NONE if gate is None else _rows(gate)
     a = _lib.GpaNormArgs(
         _lib.ptr(h), _lib.ptr(y), _lib.ptr(g), weight.data_ptr(), _lib.ptr(post_weight),
-        _lib.ptr(scale), math.prod(shape[:-2]) if inner else 0, inner, h0, h1, y0, y1, g0, g1, width, _DTYPES[stream_dtype], _DTYPES[update_dtype], 0 if g is None else _DTYPES[g.dtype],
+        _lib.ptr(scale), math.prod(shape[:-2]) if inner else 0, inner, h0, h1, y0, y1, g0, g1,
+        width, _DTYPES[stream_dtype], _DTYPES[update_dtype], 0 if g is None else _DTYPES[g.dtype],
         _DTYPES[out_dtype], 0 if g is None else 2 if g.shape[-1] == width else 1, eps, const)
     return a, (h, y, g)
 

@@ -239,7 +239,8 @@ typedef struct GpaNormGrads {
 
 /* stream [rows, width] (stream_dtype; ignored for the plain norm), normed [rows, width]. */
 int gpa_b200_norm_forward(const GpaNormArgs* args, void* stream_out, void* normed, void* stream);
-/* Bytes of the backward's scratch (0 for arguments the entry points refuse). */
+/* Bytes of the backward's scratch (0 for arguments the entry points refuse); it starts on 16
+ * bytes. */
 size_t gpa_b200_norm_scratch_bytes(const GpaNormArgs* args);
 /* stream_in: the forward's stream_out.  dstream / dnormed may be NULL (zero).  args->update is
  * read only for the plain norm or with a post weight, gate or scale vector; args->residual is

@@ -69,6 +69,8 @@ def test_norm_entry_points_refuse_missing_tensors():
     g.dweight = 16  # a weight gradient needs scratch
     assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, None, 0, None) == 1
     assert "scratch" in _message()
+    assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, 20, 1 << 30, None) == 1
+    assert "16 bytes" in _message()
     a = _args()
     assert lib.gpa_b200_norm_scratch_bytes(a) >= 2 * 8 * 4
 
