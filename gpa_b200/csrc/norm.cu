@@ -46,7 +46,8 @@ struct Bwd {
   Fwd f;                  // stream: the rounded h' of the forward (NULL for the plain norm)
   const void *dn, *ds;    // contiguous gradients of n and h' (either may be NULL)
   void *dh, *dy, *dgate;
-  float *part;            // [blocks][sums][width]
+  float *part;            // [blocks][sums][width], or NULL: one block, which writes the sums themselves
+  float *sums_out[3];     // by slot
   int sum_w, sum_p, sum_c, sums;  // slot of dw / dwp / dc in a partial row, or -1
 };
 
@@ -299,6 +300,11 @@ __global__ void __launch_bounds__(MT) k_norm_fwd(const Fwd p) {
   }
 }
 
+// where a block leaves its column sums of one weight
+GPA_DEV float* sums_at(const Bwd& b, int slot) {
+  return b.part ? b.part + ((int64_t)blockIdx.x * b.sums + slot) * b.f.width : b.sums_out[slot];
+}
+
 // Column sums of a block's rows into its partial row: registers of one group, or of the block's
 // groups added through shared memory.
 template <int G, int VEC, int ITER>
@@ -455,9 +461,8 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
       stv<VEC>(b.dy, at + c, y_dt, d[i]);
     }
   }
-  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width;
   auto emit = [&](int slot, const float (&a)[ITER][VEC]) {
-    if (slot >= 0) emit_sums<G, VEC, ITER>(part + (int64_t)slot * p.width, a, p.width, g, t, mine, per, fold);
+    if (slot >= 0) emit_sums<G, VEC, ITER>(sums_at(b, slot), a, p.width, g, t, mine, per, fold);
   };
   emit(b.sum_w, aw);
   emit(b.sum_p, ap);
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
       stv<8>(b.dy, at, p.y_dt, d);
     }
   }
-  if (b.sum_w >= 0) emit_sums<G, 8, 1>(b.part + (int64_t)blockIdx.x * p.width, aw, p.width, g, t, mine, per, fold);
+  if (b.sum_w >= 0) emit_sums<G, 8, 1>(sums_at(b, b.sum_w), aw, p.width, g, t, mine, per, fold);
 }
 
 // Backward with a post weight, a gate or a scale, over rows of whole blocks with 8 channels a
@@ -725,10 +730,9 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (!in) return;
-  float* part = b.part + (int64_t)blockIdx.x * b.sums * p.width + c;
-  if (b.sum_w >= 0) stv<8>(part + (int64_t)b.sum_w * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(aw));
-  if (b.sum_p >= 0) stv<8>(part + (int64_t)b.sum_p * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(ap));
-  if (b.sum_c >= 0) stv<8>(part + (int64_t)b.sum_c * p.width, 0, kF32, reinterpret_cast<const float(&)[8]>(ac));
+  if (b.sum_w >= 0) store(sums_at(b, b.sum_w), c, kF32, aw);
+  if (b.sum_p >= 0) store(sums_at(b, b.sum_p), c, kF32, ap);
+  if (b.sum_c >= 0) store(sums_at(b, b.sum_c), c, kF32, ac);
 }
 
 // out[k][c] = sum over blocks of part[block][k][c] (k: blockIdx.y), always in the same order: 32
@@ -868,6 +872,10 @@ bool vec_ok(const Fwd& f) {
 // Blocks of the backward: as many as run at once, each with many rows, so that its column sums
 // are added in registers and few partial rows are left.  At most 8 blocks of 128 threads an SM.
 int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
+// Few rows go to one block, which writes the sums itself: up to 8 turns of narrow rows (28 x 96: 105
+// -> 97 us eager, most of it the host's, 8.3 us replayed either way), 2 of wide ones (6 x 647 in one
+// block: 139 -> 130 us eager, but 16 -> 35 us replayed).
+uint32_t one_block(const Shape& s) { return s.group ? 8 : 2; }
 // 0: the kernel cannot have its shared memory.  Known: a kernel's blocks per SM by device and warps
 // of a block, 0 where not asked yet.
 using Known = std::atomic<int>[8][33];
@@ -886,7 +894,8 @@ int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, K
     if (dev < 8) known[dev][s.threads / 32].store(at_once, std::memory_order_relaxed);
   }
   const uint32_t need = (rows + per - 1) / per;
-  return (int)std::max(1u, std::min(need, (uint32_t)std::min(148 * at_once, most_blocks(s))));
+  if (need <= one_block(s)) return 1;
+  return (int)std::min(need, (uint32_t)std::min(148 * at_once, most_blocks(s)));
 }
 
 }  // namespace
@@ -938,8 +947,13 @@ int norm_forward(const GpaNormArgs* a, void* stream_out, void* normed, cudaStrea
 namespace {
 // whichever variant runs, its partial rows fit
 size_t partial_floats(const Fwd& f) {
-  const int b = std::max(most_blocks(shape_of(f, true)), most_blocks(shape_of(f, false)));
-  return (size_t)std::min<int64_t>(b, f.rows) * 3 * f.width;
+  size_t most = 0;
+  for (bool vec : {true, false}) {
+    const Shape s = shape_of(f, vec);
+    const uint32_t per = s.group ? s.threads / s.group : 1, need = (f.rows + per - 1) / per;
+    if (need > one_block(s)) most = std::max<size_t>(most, std::min<size_t>(need, most_blocks(s)));
+  }
+  return most * 3 * f.width;
 }
 }  // namespace
 
@@ -982,11 +996,12 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
       }
     return GPA_B200_OK;
   }
-  if (b.sums && (!scratch || scratch_bytes < partial_floats(f) * sizeof(float))) {
+  const size_t want = partial_floats(f) * sizeof(float);
+  if (b.sums && want && (!scratch || scratch_bytes < want)) {
     *why = "scratch is smaller than gpa_b200_norm_scratch_bytes";
     return GPA_B200_BAD_ARGUMENT;
   }
-  if (b.sums && !aligned8(scratch)) {
+  if (b.sums && want && !aligned8(scratch)) {
     *why = "scratch must start on 16 bytes";
     return GPA_B200_BAD_ARGUMENT;
   }
@@ -997,9 +1012,11 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
   b.dh = g->dresidual;
   b.dy = g->dupdate;
   b.dgate = g->dgate;
-  b.part = static_cast<float*>(scratch);
+  for (int k = 0, slot = 0; k < 3; ++k)
+    if (out[k]) b.sums_out[slot++] = out[k];
   const bool vec = vec_ok(f) && aligned8(dnormed) && aligned8(dstream) && aligned8(g->dresidual) &&
-                   aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate));
+                   aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate)) && aligned8(g->dweight) &&
+                   aligned8(g->dpost_weight) && aligned8(g->dscale);
   const Shape s = shape_of(f, vec);
   const bool light = s.vec == 8 && s.iter == 1 && !f.wp && !f.scale && !f.gate;
   int blocks = 0;
@@ -1010,6 +1027,7 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     static Known known;                                                          \
     const size_t smem = (SMEM);                                                  \
     blocks = bwd_blocks(s, f.rows, reinterpret_cast<const void*>(&K), smem, known); \
+    b.part = blocks > 1 ? static_cast<float*>(scratch) : nullptr;                \
     if (blocks) K<<<blocks, s.threads, smem, st>>>(b);                           \
   } while (0)
 #define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>), fold_smem)
@@ -1043,10 +1061,9 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
       return GPA_B200_LAUNCH_FAILURE;
     }
   }
-  if (!b.sums) return GPA_B200_OK;
+  if (!b.sums || blocks == 1) return GPA_B200_OK;
   Sums sums = {};
-  for (int k = 0, slot = 0; k < 3; ++k)
-    if (out[k]) sums.out[slot++] = out[k];
+  for (int k = 0; k < 3; ++k) sums.out[k] = b.sums_out[k];
   Launch scope("norm_fold", st);
   k_norm_fold<<<dim3((f.width + 31) / 32, b.sums), dim3(32, 32), 0, st>>>(b.part, blocks, b.sums, f.width, sums);
   if (cudaGetLastError() != cudaSuccess) {

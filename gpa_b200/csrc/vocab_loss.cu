@@ -1,6 +1,6 @@
 // Softmax cross entropy of z = x W^T over a large vocabulary, in pieces of it, without keeping z:
 //   m_i = max_v z_iv    s_i = sum_v exp(z_iv - m_i)    loss_i = m_i - z_{i, y_i} + log s_i
-//   P_iv = (exp(z_iv - m_i) / s_i - [v = y_i]) r_i        dx = s P W        dW = s P^T x
+//   P_iv = exp(z_iv - m_i) / s_i - [v = y_i]        dx_i = s r_i (P W)_i        dW = s P^T (r x)
 // with the upstream gradient of row i written as s r_i (see Upstream).
 //
 // Rows without a label are dropped first: the labelled ones are packed (k_pack), so masked
@@ -258,8 +258,8 @@ __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, 
   }
 }
 
-// fp16, a gradient for each row: s = the largest magnitude, r = its share (fp16's range would lose
-// the products otherwise).
+// fp16, a gradient for each row: s = the largest magnitude, r = its share (x times r would leave
+// fp16's range otherwise).
 __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Call c, float* r, float* scale) {
   __shared__ float sm[32];
   const int n = *c.n_rows;
@@ -274,15 +274,38 @@ __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Ca
   if (threadIdx.x == 0) *scale = s;
 }
 
-// dx of the caller's rows: the parts added in order, scaled, rounded; zero for rows without a
-// label.  kV channels a thread at a time.
+// The packed rows times their r, as dW takes them where each has a gradient of its own: rounded
+// once more to the inputs' type (fp32: its parts formed again).  A warp a row, zero behind the
+// last one up to a multiple of 64.
+template <typename T>
+__global__ void __launch_bounds__(256) k_scale(const Call c, const Upstream up, typename Part<T>::type* dst) {
+  using E = typename Part<T>::type;
+  const int rows = *c.n_rows;
+  const int64_t j = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), plane = c.n_pad * c.pitch;
+  if (j >= (rows + 63) / 64 * 64) return;
+  const float r = j < rows ? up.r(c, j) : 0.f;
+  const E* src = static_cast<const E*>(c.x) + j * c.pitch;
+  E* d = dst + j * c.pitch;
+  for (int k = threadIdx.x & 31; k < c.pitch; k += 32) {
+    if (j >= rows) {
+      put(d + k, plane, T(0.f));
+    } else if constexpr (sizeof(T) == 4) {
+      put(d + k, plane, ((float)src[k] + (float)src[plane + k] + (float)src[2 * plane + k]) * r);
+    } else {
+      put(d + k, plane, T((float)src[k] * r));
+    }
+  }
+}
+
+// dx of the caller's rows: the parts added in order, times the row's gradient, rounded; zero for rows
+// without a label.  kV channels a thread at a time.
 template <typename T, int kV>
 __global__ void k_finish(const float* __restrict__ part, int64_t part_stride, const Call c, const int* pos,
                          const Upstream up, float unit, T* __restrict__ dx) {
   after_previous();
   const int64_t i = blockIdx.x;
   const int j = pos[i], parts = c.n_rows[2];
-  const float s = up.scale(*c.n_rows) * unit;
+  const float s = j < 0 ? 0.f : up.scale(*c.n_rows) * up.r(c, j) * unit;
   T* out = dx + i * c.width;
   const float* p = part + (int64_t)j * c.pitch;
   for (int k = threadIdx.x * kV; k < c.width; k += blockDim.x * kV) {
@@ -328,7 +351,7 @@ struct Plan {
   int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
   // scratch
   int64_t count, part, z_label, loss, fwd_bytes;
-  int64_t p, dxp, dwp, r, scale, bwd_bytes;
+  int64_t p, dxp, dwp, xr, r, scale, bwd_bytes;
 };
 
 const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
@@ -410,6 +433,7 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->p = take(c.planes * c.n_pad * p->piece * 2);
   p->dxp = take((int64_t)p->split.most * c.n_pad * c.pitch * 4);
   p->dwp = take(p->piece * c.pitch * p->es);
+  p->xr = take(a->reduction == GPA_B200_LOSS_NONE ? c.planes * c.n_pad * c.pitch * 2 : 0);
   p->r = take(4 * c.n);
   p->scale = take(4);
   p->bwd_bytes = at;
@@ -597,26 +621,35 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
   const bool none = a->reduction == GPA_B200_LOSS_NONE;
-  Upstream up = {none ? dloss : nullptr, true, none ? nullptr : dloss, a->reduction == GPA_B200_LOSS_MEAN};
-  if (none && a->dtype == GPA_B200_F16) {
-    float* r = reinterpret_cast<float*>(sc + p.r);
-    float* s = reinterpret_cast<float*>(sc + p.scale);
-    Launch scope("loss_row_scale", st);
-    k_row_scale<<<1, 1024, 0, st>>>(dloss, c, r, s);
-    OK_OR("loss_row_scale launch failed");
-    up = {r, false, s, false};
+  const Upstream up = {none ? dloss : nullptr, true, none ? nullptr : dloss, a->reduction == GPA_B200_LOSS_MEAN};
+  Upstream up_w = up;
+  const void* x = c.x;
+  if (none && dweight) {
+    if (a->dtype == GPA_B200_F16) {
+      float* r = reinterpret_cast<float*>(sc + p.r);
+      float* s = reinterpret_cast<float*>(sc + p.scale);
+      Launch scope("loss_row_scale", st);
+      k_row_scale<<<1, 1024, 0, st>>>(dloss, c, r, s);
+      OK_OR("loss_row_scale launch failed");
+      up_w = {r, false, s, false};
+    }
+    Launch scope("loss_scale", st);
+    BY_TYPE(a->dtype, (k_scale<T><<<(unsigned)(c.n_pad / 8), 256, 0, st>>>(
+                          c, up_w, reinterpret_cast<typename Part<T>::type*>(sc + p.xr))));
+    OK_OR("loss_scale launch failed");
+    x = sc + p.xr;
   }
   const int64_t part_stride = c.n_pad * c.pitch;
   // pieces start at multiples of 256 rows: every row of dW on 16 bytes (32 for fp32), or none
   const bool in_place = c.width == c.pitch && (reinterpret_cast<uintptr_t>(dweight) & (p.es == 4 ? 31 : 15)) == 0;
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
-    if (!tc_probs(c, v0, vn, lse, up, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
+    if (!tc_probs(c, v0, vn, lse, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
     if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.split.most, v0 > 0, dxp, part_stride, st))
       FAIL("loss_dx_tc5 launch failed");
     if (!dweight) continue;
     char* dw = static_cast<char*>(dweight) + v0 * c.width * p.es;
-    if (!tc_dw(c, pr, p.piece, v0, vn, up, in_place ? dw : sc + p.dwp, c.pitch, st)) FAIL("loss_dw_tc5 launch failed");
+    if (!tc_dw(c, pr, p.piece, v0, vn, x, up_w, in_place ? dw : sc + p.dwp, c.pitch, st)) FAIL("loss_dw_tc5 launch failed");
     if (!in_place) {
       Launch scope("loss_unpad", st);
       BY_TYPE(a->dtype, (k_unpad<T><<<(unsigned)((vn + 7) / 8), 256, 0, st>>>(

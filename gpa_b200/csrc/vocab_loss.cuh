@@ -28,8 +28,8 @@ struct Call {
   int few;            // 32 or 128: at least n, and z and dx are formed transposed; 0: more rows
 };
 
-// The gradient of a packed row's loss, as s r with |r| <= 1 where fp16 needs it:
-//   r: 1 (each == NULL), each[row] (by_row) or each[packed row];  NaN for a label outside the vocabulary
+// The gradient of a packed row's loss, s r:
+//   r: 1 (each == NULL), each[row] (by_row) or each[packed row]
 //   s: *s (1 if NULL), over the number of labelled rows for a mean
 struct Upstream {
   const float* each;
@@ -37,7 +37,6 @@ struct Upstream {
   const float* s;
   bool mean;
   __device__ __forceinline__ float r(const Call& c, int64_t j) const {
-    if (c.label[j] < 0) return NAN;
     return !each ? 1.f : each[by_row ? c.row[j] : j];
   }
   __device__ __forceinline__ float scale(int n_rows) const {
@@ -98,13 +97,12 @@ int tc_pairs();
 int tc_stats_parts(const Call& c);  // (max, sum) pairs of a row that tc_stats leaves
 float tc_p_scale(int dtype);  // P is stored times this
 bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st);
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
-              int64_t p_pitch, cudaStream_t st);
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, void* p, int64_t p_pitch, cudaStream_t st);
 bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, int most_parts, bool add,
            float* dx, int64_t dx_part, cudaStream_t st);
-// dW of a piece; its rows are a multiple of 8 values long and start on 16 bytes (fp32: 32)
-bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
-           int64_t dw_pitch, cudaStream_t st);
+// dW of a piece, from x or its rows times their r (the same planes); its rows are a multiple of 8 values long and start on 16 bytes (fp32: 32)
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const void* x, const Upstream& up,
+           void* dw, int64_t dw_pitch, cudaStream_t st);
 
 }  // namespace vloss
 

@@ -344,13 +344,14 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
     }
     if (live) a.part[(int64_t)(F32 ? 4 * t.n + group : t.n) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
-    // P is rounded once to the type of its product's other operand: the relative error of a logit's
-    // gradient is half a step of that type, the same as the caller's own rounding of dx and dW.
-    // (fp32: three parts, 24 bits.)  fp16 takes it times 2^14 (tc_p_scale): a probability of
-    // 2^-28 keeps its full precision, and the largest value is 2^14 |r|.
+    // P is rounded once to the type of its product's other operand, half a step of it (fp32: three
+    // parts, 24 bits), without the row's gradient r: where the label's entry outweighs the others
+    // it stays near -1 and its rounding is small.  fp16 takes P times 2^14 (tc_p_scale): a
+    // probability of 2^-28 keeps its full precision.
     const bool live = row < n_rows;
     const float2 l = live ? a.lse[row] : make_float2(0.f, 0.f);
-    const float r = live ? a.up.r(a.c, row) * a.p_scale : 0.f, f = l.y * r, off = l.x * kLog2e;
+    const float one = live && a.c.label[row] < 0 ? NAN : a.p_scale;  // no such label: the row is NaN
+    const float f = l.y * one, off = l.x * kLog2e;
     const int64_t y = live ? (int64_t)a.c.label[row] - a.v0 - col0 : -1;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p) + row * a.p_pitch + col0);
     const int64_t plane = a.c.n_pad * a.p_pitch / 2;
@@ -363,7 +364,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (y == c + i) v[i] -= r;
+          if (y == c + i) v[i] -= one;
       }
       const int64_t left = live ? a.vn - col0 - c : 0;
 #pragma unroll
@@ -515,14 +516,14 @@ struct Stats {
   }
 };
 
-// {max (times log2 e for 16-bit inputs), factor of the exp, r, label within the piece} of row j of x
+// {max (times log2 e for 16-bit inputs), factor of the exp, P's unit, label within the piece} of row j of x
 template <bool F32>
 GPA_DEV float4 row_of(const Args& a, int j, int n_rows) {
   if (j >= n_rows) return make_float4(0.f, 0.f, 0.f, __int_as_float(-2));  // no row
   const float2 l = a.lse[j];
-  const float r = a.up.r(a.c, j) * a.p_scale;
+  const float one = a.c.label[j] < 0 ? NAN : a.p_scale;
   const int64_t y = (int64_t)a.c.label[j] - a.v0;
-  return make_float4(F32 ? l.x : l.x * kLog2e, l.y * r, r, __int_as_float(y >= 0 && y < a.vn ? (int)y : -1));
+  return make_float4(F32 ? l.x : l.x * kLog2e, l.y * one, one, __int_as_float(y >= 0 && y < a.vn ? (int)y : -1));
 }
 
 template <Mode M, bool F32, int BN>
@@ -917,14 +918,12 @@ bool tc_stats(const Call& c, float2* part, float* z_label, cudaStream_t st) {
   return launch<kStats, 256>("loss_stats_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile), st);
 }
 
-bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, const Upstream& up, void* p,
-              int64_t p_pitch, cudaStream_t st) {
+bool tc_probs(const Call& c, int64_t v0, int64_t vn, const float2* lse, void* p, int64_t p_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   Args a = base_args(c);
   a.v0 = v0;
   a.vn = vn;
   a.lse = lse;
-  a.up = up;
   a.p = p;
   a.p_pitch = p_pitch;
   if (c.few) return launch_z_t<kProbsT>("loss_probs_tc5", a, st);
@@ -963,12 +962,12 @@ bool tc_dx(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
   return launch<kDx, 256>("loss_dx_tc5", ma, mb, a, (int64_t)a.tiles_n * (c.n_pad / kTile) * most_parts, st);
 }
 
-bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const Upstream& up, void* dw,
-           int64_t dw_pitch, cudaStream_t st) {
+bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn, const void* x, const Upstream& up,
+           void* dw, int64_t dw_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
   if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kBK, f16) ||
-      !make_map(&mb, c.x, c.pitch, c.planes * c.n_pad, c.pitch, kBK, f16))
+      !make_map(&mb, x, c.pitch, c.planes * c.n_pad, c.pitch, kBK, f16))
     return false;
   Args a = base_args(c);
   a.v0 = v0;

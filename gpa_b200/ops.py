@@ -29,7 +29,7 @@ MAX_NORM_WIDTH = 16384
 
 
 def _on(device):
-    """`device` as the current one: the library sizes its workspaces and launches for that."""
+    """`device` as the current one: the library sizes the loss's workspaces for that."""
     return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
@@ -68,8 +68,13 @@ def _first_order(backward):
 
 
 def _call(fn, device, *args):
-    """`fn(*args, stream)` on the current stream of `device`, which is current."""
-    rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    """`fn(*args, stream)` on the current stream of `device`, made the current device."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
     if rc:
         _lib.check(rc, fn.__name__)
 
@@ -141,11 +146,10 @@ def _norm_args(residual, update, weight, post_weight, gate, scale, eps, const, s
 def _norm_backward(a, device, stream_in, dstream, dnormed, grads):
     lib = _lib.load()
     g = _lib.GpaNormGrads(*[None if t is None else t.data_ptr() for t in grads])
-    with _on(device):
-        nbytes = lib.gpa_b200_norm_scratch_bytes(a)
-        scratch = _scratch(nbytes, device)
-        _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
-              _lib.ptr(dnormed), g, scratch.data_ptr(), nbytes)
+    nbytes = lib.gpa_b200_norm_scratch_bytes(a)
+    scratch = _scratch(nbytes, device) if nbytes else None
+    _call(lib.gpa_b200_norm_backward, device, a, _lib.ptr(stream_in), _lib.ptr(dstream),
+          _lib.ptr(dnormed), g, _lib.ptr(scratch), nbytes)
 
 
 _DENSE = torch.contiguous_format
@@ -159,8 +163,7 @@ def _rms_forward(x, weight, eps, out_dtype, args=None):
     out = torch.empty_like(x, dtype=out_dtype, memory_format=_DENSE)
     if out.numel():
         a, keep = _rms_args(x, weight, eps, out_dtype) if args is None else args
-        with _on(x.device):
-            _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
+        _call(_lib.load().gpa_b200_norm_forward, x.device, a, None, out.data_ptr())
     return out
 
 
@@ -222,9 +225,8 @@ def _residual_forward(residual, update, weight, post_weight, gate, scale, eps, c
     if stream.numel():
         a, keep = args or _residual_args(residual, update, weight, post_weight, gate, scale, eps,
                                          const, out_dtype)
-        with _on(residual.device):
-            _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
-                  normed.data_ptr())
+        _call(_lib.load().gpa_b200_norm_forward, residual.device, a, stream.data_ptr(),
+              normed.data_ptr())
     return stream, normed
 
 
@@ -416,7 +418,8 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
 
     ``reduction``: "mean" over the labelled tokens (0 when there is none), "sum", or "none" (a
     loss for each token, 0 where ignored).  Gradients: hidden and weight, rounded once to their
-    dtype; with 16-bit inputs the gradient of each logit is rounded to that type on the way.
+    dtype; with 16-bit inputs the gradient of each logit is rounded to that type on the way, and
+    under "none" so are the hidden rows times their own gradients, for the weight's.
     """
     _check_tensor("hidden", hidden)
     dev = hidden.device

@@ -5,7 +5,8 @@ products (16-bit inputs; each rounded once more for fp32 ones) whose additions l
 the running magnitude each, whether they round or truncate: Ez = 2 (D + 2) U sum |x| |w|.  The
 loss takes two logits and an exp / log of relative error below 64 U.  A gradient of a logit is
 P = exp(z - lse) - [v = y]: its exp part is off by that relative error plus 2 max Ez, and P is
-rounded once to the input's type when that has 16 bits.  The products with P then add
+rounded once to the input's type when that has 16 bits.  Each row's own gradient (reduction "none")
+multiplies dx in fp32, and the rows that dW takes, rounded to their type.  The products with P then add
 2 (n + 2) U sum |P| |w| over their n terms, and the result is rounded once.
 """
 from __future__ import annotations
@@ -60,15 +61,16 @@ def _reference(x, w, y, up, reduction):
     ep = soft * (2 * worst + 64 * U) + U * (soft + hot)
     p = soft - hot
     if dtype != F32:
-        # rounded once to the type, with the row's factor g / max g in it: fp16 underflows at
-        # 2^-25 of the scale 2^14 that keeps small probabilities in range
-        ep = ep + HALF[dtype] * (p.abs() + ep)
-        if dtype == F16:
-            big = g.abs().max() if n else 1.0
-            ep = ep + 2.0 ** -39 * big / g.abs().clamp_min(1e-300)
+        # rounded once to the type: fp16 underflows at 2^-25 of the scale 2^14 that keeps small
+        # probabilities in range
+        ep = ep + HALF[dtype] * (p.abs() + ep) + (2.0 ** -39 if dtype == F16 else 0.0)
     p, ep = p * g, ep * g.abs() * (1 + 4 * U)
     dx, ex = p @ w, ep @ w.abs() + 2 * (v + 2) * U * (p.abs() @ w.abs())
     dw, ew = p.T @ xk, ep.T @ xk.abs() + 2 * (n + 2) * U * (p.abs().T @ xk.abs())
+    if dtype != F32 and reduction == "none" and n:
+        # dW takes the rows times their own gradients, rounded once more (fp16: as shares of the
+        # largest gradient, which may fall below its normal range)
+        ew = ew + HALF[dtype] * (p.abs().T @ xk.abs()) + TINY[dtype] * g.abs().max() * (soft + hot).sum(0)[:, None]
     fx, fe = torch.zeros_like(x), torch.zeros_like(x)
     fx[keep], fe[keep] = dx, ex + (HALF[dtype] + 4 * U) * (dx.abs() + ex) + TINY[dtype]
     out["dhidden"] = (fx.view(shape), fe.view(shape))

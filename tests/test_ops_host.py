@@ -66,13 +66,14 @@ def test_norm_entry_points_refuse_missing_tensors():
     assert lib.gpa_b200_norm_backward(_args(), None, None, None, g, None, 0, None) == 1  # no dupdate
     g.dresidual = 16
     assert lib.gpa_b200_norm_backward(_args(residual=16), None, None, None, g, None, 0, None) == 1
-    g.dweight = 16  # a weight gradient needs scratch
-    assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, None, 0, None) == 1
+    g.dweight = 16  # a weight gradient over many rows needs scratch
+    many = _args(residual=16, outer=1000)
+    assert lib.gpa_b200_norm_backward(many, 16, None, None, g, None, 0, None) == 1
     assert "scratch" in _message()
-    assert lib.gpa_b200_norm_backward(_args(residual=16), 16, None, None, g, 20, 1 << 30, None) == 1
+    assert lib.gpa_b200_norm_backward(many, 16, None, None, g, 20, 1 << 30, None) == 1
     assert "16 bytes" in _message()
-    a = _args()
-    assert lib.gpa_b200_norm_scratch_bytes(a) >= 2 * 8 * 4
+    assert lib.gpa_b200_norm_scratch_bytes(many) >= 5 * 8 * 4
+    assert lib.gpa_b200_norm_scratch_bytes(_args()) == 0  # one block takes so few rows
 
 
 @pytest.mark.parametrize("name", ["dpost_weight", "dscale", "dgate"])
