@@ -12,7 +12,8 @@
 // epilogue warps empty one while the next tile's products go to the other.
 //
 //   warp 0: copies     warp 1: products (first CTA of the pair)     warp 2: tensor memory
-//   warps 4-7: epilogue, a thread for each row of the tile
+//   warps 4-11: epilogue, two threads for each row of the tile (one: D of 135 channels leaves so few
+//   products to a tile that its epilogue bounds it; 21010 x 135 x 9393 bf16 step 646 -> 612 us)
 //
 // Up to 128 rows of x would leave most of such a tile empty, and what counts then is how fast W
 // comes by.  There z and dx are formed the other way round (kStatsT, kProbsT, kDxT): 256 vocabulary
@@ -80,7 +81,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode { kStats, kProbs, kDx, kDw, kStatsT, kProbsT, kDxT };
 // groups of four epilogue warps: threads that share a row of the tile
-__host__ __device__ constexpr int groups_of(Mode m, bool f32) { return !f32 ? 1 : m >= kStatsT ? 2 : 4; }
+__host__ __device__ constexpr int groups_of(Mode m, bool f32) {
+  return f32 ? (m >= kStatsT ? 2 : 4) : m >= kStatsT ? 1 : 2;
+}
 __host__ __device__ constexpr int threads_of(Mode m, bool f32) { return 128 + 128 * groups_of(m, f32); }
 
 struct Args {
@@ -304,11 +307,11 @@ struct Row<true, CW> {
 
 template <Mode M, bool F32, bool EXACT>
 GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& held, int rank, bool empty) {
-  constexpr int kChunks = F32 ? 2 : 8, kUnroll = F32 ? 2 : 1;
-  const int group = F32 ? (threadIdx.x - 128) >> 7 : 0;  // of the tile's columns
+  constexpr int kGroups = groups_of(M, F32), kChunks = 8 / kGroups, kUnroll = F32 ? kChunks : 1;
+  const int group = (threadIdx.x - 128) >> 7;  // of the tile's columns
   const int in_tile = rank * kHalf + (threadIdx.x & 127);
   const int64_t row = (int64_t)t.m * kTile + in_tile;
-  const int64_t col0 = (int64_t)t.n * kTile + group * 64;
+  const int64_t col0 = (int64_t)t.n * kTile + group * (kTile / kGroups);
   float buffer[32];
   if (M == kStats) {
     const bool live = row < n_rows;
@@ -342,7 +345,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
       sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
     }
-    if (live) a.part[(int64_t)(F32 ? 4 * t.n + group : t.n) * a.c.n_pad + row] = make_float2(big, sum);
+    if (live) a.part[((int64_t)t.n * kGroups + group) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
     // P is rounded once to the type of its product's other operand, half a step of it (fp32: three
     // parts, 24 bits), without the row's gradient r: where the label's entry outweighs the others
@@ -734,7 +737,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
             }
           }
         } else {
-          held.tmem = tmem + buf * kTile;
+          held.tmem = tmem + buf * kTile + (kT ? 0 : half * 128);
           done(false);
         }
         tc5::fence_before_sync();
@@ -892,7 +895,7 @@ int tc_pairs() {
 int tc_stats_parts(const Call& c) {
   const int64_t tiles = (c.vocab + kTile - 1) / kTile;
   const bool exact = exact_stats(c);
-  if (!c.few) return (int)(exact ? 4 * tiles : tiles);
+  if (!c.few) return (int)tiles * groups_of(kStats, exact);
   const int lanes = exact && c.few == 32 ? Cols<true, 32>::kLanes : Cols<false, 32>::kLanes;
   return (int)(2 * std::min<int64_t>(tiles, tc_pairs())) * lanes;
 }
