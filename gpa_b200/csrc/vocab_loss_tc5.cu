@@ -148,8 +148,11 @@ GPA_DEV void commit2(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// Hands an accumulator back.  It was read, and the reads waited for (ld32, ld16), so the arrival has no
+// memory to publish; a release would first wait until the tile's results have reached memory, which
+// held the accumulator 1900 cycles longer (16384 x 256 x 32000: statistics 309 -> 255 us, P 401 -> 312 us).
 GPA_DEV void arrive_first(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 GPA_DEV bool try_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -206,6 +209,27 @@ GPA_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// The epilogues of 16-bit inputs are bound by instructions where channels are few: two values at an
+// instruction where there is one, and P's factor as a term of its exponent (16384 x 256 x 32000: P 453 -> 401
+// us, statistics 317 -> 309 us; with 1024 channels, under the power limit, P 848 -> 764 us).
+
+// v log2(e) - off
+GPA_DEV void scaled2(float& a, float& b, float off) {
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %2};\nmov.b64 z, {%3, %3};\n"
+      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(kLog2e), "f"(-off));
+}
+GPA_DEV void add2(float& a, float& b, float x, float y) {
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}"
+      : "+f"(a), "+f"(b)
+      : "f"(x), "f"(y));
+}
+GPA_DEV float max3(float a, float b, float c) {
+  float m;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
 }
 GPA_DEV uint32_t pack2(float a, float b, bool f16) {
   if (f16) {
@@ -305,8 +329,26 @@ struct Row<true, CW> {
   }
 };
 
+// What the statistics and P take from memory for a thread's row, read while the tile before is dealt
+// with (16384 x 256 x 32000: statistics 255 -> 245 us, P 314 -> 308 us).
+struct RowIn {
+  int label;   // -1: no row, or no such label
+  float2 lse;  // zero: no row
+};
+template <Mode M>
+GPA_DEV RowIn row_in(const Args& a, const Tile& t, int n_rows, int rank) {
+  const int64_t row = (int64_t)t.m * kTile + rank * kHalf + (threadIdx.x & 127);
+  RowIn in = {-1, {0.f, 0.f}};
+  if ((M == kStats || M == kProbs) && row < n_rows) {
+    in.label = a.c.label[row];
+    if (M == kProbs) in.lse = a.lse[row];
+  }
+  return in;
+}
+
 template <Mode M, bool F32, bool EXACT>
-GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& held, int rank, bool empty) {
+GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& held, const RowIn& in, int rank,
+                      bool empty) {
   constexpr int kGroups = groups_of(M, F32), kChunks = 8 / kGroups, kUnroll = F32 ? kChunks : 1;
   const int group = (threadIdx.x - 128) >> 7;  // of the tile's columns
   const int in_tile = rank * kHalf + (threadIdx.x & 127);
@@ -315,7 +357,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
   float buffer[32];
   if (M == kStats) {
     const bool live = row < n_rows;
-    const int64_t y = live ? (int64_t)a.c.label[row] - col0 : -1;
+    const int64_t y = in.label - col0;  // not in the tile when negative
     float big = -INFINITY, sum = 0.f;
 #pragma unroll kUnroll
     for (int k = 0; k < kChunks; ++k) {
@@ -332,15 +374,19 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
         for (int i = 0; i < 32; ++i)
           if (i >= left) v[i] = -INFINITY;
       }
-      float m = big;
+      float m = big, m1 = v[0];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+      for (int i = 0; i < 32; i += 4) {
+        m = max3(m, v[i], v[i + 1]);
+        m1 = max3(m1, v[i + 2], v[i + 3]);
+      }
+      m = fmaxf(m, m1);
       const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        s0 += EXACT ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
-        s1 += EXACT ? expf(v[i + 1] - safe) : ex2(fmaf(v[i + 1], kLog2e, -off));
+        if (!EXACT) scaled2(v[i], v[i + 1], off);
+        add2(s0, s1, EXACT ? expf(v[i] - safe) : ex2(v[i]), EXACT ? expf(v[i + 1] - safe) : ex2(v[i + 1]));
       }
       sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
@@ -352,10 +398,10 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
     // it stays near -1 and its rounding is small.  fp16 takes P times 2^14 (tc_p_scale): a
     // probability of 2^-28 keeps its full precision.
     const bool live = row < n_rows;
-    const float2 l = live ? a.lse[row] : make_float2(0.f, 0.f);
-    const float one = live && a.c.label[row] < 0 ? NAN : a.p_scale;  // no such label: the row is NaN
-    const float f = l.y * one, off = l.x * kLog2e;
-    const int64_t y = live ? (int64_t)a.c.label[row] - a.v0 - col0 : -1;
+    const float2 l = in.lse;
+    const float one = live && in.label < 0 ? NAN : a.p_scale;  // no such label: the row is NaN
+    const float f = l.y * one, off = EXACT ? l.x : fmaf(l.x, kLog2e, -log2f(f));
+    const int64_t y = in.label - a.v0 - col0;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.p) + row * a.p_pitch + col0);
     const int64_t plane = a.c.n_pad * a.p_pitch / 2;
 #pragma unroll kUnroll
@@ -363,16 +409,22 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
       const int c = 32 * k;
       float (&v)[32] = held.take(k, buffer);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = (EXACT ? expf(v[i] - l.x) : ex2(fmaf(v[i], kLog2e, -off))) * f;
+      for (int i = 0; i < 32; i += 2) {
+        if (!EXACT) scaled2(v[i], v[i + 1], off);
+        v[i] = EXACT ? expf(v[i] - off) * f : ex2(v[i]);
+        v[i + 1] = EXACT ? expf(v[i + 1] - off) * f : ex2(v[i + 1]);
+      }
       if (y >= c && y < c + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (y == c + i) v[i] -= one;
       }
       const int64_t left = live ? a.vn - col0 - c : 0;
+      if (left < 32) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i >= left) v[i] = 0.f;
+        for (int i = 0; i < 32; ++i)
+          if (i >= left) v[i] = 0.f;
+      }
 #pragma unroll
       for (int q = 0; q < (F32 ? 3 : 1); ++q) {
         uint32_t w[16];
@@ -709,15 +761,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
     Stats<F32, BN, kPlanes> stats;
     float* square = reinterpret_cast<float*>(sm + S::kSquares) + half * 32 * kSquare;
     if constexpr (M == kStatsT) stats.start(a, walk.n_rows);
+    constexpr bool kRows = M == kStats || M == kProbs;
+    RowIn next = {};
+    if (kRows && pair < walk.total) next = row_in<M>(a, walk.at(pair), walk.n_rows, rank);
     for (int t = pair; t < walk.total && ok; t += pairs) {
       const Tile x = walk.at(t);
+      const RowIn in = next;
+      if (kRows && t + pairs < walk.total) next = row_in<M>(a, walk.at(t + pairs), walk.n_rows, rank);
       Row<F32, kCw> held;
       const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (dx)
       if (none && M != kDw) continue;
       auto done = [&](bool empty) {
         if constexpr (M == kStatsT) stats.tile(a, x, held, rank, square);
         else if constexpr (kT) epilogue_t<M, F32, BN>(a, x, walk.n_rows, held, rank, table);
-        else epilogue<M, F32, kPlanes>(a, x, walk.n_rows, held, rank, empty);
+        else epilogue<M, F32, kPlanes>(a, x, walk.n_rows, held, in, rank, empty);
       };
       for (int k0 = x.k0; k0 < x.k1; k0 = segment_end(k0, x.k1), ++count) {
         const uint32_t buf = count & 1, use = count >> 1;
@@ -737,7 +794,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
             }
           }
         } else {
-          held.tmem = tmem + buf * kTile + (kT ? 0 : half * 128);
+          held.tmem = tmem + buf * kTile + (kT ? 0 : half * (kTile / groups_of(M, F32)));
           done(false);
         }
         tc5::fence_before_sync();
