@@ -148,7 +148,7 @@ GPA_DEV void commit2(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
-// Hands an accumulator back.  It was read, and the reads waited for (ld32, ld16), so the arrival has no
+// Hands an accumulator back.  It was read, and the reads waited for (ld32, ld8), so the arrival has no
 // memory to publish; a release would first wait until the tile's results have reached memory, which
 // held the accumulator 1900 cycles longer (16384 x 256 x 32000: statistics 309 -> 255 us, P 401 -> 312 us).
 GPA_DEV void arrive_first(uint32_t bar) {
@@ -200,9 +200,16 @@ GPA_DEV void ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-GPA_DEV void ld16(uint32_t taddr, float (&v)[16]) {
-  tc5::tmem_ld16(taddr, v);
+// 8 at a time where 64 sums stay in registers: 16 would spill more of them (16384 x 1024 x 32000, fp32: P 1766
+// -> 1712 us a piece).
+GPA_DEV void ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
   tc5::tmem_wait_ld();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 GPA_DEV float ex2(float x) {
@@ -330,7 +337,7 @@ struct Row<true, CW> {
 };
 
 // What the statistics and P take from memory for a thread's row, read while the tile before is dealt
-// with (16384 x 256 x 32000: statistics 255 -> 245 us, P 314 -> 308 us).
+// with (16384 x 256 x 32000: statistics 255 -> 245 us, P 314 -> 308 us); not where sums fill the registers.
 struct RowIn {
   int label;   // -1: no row, or no such label
   float2 lse;  // zero: no row
@@ -385,8 +392,13 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        if (!EXACT) scaled2(v[i], v[i + 1], off);
-        add2(s0, s1, EXACT ? expf(v[i] - safe) : ex2(v[i]), EXACT ? expf(v[i + 1] - safe) : ex2(v[i + 1]));
+        if (F32) {  // one at a time: pairs would spill more of the sums (2048 x 2048 x 50000: 364 -> 341 us)
+          s0 += EXACT ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
+          s1 += EXACT ? expf(v[i + 1] - safe) : ex2(fmaf(v[i + 1], kLog2e, -off));
+          continue;
+        }
+        scaled2(v[i], v[i + 1], off);
+        add2(s0, s1, ex2(v[i]), ex2(v[i + 1]));
       }
       sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
       big = m;
@@ -761,20 +773,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
     Stats<F32, BN, kPlanes> stats;
     float* square = reinterpret_cast<float*>(sm + S::kSquares) + half * 32 * kSquare;
     if constexpr (M == kStatsT) stats.start(a, walk.n_rows);
-    constexpr bool kRows = M == kStats || M == kProbs;
+    constexpr bool kAhead = !F32 && (M == kStats || M == kProbs);
     RowIn next = {};
-    if (kRows && pair < walk.total) next = row_in<M>(a, walk.at(pair), walk.n_rows, rank);
+    if (kAhead && pair < walk.total) next = row_in<M>(a, walk.at(pair), walk.n_rows, rank);
     for (int t = pair; t < walk.total && ok; t += pairs) {
       const Tile x = walk.at(t);
       const RowIn in = next;
-      if (kRows && t + pairs < walk.total) next = row_in<M>(a, walk.at(t + pairs), walk.n_rows, rank);
+      if (kAhead && t + pairs < walk.total) next = row_in<M>(a, walk.at(t + pairs), walk.n_rows, rank);
       Row<F32, kCw> held;
       const bool none = x.k0 >= x.k1;  // no labelled row (kDw), or no entry of the piece (dx)
       if (none && M != kDw) continue;
       auto done = [&](bool empty) {
         if constexpr (M == kStatsT) stats.tile(a, x, held, rank, square);
         else if constexpr (kT) epilogue_t<M, F32, BN>(a, x, walk.n_rows, held, rank, table);
-        else epilogue<M, F32, kPlanes>(a, x, walk.n_rows, held, in, rank, empty);
+        else
+          epilogue<M, F32, kPlanes>(a, x, walk.n_rows, held, kAhead ? in : row_in<M>(a, x, walk.n_rows, rank), rank,
+                                    empty);
       };
       for (int k0 = x.k0; k0 < x.k1; k0 = segment_end(k0, x.k1), ++count) {
         const uint32_t buf = count & 1, use = count >> 1;
@@ -784,11 +798,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
         tc5::fence_after_sync();
         if constexpr (F32) {
 #pragma unroll
-          for (int c = 0; c < kCw; c += 16) {
-            float v[16];
-            ld16(tc5::tmem_at(tmem, buf * kTile + half * kCw + c), v);
+          for (int c = 0; c < kCw; c += 8) {
+            float v[8];
+            ld8(tc5::tmem_at(tmem, buf * kTile + half * kCw + c), v);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < 8; ++i) {
               float& sum = held.acc[(c + i) / held.kCh][(c + i) % held.kCh];
               sum = k0 == x.k0 ? v[i] : sum + v[i];
             }
