@@ -34,10 +34,10 @@
 // in two).
 //
 // Measured (GPU time of one launch, B200): 65536 rows x 1024 channels x 151936 entries, bf16:
-// statistics 16.3 ms = 1.25 PFLOP/s, P 18.4 ms, dx 15.7 ms, dW 15.4 ms (1.30 PFLOP/s; a library
+// statistics 16.4 ms = 1.24 PFLOP/s, P 16.7 ms, dx 15.5 ms, dW 15.3 ms (1.33 PFLOP/s; a library
 // product of 8192^3 sustains 1.38 under the power limit, which bounds all four).  2048 x 2048 x
-// 50000, fp16: dW 275 us = 1.53 PFLOP/s (1.65 in a burst).  1026 x 512 x 16001, fp32: dW 107 us =
-// 157 TFLOP/s of fp32 products, 940 of bf16 ones.  8 x 1024 x 151936, bf16: statistics 53 us =
+// 50000, fp16: dW 275 us = 1.53 PFLOP/s (1.65 in a burst).  1026 x 512 x 16001, fp32: dW 97 us =
+// 173 TFLOP/s of fp32 products, 1040 of bf16 ones.  8 x 1024 x 151936, bf16: statistics 53 us =
 // 5.9 TB/s of W.  One CTA instead of the pair was not built: its shared memory would bound it.
 //
 // Every wait is bounded (tc5.cuh); a wait that gives up sets the device status and the kernel
