@@ -13,7 +13,7 @@ from ctypes import (POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_
 
 MAX_LEVELS = 8
 MAX_EDGES = 56
-ABI_VERSION = 3
+ABI_VERSION = 4
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgpa_b200.so")
 
 STATUS = {0: "ok", 1: "bad argument", 2: "unsupported configuration", 3: "CUDA launch failure",
@@ -83,8 +83,8 @@ EXPORTS = ("gpa_b200_saved_bytes", "gpa_b200_scratch_bytes", "gpa_b200_forward",
            "gpa_b200_profile_stop", "gpa_b200_forward_noalloc", "gpa_b200_noalloc_capacity",
            "gpa_b200_step", "gpa_b200_umma_selftest", "gpa_b200_device_status",
            "gpa_b200_norm_forward", "gpa_b200_norm_scratch_bytes", "gpa_b200_norm_backward",
-           "gpa_b200_loss_saved_bytes", "gpa_b200_loss_scratch_bytes", "gpa_b200_loss_forward",
-           "gpa_b200_loss_backward")
+           "gpa_b200_loss_saved_bytes", "gpa_b200_loss_scratch_bytes", "gpa_b200_loss_cut",
+           "gpa_b200_loss_forward", "gpa_b200_loss_backward")
 
 _lib = None
 
@@ -137,6 +137,8 @@ def load():
     lib.gpa_b200_loss_saved_bytes.restype = c_size_t
     lib.gpa_b200_loss_scratch_bytes.argtypes = [POINTER(GpaLossArgs), c_int]
     lib.gpa_b200_loss_scratch_bytes.restype = c_size_t
+    lib.gpa_b200_loss_cut.argtypes = [POINTER(GpaLossArgs), c_int64, POINTER(c_int64)]
+    lib.gpa_b200_loss_cut.restype = c_int
     lib.gpa_b200_loss_forward.argtypes = [POINTER(GpaLossArgs), c_void_p, c_void_p, c_size_t,
                                           c_void_p, c_size_t, c_void_p]
     lib.gpa_b200_loss_forward.restype = c_int

@@ -1125,6 +1125,13 @@ size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward) {
   return gpa::loss_scratch_bytes(args, backward);
 }
 
+int gpa_b200_loss_cut(const GpaLossArgs* args, int64_t labelled, int64_t* cut) {
+  g_last_error.clear();
+  const char* why = "";
+  const int rc = gpa::loss_cut(args, labelled, cut, &why);
+  return rc ? fail(rc, why) : rc;
+}
+
 int gpa_b200_loss_forward(const GpaLossArgs* args, float* loss, void* saved, size_t saved_bytes,
                           void* scratch, size_t scratch_bytes, void* stream) {
   g_last_error.clear();
@@ -1151,7 +1158,7 @@ int gpa_b200_last_error(char* buf, size_t len) {
   return g_last_error.empty() ? 0 : 1;
 }
 
-int gpa_b200_abi_version(void) { return 3; }
+int gpa_b200_abi_version(void) { return 4; }
 
 long long gpa_b200_launch_count(void) { return g_launches.load(); }
 

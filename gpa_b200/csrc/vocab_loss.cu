@@ -396,12 +396,14 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   for (int64_t t = best; t >= 1 && t >= std::min(tiles_v, most) / 2; --t)
     if (turns_of(t) < turns) turns = turns_of(t), best = t;
   p->piece = best * kTile;
-  // dx: parts of at least 512 entries, and of 256 MB in all beside the first.  A turn over a piece
-  // goes at about 1.4 PFLOP/s, the parts in fp32 at about 5 TB/s.
+  // dx: at most one part for every 512 entries, and 256 MB of them in all beside the first; the last
+  // one holds what is left.  Cut by the blocks that the first piece has, not by its tiles: every part
+  // of it then holds a block and is written, and later pieces, which add to the parts, may leave some
+  // out.  A turn over a piece goes at about 1.4 PFLOP/s, the parts in fp32 at about 5 TB/s.
   Split& d = p->split;
   d.tiles_d = (int)tiles_d;
   d.at_once = at_once;
-  d.blocks = (int)(p->piece / 64);
+  d.blocks = (int)((std::min(p->piece, c.vocab) + 63) / 64);
   const int64_t one = c.n_pad * c.pitch * 4;
   d.most = (int)std::max<int64_t>(1, std::min<int64_t>({tiles_m == 1 ? 2 * at_once : 16, p->piece / 512,
                                                         1 + (int64_t(1) << 28) / one}));
@@ -541,6 +543,23 @@ size_t loss_scratch_bytes(const GpaLossArgs* a, int backward) {
   Plan p;
   int code;
   return plan_of(a, &p, &code) ? 0 : backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+int loss_cut(const GpaLossArgs* a, int64_t labelled, int64_t* cut, const char** why) {
+  Plan p;
+  int code;
+  if ((*why = plan_of(a, &p, &code))) return code;
+  if (!cut || labelled < 0 || labelled > p.c.n) {
+    *why = "cut is NULL, or labelled not between 0 and the rows";
+    return GPA_B200_BAD_ARGUMENT;
+  }
+  int parts = p.split.parts, k_part = p.split.k_part;
+  if (!parts) parts = parts_of(p.split, (int)((labelled + kTile - 1) / kTile), &k_part);
+  cut[0] = std::min(p.piece, p.c.vocab);
+  cut[1] = (cut[0] + 63) / 64;
+  cut[2] = parts;
+  cut[3] = k_part;
+  return GPA_B200_OK;
 }
 
 int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_bytes, void* scratch,

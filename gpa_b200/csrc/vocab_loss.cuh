@@ -51,7 +51,7 @@ __host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1)
 // known; n_rows[2] holds the parts and n_rows[3] the reduction blocks (of 64) of each.
 struct Split {
   int tiles_d, at_once;  // tiles across dx, tiles that run at a time
-  int blocks;            // reduction blocks of a piece
+  int blocks;            // reduction blocks of 64 that the first piece has
   int most;              // parts that the buffer holds
   float turn, pass;      // seconds of a turn over a piece, and of writing and reading one part's tile row
   int parts, k_part;     // decided on the host where one row of tiles is all there can be (parts > 0)
@@ -107,6 +107,7 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
 }  // namespace vloss
 
 int loss_device_status(bool clear);
+int loss_cut(const GpaLossArgs* a, int64_t labelled, int64_t* cut, const char** why);
 int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_bytes, void* scratch,
                  size_t scratch_bytes, cudaStream_t st, const char** why);
 int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, const float* dloss,

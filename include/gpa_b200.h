@@ -274,6 +274,10 @@ typedef struct GpaLossArgs {
  * not start on 16 bytes). */
 size_t gpa_b200_loss_saved_bytes(const GpaLossArgs* args);
 size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward);
+/* How the backward sums dhidden over the vocabulary for `labelled` of the rows (on the host; for
+ * checks): cut[0] entries of the first piece, cut[1] its blocks of 64, cut[2] the parts that are summed
+ * apart and added, cut[3] blocks of each part (the last one has what is left, at least one). */
+int gpa_b200_loss_cut(const GpaLossArgs* args, int64_t labelled, int64_t* cut);
 /* loss: one fp32, or one per row for GPA_B200_LOSS_NONE (0 for rows without a label). */
 int gpa_b200_loss_forward(const GpaLossArgs* args, float* loss, void* saved, size_t saved_bytes,
                           void* scratch, size_t scratch_bytes, void* stream);
@@ -287,7 +291,7 @@ int gpa_b200_loss_backward(const GpaLossArgs* args, const void* saved, size_t sa
 /* Message of the last failure on the calling thread (0 if none). */
 int gpa_b200_last_error(char* buf, size_t len);
 
-/* ABI version of this header: 3 (the norm and loss entry points; 2: GpaDims.reader_mode, positional_moments and
+/* ABI version of this header: 4 (gpa_b200_loss_cut; 3: the norm and loss entry points; 2: GpaDims.reader_mode, positional_moments and
  * position; GpaParams / GpaParamGrads.moment_gain; GpaStateRef.moment; a third
  * offset word of gpa_b200_step). */
 int gpa_b200_abi_version(void);

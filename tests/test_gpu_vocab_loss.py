@@ -409,3 +409,32 @@ def test_first_call_of_a_process_may_be_captured():
 
 def test_no_tensor_core_kernel_timed_out():
     assert _lib.device_status() == 0
+
+
+def _spoil(nbytes):
+    """Memory that the next allocations get, filled with NaN."""
+    torch.cuda.empty_cache()
+    for size in nbytes:
+        torch.full((max(1, size // 4),), float("nan"), device="cuda")
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,labelled,width,vocab", [
+    (16, 16, 1024, 7000), (100, 100, 640, 8000), (200, 200, 384, 28996), (16, 16, 256, 6200), (100, 90, 512, 28996),
+    (512, 512, 512, 7000), (768, 768, 512, 7000), (4096, 200, 1024, 7000),
+])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_nothing_of_the_scratch_reaches_the_gradients(rows, labelled, width, vocab, dtype, reduction):
+    """Vocabularies that end in the last tile's first blocks of 64: the parts of dhidden that are
+    added up are all written.  The workspaces come from memory full of NaN."""
+    x, w, y = _inputs(rows + vocab, (rows,), width, vocab, dtype)
+    y[torch.randperm(rows, generator=torch.Generator().manual_seed(1)).cuda()[labelled:]] = -100
+    xr, wr = x.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = linear_cross_entropy(xr, wr, y, reduction=reduction)
+    up = torch.randn(loss.shape, generator=torch.Generator().manual_seed(2)).cuda()
+    _spoil([1 << 30])
+    dx, dw = torch.autograd.grad(loss, (xr, wr), up)
+    want = _reference(x, w, y, up, reduction)
+    _check("dhidden", dx, want["dhidden"])
+    _check("dweight", dw, want["dweight"])

@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes
+import math
+import random
 
 import pytest
 import torch
@@ -145,3 +147,38 @@ def test_loss_workspace_of_a_training_step_stays_small():
     lib = _lib.load()
     a = _loss_args(outer=8, inner=8192, width=1024, vocab=151936, weight_stride=1024)
     assert lib.gpa_b200_loss_scratch_bytes(a, 0) < 2.5e9 and lib.gpa_b200_loss_scratch_bytes(a, 1) < 2.5e9
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def _cut(rows, labelled, width, vocab, dtype):
+    a = _loss_args(outer=1, inner=rows, width=width, vocab=vocab, weight_stride=width, dtype=dtype)
+    cut = (ctypes.c_int64 * 4)()
+    assert _lib.load().gpa_b200_loss_cut(a, labelled, cut) == 0
+    return tuple(cut)
+
+
+def test_every_part_of_dhidden_is_written():
+    """The parts that are added up are fresh memory: each holds a block of the first piece, also
+    where the vocabulary ends inside a tile of 256."""
+    sizes = [(256, 256, 1024, 7000, 1), (17, 17, 640, 8000, 1), (256, 256, 384, 16000, 2), (1, 1, 384, 28996, 1),
+             (256, 256, 512, 28996, 0), (512, 512, 512, 7000, 1), (768, 768, 512, 7000, 0), (4096, 200, 1024, 7000, 1)]
+    rng = random.Random(5)
+    for _ in range(20000):
+        rows = _log(rng, 1, 20000)
+        sizes.append((rows, max(1, int(rows * rng.choice([1, 0.4, 0.05]))), _log(rng, 8, 8192), _log(rng, 1, 300000),
+                      rng.randrange(3)))
+    for size in sizes:
+        entries, blocks, parts, each = _cut(*size)
+        assert 1 <= entries <= size[3] and blocks == -(-entries // 64)
+        assert (parts - 1) * each < blocks <= parts * each, (size, blocks, parts, each)
+
+
+def test_cut_refuses_bad_arguments():
+    lib, cut = _lib.load(), (ctypes.c_int64 * 4)()
+    assert lib.gpa_b200_loss_cut(_loss_args(), -1, cut) == 1 and "labelled" in _message()
+    assert lib.gpa_b200_loss_cut(_loss_args(), 4, cut) == 1 and "labelled" in _message()
+    assert lib.gpa_b200_loss_cut(_loss_args(), 3, None) == 1
+    assert lib.gpa_b200_loss_cut(_loss_args(vocab=0), 3, cut) == 1 and "vocab" in _message()
