@@ -101,6 +101,29 @@ def _rows(t: Tensor):
     return _rows(t.contiguous())
 
 
+def _kept(tensors, as_saved):
+    """Saved tensors, checked for what the kernels take from the forward: whoever kept them
+    meanwhile (hooks on saved tensors, sharded parameters) may bring them back at another address
+    and with other strides, but not with another shape, type or device."""
+    for t, want in zip(tensors, as_saved):
+        if t is not None and (t.shape, t.dtype, t.device) != want:
+            raise RuntimeError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}, not "
+                               f"as {want[1]} {list(want[0])} on {want[2]}")
+    return tensors
+
+
+def _as_saved(*tensors):
+    return tuple(None if t is None else (t.shape, t.dtype, t.device) for t in tensors)
+
+
+def _stride(t):
+    return None if t is None else t.stride()
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def _check_tensor(name: str, t: Tensor, device=None):
     if t.is_cuda and t.dtype in _DTYPES and (device is None or t.device == device):
         return
@@ -174,20 +197,24 @@ class _RMSNorm(torch.autograd.Function):
         ctx.save_for_backward(x, weight)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args if args[1][1] is x else None
+        ctx.as_saved, ctx.stride = _as_saved(x, weight), x.stride()
         ctx.eps, ctx.out_dtype = eps, out_dtype
         return _rms_forward(x, weight, eps, out_dtype, args)
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
-        x, weight = ctx.saved_tensors
+        x, weight = _kept(ctx.saved_tensors, ctx.as_saved)
+        weight = _dense(weight)
         dx = torch.empty_like(x, memory_format=_DENSE)
         if not x.numel():
             return dx, torch.zeros_like(weight), None, None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        a, keep = ctx.args or _rms_args(x, weight, ctx.eps, ctx.out_dtype)
-        if ctx.args:  # the tensors may have moved since (sharded parameters do)
-            a.update, a.weight = x.data_ptr(), weight.data_ptr()
+        if ctx.args and x.stride() == ctx.stride:
+            a, keep = ctx.args
+            a.update, a.weight = x.data_ptr(), weight.data_ptr()  # which may have moved
+        else:
+            a, keep = _rms_args(x, weight, ctx.eps, ctx.out_dtype)
         _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
         return dx, dw, None, None
 
@@ -241,6 +268,8 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args[0] if args[1][1] is update and args[1][2] is gate else None
+        ctx.as_saved = _as_saved(stream, update, weight, post_weight, gate, scale)
+        ctx.strides = update.stride() if read else None, _stride(gate)
         ctx.update_dtype = update.dtype
         ctx.eps, ctx.const, ctx.out_dtype = eps, const, out_dtype
         ctx.set_materialize_grads(False)
@@ -251,7 +280,8 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dstream, dnormed):
         if dstream is None and dnormed is None:
             return (None,) * 9
-        stream, update, weight, post_weight, gate, scale = ctx.saved_tensors
+        stream, update, weight, post_weight, gate, scale = _kept(ctx.saved_tensors, ctx.as_saved)
+        stream, weight, post_weight, scale = map(_dense, (stream, weight, post_weight, scale))
         need = ctx.needs_input_grad
         dres = torch.empty_like(stream) if need[0] else None
         dupd = torch.empty_like(stream, dtype=ctx.update_dtype) if need[1] else None
@@ -265,10 +295,10 @@ class _ResidualNorm(torch.autograd.Function):
         dstream = None if dstream is None else dstream.contiguous()
         dnormed = None if dnormed is None else dnormed.contiguous()
         a, keep = ctx.args, None
-        if a is None:
+        if a is None or (_stride(update), _stride(gate)) != ctx.strides:
             a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
                                  stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
-        else:  # the tensors may have moved since (sharded parameters do)
+        else:  # the tensors may have moved
             a.update, a.weight, a.gate = _lib.ptr(update), weight.data_ptr(), _lib.ptr(gate)
             a.post_weight, a.scale = _lib.ptr(post_weight), _lib.ptr(scale)
         _norm_backward(a, stream.device, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
@@ -379,6 +409,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss, saved, ctx.args = _loss_forward(hidden, weight, labels, ignore_index, reduction, True)
         # the labelled rows are packed into `saved`: hidden and labels are not needed again
         ctx.save_for_backward(weight, saved)
+        ctx.as_saved, ctx.stride = _as_saved(weight, saved), weight.stride()
         ctx.hidden = hidden.shape, hidden.dtype
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
@@ -386,15 +417,18 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, dloss):
-        weight, saved = ctx.saved_tensors
+        weight, saved = _kept(ctx.saved_tensors, ctx.as_saved)
+        saved = _dense(saved)
         shape, dtype = ctx.hidden
         lib = _lib.load()
         dev = weight.device
         a, keep = ctx.args, None
-        if a is None:
+        if a is None or weight.stride() != ctx.stride or weight.data_ptr() != a.weight:
             a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
-        else:
-            a.weight = weight.data_ptr()  # which may have moved since (sharded parameters do)
+            if lib.gpa_b200_loss_saved_bytes(a) > saved.numel():
+                # the forward read the weight in place; where it is now that takes a copy of it
+                a, keep = _loss_args(weight.clone(memory_format=_DENSE), shape, dtype, ctx.ignore_index,
+                                     ctx.reduction)
         dx = torch.empty(shape, device=dev, dtype=dtype) if ctx.needs_input_grad[0] else None
         dw = torch.empty_like(weight, memory_format=_DENSE) if ctx.needs_input_grad[1] else None
         dloss = dloss.contiguous()

@@ -386,3 +386,28 @@ def test_gates_at_the_ends_of_their_range():
         assert da.isfinite().all() and not da[:3].any() and not da[-3:].any()
     nan = torch.full((16, 1), float("nan"), device="cuda")
     assert residual_norm(h, u, w, EPS, gate=nan)[0].isnan().all()
+
+
+def test_saved_tensors_that_come_back_with_other_strides():
+    """Kept on the host between forward and backward, strided inputs come back dense.  The gate then
+    starts on 16 bytes, which it does not in place: other sums, the same bounds."""
+    g = _gen(32)
+    joint, wide = _randn(g, (3, 50, 96), BF16), _randn(g, (3, 50, 200), BF16)
+    x, gate = (t.detach().requires_grad_() for t in (joint[..., 16:48], wide[..., 100:132]))
+    h, w = _randn(g, (3, 50, 32)), (1 + 0.1 * _randn(g, (32,))).requires_grad_()
+    up, upn = _randn(g, (3, 50, 32)), _randn(g, (3, 50, 32), BF16)
+
+    post = w.detach().clone().requires_grad_()
+
+    def step():
+        s, n = residual_norm(h, x, w, EPS, gate=gate, post_weight=post)
+        y = rms_norm(x, w)
+        return s, torch.autograd.grad((s, n), (x, gate, w, post), (up, upn)), torch.autograd.grad(y, (x, w), upn)
+
+    with torch.autograd.graph.save_on_cpu():
+        s, parts, plain = step()
+    want = ref.backward(s, x, w, post, gate, None, 1.0, EPS, up, upn)
+    for name, t in zip(("update", "gate", "weight", "post_weight"), parts):
+        ref.check("d" + name, t, want["d" + name])
+    for a, b in zip(step()[2], plain):
+        assert torch.equal(a, b)

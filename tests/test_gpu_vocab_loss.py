@@ -438,3 +438,17 @@ def test_nothing_of_the_scratch_reaches_the_gradients(rows, labelled, width, voc
     want = _reference(x, w, y, up, reduction)
     _check("dhidden", dx, want["dhidden"])
     _check("dweight", dw, want["dweight"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead", [(40,), (300,)])
+def test_saved_tensors_that_come_back_with_other_strides(lead, dtype):
+    """Kept on the host between forward and backward, a strided weight comes back dense."""
+    x, w, y = _inputs(18, lead, 64, 700, dtype)
+    wide = torch.zeros(700, 208, device="cuda", dtype=dtype)
+    wide[:, 16:80] = w
+    want = _run(x, w, y, "none")
+    with torch.autograd.graph.save_on_cpu():
+        got = _run(x, wide[:, 16:80], y, "none")
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)

@@ -1,6 +1,7 @@
 """Refusals of the language-model operators: checked on the host, before any CUDA call."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import random
@@ -8,7 +9,7 @@ import random
 import pytest
 import torch
 
-from gpa_b200 import _lib, linear_cross_entropy, residual_norm, rms_norm
+from gpa_b200 import _lib, ops, linear_cross_entropy, residual_norm, rms_norm
 
 
 def _message():
@@ -182,3 +183,133 @@ def test_cut_refuses_bad_arguments():
     assert lib.gpa_b200_loss_cut(_loss_args(), 4, cut) == 1 and "labelled" in _message()
     assert lib.gpa_b200_loss_cut(_loss_args(), 3, None) == 1
     assert lib.gpa_b200_loss_cut(_loss_args(vocab=0), 3, cut) == 1 and "vocab" in _message()
+
+
+class _Calls:
+    """The operators on CPU tensors, with the library's launches recorded instead of made.  Each
+    record holds the entry point's name and the arguments; the structures are copied."""
+
+    def __init__(self, monkeypatch):
+        self.made = []
+        monkeypatch.setattr(ops, "_check_tensor", lambda name, t, device=None: None)
+        monkeypatch.setattr(ops, "_on", lambda device: contextlib.nullcontext())
+        monkeypatch.setattr(ops, "_call", self._record)
+
+    def _record(self, fn, device, *args):
+        copied = [type(a).from_buffer_copy(a) if isinstance(a, ctypes.Structure) else a for a in args]
+        self.made.append((fn.__name__, copied))
+
+    def last(self, name):
+        return [a for n, a in self.made if n == name][-1]
+
+
+def _rows_inside(pointer, tensor, outer, inner, strides, width):
+    """Whether outer x inner rows at `strides` lie in the memory of `tensor`."""
+    last = (outer - 1) * strides[0] + (inner - 1) * strides[1] + width
+    end = tensor.untyped_storage().data_ptr() + tensor.untyped_storage().nbytes()
+    return pointer == tensor.data_ptr() and pointer + last * tensor.element_size() <= end
+
+
+def _packed(kept):
+    """Saved tensors come back as dense copies, as tensors kept on another device do."""
+    def back(t):
+        kept.append(t.clone(memory_format=torch.contiguous_format))
+        return kept[-1]
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, back)
+
+
+def test_norm_backward_reads_saved_tensors_where_they_are(monkeypatch):
+    calls, kept = _Calls(monkeypatch), []
+    joint = torch.randn(3, 5, 96)
+    x = joint[..., 16:48].detach().requires_grad_()  # rows 96 apart, inside the joint tensor
+    assert not x.is_contiguous()
+    w = torch.ones(32, requires_grad=True)
+    with _packed(kept):
+        y = rms_norm(x, w)
+    torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    a = calls.last("gpa_b200_norm_backward")[0]
+    assert a.width == 32 and a.outer * a.inner == 15
+    back = next(t for t in kept if t.shape == x.shape)
+    assert _rows_inside(a.update, back, a.outer, a.inner, (a.update_outer, a.update_inner), 32)
+
+
+def test_residual_norm_backward_reads_saved_tensors_where_they_are(monkeypatch):
+    calls, kept = _Calls(monkeypatch), []
+    joint, wide = torch.randn(3, 5, 96), torch.randn(3, 5, 200)
+    residual, update = torch.randn(3, 5, 32), joint[..., 16:48].detach().requires_grad_()
+    gate = wide[..., 100:132].detach().requires_grad_()
+    with _packed(kept):
+        s, n = residual_norm(residual, update, torch.ones(32), gate=gate, post_weight=torch.ones(32))
+    torch.autograd.grad((s, n), (update, gate), (torch.ones_like(s), torch.ones_like(n)))
+    a = calls.last("gpa_b200_norm_backward")[0]
+    inside = [t for t in kept if t.shape == update.shape]
+    assert any(_rows_inside(a.update, t, a.outer, a.inner, (a.update_outer, a.update_inner), 32) for t in inside)
+    assert any(_rows_inside(a.gate, t, a.outer, a.inner, (a.gate_outer, a.gate_inner), 32) for t in inside)
+
+
+def test_loss_backward_reads_the_saved_weight_where_it_is(monkeypatch):
+    calls, kept = _Calls(monkeypatch), []
+    x = torch.randn(6, 32).bfloat16().requires_grad_()
+    w = torch.randn(50, 96).bfloat16()[:, 16:48].detach().requires_grad_()  # rows 96 apart
+    assert not w.is_contiguous()
+    with _packed(kept):
+        loss = linear_cross_entropy(x, w, torch.zeros(6, dtype=torch.long))
+    torch.autograd.grad(loss, (x, w))
+    a, saved, nbytes = calls.last("gpa_b200_loss_backward")[:3]
+    back = next(t for t in kept if t.shape == w.shape)
+    assert _rows_inside(a.weight, back, 1, 50, (0, a.weight_stride), 32)
+    assert nbytes >= _lib.load().gpa_b200_loss_saved_bytes(a)
+
+
+def test_loss_backward_of_a_weight_that_moved_off_its_alignment(monkeypatch):
+    """The forward read the weight in place; the copy that comes back starts off 16 bytes."""
+    calls, kept = _Calls(monkeypatch), []
+    x = torch.randn(6, 32).bfloat16().requires_grad_()
+    w = torch.randn(50, 32).bfloat16().requires_grad_()
+
+    def back(t):
+        if t.shape != w.shape:
+            return t
+        moved = torch.empty(t.numel() + 1, dtype=t.dtype)[1:].view(t.shape)
+        kept.append(moved.copy_(t))
+        return moved
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+        loss = linear_cross_entropy(x, w, torch.zeros(6, dtype=torch.long))
+    assert kept == []
+    torch.autograd.grad(loss, (x, w))
+    assert kept[0].data_ptr() % 16
+    a, saved, nbytes = calls.last("gpa_b200_loss_backward")[:3]
+    assert a.weight % 16 == 0 and nbytes >= _lib.load().gpa_b200_loss_saved_bytes(a)
+
+
+def test_loss_backward_of_a_weight_that_comes_back_strided(monkeypatch):
+    calls, kept = _Calls(monkeypatch), []
+    x = torch.randn(6, 32).bfloat16().requires_grad_()
+    w = torch.randn(50, 32).bfloat16().requires_grad_()
+
+    def back(t):
+        if t.shape != w.shape:
+            return t
+        kept.append(torch.zeros(50, 43, dtype=t.dtype)[:, 3:35].copy_(t))
+        return kept[-1]
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+        loss = linear_cross_entropy(x, w, torch.zeros(6, dtype=torch.long))
+    torch.autograd.grad(loss, (x, w))
+    a, saved, nbytes = calls.last("gpa_b200_loss_backward")[:3]
+    assert a.weight % 16 == 0 and a.weight_stride == 32
+    assert nbytes >= _lib.load().gpa_b200_loss_saved_bytes(a)
+
+
+@pytest.mark.parametrize("spoil", [lambda t: t.double() if t.is_floating_point() else t, lambda t: t[..., :-1]])
+def test_saved_tensors_of_another_type_or_shape_are_refused(monkeypatch, spoil):
+    _Calls(monkeypatch)
+    x, w = torch.randn(4, 32, requires_grad=True), torch.ones(32, requires_grad=True)
+    e = torch.randn(50, 32, requires_grad=True)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spoil):
+        outs = [rms_norm(x, w), residual_norm(x, x, w, post_weight=w)[0],
+                linear_cross_entropy(x, e, torch.zeros(4, dtype=torch.long))]
+    for out in outs:
+        with pytest.raises(RuntimeError, match="saved"):
+            out.backward(torch.ones_like(out))
