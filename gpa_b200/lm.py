@@ -82,6 +82,17 @@ def _projection_dtype(x: Tensor) -> torch.dtype:
     return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
 
 
+def _bare(m: nn.Module, kind: type) -> bool:
+    """Whether a call of `m` would run `kind`'s own forward and nothing round it: no subclass or
+    wrapper, no hook, no forward put in its place.  What is not bare is called, never taken apart:
+    fusing across it would leave out what was put there (adapters, sharding, recorders)."""
+    g = nn.modules.module
+    return (type(m) is kind and "forward" not in m.__dict__ and m._compiled_call_impl is None and
+            not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or
+                 g._global_forward_hooks or g._global_forward_pre_hooks or g._global_backward_hooks or
+                 g._global_backward_pre_hooks))
+
+
 class RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float):
         super().__init__()
@@ -186,6 +197,11 @@ class SwiGLU(nn.Module):
         return self.down_proj(F.silu(self.gate_proj(x)) * self.up_proj(x))
 
 
+def _normed(norm: nn.Module, x: Tensor, dtype: torch.dtype) -> Tensor:
+    """norm(x), straight in the dtype its reader takes where the norm is RMSNorm alone."""
+    return norm(x, dtype) if _bare(norm, RMSNorm) else norm(x)
+
+
 class BlockOutput(nn.Module):
     """What happens to a block's output on its way into the residual stream: by default nothing;
     with the options of GPALMConfig a norm, a gate from the block's input and a scale."""
@@ -211,14 +227,15 @@ class BlockOutput(nn.Module):
             update = self.scale * update
         return x + update
 
-    def add_and_norm(self, x: Tensor, update: Tensor, gate: Tensor | None, norm: RMSNorm):
-        """(x + the update's share, its norm for the next projections)."""
-        if _kernels(x):
+    def add_and_norm(self, x: Tensor, update: Tensor, gate: Tensor | None, norm: nn.Module, dtype: torch.dtype):
+        """(x + the update's share, its norm in the dtype its reader takes)."""
+        post = self.post
+        if _kernels(x) and _bare(norm, RMSNorm) and (
+                post is None or (_bare(post, RMSNorm) and post.eps == norm.eps)):
             return residual_norm(x, update, norm.weight, norm.eps, gate=gate, scale=self.scale,
-                                 post_weight=None if self.post is None else self.post.weight,
-                                 out_dtype=_projection_dtype(x))
+                                 post_weight=None if post is None else post.weight, out_dtype=dtype)
         x = self.add(x, update, gate)
-        return x, norm(x)
+        return x, _normed(norm, x, dtype)
 
 
 class GPABlock(nn.Module):
@@ -237,12 +254,13 @@ class GPABlock(nn.Module):
         ``gate`` are the previous block's, ``before`` its output stage (None for the first
         block).  Returns (x, update, gate, memory) of this block, for the next one.  ``attend``
         stands in for the attention (decoding sessions)."""
+        dtype = _projection_dtype(x)
         if update is None:
-            n = self.input_norm(x, _projection_dtype(x))
+            n = _normed(self.input_norm, x, dtype)
         else:
-            x, n = before.add_and_norm(x, update, gate, self.input_norm)
+            x, n = before.add_and_norm(x, update, gate, self.input_norm, dtype)
         y, memory = self.attn(n, memory) if attend is None else (attend(n), memory)
-        x, m = self.attn_out.add_and_norm(x, y, self.attn_out.gate_of(n), self.post_norm)
+        x, m = self.attn_out.add_and_norm(x, y, self.attn_out.gate_of(n), self.post_norm, dtype)
         return x, self.mlp(m), self.mlp_out.gate_of(m), memory
 
     def forward(self, x: Tensor, memory: LayerMemory | None = None):
@@ -289,19 +307,26 @@ class GPALM(nn.Module):
         with torch.autocast("cuda", dtype=torch.bfloat16, enabled=x.is_cuda and self.autocast):
             for i, blk in enumerate(self.blocks):
                 old = None if cache is None else cache.layers[i]
+                bare, mem = _bare(blk, GPABlock), None
+                if not bare and update is not None:  # whatever is round the block meets the whole stream
+                    x, update, gate = before.add(x, update, gate), None, None
                 if self.training and self.gradient_checkpointing:
                     # reentrant: the layer's forward runs without a graph, so the core's
                     # forward workspace is freed at once and rebuilt in the backward
-                    x, update, gate = checkpoint(
-                        lambda y, u, g, blk=blk, before=before: blk.step(y, u, g, before)[:3],
-                        x, update, gate, use_reentrant=True)
-                else:
+                    if bare:
+                        x, update, gate = checkpoint(
+                            lambda y, u, g, blk=blk, before=before: blk.step(y, u, g, before)[:3],
+                            x, update, gate, use_reentrant=True)
+                    else:
+                        x = checkpoint(lambda y, blk=blk: blk(y)[0], x, use_reentrant=True)
+                elif bare:
                     x, update, gate, mem = blk.step(x, update, gate, before, old)
-                    if cache is not None:
-                        cache.layers[i] = mem
-                before = blk.mlp_out
-            x = (self.norm(x, _projection_dtype(x)) if update is None else
-                 before.add_and_norm(x, update, gate, self.norm)[1])
+                else:
+                    x, mem = blk(x, old)
+                if cache is not None:
+                    cache.layers[i] = mem
+                before = blk.mlp_out if bare else None
+            x = self._final_norm(x, update, gate, before)
             if cache is not None:
                 cache.seen_tokens += ids.shape[1]
             if labels is None:
@@ -310,10 +335,22 @@ class GPALM(nn.Module):
                 raise ValueError("labels must match ids")
             return self._loss(x, labels), cache
 
+    def _final_norm(self, x: Tensor, update, gate, before) -> Tensor:
+        """The last norm, after the addition that is still to be made (if any)."""
+        dtype = _projection_dtype(x) if _bare(self.lm_head, nn.Linear) else x.dtype
+        if update is None:
+            return _normed(self.norm, x, dtype)
+        return before.add_and_norm(x, update, gate, self.norm, dtype)[1]
+
+    def _fused_loss(self, x: Tensor) -> bool:
+        """Whether linear_cross_entropy takes this loss: a head that is a product with its weight alone."""
+        head = self.lm_head
+        return x.is_cuda and x.dtype in _DTYPES and _bare(head, nn.Linear) and head.bias is None
+
     def _loss(self, x: Tensor, labels: Tensor) -> Tensor:
         """Mean next-token cross entropy over labels[:, 1:] != -100."""
         t = x.shape[1]
-        if x.is_cuda and x.dtype in _DTYPES:
+        if self._fused_loss(x):
             # position i predicts token i + 1; the last position predicts nothing
             shifted = F.pad(labels[:, 1:], (0, 1), value=-100)
             return linear_cross_entropy(x, self.lm_head.weight.to(x.dtype), shifted)
@@ -380,7 +417,7 @@ class GPALM(nn.Module):
 
                     x, update, gate, _ = blk.step(x, update, gate, before, attend=attend)
                     before = blk.mlp_out
-                x = before.add_and_norm(x, update, gate, self.norm)[1]
+                x = self._final_norm(x, update, gate, before)
                 tok.copy_(self.lm_head(x[:, -1]).float().argmax(-1))
 
         # every decode step is the same sequence of launches on fixed buffers: record one in a

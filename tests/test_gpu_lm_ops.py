@@ -15,6 +15,7 @@ import torch
 from gpa_b200 import _lib
 from gpa_b200.lm import GPALM, GPALMConfig
 from gpa_b200.training_graph import GradientGraph
+from lm_around import Adapted, Round, shard
 from lm_oracle import oracle_lm
 from parity_util import rel
 
@@ -123,3 +124,73 @@ def test_no_label_at_all_gives_zero_loss_and_gradients():
     loss, _ = m(ids, labels=torch.full_like(ids, -100))
     loss.backward()
     assert float(loss) == 0 and not m.embed.weight.grad.any()
+
+
+def _step(m, ids, labels):
+    m.zero_grad(set_to_none=True)
+    loss, _ = m(ids, labels=labels)
+    loss.backward()
+    return loss.detach(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+
+
+@pytest.mark.parametrize("checkpointing", [False, True])
+@pytest.mark.parametrize("options", [{}, OPTIONS[3]])
+@pytest.mark.parametrize("what", ["blocks", "norms", "head", "posts"])
+def test_hooked_modules_are_called(what, options, checkpointing):
+    # a head of its own: the embedding reads its table outside the head's forward
+    m = _model(dataclasses.replace(CFG, tie_embeddings=False, **options), seed=7).cuda().train()
+    m.gradient_checkpointing, m.autocast = checkpointing, False
+    ids = torch.randint(0, CFG.vocab_size, (2, 70), generator=torch.Generator().manual_seed(8)).cuda()
+    want, grads = _step(m, ids, ids)
+    some = {"blocks": list(m.blocks), "head": [m.lm_head],
+            "norms": [n for b in m.blocks for n in (b.input_norm, b.post_norm)] + [m.norm],
+            "posts": [o.post for b in m.blocks for o in (b.attn_out, b.mlp_out) if o.post is not None]}[what]
+    calls, handles = [], [mod.register_forward_hook(lambda mod, a, o: calls.append(mod)) for mod in some]
+    got, again = _step(m, ids, ids)
+    assert {id(c) for c in calls} == {id(mod) for mod in some}
+    assert rel(got, want) <= 1e-5
+    bad = {n: rel(again[n], g) for n, g in grads.items() if not rel(again[n], g) <= 1e-3}
+    assert not bad and set(again) == set(grads), bad
+    for h in handles:
+        h.remove()
+    back = [shard(mod) for mod in some]
+    with torch.no_grad():
+        assert rel(m(ids, labels=ids)[0], want) <= 1e-5
+    for f in back:
+        f()
+
+
+@pytest.mark.parametrize("head", ["adapted", "biased", "wrapped"])
+def test_replaced_heads_are_called(head, cpu_threads):
+    m = _model(CFG, seed=9)
+    m.lm_head.weight = torch.nn.Parameter(m.lm_head.weight.detach().clone())
+    if head == "adapted":
+        m.lm_head = Adapted(m.lm_head)
+    elif head == "biased":
+        m.lm_head.bias = torch.nn.Parameter(torch.randn(CFG.vocab_size, generator=torch.Generator().manual_seed(1)))
+    else:
+        m.lm_head = Round(m.lm_head)
+    twin = oracle_lm(m).train()
+    ids = torch.randint(0, CFG.vocab_size, (2, 70), generator=torch.Generator().manual_seed(10))
+    ref, wanted = _step(twin, ids, ids)
+    gpu = m.cuda().train()
+    gpu.autocast = False
+    loss, got = _step(gpu, ids.cuda(), ids.cuda())
+    assert rel(loss, ref) <= 1e-5
+    bad = {n: rel(g, wanted[n.replace("gpa.", "gpa.inner.")]) for n, g in got.items()
+           if not rel(g, wanted[n.replace("gpa.", "gpa.inner.")]) <= 1e-3}
+    assert not bad, bad
+
+
+def test_every_option_gets_its_gradient():
+    m = _model(dataclasses.replace(CFG, **OPTIONS[3]), seed=11).cuda().train()
+    ids = torch.randint(0, CFG.vocab_size, (2, 70), generator=torch.Generator().manual_seed(12)).cuda()
+    grads = _step(m, ids, ids)[1]
+    wanted = {n for n, _ in m.named_parameters() if "attn_out" in n or "mlp_out" in n or "norm" in n}
+    assert wanted and wanted <= set(grads) and all(grads[n].any() for n in wanted)
+
+
+def test_a_model_without_layers_generates():
+    m = GPALM(dataclasses.replace(CFG, num_layers=0)).cuda().eval()
+    ids = torch.randint(0, CFG.vocab_size, (2, 5), generator=torch.Generator().manual_seed(15)).cuda()
+    assert torch.equal(m.generate(ids, 3), m.generate(ids, 3, fused_decode=False))

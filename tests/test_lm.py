@@ -9,10 +9,12 @@ cores inside the same model.
 """
 from __future__ import annotations
 
+import pytest
 import torch
 import torch.nn.functional as F
 
 from gpa_b200.lm import GPALM, GPALMConfig, num_parameters
+from lm_around import Round, shard
 from lm_oracle import oracle_lm
 
 SMALL = GPALMConfig(vocab_size=97, hidden_size=32, num_layers=2, num_heads=2, num_kv_heads=1,
@@ -106,3 +108,67 @@ def test_qwen_shaped_parameter_count():
     gpa = num_parameters(m.blocks[0].attn.gpa)
     assert gpa == 6_128_896
     assert 700e6 < n < 800e6, n
+
+
+def _pass(m, training=False, seed=8):
+    ids = torch.randint(0, SMALL.vocab_size, (2, 9), generator=torch.Generator().manual_seed(seed))
+    m.train(training)
+    return m(ids, labels=ids)[0], m(ids)[0] if not training else None
+
+
+def _hooked():
+    m = _model(seed=9)
+    return m, [*m.blocks, *(n for blk in m.blocks for n in (blk.input_norm, blk.post_norm)), m.norm]
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_forward_hooks_of_blocks_and_norms_run(training):
+    m, modules = _hooked()
+    m.gradient_checkpointing = training
+    want = _pass(m, training)
+    seen = []
+    for k, mod in enumerate(modules):
+        mod.register_forward_hook(lambda mod, args, out, k=k: seen.append((k, args, out)))
+    got = _pass(m, training)
+    # a step each: loss alone in training (its backward would run the layers again), loss and logits else
+    assert sorted(k for k, _, _ in seen) == sorted(list(range(len(modules))) * (1 if training else 2))
+    assert torch.allclose(got[0], want[0], atol=1e-12)
+    # what a block returns is the stream that the next one, or the last norm, takes
+    first = {}
+    for k, args, out in seen:
+        first.setdefault(k, (args, out))
+    assert torch.equal(first[0][1][0], first[1][0][0])
+    assert torch.equal(first[1][1][0], first[len(modules) - 1][0][0])
+
+
+def test_a_hook_may_change_what_a_block_returns():
+    m, _ = _hooked()
+    m.blocks[0].register_forward_hook(lambda mod, args, out: (out[0] * 0, out[1]))
+    a = _pass(m)[1]
+    for p in m.blocks[0].parameters():
+        torch.nn.init.normal_(p)
+    assert torch.equal(_pass(m)[1], a)
+
+
+@pytest.mark.parametrize("training", [False, True])
+@pytest.mark.parametrize("what", ["blocks", "norms", "head"])
+def test_weights_may_be_there_during_a_module_s_own_forward_alone(what, training):
+    m, modules = _hooked()
+    want = _pass(m, training)[0]
+    m.lm_head.weight = torch.nn.Parameter(m.lm_head.weight.detach().clone())  # sharded apart from the embedding
+    some = {"blocks": list(m.blocks), "norms": modules[len(m.blocks):], "head": [m.lm_head]}[what]
+    back = [shard(mod) for mod in some]
+    assert torch.allclose(_pass(m, training)[0], want, atol=1e-12)
+    for f in back:
+        f()
+
+
+def test_wrapped_and_replaced_modules_are_called():
+    m, _ = _hooked()
+    want = _pass(m)
+    m.blocks[1] = Round(m.blocks[1])
+    m.blocks[0].post_norm = Round(m.blocks[0].post_norm)
+    m.norm = Round(m.norm)
+    got = _pass(m)
+    assert torch.allclose(got[0], want[0], atol=1e-12) and torch.allclose(got[1], want[1], atol=1e-12)
+    assert m.blocks[1].calls == m.blocks[0].post_norm.calls == m.norm.calls == 2
