@@ -38,7 +38,7 @@ from torch.utils.checkpoint import checkpoint
 
 from .config import GPAConfig
 from .core import DenseGPA
-from .ops import _DTYPES, MAX_NORM_WIDTH, linear_cross_entropy, residual_norm, rms_norm
+from .ops import _DTYPES, MAX_NORM_WIDTH, linear_cross_entropy, loss_limits, residual_norm, rms_norm
 from .state import GPAState, _map
 
 
@@ -343,9 +343,12 @@ class GPALM(nn.Module):
         return before.add_and_norm(x, update, gate, self.norm, dtype)[1]
 
     def _fused_loss(self, x: Tensor) -> bool:
-        """Whether linear_cross_entropy takes this loss: a head that is a product with its weight alone."""
+        """Whether linear_cross_entropy takes this loss: a head that is a product with its weight
+        alone, sizes it takes, and something to predict."""
         head = self.lm_head
-        return x.is_cuda and x.dtype in _DTYPES and _bare(head, nn.Linear) and head.bias is None
+        return (x.is_cuda and x.dtype in _DTYPES and x.shape[1] > 1 and _bare(head, nn.Linear) and
+                head.bias is None and
+                loss_limits(x.shape[0] * x.shape[1], *head.weight.shape[::-1]) is None)
 
     def _loss(self, x: Tensor, labels: Tensor) -> Tensor:
         """Mean next-token cross entropy over labels[:, 1:] != -100."""

@@ -365,6 +365,17 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
     return _residual_forward(*args)
 
 
+def loss_limits(tokens: int, width: int, vocab: int) -> str | None:
+    """What `linear_cross_entropy` says of sizes it does not take, or None."""
+    if not 1 <= width <= 65536 or not 1 <= vocab <= 1 << 29:
+        return f"1 to 65536 channels and 1 to 2^29 vocabulary entries, not {width} and {vocab}"
+    if tokens > 1 << 22:
+        return f"at most 2^22 tokens in a call, not {tokens}"
+    if -(-tokens // 256) * -(-vocab // 256) > 1 << 30:
+        return f"at most 2^30 tiles of 256 x 256 logits in a call, not {tokens} x {vocab}"
+    return None
+
+
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
@@ -472,11 +483,9 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
         raise ValueError(f"labels is on {labels.device}, the other tensors are on {dev}")
     if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
         raise ValueError(f"labels must be integers, not {labels.dtype}")
-    if not 1 <= hidden.shape[-1] <= 65536 or not 1 <= weight.shape[0] <= 1 << 29:
-        raise ValueError(f"1 to 65536 channels and 1 to 2^29 vocabulary entries, not {weight.shape[1]} "
-                         f"and {weight.shape[0]}")
-    if labels.numel() > 1 << 22:
-        raise ValueError(f"at most 2^22 tokens in a call, not {labels.numel()}")
+    too_large = loss_limits(labels.numel(), weight.shape[1], weight.shape[0])
+    if too_large:
+        raise ValueError(too_large)
     if labels.dtype != torch.int64 or not labels.is_contiguous():
         labels = labels.long().contiguous()
     args = (hidden, weight, labels, int(ignore_index), _REDUCTIONS[reduction])

@@ -190,6 +190,39 @@ def test_every_option_gets_its_gradient():
     assert wanted and wanted <= set(grads) and all(grads[n].any() for n in wanted)
 
 
+def _expected(x, head, labels):
+    z = x.double().flatten(0, 1) @ head.double().T
+    y = torch.nn.functional.pad(labels[:, 1:], (0, 1), value=-100).flatten()
+    return torch.nn.functional.cross_entropy(z, y, ignore_index=-100)
+
+
+@pytest.mark.parametrize("tokens,grad", [((1 << 22) + 2, True), (9, False), (9, True)])
+def test_losses_of_every_size_are_answered(tokens, grad):
+    """More tokens than linear_cross_entropy takes in a call, and few: 1e-5 relative, fp32's
+    rounding over 8 channels and a mean with room."""
+    m = GPALM(dataclasses.replace(CFG, vocab_size=16, hidden_size=8, num_layers=0, loss_chunk_size=1 << 20)).cuda().eval()
+    g = torch.Generator().manual_seed(13)
+    x = torch.randn(1, tokens, 8, generator=g).cuda().requires_grad_(grad)
+    labels = torch.randint(0, 16, (1, tokens), generator=g).cuda()
+    with torch.set_grad_enabled(grad):
+        loss = m._loss(x, labels)
+    ref = _expected(x.detach(), m.lm_head.weight.detach(), labels)
+    assert loss.dtype == torch.float32 and rel(loss, ref) <= 1e-5
+    if grad:
+        (dx,) = torch.autograd.grad(loss, x)
+        assert dx.isfinite().all() and dx[:, :-1].any(-1).all() and not dx[:, -1].any()
+
+
+def test_one_token_with_its_label_has_no_loss():
+    m = _model(CFG, seed=14).cuda().train()
+    ids = torch.zeros(3, 1, dtype=torch.long, device="cuda")
+    _lib.profile_start()
+    loss, grads = _step(m, ids, ids)
+    counts = _lib.profile_stop()
+    assert float(loss) == 0 and not any("loss" in k for k in counts)
+    assert loss.dtype == torch.float32 and not any(g.any() for g in grads.values())
+
+
 def test_a_model_without_layers_generates():
     m = GPALM(dataclasses.replace(CFG, num_layers=0)).cuda().eval()
     ids = torch.randint(0, CFG.vocab_size, (2, 5), generator=torch.Generator().manual_seed(15)).cuda()
