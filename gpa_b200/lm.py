@@ -34,6 +34,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from .config import GPAConfig
@@ -73,8 +74,10 @@ class GPALMConfig:
 
 
 def _kernels(x: Tensor) -> bool:
-    """Whether the norm kernels take rows like x's (else the plain torch form runs)."""
-    return x.is_cuda and x.dtype in _DTYPES and x.shape[-1] <= MAX_NORM_WIDTH
+    """Whether the norm kernels take rows like x's (else the plain torch form runs, as it does under
+    forward-mode differentiation and function transforms, which the kernels have no rules for)."""
+    return (x.is_cuda and x.dtype in _DTYPES and x.shape[-1] <= MAX_NORM_WIDTH and
+            forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active())
 
 
 def _projection_dtype(x: Tensor) -> torch.dtype:

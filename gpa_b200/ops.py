@@ -8,7 +8,8 @@
 
 They take CUDA tensors in float32, bfloat16 or float16 (the norms any mix of them), sum in fp32,
 run on the current stream without synchronising, allocate through PyTorch, can be captured in a
-CUDA graph and have first-order gradients.  They raise ``ValueError`` for arguments they refuse.
+CUDA graph and have first-order gradients in reverse mode; other derivatives are a
+``RuntimeError``.  They raise ``ValueError`` for arguments they refuse.
 
 As for any PyTorch operator, a backward that is captured must find no eager graph of the same
 leaves alive: their gradient accumulators would belong to the eager stream.
@@ -21,6 +22,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -65,6 +67,15 @@ def _first_order(backward):
         return tuple(None if g is None else next(marked) for g in out)
 
     return run
+
+
+def _no_tangents(*tensors):
+    """Without reverse-mode gradients an operator runs outside autograd, which would drop the
+    tangents of forward-mode differentiation without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("forward-mode derivatives of this operator are not implemented")
 
 
 def _call(fn, device, *args):
@@ -228,6 +239,7 @@ def rms_norm(x: Tensor, weight: Tensor, eps: float = 1e-6, *,
     default).  Gradients: x (in x's dtype) and weight.
     """
     _check_tensor("x", x)
+    _no_tangents(x, weight)
     if x.ndim < 1:
         raise ValueError("x must have at least one axis")
     _check_width(x.shape[-1])
@@ -324,6 +336,7 @@ def residual_norm(residual: Tensor, update: Tensor, weight: Tensor, eps: float =
     the rounded stream.  Gradients: every tensor argument.
     """
     _check_tensor("residual", residual)
+    _no_tangents(residual, update, weight, post_weight, gate, scale)
     dev = residual.device
     _check_tensor("update", update, dev)
     if residual.ndim < 1 or residual.shape != update.shape:
@@ -467,6 +480,7 @@ def linear_cross_entropy(hidden: Tensor, weight: Tensor, labels: Tensor, *,
     under "none" so are the hidden rows times their own gradients, for the weight's.
     """
     _check_tensor("hidden", hidden)
+    _no_tangents(hidden, weight)
     dev = hidden.device
     _check_tensor("weight", weight, dev)
     if reduction not in _REDUCTIONS:

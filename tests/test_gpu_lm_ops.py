@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from gpa_b200 import _lib
-from gpa_b200.lm import GPALM, GPALMConfig
+from gpa_b200.lm import GPALM, GPALMConfig, RMSNorm
 from gpa_b200.training_graph import GradientGraph
 from lm_around import Adapted, Round, shard
 from lm_oracle import oracle_lm
@@ -227,3 +227,17 @@ def test_a_model_without_layers_generates():
     m = GPALM(dataclasses.replace(CFG, num_layers=0)).cuda().eval()
     ids = torch.randint(0, CFG.vocab_size, (2, 5), generator=torch.Generator().manual_seed(15)).cuda()
     assert torch.equal(m.generate(ids, 3), m.generate(ids, 3, fused_decode=False))
+
+
+def test_the_model_s_norm_keeps_forward_mode_and_transforms():
+    norm = RMSNorm(48, 1e-6).cuda()
+    g = torch.Generator().manual_seed(16)
+    x, t = (torch.randn(5, 48, generator=g).cuda() for _ in range(2))
+    out, tangent = torch.func.jvp(norm, (x,), (t,))
+    xd, td = x.double(), t.double()
+    r = 1 / (xd.square().mean(-1, keepdim=True) + 1e-6).sqrt()
+    want = td * r - xd * r ** 3 * (xd * td).mean(-1, keepdim=True)
+    # each term carries a few fp32 roundings and a mean of 48: 64 of them are room enough
+    mag = (td.abs() * r + xd.abs() * r ** 3 * (xd * td).abs().mean(-1, keepdim=True))
+    assert ((tangent.double() - want).abs() <= 64 * 2.0 ** -24 * mag).all()
+    assert torch.allclose(torch.func.vmap(norm)(x), norm(x), atol=0, rtol=1e-5)

@@ -313,3 +313,22 @@ def test_saved_tensors_of_another_type_or_shape_are_refused(monkeypatch, spoil):
     for out in outs:
         with pytest.raises(RuntimeError, match="saved"):
             out.backward(torch.ones_like(out))
+
+
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    _Calls(monkeypatch)
+    x, w, e = torch.randn(4, 32), torch.ones(32), torch.randn(50, 32)
+    labels = torch.zeros(4, dtype=torch.long)
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        dw = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: rms_norm(d, w), lambda: rms_norm(x, dw), lambda: residual_norm(d, x, w),
+                     lambda: residual_norm(x, d, w), lambda: residual_norm(x, x, w, post_weight=dw),
+                     lambda: residual_norm(x, x, w, gate=d), lambda: residual_norm(x, x, w, scale=dw),
+                     lambda: linear_cross_entropy(d, e, labels),
+                     lambda: linear_cross_entropy(x, torch.autograd.forward_ad.make_dual(e, e), labels)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        rms_norm(x, w)  # nothing to differentiate: as ever
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: rms_norm(t, w), (x,), (x,))
