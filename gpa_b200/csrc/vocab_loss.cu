@@ -614,7 +614,7 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   int code;
   if ((*why = plan_of(a, &p, &code))) return code;
   const Call& c = p.c;
-  if (!a->weight || !saved || !scratch || (c.n && !dloss) || (!dhidden && !dweight)) {
+  if (!a->weight || !saved || !scratch || (c.n && (!dloss || (!dhidden && !dweight)))) {
     *why = "a tensor is NULL";
     return GPA_B200_BAD_ARGUMENT;
   }

@@ -452,3 +452,13 @@ def test_saved_tensors_that_come_back_with_other_strides(lead, dtype):
         got = _run(x, wide[:, 16:80], y, "none")
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_no_token_and_a_frozen_weight(dtype, reduction):
+    x, w, y = _inputs(19, (0,), 64, 300, dtype)
+    x.requires_grad_()
+    loss = linear_cross_entropy(x, w, y, reduction=reduction)
+    (dx,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert dx.shape == (0, 64) and dx.dtype == dtype

@@ -332,3 +332,11 @@ def test_forward_mode_derivatives_are_refused(monkeypatch):
         rms_norm(x, w)  # nothing to differentiate: as ever
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: rms_norm(t, w), (x,), (x,))
+
+
+def test_loss_backward_without_rows_needs_no_gradient_to_write():
+    """The gradient of an empty hidden has no memory; with a frozen weight nothing is left to do."""
+    lib = _lib.load()
+    a = _loss_args(outer=0)
+    saved, scratch = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 1)
+    assert lib.gpa_b200_loss_backward(a, 32, saved, None, None, None, 32, scratch, None) == 0
