@@ -401,10 +401,12 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
       if (!live || c >= p.width) continue;
       float w[VEC], a[VEC];
       ldv<VEC>(p.w, c, kF32, w);
+      if (b.dn) {  // without: nothing reaches the row through its norm, whatever it holds
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        aw[i][k] += d[i][k] * x[i][k] * r;
-        d[i][k] = r * (w[k] * d[i][k] - x[i][k] * q);
+        for (int k = 0; k < VEC; ++k) {
+          aw[i][k] += d[i][k] * x[i][k] * r;
+          d[i][k] = r * (w[k] * d[i][k] - x[i][k] * q);
+        }
       }
       if (b.ds) {
         held_s[i].get(h_dt, a);
@@ -548,11 +550,16 @@ __global__ void __launch_bounds__(MT) k_norm_bwd_light(const Bwd b) {
     const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
     if (row >= p.rows || !in) continue;
     const int64_t at = (int64_t)row * p.width + c;
+    if (b.dn) {  // without: nothing reaches the row through its norm, whatever it holds
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      aw[0][k] += d[k] * x[k] * r;
-      d[k] = r * (w[k] * d[k] - x[k] * q);
-      if (b.ds) d[k] += e[k];
+      for (int k = 0; k < 8; ++k) {
+        aw[0][k] += d[k] * x[k] * r;
+        d[k] = r * (w[k] * d[k] - x[k] * q);
+      }
+    }
+    if (b.ds) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] += e[k];
     }
     if (b.dh) stv<8>(b.dh, at, p.h_dt, d);
     if (b.dy) {

@@ -411,3 +411,18 @@ def test_saved_tensors_that_come_back_with_other_strides():
         ref.check("d" + name, t, want["d" + name])
     for a, b in zip(step()[2], plain):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("parts", [False, True])
+@pytest.mark.parametrize("width", [24, 64, 1001, 1024, 8200])
+def test_infinities_stay_out_of_the_gradient_of_the_stream_alone(width, parts):
+    """Only the stream has a gradient: it is the residual's, also in rows that overflowed."""
+    g = _gen(33)
+    h, u, up = _randn(g, (6, width)), _randn(g, (6, width)), _randn(g, (6, width))
+    h[1, 3], h[2, 5] = float("inf"), float("nan")
+    h.requires_grad_()
+    u.requires_grad_()
+    w = torch.ones(width, device="cuda", requires_grad=True)
+    s, n = residual_norm(h, u, w, EPS, scale=torch.full((width,), 0.5, device="cuda") if parts else 0.5)
+    dh, du = torch.autograd.grad(s, (h, u), up)
+    assert torch.equal(dh, up) and torch.equal(du, 0.5 * up)
