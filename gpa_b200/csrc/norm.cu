@@ -151,9 +151,12 @@ GPA_DEV float gate_of(float a) {
   return a < -87.f ? 0.f : r;
 }
 
-// The gate in the backward, whose results are not rounded next to a border of another tensor's:
-// exp2 and reciprocal units alone (7 us less there).
-GPA_DEV float gate_near(float a) { return __fdividef(1.f, 1.f + __expf(-a)); }
+// The gate in the backward.  16-bit gates: exp2 and reciprocal units alone (7 us less), whose error,
+// 2^-24 |a| and so about a hundredth of the rounding of the gate's own gradient, moves no result next
+// to a border of another tensor's.  fp32 ones, whose gradients are fp32: as in the forward.
+GPA_DEV float gate_back(float a, int dt) {
+  return dt == kF32 ? gate_of(a) : __fdividef(1.f, 1.f + __expf(-a));
+}
 
 GPA_DEV float round_to(float x, int dt) {
   if (dt == kBF16) return __bfloat162float(__float2bfloat16(x));
@@ -393,7 +396,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
     const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
     const float ry = p.wp ? rsqrtf(s[2] * inv + p.eps) : 1.f;
     float gr = 1.f;
-    if (live && p.gate && !p.gate_full) gr = gate_near(load_in(p.gate, og, g_dt));
+    if (live && p.gate && !p.gate_full) gr = gate_back(load_in(p.gate, og, g_dt), g_dt);
     float s2[2] = {0.f, 0.f};  // wp du y, row-gate gradient
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -432,7 +435,7 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
       if (p.gate && p.gate_full) {
         held_g[i].get(g_dt, a);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a[k] = gate_near(a[k]);
+        for (int k = 0; k < VEC; ++k) a[k] = gate_back(a[k], g_dt);
       }
       float dg[VEC];
 #pragma unroll
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
     const float r = rsqrtf(sums[0] * inv + p.eps), q = sums[1] * inv * r * r;
     const float ry = p.wp ? rsqrtf(sums[2] * inv + p.eps) : 1.f;
     float gr = 1.f;
-    if (p.gate && !full) gr = gate_near(load_in(p.gate, row_at(p.rg, row, p.inner), g_dt));
+    if (p.gate && !full) gr = gate_back(load_in(p.gate, row_at(p.rg, row, p.inner), g_dt), g_dt);
     float two[2] = {0.f, 0.f};  // wp du y, row-gate gradient
     V8 d;
     if (in) {
@@ -694,7 +697,7 @@ __global__ void __launch_bounds__(MT, MT == 320 ? 2 : 1) k_norm_bwd_parts(const 
       if (full) {
         a = read(s + sg * n, g_dt);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a.v[k] = make_float2(gate_near(a.v[k].x), gate_near(a.v[k].y));
+        for (int k = 0; k < 4; ++k) a.v[k] = make_float2(gate_back(a.v[k].x, g_dt), gate_back(a.v[k].y, g_dt));
       }
       V8 cs, wp;
 #pragma unroll

@@ -426,3 +426,23 @@ def test_infinities_stay_out_of_the_gradient_of_the_stream_alone(width, parts):
     s, n = residual_norm(h, u, w, EPS, scale=torch.full((width,), 0.5, device="cuda") if parts else 0.5)
     dh, du = torch.autograd.grad(s, (h, u), up)
     assert torch.equal(dh, up) and torch.equal(du, 0.5 * up)
+
+
+@pytest.mark.parametrize("width", [40, 1001, 1024])
+def test_fp32_gates_near_zero_keep_their_gradients_digits(width):
+    """Gates of e^-1 to e^-60, whose gradients shrink with them.  The exponential is within 4 U, the
+    reciprocal, the products and 1 - s add 10 U to a gradient of every channel; a row's gate adds
+    up positive terms, in at most 26 additions (see norm_reference)."""
+    g = _gen(34)
+    h, u, up = (_randn(g, (12, width)) for _ in range(3))
+    up = up.abs() * u.sign()
+    w = torch.ones(width, device="cuda")
+    for shape, room in (((12, width), 16), ((12, 1), 16 + 26)):
+        a = (-1 - 59 * torch.rand(shape, generator=g)).cuda().requires_grad_()
+        s, n = residual_norm(h, u, w, EPS, gate=a)
+        (da,) = torch.autograd.grad(s, a, up)
+        gate = torch.sigmoid(a.detach().double())
+        want = up.double() * u.double() * gate * (1 - gate)
+        if shape[1] == 1:
+            want = want.sum(-1, keepdim=True)
+        assert ((da.double() - want).abs() <= room * ref.U * want.abs()).all(), shape
