@@ -886,14 +886,19 @@ int most_blocks(const Shape& s) { return 148 * std::max(1, 1024 / s.threads); }
 // -> 97 us eager, most of it the host's, 8.3 us replayed either way), 2 of wide ones (6 x 647 in one
 // block: 139 -> 130 us eager, but 16 -> 35 us replayed).
 uint32_t one_block(const Shape& s) { return s.group ? 8 : 2; }
-// 0: the kernel cannot have its shared memory.  Known: a kernel's blocks per SM by device and warps
-// of a block, 0 where not asked yet.
-using Known = std::atomic<int>[8][33];
+// 0: the kernel cannot have its shared memory.  Known: a kernel's blocks per SM by device, warps of a
+// block and 32-byte units of shared memory a thread (two stages of a slot; the types of a call set
+// them), 0 where not asked yet.  The grid says how the column sums are grouped, so it follows from
+// the call alone.
+constexpr int kUnits = 11;
+using Known = std::atomic<int>[8][33][kUnits];
 int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, Known& known) {
   const uint32_t per = s.group ? s.threads / s.group : 1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  int at_once = dev < 8 ? known[dev][s.threads / 32].load(std::memory_order_relaxed) : 0;
+  const size_t units = smem / (32 * s.threads);
+  const bool keep = dev < 8 && units < kUnits;
+  int at_once = keep ? known[dev][s.threads / 32][units].load(std::memory_order_relaxed) : 0;
   if (!at_once) {
     // rows of whole blocks: up to 2 x 10 slots of 16 bytes for 512 threads, whatever the types of this call
     if (!s.group && smem &&
@@ -901,7 +906,7 @@ int bwd_blocks(const Shape& s, uint32_t rows, const void* kernel, size_t smem, K
       return 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kernel, s.threads, smem) != cudaSuccess || at_once < 1)
       at_once = 1;
-    if (dev < 8) known[dev][s.threads / 32].store(at_once, std::memory_order_relaxed);
+    if (keep) known[dev][s.threads / 32][units].store(at_once, std::memory_order_relaxed);
   }
   const uint32_t need = (rows + per - 1) / per;
   if (need <= one_block(s)) return 1;

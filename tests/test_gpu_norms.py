@@ -446,3 +446,34 @@ def test_fp32_gates_near_zero_keep_their_gradients_digits(width):
         if shape[1] == 1:
             want = want.sum(-1, keepdim=True)
         assert ((da.double() - want).abs() <= room * ref.U * want.abs()).all(), shape
+
+
+OTHER_TYPES_FIRST = """
+import sys, torch
+from gpa_b200 import residual_norm
+def step(stream, update, gate, out, width):
+    g = torch.Generator().manual_seed(width)
+    h, u, a = (torch.randn(4000, width, generator=g).to(t).cuda().requires_grad_() for t in (stream, update, gate))
+    w, p, c = ((1 + 0.1 * torch.randn(width, generator=g)).cuda().requires_grad_() for _ in range(3))
+    s, n = residual_norm(h, u, w, post_weight=p, gate=a, scale=c, out_dtype=out)
+    return torch.autograd.grad((s, n), (w, p, c), (torch.ones_like(s), torch.ones_like(n)))
+F, B, H = torch.float32, torch.bfloat16, torch.float16
+for width in (384, 768, 1280, 1792, 2560, 4096):
+    if sys.argv[1] == "first":
+        step(H, H, H, H, width)
+    torch.save(step(F, F, B, F, width), f"{sys.argv[2]}/{sys.argv[1]}{width}.pt")
+"""
+
+
+def test_column_sums_do_not_depend_on_earlier_calls(tmp_path):
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for order in ("first", "alone"):
+        r = subprocess.run([sys.executable, "-c", OTHER_TYPES_FIRST, order, str(tmp_path)], cwd=root,
+                           capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stderr[-2000:]
+    for width in (384, 768, 1280, 1792, 2560, 4096):
+        a, b = (torch.load(f"{tmp_path}/{order}{width}.pt") for order in ("first", "alone"))
+        assert all(torch.equal(x, y) for x, y in zip(a, b)), width
