@@ -337,8 +337,11 @@ GPA_DEV void emit_sums(float* dst, const float (&a)[ITER][VEC], int width, int g
   }
 }
 
-template <int G, int VEC, int ITER, int MT>
-__global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
+// PARTS: with a post weight, a gate or a scale.  Without, the update and its sums take no registers,
+// which blocks of 1024 threads are short of (1864 x 9001 in bf16, step: 807 -> 638 us, where plain
+// PyTorch takes 662; with parts they spill still: 1307, 1631).
+template <int G, int VEC, int ITER, int MT, bool PARTS>
+__global__ void __launch_bounds__(MT, 1) k_norm_bwd(const Bwd b) {
   const Fwd& p = b.f;
   NORM_TYPES(kAny);
   __shared__ float sm[2][3][32];
@@ -348,55 +351,64 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
   const int t = G == 0 ? (int)threadIdx.x : (int)(threadIdx.x % G);
   const uint32_t per = G == 0 ? 1u : blockDim.x / G;
   const uint32_t mine = G == 0 ? 0u : threadIdx.x / G;
-  const bool plain = p.h_dt < 0;
+  const bool plain = !PARTS && p.h_dt < 0;
   const float inv = 1.f / (float)p.width;
-  float aw[ITER][VEC], ap[ITER][VEC], ac[ITER][VEC];
+  constexpr int kP = PARTS ? ITER : 1;
+  float aw[ITER][VEC], ap[kP][VEC], ac[kP][VEC];
 #pragma unroll
   for (int i = 0; i < ITER; ++i)
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) aw[i][k] = ap[i][k] = ac[i][k] = 0.f;
+    for (int k = 0; k < VEC; ++k) {
+      aw[i][k] = 0.f;
+      if constexpr (PARTS) ap[i][k] = ac[i][k] = 0.f;
+    }
   const uint32_t step = gridDim.x * per;
   for (uint32_t base = blockIdx.x * per; base < p.rows; base += step) {
     const uint32_t row = base + mine;
     const bool live = row < p.rows;
     const int64_t at = (int64_t)row * p.width;
     const int64_t oy = live ? row_at(p.ry, row, p.inner) : 0;
-    const int64_t og = live && p.gate ? row_at(p.rg, row, p.inner) : 0;
-    const bool use_y = !plain && p.y != nullptr;
-    float x[ITER][VEC], d[ITER][VEC], y[ITER][VEC];
-    float s[3] = {0.f, 0.f, 0.f};  // x^2, w dn x, y^2
-    Held<VEC> held_s[ITER], held_g[ITER];  // read after the sums, on their way before them
+    const int64_t og = PARTS && live && p.gate ? row_at(p.rg, row, p.inner) : 0;
+    float x[ITER][VEC], d[ITER][VEC], y[kP][VEC];
+    float s[PARTS ? 3 : 2] = {};  // x^2, w dn x, y^2
+    Held<VEC> held_s[ITER], held_g[kP];  // read after the sums, on their way before them
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
       if (!live || c >= p.width) continue;
       if (b.ds) held_s[i].load(b.ds, at + c, h_dt);
-      if (p.gate && p.gate_full) held_g[i].load(p.gate, og + c, g_dt);
+      if constexpr (PARTS)
+        if (p.gate && p.gate_full) held_g[i].load(p.gate, og + c, g_dt);
     }
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
       const int c = (i * g + t) * VEC;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[i][k] = d[i][k] = y[i][k] = 0.f;
+      for (int k = 0; k < VEC; ++k) {
+        x[i][k] = d[i][k] = 0.f;
+        if constexpr (PARTS) y[i][k] = 0.f;
+      }
       if (!live || c >= p.width) continue;
       if (plain) ldv<VEC>(p.y, oy + c, y_dt, x[i]);
       else ldv<VEC>(p.stream, at + c, h_dt, x[i]);
       if (b.dn) ldv<VEC>(b.dn, at + c, out_dt, d[i]);
-      if (use_y) ldv<VEC>(p.y, oy + c, y_dt, y[i]);
+      if constexpr (PARTS) ldv<VEC>(p.y, oy + c, y_dt, y[i]);
       float w[VEC];
       ldv<VEC>(p.w, c, kF32, w);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         s[0] += x[i][k] * x[i][k];
         s[1] += w[k] * d[i][k] * x[i][k];
-        s[2] += y[i][k] * y[i][k];
+        if constexpr (PARTS) s[2] += y[i][k] * y[i][k];
       }
     }
-    group_sum<G, 3>(s, sm, buf);
+    group_sum<G, PARTS ? 3 : 2>(s, sm, buf);
     const float r = rsqrtf(s[0] * inv + p.eps), q = s[1] * inv * r * r;
-    const float ry = p.wp ? rsqrtf(s[2] * inv + p.eps) : 1.f;
-    float gr = 1.f;
-    if (live && p.gate && !p.gate_full) gr = gate_back(load_in(p.gate, og, g_dt), g_dt);
+    float ry = 1.f, gr = 1.f;
+    if constexpr (PARTS) {
+      if (p.wp) ry = rsqrtf(s[2] * inv + p.eps);
+      if (live && p.gate && !p.gate_full) gr = gate_back(load_in(p.gate, og, g_dt), g_dt);
+    }
     float s2[2] = {0.f, 0.f};  // wp du y, row-gate gradient
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
@@ -416,62 +428,69 @@ __global__ void __launch_bounds__(MT) k_norm_bwd(const Bwd b) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[i][k] += a[k];
       }
-      if (plain) {
-        stv<VEC>(b.dy, at + c, y_dt, d[i]);
-        continue;
+      if (!plain && b.dh) stv<VEC>(b.dh, at + c, h_dt, d[i]);
+      if constexpr (!PARTS) {
+        if (!plain) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) d[i][k] *= p.c;
+        }
+        if (b.dy) stv<VEC>(b.dy, at + c, y_dt, d[i]);
+      } else {
+        float wp[VEC], cs[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) wp[k] = 1.f, cs[k] = p.c;
+        if (p.wp) ldv<VEC>(p.wp, c, kF32, wp);
+        if (p.scale) {
+          ldv<VEC>(p.scale, c, kF32, a);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) cs[k] *= a[k];
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) a[k] = gr;
+        if (p.gate && p.gate_full) {
+          held_g[i].get(g_dt, a);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) a[k] = gate_back(a[k], g_dt);
+        }
+        float dg[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const float u = y[i][k] * ry * wp[k], G_ = d[i][k];
+          ac[i][k] += G_ * a[k] * u * p.c;
+          dg[k] = G_ * cs[k] * u * a[k] * (1.f - a[k]);
+          s2[1] += dg[k];
+          const float du = G_ * cs[k] * a[k];
+          ap[i][k] += du * y[i][k] * ry;
+          d[i][k] = du * wp[k];
+          s2[0] += d[i][k] * y[i][k];
+        }
+        if (p.gate && p.gate_full && b.dgate) stv<VEC>(b.dgate, at + c, g_dt, dg);
       }
-      if (b.dh) stv<VEC>(b.dh, at + c, h_dt, d[i]);
-      float wp[VEC], cs[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) wp[k] = 1.f, cs[k] = p.c;
-      if (p.wp) ldv<VEC>(p.wp, c, kF32, wp);
-      if (p.scale) {
-        ldv<VEC>(p.scale, c, kF32, a);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) cs[k] *= a[k];
-      }
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) a[k] = gr;
-      if (p.gate && p.gate_full) {
-        held_g[i].get(g_dt, a);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) a[k] = gate_back(a[k], g_dt);
-      }
-      float dg[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float u = y[i][k] * ry * wp[k], G_ = d[i][k];
-        ac[i][k] += G_ * a[k] * u * p.c;
-        dg[k] = G_ * cs[k] * u * a[k] * (1.f - a[k]);
-        s2[1] += dg[k];
-        const float du = G_ * cs[k] * a[k];
-        ap[i][k] += du * y[i][k] * ry;
-        d[i][k] = du * wp[k];
-        s2[0] += d[i][k] * y[i][k];
-      }
-      if (p.gate && p.gate_full && b.dgate) stv<VEC>(b.dgate, at + c, g_dt, dg);
     }
-    if (plain) continue;
-    const bool row_gate = p.gate && !p.gate_full && b.dgate;
-    if (p.wp || row_gate) group_sum<G, 2>(s2, sm, buf);
-    if (row_gate && live && t == 0) store_out(b.dgate, row, s2[1], g_dt);
-    if (!b.dy) continue;
-    const float qy = p.wp ? s2[0] * inv * ry * ry : 0.f;
+    if constexpr (PARTS) {
+      const bool row_gate = p.gate && !p.gate_full && b.dgate;
+      if (p.wp || row_gate) group_sum<G, 2>(s2, sm, buf);
+      if (row_gate && live && t == 0) store_out(b.dgate, row, s2[1], g_dt);
+      if (!b.dy) continue;
+      const float qy = p.wp ? s2[0] * inv * ry * ry : 0.f;
 #pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-      const int c = (i * g + t) * VEC;
-      if (!live || c >= p.width) continue;
+      for (int i = 0; i < ITER; ++i) {
+        const int c = (i * g + t) * VEC;
+        if (!live || c >= p.width) continue;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) d[i][k] = ry * (d[i][k] - y[i][k] * qy);
-      stv<VEC>(b.dy, at + c, y_dt, d[i]);
+        for (int k = 0; k < VEC; ++k) d[i][k] = ry * (d[i][k] - y[i][k] * qy);
+        stv<VEC>(b.dy, at + c, y_dt, d[i]);
+      }
     }
   }
   auto emit = [&](int slot, const float (&a)[ITER][VEC]) {
     if (slot >= 0) emit_sums<G, VEC, ITER>(sums_at(b, slot), a, p.width, g, t, mine, per, fold);
   };
   emit(b.sum_w, aw);
-  emit(b.sum_p, ap);
-  emit(b.sum_c, ac);
+  if constexpr (PARTS) {
+    emit(b.sum_p, ap);
+    emit(b.sum_c, ac);
+  }
 }
 
 // The plain norm over narrow rows: each group takes kNarrow rows at once, all their loads in
@@ -1033,7 +1052,7 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
                    aligned8(g->dupdate) && (!f.gate_full || aligned8(g->dgate)) && aligned8(g->dweight) &&
                    aligned8(g->dpost_weight) && aligned8(g->dscale);
   const Shape s = shape_of(f, vec);
-  const bool light = s.vec == 8 && s.iter == 1 && !f.wp && !f.scale && !f.gate;
+  const bool parts = f.wp || f.scale || f.gate, light = s.vec == 8 && s.iter == 1 && !parts;
   int blocks = 0;
   {
     Launch scope("norm_bwd", st);
@@ -1046,7 +1065,12 @@ int norm_backward(const GpaNormArgs* a, const void* stream_in, const void* dstre
     if (blocks) K<<<blocks, s.threads, smem, st>>>(b);                           \
   } while (0)
 #define LIGHT(G, M) RUN((k_norm_bwd_light<G, M>), fold_smem)
-#define CALL(G, V, I, M) RUN((k_norm_bwd<G, V, I, M>), fold_smem)
+#define CALL(G, V, I, M)                                                   \
+  do {                                                                     \
+    /* 8 channels a thread in one turn without parts: k_norm_bwd_light */ \
+    if (parts || ((V) == 8 && (I) == 1)) RUN((k_norm_bwd<G, V, I, M, true>), fold_smem); \
+    else RUN((k_norm_bwd<G, V, I, M, (V) == 8 && (I) == 1>), fold_smem);   \
+  } while (0)
 #define TYPED(M, T) RUN((k_norm_bwd_parts<M, T>), slot_smem)
 #define BLOCK                                            \
   if (s.threads <= 320) NORM_TYPED(types, TYPED, 320);   \

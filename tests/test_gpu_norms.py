@@ -477,3 +477,11 @@ def test_column_sums_do_not_depend_on_earlier_calls(tmp_path):
     for width in (384, 768, 1280, 1792, 2560, 4096):
         a, b = (torch.load(f"{tmp_path}/{order}{width}.pt") for order in ("first", "alone"))
         assert all(torch.equal(x, y) for x, y in zip(a, b)), width
+
+
+@pytest.mark.parametrize("stream,update", [(F32, BF16), (F16, F16)])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_residual_norm_widths_without_parts(width, stream, update):
+    shape = (3, width)
+    t, const, ds, dn = _inputs(width, shape, stream, update, update, False, None, "number")
+    _check_case(t, const, ds, dn, update)
