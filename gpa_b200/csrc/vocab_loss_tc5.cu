@@ -28,10 +28,10 @@
 // x1 y0, x0 y1, x0 y0.  The tensor core drops the bits below its accumulator's last with every
 // step of 16, so a long reduction would lose what the parts gained: the accumulator is emptied
 // after a segment of it and the segments are added in registers, in round-to-nearest fp32, by
-// more epilogue warps (four threads a row of 256 columns, 64 registers each).  The statistics of
-// 16-bit inputs are formed the same way beyond 1024 channels: the loss is an fp32 result, and its
-// error would grow with the width (2048 channels: 1.1e-6 of the loss in one accumulator, 0.5e-6
-// in two).
+// more epilogue warps (four threads a row of 256 columns, 64 registers each).  So is dW of 16-bit
+// inputs over very many rows (see kSegmentDw), and so are the statistics of 16-bit inputs beyond
+// 1024 channels: the loss is an fp32 result, and its error would grow with the width (2048
+// channels: 1.1e-6 of the loss in one accumulator, 0.5e-6 in two).
 //
 // Measured (GPU time of one launch, B200): 65536 rows x 1024 channels x 151936 entries, bf16:
 // statistics 16.4 ms = 1.24 PFLOP/s, P 16.7 ms, dx 15.5 ms, dW 15.3 ms (1.33 PFLOP/s; a library
@@ -74,8 +74,15 @@ struct Smem {
 };
 // Reduction blocks between two additions in registers: 512 for the six products of fp32 parts one
 // after the other, 128 where the products of a part follow one another in every block (few rows,
-// see below), 1024 for single products.
+// see below), 1024 for single products of z.
 constexpr int kSegmentF32 = 8, kSegmentShare = 2, kSegment16 = 16;
+// dW of 16-bit inputs: the reduction runs over the rows, and what the accumulator drops was measured
+// at 1.04e-7 of the sum with every 16 of them (2^22 rows of one sign: 2.7e-2 of dW, 262144 of fp16:
+// 2e-3).  Up to 65536 rows (fp16: 8192) that stays below an eighth of the half step to which dW is
+// rounded; more are added up in registers 8192 at a time, which takes 3 % longer (65536 x 1024 x
+// 151936: 14.8 -> 15.3 ms).
+constexpr int kSegmentDw = 128;
+bool long_dw(const Call& c) { return c.n > (c.dtype == GPA_B200_F16 ? 8192 : 65536); }
 constexpr int kGroup = 16;  // row tiles that walk over the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -485,7 +492,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
       const int64_t left = a.dw_pitch - col0 - c;  // a multiple of 8
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = empty ? 0.f : v[i] * s;
-      if (F32) {
+      if (EXACT) {
         float* out = static_cast<float*>(a.dw) + at + c;
 #pragma unroll
         for (int i = 0; i < 32; i += 8)
@@ -650,7 +657,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(M, F32), 
   constexpr bool kT = M == kStatsT || M == kProbsT || M == kDxT;
   constexpr bool kAMn = M == kDw || M == kDxT, kBMn = M == kDx || M == kDw;
   constexpr bool kPlanes = PRODUCTS > 1, kShare = kPlanes && kT;
-  constexpr int kSegment = kShare ? kSegmentShare : kPlanes ? kSegmentF32 : kSegment16;
+  constexpr int kSegment = kShare ? kSegmentShare : kPlanes ? kSegmentF32 : M == kDw ? kSegmentDw : kSegment16;
   constexpr int kPasses = kShare ? 3 : PRODUCTS;  // over a segment
   using S = Smem<BN, kShare>;
   constexpr int kStages = S::kStages;
@@ -911,6 +918,8 @@ bool launch(const char* name, const CUtensorMap& ma, const CUtensorMap& mb, cons
   if (a.c.dtype == GPA_B200_F32) return launch_as<M, true, BN, 6>(name, ma, mb, a, tiles, st);
   if constexpr (M == kStats || M == kStatsT)
     if (exact_stats(a.c)) return launch_as<M, true, BN, 1>(name, ma, mb, a, tiles, st);
+  if constexpr (M == kDw)
+    if (long_dw(a.c)) return launch_as<M, true, BN, 1>(name, ma, mb, a, tiles, st);
   return launch_as<M, false, BN, 1>(name, ma, mb, a, tiles, st);
 }
 

@@ -462,3 +462,30 @@ def test_no_token_and_a_frozen_weight(dtype, reduction):
     loss = linear_cross_entropy(x, w, y, reduction=reduction)
     (dx,) = torch.autograd.grad(loss, x, torch.ones_like(loss))
     assert dx.shape == (0, 64) and dx.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype,rows", [(F16, 8193), (F16, 1 << 18), (BF16, 65537), (BF16, 1 << 20), (F32, 1 << 18)])
+@pytest.mark.parametrize("width,vocab", [(64, 64), (40, 300)])
+def test_weight_gradient_over_very_many_rows(dtype, rows, width, vocab):
+    """Sums of one sign over the rows: entry 0 is nobody's label.  P is off by the logits' error and
+    half a step of its type, dW is rounded once more; in between an accumulator loses at most 2^-23
+    of itself with each 16 rows, over 8192 of them at a time (fp16; fp32 less), and these are added
+    with at most one rounding each: 2^-14 + rows / 8192 U.  bf16 adds 65536 at a time: 2^-11."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (0.5 + torch.rand(rows, width, generator=g, device="cuda")).to(dtype)
+    w = (torch.randn(vocab, width, generator=g, device="cuda") * 0.05).to(dtype).requires_grad_()
+    y = torch.randint(1, vocab, (rows,), generator=g, device="cuda")
+    (dw,) = torch.autograd.grad(linear_cross_entropy(x, w, y), w)
+    wd = w.detach().double()
+    want, size, worst = torch.zeros_like(wd), torch.zeros_like(wd), 0.0
+    for i in range(0, rows, 1 << 16):
+        xd, yd = x[i:i + (1 << 16)].double(), y[i:i + (1 << 16), None]
+        worst = max(worst, 2 * (width + 2) * U * float((xd @ wd.abs().T).amax()))
+        p = torch.softmax(xd @ wd.T, -1)
+        full = p.scatter_add(1, yd, torch.ones_like(yd, dtype=torch.float64))  # softmax + onehot
+        want += (p.scatter_add(1, yd, -torch.ones_like(yd, dtype=torch.float64))).T @ xd / rows
+        size += full.T @ xd / rows
+    kept = 0.0 if dtype == F32 else 2.0 ** -14 if dtype == F16 else 2.0 ** -11
+    off = 2 * worst + 64 * U + HALF[dtype] + kept + (rows / 8192 + 4) * U + (1024 * U if dtype == F32 else 0.0)
+    bound = off * size + HALF[dtype] * want.abs() + TINY[dtype]
+    assert ((dw.double() - want).abs() <= bound).all(), float(((dw.double() - want).abs() / bound).max())
