@@ -245,6 +245,12 @@ GPA_DEV float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
   return m;
 }
+// Powers of 2 are taken of v log2(e) - base, base = m log2(e) as rounded, and so are all off by what
+// that rounding left: 4e-5 at m = 1000, enough for a loss below 0.  base_rest is the factor that puts
+// it right, once for a row; no m at all (-inf) has the base 0.
+GPA_DEV float scaled(float m) { return __fmul_rn(m, kLog2e); }  // rounded: never part of an fma
+GPA_DEV float base_of(float m) { return m == -INFINITY ? 0.f : scaled(m); }
+GPA_DEV float base_rest(float m) { return m == -INFINITY ? 1.f : ex2(-fmaf(m, kLog2e, -scaled(m))); }
 GPA_DEV uint32_t pack2(float a, float b, bool f16) {
   if (f16) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -395,7 +401,7 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
         m1 = max3(m1, v[i + 2], v[i + 3]);
       }
       m = fmaxf(m, m1);
-      const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
+      const float safe = m == -INFINITY ? 0.f : m, off = base_of(m);
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
@@ -407,9 +413,10 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
         scaled2(v[i], v[i + 1], off);
         add2(s0, s1, ex2(v[i]), ex2(v[i + 1]));
       }
-      sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(fmaf(big, kLog2e, -off)), s0 + s1);
+      sum = fmaf(sum, EXACT ? expf(big - safe) : ex2(scaled(big) - off), s0 + s1);
       big = m;
     }
+    if (!EXACT) sum *= base_rest(big);
     if (live) a.part[((int64_t)t.n * kGroups + group) * a.c.n_pad + row] = make_float2(big, sum);
   } else if (M == kProbs) {
     // P is rounded once to the type of its product's other operand, half a step of it (fp32: three
@@ -434,9 +441,12 @@ GPA_DEV void epilogue(const Args& a, const Tile& t, int n_rows, Row<F32, 64>& he
         v[i + 1] = EXACT ? expf(v[i + 1] - off) * f : ex2(v[i + 1]);
       }
       if (y >= c && y < c + 32) {
+        // off is rounded, which moves all of a row alike: within P's own rounding, but not here, where
+        // one goes off what may be nearly one
+        const float base = scaled(l.x), rest = EXACT ? 1.f : ex2((off - base) + log2f(f) - fmaf(l.x, kLog2e, -base));
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (y == c + i) v[i] -= one;
+          if (y == c + i) v[i] = fmaf(v[i], rest, -one);
       }
       const int64_t left = live ? a.vn - col0 - c : 0;
       if (left < 32) {
@@ -571,11 +581,11 @@ struct Stats {
         v[i] = s[i];
         m = fmaxf(m, v[i]);
       }
-      const float safe = m == -INFINITY ? 0.f : m, off = safe * kLog2e;
+      const float safe = m == -INFINITY ? 0.f : m, off = base_of(m);
       float more = 0.f;
 #pragma unroll
       for (int i = 0; i < C::kCh; ++i) more += EXACT ? expf(v[i] - safe) : ex2(fmaf(v[i], kLog2e, -off));
-      sum[k] = fmaf(sum[k], EXACT ? expf(big[k] - safe) : ex2(fmaf(big[k], kLog2e, -off)), more);
+      sum[k] = fmaf(sum[k], EXACT ? expf(big[k] - safe) : ex2(scaled(big[k]) - off), more);
       big[k] = m;
       const int64_t y = label[k] - base - lane * C::kCh;
       if (label[k] >= 0 && y >= 0 && y < C::kCh) a.z_label[column(k)] = s[y];
@@ -586,18 +596,20 @@ struct Stats {
 #pragma unroll
     for (int k = 0; k < C::kChunks; ++k)
       if (column(k) < n_rows)
-        a.part[((int64_t)blockIdx.x * C::kLanes + lane) * a.c.n_pad + column(k)] = make_float2(big[k], sum[k]);
+        a.part[((int64_t)blockIdx.x * C::kLanes + lane) * a.c.n_pad + column(k)] =
+            make_float2(big[k], EXACT ? sum[k] : sum[k] * base_rest(big[k]));
   }
 };
 
-// {max (times log2 e for 16-bit inputs), factor of the exp, P's unit, label within the piece} of row j of x
+// {max (16-bit inputs: its base), factor of the exp, P's unit, label within the piece} of row j of x
 template <bool F32>
 GPA_DEV float4 row_of(const Args& a, int j, int n_rows) {
   if (j >= n_rows) return make_float4(0.f, 0.f, 0.f, __int_as_float(-2));  // no row
   const float2 l = a.lse[j];
   const float one = a.c.label[j] < 0 ? NAN : a.p_scale;
   const int64_t y = (int64_t)a.c.label[j] - a.v0;
-  return make_float4(F32 ? l.x : l.x * kLog2e, l.y * one, one, __int_as_float(y >= 0 && y < a.vn ? (int)y : -1));
+  return make_float4(F32 ? l.x : scaled(l.x), F32 ? l.y * one : l.y * one * base_rest(l.x), one,
+                     __int_as_float(y >= 0 && y < a.vn ? (int)y : -1));
 }
 
 template <Mode M, bool F32, int BN>

@@ -11,6 +11,8 @@ multiplies dx in fp32, and the rows that dW takes, rounded to their type.  The p
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -489,3 +491,35 @@ def test_weight_gradient_over_very_many_rows(dtype, rows, width, vocab):
     off = 2 * worst + 64 * U + HALF[dtype] + kept + (rows / 8192 + 4) * U + (1024 * U if dtype == F32 else 0.0)
     bound = off * size + HALF[dtype] * want.abs() + TINY[dtype]
     assert ((dw.double() - want).abs() <= bound).all(), float(((dw.double() - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,width", [(20, 64), (100, 64), (300, 64), (300, 1500), (20, 1500)])
+@pytest.mark.parametrize("big", [300.0, 1000.0, 3000.0, 20000.0])
+def test_a_token_that_has_all_the_probability(dtype, rows, width, big):
+    """One entry's logit is big x for 0.3 < x < 1, every other one 0: the loss is 0 and so are the
+    gradients.  An exp2 of a value near 0 and its correction are within 4 U of 1 each, their
+    product, the sum of one term, its log and reciprocal within 8 more: 16 U of a probability.  The
+    2999 entries of logit 0 have at most e^(-0.3 big) each, 2.5e-36 in all at 300: fp32 holds that."""
+    g = torch.Generator().manual_seed(int(big))
+    x = torch.zeros(rows, width)
+    x[:, 0] = 0.3 + 0.7 * torch.rand(rows, generator=g)
+    w = torch.randn(3000, width, generator=g) * 0.5
+    w[:, 0] = 0
+    w[1234] = 0
+    w[1234, 0] = big
+    x, w, y = x.to(dtype).cuda(), w.to(dtype).cuda(), torch.full((rows,), 1234).cuda()
+    for label, expected in ((1234, 0.0), (77, 1.0)):
+        y.fill_(label)
+        xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = linear_cross_entropy(xr, wr, y, reduction="none")
+        want = x[:, 0].double() * w[1234, 0].double() * expected
+        assert ((loss.double() - want).abs() <= 16 * U + 2 * U * want).all()
+        dx, dw = torch.autograd.grad(loss.sum(), (xr, wr))
+        # of each row: (P - hot) w over the two entries that matter
+        p = expected * (w[1234].double() - w[label].double())
+        off = (16 * U + HALF[dtype]) * expected + 16 * U
+        assert ((dx.double() - p).abs() <= off * (w[1234].abs() + w[label].abs()).double() +
+                HALF[dtype] * p.abs() + TINY[dtype] + 3000 * math.exp(-0.3 * big) * w.abs().double().amax()).all()
+        total = x.double().abs().sum(0)
+        assert (dw[1234].double().abs() <= expected * total * (1 + 1e-2) + 16 * U * total + TINY[dtype]).all()
