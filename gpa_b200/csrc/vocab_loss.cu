@@ -13,6 +13,7 @@
 #include "vocab_loss.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace gpa {
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(256) k_pack(const Pack p, const T* src, typena
 }
 
 // The weight where the tensor cores cannot read the caller's: rows that do not start on 16 bytes,
-// or fp32.  A warp a row; rows behind the last (of a plane) become zero.
+// or fp32 (few rows: in the backward alone, see k_few).  A warp a row; rows behind the last (of a plane) become zero.
 template <typename T>
 __global__ void __launch_bounds__(256) k_weight(const T* src, int64_t stride, int64_t vocab, int64_t rows, int width,
                                                 int pitch, int64_t plane, bool vec, typename Part<T>::type* dst) {
@@ -258,6 +259,139 @@ __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, 
   }
 }
 
+// ------------------------------------------------------------------ statistics of few fp32 rows
+// (max, sum of exp) of z for R of the packed rows a blockIdx.y, with fp32 multiply-adds on the weight as
+// it is.  The tensor cores take fp32 as three bf16 parts, and writing and reading those (12 bytes a value
+// beside the 4) is most of the time where rows are few.  Scores against 151936 entries of 1024 channels:
+// 8 rows 584 -> 198 us, 16 -> 221, 32 -> 354; 64 rows would take two turns of W, as long as their parts.
+//
+// A warp takes E entries at a time, its lanes four channels each of every 128; x lies in shared memory
+// as pairs of rows, and two rows go to an instruction.  W's next values are on their way meanwhile: with
+// 8 rows it comes by at 4.1 TB/s (eight warps of 200 registers an SM), with 32 instructions bound it.
+// The E R sums are added over the lanes 32 at a time, so that lane l ends up with the l-th of them.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewShared = 192 * 1024;
+
+struct Few {
+  const float *w, *x;     // the caller's weight and rows
+  int64_t w_stride, so, si, inner;
+  int pitch;              // channels up to a multiple of 128
+  bool vec;               // rows of both start on 16 bytes
+  float2* part;
+  float* z_label;
+};
+
+GPA_DEV float4 few_load(const float* p, int d, int width, bool vec) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vec) {
+    if (d < width) v = __ldcs(reinterpret_cast<const float4*>(p + d));  // width is a multiple of 4
+  } else {
+    if (d < width) v.x = p[d];
+    if (d + 1 < width) v.y = p[d + 1];
+    if (d + 2 < width) v.z = p[d + 2];
+    if (d + 3 < width) v.w = p[d + 3];
+  }
+  return v;
+}
+
+template <int R, int E>
+__global__ void __launch_bounds__(kFewThreads, 1) k_few(const Call c, const Few f) {
+  // [R / 2][channels 0, 1 or 2, 3 of four][pitch / 4]: {row, next row} of two channels; neighbouring
+  // lanes read neighbouring 16 bytes
+  extern __shared__ float4 xs[];
+  __shared__ float2 joined[kFewWarps][R];
+  constexpr int kAtOnce = 32 / R;  // entries whose sums fill the lanes
+  let_next();
+  after_previous();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.y * R, quads = f.pitch / 4;
+  const int rows = min(*c.n_rows - first, R);
+  if (rows <= 0) return;
+  const int row = lane % R;
+  const int label = row < rows ? c.label[first + row] : -1;
+  for (int i = threadIdx.x; i < R * quads; i += kFewThreads) {
+    const int j = i / quads, q = i % quads;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (j < rows) {
+      const int64_t at = c.row[first + j];
+      v = few_load(f.x + (at / f.inner) * f.so + (at % f.inner) * f.si, q * 4, c.width, f.vec);
+    }
+    float* to = reinterpret_cast<float*>(xs + (j >> 1) * 2 * quads + q) + (j & 1);
+    to[0] = v.x, to[2] = v.y;
+    to += 4 * quads;
+    to[0] = v.z, to[2] = v.w;
+  }
+  __syncthreads();
+  float m = -INFINITY, s = 0.f;
+  const int64_t step = (int64_t)gridDim.x * kFewWarps * E;
+  for (int64_t v0 = ((int64_t)blockIdx.x * kFewWarps + warp) * E; v0 < c.vocab; v0 += step) {
+    const float* w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = f.w + (v0 + e < c.vocab ? v0 + e : c.vocab - 1) * f.w_stride;
+    float2 acc[E][R / 2];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int r = 0; r < R / 2; ++r) acc[e][r] = make_float2(0.f, 0.f);
+    float4 next[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) next[e] = few_load(w[e], lane * 4, c.width, f.vec);
+    for (int d = lane * 4; d < f.pitch; d += 128) {
+      float4 now[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        now[e] = next[e];
+        next[e] = few_load(w[e], d + 128, c.width, f.vec);
+      }
+#pragma unroll
+      for (int r = 0; r < R / 2; ++r) {
+        const float4 a = xs[2 * r * quads + d / 4], b = xs[(2 * r + 1) * quads + d / 4];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float2 v = acc[e][r];
+          v = __ffma2_rn(make_float2(a.x, a.y), make_float2(now[e].x, now[e].x), v);
+          v = __ffma2_rn(make_float2(a.z, a.w), make_float2(now[e].y, now[e].y), v);
+          v = __ffma2_rn(make_float2(b.x, b.y), make_float2(now[e].z, now[e].z), v);
+          acc[e][r] = __ffma2_rn(make_float2(b.z, b.w), make_float2(now[e].w, now[e].w), v);
+        }
+      }
+    }
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += kAtOnce) {
+      float v[32];
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const float2 a = acc[e0 + i / R][i % R / 2];
+        v[i] = a.x, v[i + 1] = a.y;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+          const bool high = lane & o;
+          const float mine = high ? v[i + o] : v[i], other = high ? v[i] : v[i + o];
+          v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+        }
+      const int64_t entry = v0 + e0 + lane / R;
+      const bool is = entry < c.vocab;
+      if (is && entry == label) f.z_label[first + row] = v[0];
+      merge(m, s, is ? v[0] : -INFINITY, is ? 1.f : 0.f);
+    }
+  }
+#pragma unroll
+  for (int o = R; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    merge(m, s, m2, s2);
+  }
+  if (lane < R) joined[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x < rows) {
+    float2 a = joined[0][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < kFewWarps; ++k) merge(a.x, a.y, joined[k][threadIdx.x].x, joined[k][threadIdx.x].y);
+    f.part[blockIdx.x * c.n_pad + first + threadIdx.x] = a;
+  }
+}
+
 // fp16, a gradient for each row: s = the largest magnitude, r = its share (x times r would leave
 // fp16's range otherwise).
 __global__ void __launch_bounds__(1024) k_row_scale(const float* dloss, const Call c, float* r, float* scale) {
@@ -343,6 +477,7 @@ constexpr int64_t kPieceBytes = int64_t(3) << 29;  // of P at a time
 struct Plan {
   Call c;
   bool copy_w;             // the weight is copied first (k_weight)
+  int few_rows;            // the forward's statistics by k_few: its rows a block (8, 16 or 32); or 0
   int es;                  // bytes of an element of the caller's tensors
   int parts_v;             // (max, sum) pairs of a row
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
@@ -351,8 +486,15 @@ struct Plan {
   int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
   // scratch
   int64_t count, part, z_label, loss, fwd_bytes;
-  int64_t p, dxp, dwp, xr, r, scale, bwd_bytes;
+  int64_t p, dxp, dwp, xr, r, scale, w, again, lse, bwd_bytes;
 };
+
+// fp32 rows that k_few takes, in one turn of the weight or, where their x fills shared memory, two
+constexpr int64_t kFewRows = 32;
+int few_entries(const Plan& p) { return kFewWarps * (p.few_rows == 32 ? 4 : 8); }  // of a block's turn
+int few_blocks(const Plan& p) {
+  return (int)std::min<int64_t>((p.c.vocab + few_entries(p) - 1) / few_entries(p), 2 * tc_pairs());
+}
 
 const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   *code = GPA_B200_BAD_ARGUMENT;
@@ -384,7 +526,11 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   const int64_t tiles_d = (c.pitch + kTile - 1) / kTile;
   if (tiles_v * tiles_m > (int64_t(1) << 30)) return "at most 2^30 tiles of 256 x 256 logits in a call";
   c.few = c.n <= 32 ? 32 : c.n <= 128 ? 128 : 0;
-  p->parts_v = tc_stats_parts(c);
+  p->few_rows = !f32 || c.n > kFewRows ? 0 : c.n <= 8 ? 8 : c.n <= 16 ? 16 : 32;
+  while (p->few_rows && p->few_rows * up(c.width, 128) * 4 > kFewShared)
+    p->few_rows = p->few_rows > 8 ? p->few_rows / 2 : 0;
+  if (p->few_rows * 2 < c.n) p->few_rows = 0;
+  p->parts_v = p->few_rows ? few_blocks(*p) : tc_stats_parts(c);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
   // come out in fewer turns of the whole GPU (the pieces' turns added up).
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * 2 * c.planes) / kTile);
@@ -423,7 +569,8 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->s_pos = take(4 * c.n);
   p->s_lse = take(8 * c.n);
   p->s_x = take(c.planes * c.n_pad * c.pitch * 2);
-  p->s_w = take(p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0);
+  const int64_t w_bytes = p->copy_w ? c.planes * up(c.vocab, kTile) * c.pitch * 2 : 0;
+  p->s_w = take(p->few_rows ? 0 : w_bytes);
   p->s_bytes = at;
   at = 0;
   p->count = take(4 * (up(c.n, kRun) / kRun));
@@ -438,6 +585,9 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->xr = take(a->reduction == GPA_B200_LOSS_NONE ? c.planes * c.n_pad * c.pitch * 2 : 0);
   p->r = take(4 * c.n);
   p->scale = take(4);
+  p->w = take(p->few_rows ? w_bytes : 0);
+  p->again = take(p->few_rows ? (int64_t)tc_stats_parts(c) * c.n_pad * 8 : 0);
+  p->lse = take(p->few_rows ? 8 * c.n : 0);
   p->bwd_bytes = at;
   return nullptr;
 }
@@ -476,14 +626,58 @@ void pack(const GpaLossArgs* a, const Plan& p, char* saved, char* scratch, cudaS
 }
 
 template <typename T>
-void copy_weight(const GpaLossArgs* a, const Plan& p, char* saved, cudaStream_t st) {
+void copy_weight(const GpaLossArgs* a, const Plan& p, char* to, cudaStream_t st) {
   const Call& c = p.c;
   const int64_t rows = c.planes > 1 ? up(c.vocab, kTile) : c.vocab;
   const bool vec = c.width % 8 == 0 && a->weight_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(a->weight) & 15) == 0;
   Launch scope("loss_weight", st);
   k_weight<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(
       static_cast<const T*>(a->weight), a->weight_stride, c.vocab, rows, c.width, c.pitch, rows * c.pitch, vec,
-      reinterpret_cast<typename Part<T>::type*>(saved + p.s_w));
+      reinterpret_cast<typename Part<T>::type*>(to));
+}
+
+template <int R, int E>
+bool few_as(const Plan& p, const Few& f, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(k_few<R, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared) != cudaSuccess)
+      return false;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  Launch scope("loss_stats_few", st);
+  return launch_next(k_few<R, E>, dim3(p.parts_v, (unsigned)((p.c.n + R - 1) / R)), kFewThreads,
+                     (size_t)R * f.pitch * 4, st, p.c, f);
+}
+
+// the losses to `each` (by the caller's rows), or their sum or mean to `total`
+bool join(const Plan& p, const float2* part, int parts, const float* z_label, float2* lse, float* each, float* packed,
+          float* total, const char* saved, int* counter, bool mean, cudaStream_t st) {
+  const Call& c = p.c;
+  const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;  // few rows: more lanes for the tiles of each
+  Launch scope("loss_join", st);
+  return launch_next(k_join, (unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st, c,
+                     part, parts, z_label, lse, each, reinterpret_cast<const int*>(saved + p.s_pos), packed, total, mean,
+                     counter);
+}
+
+bool few_stats(const GpaLossArgs* a, const Plan& p, float2* part, float* z_label, cudaStream_t st) {
+  Few f;
+  f.w = static_cast<const float*>(a->weight);
+  f.x = static_cast<const float*>(a->hidden);
+  f.w_stride = a->weight_stride;
+  f.so = a->hidden_stride[0];
+  f.si = a->hidden_stride[1];
+  f.inner = std::max<int64_t>(a->inner, 1);
+  f.pitch = (int)up(p.c.width, 128);
+  f.vec = a->width % 4 == 0 && f.w_stride % 4 == 0 && f.so % 4 == 0 && f.si % 4 == 0 &&
+          ((reinterpret_cast<uintptr_t>(f.w) | reinterpret_cast<uintptr_t>(f.x)) & 15) == 0;
+  f.part = part;
+  f.z_label = z_label;
+  if (p.few_rows == 8) return few_as<8, 8>(p, f, st);
+  return p.few_rows == 16 ? few_as<16, 8>(p, f, st) : few_as<32, 4>(p, f, st);
 }
 
 template <typename T>
@@ -508,7 +702,7 @@ void bind(Plan* p, const void* saved) {
   p->c.row = reinterpret_cast<const int*>(s + p->s_row);
   p->c.label = reinterpret_cast<const int*>(s + p->s_label);
   p->c.x = s + p->s_x;
-  if (p->copy_w) p->c.w = s + p->s_w;
+  if (p->copy_w && !p->few_rows) p->c.w = s + p->s_w;
 }
 
 #define BY_TYPE(DT, CALL)                                  \
@@ -589,21 +783,17 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
   float2* part = reinterpret_cast<float2*>(sc + p.part);
   BY_TYPE(a->dtype, pack<T>(a, p, sv, sc, st));
   OK_OR("loss_pack launch failed");
-  if (p.copy_w && c.n) {
-    BY_TYPE(a->dtype, copy_weight<T>(a, p, sv, st));
+  if (p.copy_w && !p.few_rows && c.n) {
+    BY_TYPE(a->dtype, copy_weight<T>(a, p, sv + p.s_w, st));
     OK_OR("loss_weight launch failed");
   }
-  if (c.n && !tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
-  if (c.n || !none) {
-    // few rows: more lanes for the tiles of each
-    const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;
-    Launch scope("loss_join", st);
-    if (!launch_next(k_join, (unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st, c,
-                     part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
-                     reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
-                     a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1))
-      FAIL("loss_join launch failed");
-  }
+  if (c.n && p.few_rows && !few_stats(a, p, part, z_label, st)) FAIL("loss_stats_few launch failed");
+  if (c.n && !p.few_rows && !tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
+  if ((c.n || !none) &&
+      !join(p, part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
+            reinterpret_cast<float*>(sc + p.loss), loss, sv, reinterpret_cast<int*>(sv) + 1,
+            a->reduction == GPA_B200_LOSS_MEAN, st))
+    FAIL("loss_join launch failed");
   return GPA_B200_OK;
 }
 
@@ -637,6 +827,21 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved);
   const float2* lse = reinterpret_cast<const float2*>(sv + p.s_lse);
+  if (p.few_rows) {
+    // The products below read W in parts, and P is measured by statistics of the same logits: the
+    // forward's differ by fp32's rounding of sums, 1e-5 of P for a logit of 100, where P - 1 may be
+    // nothing.  The labels' logits and the losses, formed once more, are left where nothing lies yet.
+    copy_weight<float>(a, p, sc + p.w, st);
+    OK_OR("loss_weight launch failed");
+    p.c.w = sc + p.w;
+    float2* again = reinterpret_cast<float2*>(sc + p.again);
+    float2* to = reinterpret_cast<float2*>(sc + p.lse);
+    float *z_label = reinterpret_cast<float*>(sc + p.r), *each = reinterpret_cast<float*>(sc + p.dxp);
+    if (!tc_stats(c, again, z_label, st)) FAIL("loss_stats_tc5 launch failed");
+    if (!join(p, again, tc_stats_parts(c), z_label, to, each, nullptr, nullptr, sv, nullptr, false, st))
+      FAIL("loss_join launch failed");
+    lse = to;
+  }
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
   const bool none = a->reduction == GPA_B200_LOSS_NONE;

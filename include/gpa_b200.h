@@ -270,8 +270,8 @@ typedef struct GpaLossArgs {
 
 /* Bytes of the buffer that the forward leaves for the backward, and of either call's scratch
  * (0 for arguments the entry points refuse); both start on 32 bytes.  saved holds the labelled
- * rows, and a copy of a weight that the tensor cores cannot read in place (fp32, or rows that do
- * not start on 16 bytes). */
+ * rows, and a copy of a weight that the tensor cores cannot read in place (rows that do not start
+ * on 16 bytes, or fp32 and more than 32 rows, of wide ones fewer). */
 size_t gpa_b200_loss_saved_bytes(const GpaLossArgs* args);
 size_t gpa_b200_loss_scratch_bytes(const GpaLossArgs* args, int backward);
 /* How the backward sums dhidden over the vocabulary for `labelled` of the rows (on the host; for

@@ -200,7 +200,8 @@ def _expected(x, head, labels):
 def test_losses_of_every_size_are_answered(tokens, grad):
     """More tokens than linear_cross_entropy takes in a call, and few: 1e-5 relative, fp32's
     rounding over 8 channels and a mean with room."""
-    m = GPALM(dataclasses.replace(CFG, vocab_size=16, hidden_size=8, num_layers=0, loss_chunk_size=1 << 20)).cuda().eval()
+    cfg = dataclasses.replace(CFG, vocab_size=16, hidden_size=8, num_layers=0, loss_chunk_size=1 << 20)
+    m = GPALM(cfg).cuda().eval()
     g = torch.Generator().manual_seed(13)
     x = torch.randn(1, tokens, 8, generator=g).cuda().requires_grad_(grad)
     labels = torch.randint(0, 16, (1, tokens), generator=g).cuda()

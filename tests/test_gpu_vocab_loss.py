@@ -523,3 +523,31 @@ def test_a_token_that_has_all_the_probability(dtype, rows, width, big):
                 HALF[dtype] * p.abs() + TINY[dtype] + 3000 * math.exp(-0.3 * big) * w.abs().double().amax()).all()
         total = x.double().abs().sum(0)
         assert (dw[1234].double().abs() <= expected * total * (1 + 1e-2) + 16 * U * total + TINY[dtype]).all()
+
+
+@pytest.mark.parametrize("rows,width,vocab", [
+    (1, 1, 1), (1, 4, 5), (7, 3, 63), (8, 128, 64), (8, 6144, 700), (8, 6200, 300), (9, 130, 65), (9, 3100, 500),
+    (16, 1001, 5003), (16, 3200, 129), (17, 1500, 1187), (17, 1700, 300), (31, 64, 4800), (32, 2900, 333),
+    (32, 3200, 333), (32, 127, 9999),
+])
+@pytest.mark.parametrize("masked", [0.0, 0.5])
+def test_few_fp32_rows(rows, width, vocab, masked):
+    """Rows of one block and of two, what fits shared memory and what does not, sizes off every unit."""
+    _case(rows + width, (rows,), width, vocab, F32, "mean", masked)
+
+
+def test_few_fp32_rows_of_strided_and_spoilt_tensors():
+    x, w, y = _inputs(50, (3, 9), 96, 777, F32, 0.3)
+    want = _run(x, w, y, "none")
+    wide, tall = (torch.full(shape, float("nan"), device="cuda") for shape in ((3, 11, 107), (777, 131)))
+    wide[:, 1:10, 3:99], tall[:, 7:103] = x, w  # neither starts on 16 bytes; NaN all round
+    for a, b in zip(want, _run(wide[:, 1:10, 3:99], tall[:, 7:103], y, "none")):
+        assert torch.equal(a, b)
+    dirty = x.clone()
+    dirty[y == -100] = float("inf")
+    for a, b in zip(want, _run(dirty, w, y, "none")):
+        assert torch.equal(a, b)
+    broken = w.clone()
+    broken[5, 3] = float("nan")
+    loss = linear_cross_entropy(x, broken, y, reduction="none")
+    assert (loss.isnan() == (y != -100)).all()
