@@ -233,6 +233,7 @@ class BlockOutput(nn.Module):
     def add_and_norm(self, x: Tensor, update: Tensor, gate: Tensor | None, norm: nn.Module, dtype: torch.dtype):
         """(x + the update's share, its norm in the dtype its reader takes)."""
         post = self.post
+        x = x.to(torch.promote_types(x.dtype, update.dtype))  # the stream's type, as of x + update
         if _kernels(x) and _bare(norm, RMSNorm) and (
                 post is None or (_bare(post, RMSNorm) and post.eps == norm.eps)):
             return residual_norm(x, update, norm.weight, norm.eps, gate=gate, scale=self.scale,

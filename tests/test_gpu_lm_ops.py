@@ -13,7 +13,7 @@ import pytest
 import torch
 
 from gpa_b200 import _lib
-from gpa_b200.lm import GPALM, GPALMConfig, RMSNorm
+from gpa_b200.lm import GPALM, BlockOutput, GPALMConfig, RMSNorm
 from gpa_b200.training_graph import GradientGraph
 from lm_around import Adapted, Round, shard
 from lm_oracle import oracle_lm
@@ -242,3 +242,14 @@ def test_the_model_s_norm_keeps_forward_mode_and_transforms():
     mag = (td.abs() * r + xd.abs() * r ** 3 * (xd * td).abs().mean(-1, keepdim=True))
     assert ((tangent.double() - want).abs() <= 64 * 2.0 ** -24 * mag).all()
     assert torch.allclose(torch.func.vmap(norm)(x), norm(x), atol=0, rtol=1e-5)
+
+
+@pytest.mark.parametrize("stream,update", [(torch.float16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                           (torch.float32, torch.float16), (torch.bfloat16, torch.bfloat16)])
+def test_stream_has_the_type_of_the_addition(stream, update):
+    """As of x + y: half-precision weights under bf16 autocast leave an fp32 stream."""
+    out, norm = BlockOutput(CFG).cuda(), RMSNorm(128, 1e-6).cuda()
+    g = torch.Generator().manual_seed(17)
+    x, y = torch.randn(5, 128, generator=g).cuda().to(stream), torch.randn(5, 128, generator=g).cuda().to(update)
+    s, n = out.add_and_norm(x, y, None, norm, torch.bfloat16)
+    assert s.dtype == (x + y).dtype and torch.equal(s, x + y) and n.dtype == torch.bfloat16
