@@ -551,3 +551,17 @@ def test_few_fp32_rows_of_strided_and_spoilt_tensors():
     broken[5, 3] = float("nan")
     loss = linear_cross_entropy(x, broken, y, reduction="none")
     assert (loss.isnan() == (y != -100)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead", [(20,), (60,), (300,)])
+def test_gradients_of_extreme_logits(lead, dtype):
+    """Some entries have no probability above 2^-126 in any row: exp2 and the tensor cores' sums hold
+    no smaller numbers, so each P may be off by that much, beside the bounds of other logits."""
+    x, w, y = _inputs(8, lead, 64, 513, dtype, spread=60.0)
+    loss, dx, dw, up = _run(x, w, y, "none")
+    want = _reference(x, w, y, up, "none")
+    xd, wd, g = x.double().cpu(), w.double().cpu(), up.double().cpu()[:, None].abs()
+    (vx, bx), (vw, bw) = want["dhidden"], want["dweight"]
+    _check("dhidden", dx, (vx, bx + 2.0 ** -126 * g * wd.abs().sum(0)))
+    _check("dweight", dw, (vw, bw + 2.0 ** -126 * (g * xd.abs()).sum(0)))
