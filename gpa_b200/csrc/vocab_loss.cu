@@ -259,26 +259,36 @@ __global__ void __launch_bounds__(256) k_join(const Call c, const float2* part, 
   }
 }
 
-// ------------------------------------------------------------------ statistics of few fp32 rows
-// (max, sum of exp) of z for R of the packed rows a blockIdx.y, with fp32 multiply-adds on the weight as
-// it is.  The tensor cores take fp32 as three bf16 parts, and writing and reading those (12 bytes a value
-// beside the 4) is most of the time where rows are few.  Scores against 151936 entries of 1024 channels:
-// 8 rows 584 -> 198 us, 16 -> 221, 32 -> 354; 64 rows would take two turns of W, as long as their parts.
+// ------------------------------------------------------------------ z of few fp32 rows
+// z for R of the packed rows a blockIdx.y, with fp32 multiply-adds on the weight as it is: (max, sum of
+// exp) of each row, or P of a piece.  The tensor cores take fp32 as three bf16 parts, and writing and
+// reading those (12 bytes a value beside the 4) is most of the time where rows are few.  Scores against
+// 151936 entries of 1024 channels: 8 rows 584 -> 194 us, 16 -> 218, 32 -> 345; steps 1420 -> 1136 and
+// 1191, with 32 rows 1440 as before.  64 rows would take two turns of W, as long as their parts.  P
+// comes from here too, of the same bits of z: what it is measured by (P - 1 may be nothing) must not
+// differ by so much as a rounding.
 //
 // A warp takes E entries at a time, its lanes four channels each of every 128; x lies in shared memory
 // as pairs of rows, and two rows go to an instruction.  W's next values are on their way meanwhile: with
-// 8 rows it comes by at 4.1 TB/s (eight warps of 200 registers an SM), with 32 instructions bound it.
-// The E R sums are added over the lanes 32 at a time, so that lane l ends up with the l-th of them.
+// 8 rows it comes by at 4.1 TB/s (eight warps of 200 registers an SM), with 32 instructions bound it
+// (half a warp's lanes for either 16 rows, with half the reads of x: 308 -> 334 us).  The E R sums are
+// added over the lanes 32 at a time, so that lane l ends up with row l % R of kMine neighbouring entries.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
-constexpr int kFewShared = 192 * 1024;
+constexpr int kFewShared = 224 * 1024;
 
 struct Few {
-  const float *w, *x;     // the caller's weight and rows
-  int64_t w_stride, so, si, inner;
+  const float* w;         // the caller's weight
+  int64_t w_stride;
   int pitch;              // channels up to a multiple of 128
-  bool vec;               // rows of both start on 16 bytes
+  bool vec;               // rows of W start on 16 bytes
+  int64_t v0, end;        // entries
+  // statistics
   float2* part;
   float* z_label;
+  // P of the entries, and zeros behind the last of the vocabulary
+  const float2* lse;
+  uint16_t* p;
+  int64_t p_pitch;
 };
 
 GPA_DEV float4 few_load(const float* p, int d, int width, bool vec) {
@@ -294,36 +304,45 @@ GPA_DEV float4 few_load(const float* p, int d, int width, bool vec) {
   return v;
 }
 
-template <int R, int E>
+template <int R, int E, bool PROBS>
 __global__ void __launch_bounds__(kFewThreads, 1) k_few(const Call c, const Few f) {
   // [R / 2][channels 0, 1 or 2, 3 of four][pitch / 4]: {row, next row} of two channels; neighbouring
   // lanes read neighbouring 16 bytes
   extern __shared__ float4 xs[];
   __shared__ float2 joined[kFewWarps][R];
-  constexpr int kAtOnce = 32 / R;  // entries whose sums fill the lanes
+  constexpr int kMine = E * R / 32;  // entries of a lane in the end
   let_next();
   after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, first = blockIdx.y * R, quads = f.pitch / 4;
   const int rows = min(*c.n_rows - first, R);
   if (rows <= 0) return;
   const int row = lane % R;
-  const int label = row < rows ? c.label[first + row] : -1;
+  const bool live = row < rows;
+  const int label = live ? c.label[first + row] : -1;
+  const uint16_t* x = static_cast<const uint16_t*>(c.x) + (int64_t)first * c.pitch;
+  const int64_t x_plane = c.n_pad * c.pitch;
   for (int i = threadIdx.x; i < R * quads; i += kFewThreads) {
     const int j = i / quads, q = i % quads;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (j < rows) {
-      const int64_t at = c.row[first + j];
-      v = few_load(f.x + (at / f.inner) * f.so + (at % f.inner) * f.si, q * 4, c.width, f.vec);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (j < rows && q * 4 < c.pitch) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {  // the parts add up to the value, without a rounding
+        const uint2 u = *reinterpret_cast<const uint2*>(x + k * x_plane + (int64_t)j * c.pitch + q * 4);
+        v[0] += __uint_as_float(u.x << 16), v[1] += __uint_as_float(u.x & 0xffff0000u);
+        v[2] += __uint_as_float(u.y << 16), v[3] += __uint_as_float(u.y & 0xffff0000u);
+      }
     }
     float* to = reinterpret_cast<float*>(xs + (j >> 1) * 2 * quads + q) + (j & 1);
-    to[0] = v.x, to[2] = v.y;
+    to[0] = v[0], to[2] = v[1];
     to += 4 * quads;
-    to[0] = v.z, to[2] = v.w;
+    to[0] = v[2], to[2] = v[3];
   }
   __syncthreads();
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY, s = 0.f;  // of the row so far, or P's: its maximum and factor
+  const float one = live && label < 0 ? NAN : 1.f;  // no such label: the row is NaN
+  if (PROBS && live) m = f.lse[first + row].x, s = f.lse[first + row].y * one;
   const int64_t step = (int64_t)gridDim.x * kFewWarps * E;
-  for (int64_t v0 = ((int64_t)blockIdx.x * kFewWarps + warp) * E; v0 < c.vocab; v0 += step) {
+  for (int64_t v0 = f.v0 + ((int64_t)blockIdx.x * kFewWarps + warp) * E; v0 < f.end; v0 += step) {
     const float* w[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) w[e] = f.w + (v0 + e < c.vocab ? v0 + e : c.vocab - 1) * f.w_stride;
@@ -355,12 +374,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) k_few(const Call c, const Few 
         }
       }
     }
+    const int64_t mine = v0 + lane / R * kMine;
+    float z[kMine];
 #pragma unroll
-    for (int e0 = 0; e0 < E; e0 += kAtOnce) {
+    for (int g = 0; g < kMine; ++g) {
       float v[32];
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
-        const float2 a = acc[e0 + i / R][i % R / 2];
+        const float2 a = acc[i / R * kMine + g][i % R / 2];
         v[i] = a.x, v[i + 1] = a.y;
       }
 #pragma unroll
@@ -368,27 +389,56 @@ __global__ void __launch_bounds__(kFewThreads, 1) k_few(const Call c, const Few 
 #pragma unroll
         for (int i = 0; i < o; ++i) {
           const bool high = lane & o;
-          const float mine = high ? v[i + o] : v[i], other = high ? v[i] : v[i + o];
-          v[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+          const float keep = high ? v[i + o] : v[i], send = high ? v[i] : v[i + o];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
-      const int64_t entry = v0 + e0 + lane / R;
-      const bool is = entry < c.vocab;
-      if (is && entry == label) f.z_label[first + row] = v[0];
-      merge(m, s, is ? v[0] : -INFINITY, is ? 1.f : 0.f);
+      z[g] = v[0];
+    }
+    if constexpr (PROBS) {
+      float p[kMine];
+#pragma unroll
+      for (int g = 0; g < kMine; ++g) {
+        p[g] = expf(z[g] - m) * s - (mine + g == label ? one : 0.f);
+        if (!live || mine + g >= c.vocab) p[g] = 0.f;
+      }
+      uint16_t* out = f.p + (first + row) * f.p_pitch + (mine - f.v0);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        uint32_t b[kMine / 2];
+#pragma unroll
+        for (int g = 0; g < kMine; g += 2) {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(p[g], p[g + 1]);
+          const float2 r = __bfloat1622float2(h);
+          b[g / 2] = *reinterpret_cast<const uint32_t*>(&h);
+          p[g] -= r.x, p[g + 1] -= r.y;
+        }
+        uint32_t* to = reinterpret_cast<uint32_t*>(out + k * c.n_pad * f.p_pitch);
+        if constexpr (kMine == 4) *reinterpret_cast<uint2*>(to) = make_uint2(b[0], b[1]);
+        else *to = b[0];
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < kMine; ++g) {
+        const bool is = mine + g < c.vocab;
+        if (is && mine + g == label) f.z_label[first + row] = z[g];
+        merge(m, s, is ? z[g] : -INFINITY, is ? 1.f : 0.f);
+      }
     }
   }
+  if constexpr (!PROBS) {
 #pragma unroll
-  for (int o = R; o < 32; o <<= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    merge(m, s, m2, s2);
-  }
-  if (lane < R) joined[warp][lane] = make_float2(m, s);
-  __syncthreads();
-  if (threadIdx.x < rows) {
-    float2 a = joined[0][threadIdx.x];
+    for (int o = R; o < 32; o <<= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      merge(m, s, m2, s2);
+    }
+    if (lane < R) joined[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+      float2 a = joined[0][threadIdx.x];
 #pragma unroll
-    for (int k = 1; k < kFewWarps; ++k) merge(a.x, a.y, joined[k][threadIdx.x].x, joined[k][threadIdx.x].y);
-    f.part[blockIdx.x * c.n_pad + first + threadIdx.x] = a;
+      for (int k = 1; k < kFewWarps; ++k) merge(a.x, a.y, joined[k][threadIdx.x].x, joined[k][threadIdx.x].y);
+      f.part[blockIdx.x * c.n_pad + first + threadIdx.x] = a;
+    }
   }
 }
 
@@ -477,7 +527,7 @@ constexpr int64_t kPieceBytes = int64_t(3) << 29;  // of P at a time
 struct Plan {
   Call c;
   bool copy_w;             // the weight is copied first (k_weight)
-  int few_rows;            // the forward's statistics by k_few: its rows a block (8, 16 or 32); or 0
+  int few_rows;            // z by k_few: its rows a block (8, 16 or 32); or 0
   int es;                  // bytes of an element of the caller's tensors
   int parts_v;             // (max, sum) pairs of a row
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
@@ -486,14 +536,20 @@ struct Plan {
   int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
   // scratch
   int64_t count, part, z_label, loss, fwd_bytes;
-  int64_t p, dxp, dwp, xr, r, scale, w, again, lse, bwd_bytes;
+  int64_t p, dxp, dwp, xr, r, scale, w, bwd_bytes;
 };
 
-// fp32 rows that k_few takes, in one turn of the weight or, where their x fills shared memory, two
-constexpr int64_t kFewRows = 32;
-int few_entries(const Plan& p) { return kFewWarps * (p.few_rows == 32 ? 4 : 8); }  // of a block's turn
-int few_blocks(const Plan& p) {
-  return (int)std::min<int64_t>((p.c.vocab + few_entries(p) - 1) / few_entries(p), 2 * tc_pairs());
+int few_blocks(const Plan& p, int64_t entries) {
+  const int turn = kFewWarps * (p.few_rows == 32 ? 4 : 8);  // of a block
+  return (int)std::min<int64_t>((entries + turn - 1) / turn, 2 * tc_pairs());
+}
+// Rows that a block of k_few takes of n: all of them where their x fits shared memory, or half of up to
+// 16; 0: none, their parts on the tensor cores take less.
+int few_rows(int64_t n, int width) {
+  const int64_t fit = kFewShared / (up(width, 128) * 4);
+  for (int r : {8, 16, 32})
+    if (r <= fit && (n <= r || (r == 8 && n <= 16 && fit < 16))) return r;
+  return 0;
 }
 
 const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
@@ -526,11 +582,8 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   const int64_t tiles_d = (c.pitch + kTile - 1) / kTile;
   if (tiles_v * tiles_m > (int64_t(1) << 30)) return "at most 2^30 tiles of 256 x 256 logits in a call";
   c.few = c.n <= 32 ? 32 : c.n <= 128 ? 128 : 0;
-  p->few_rows = !f32 || c.n > kFewRows ? 0 : c.n <= 8 ? 8 : c.n <= 16 ? 16 : 32;
-  while (p->few_rows && p->few_rows * up(c.width, 128) * 4 > kFewShared)
-    p->few_rows = p->few_rows > 8 ? p->few_rows / 2 : 0;
-  if (p->few_rows * 2 < c.n) p->few_rows = 0;
-  p->parts_v = p->few_rows ? few_blocks(*p) : tc_stats_parts(c);
+  p->few_rows = f32 ? few_rows(c.n, c.width) : 0;
+  p->parts_v = p->few_rows ? few_blocks(*p, c.vocab) : tc_stats_parts(c);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
   // come out in fewer turns of the whole GPU (the pieces' turns added up).
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * 2 * c.planes) / kTile);
@@ -586,8 +639,6 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->r = take(4 * c.n);
   p->scale = take(4);
   p->w = take(p->few_rows ? w_bytes : 0);
-  p->again = take(p->few_rows ? (int64_t)tc_stats_parts(c) * c.n_pad * 8 : 0);
-  p->lse = take(p->few_rows ? 8 * c.n : 0);
   p->bwd_bytes = at;
   return nullptr;
 }
@@ -636,48 +687,51 @@ void copy_weight(const GpaLossArgs* a, const Plan& p, char* to, cudaStream_t st)
       reinterpret_cast<typename Part<T>::type*>(to));
 }
 
-template <int R, int E>
+template <int R, int E, bool PROBS>
 bool few_as(const Plan& p, const Few& f, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may take its shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return false;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(k_few<R, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared) != cudaSuccess)
+    if (cudaFuncSetAttribute(k_few<R, E, PROBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared) !=
+        cudaSuccess)
       return false;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  Launch scope("loss_stats_few", st);
-  return launch_next(k_few<R, E>, dim3(p.parts_v, (unsigned)((p.c.n + R - 1) / R)), kFewThreads,
-                     (size_t)R * f.pitch * 4, st, p.c, f);
+  Launch scope(PROBS ? "loss_probs_few" : "loss_stats_few", st);
+  return launch_next(k_few<R, E, PROBS>, dim3(few_blocks(p, f.end - f.v0), (unsigned)((p.c.n + R - 1) / R)),
+                     kFewThreads, (size_t)R * f.pitch * 4, st, p.c, f);
 }
 
-// the losses to `each` (by the caller's rows), or their sum or mean to `total`
-bool join(const Plan& p, const float2* part, int parts, const float* z_label, float2* lse, float* each, float* packed,
-          float* total, const char* saved, int* counter, bool mean, cudaStream_t st) {
-  const Call& c = p.c;
-  const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;  // few rows: more lanes for the tiles of each
-  Launch scope("loss_join", st);
-  return launch_next(k_join, (unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st, c,
-                     part, parts, z_label, lse, each, reinterpret_cast<const int*>(saved + p.s_pos), packed, total, mean,
-                     counter);
+template <bool PROBS>
+bool few(const GpaLossArgs* a, const Plan& p, Few f, cudaStream_t st) {
+  f.w = static_cast<const float*>(a->weight);
+  f.w_stride = a->weight_stride;
+  f.pitch = (int)up(p.c.width, 128);
+  f.vec = a->width % 4 == 0 && f.w_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(f.w) & 15) == 0;
+  if (p.few_rows == 8) return few_as<8, 8, PROBS>(p, f, st);
+  return p.few_rows == 16 ? few_as<16, 8, PROBS>(p, f, st) : few_as<32, 4, PROBS>(p, f, st);
 }
 
 bool few_stats(const GpaLossArgs* a, const Plan& p, float2* part, float* z_label, cudaStream_t st) {
-  Few f;
-  f.w = static_cast<const float*>(a->weight);
-  f.x = static_cast<const float*>(a->hidden);
-  f.w_stride = a->weight_stride;
-  f.so = a->hidden_stride[0];
-  f.si = a->hidden_stride[1];
-  f.inner = std::max<int64_t>(a->inner, 1);
-  f.pitch = (int)up(p.c.width, 128);
-  f.vec = a->width % 4 == 0 && f.w_stride % 4 == 0 && f.so % 4 == 0 && f.si % 4 == 0 &&
-          ((reinterpret_cast<uintptr_t>(f.w) | reinterpret_cast<uintptr_t>(f.x)) & 15) == 0;
+  Few f = {};
+  f.end = p.c.vocab;
   f.part = part;
   f.z_label = z_label;
-  if (p.few_rows == 8) return few_as<8, 8>(p, f, st);
-  return p.few_rows == 16 ? few_as<16, 8>(p, f, st) : few_as<32, 4>(p, f, st);
+  return few<false>(a, p, f, st);
+}
+
+bool few_probs(const GpaLossArgs* a, const Plan& p, int64_t v0, int64_t vn, const float2* lse, void* to,
+               cudaStream_t st) {
+  Few f = {};
+  f.v0 = v0;
+  f.end = v0 + up(vn, 64);  // dx adds up whole blocks of entries, and dW of rows
+  f.lse = lse;
+  f.p = static_cast<uint16_t*>(to);
+  f.p_pitch = p.piece;
+  if (cudaMemset2DAsync(to, p.c.n_pad * p.piece * 2, 0, 64 * p.piece * 2, 3, st) != cudaSuccess) return false;
+  return few<true>(a, p, f, st);
 }
 
 template <typename T>
@@ -789,11 +843,16 @@ int loss_forward(const GpaLossArgs* a, float* loss, void* saved, size_t saved_by
   }
   if (c.n && p.few_rows && !few_stats(a, p, part, z_label, st)) FAIL("loss_stats_few launch failed");
   if (c.n && !p.few_rows && !tc_stats(c, part, z_label, st)) FAIL("loss_stats_tc5 launch failed");
-  if ((c.n || !none) &&
-      !join(p, part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
-            reinterpret_cast<float*>(sc + p.loss), loss, sv, reinterpret_cast<int*>(sv) + 1,
-            a->reduction == GPA_B200_LOSS_MEAN, st))
-    FAIL("loss_join launch failed");
+  if (c.n || !none) {
+    // few rows: more lanes for the tiles of each
+    const int rows = c.n >= 4096 ? 32 : c.n >= 256 ? 8 : 2;
+    Launch scope("loss_join", st);
+    if (!launch_next(k_join, (unsigned)std::max<int64_t>(1, (c.n + rows - 1) / rows), dim3(rows, 256 / rows), 0, st, c,
+                     part, p.parts_v, z_label, reinterpret_cast<float2*>(sv + p.s_lse), each,
+                     reinterpret_cast<const int*>(sv + p.s_pos), reinterpret_cast<float*>(sc + p.loss), loss,
+                     a->reduction == GPA_B200_LOSS_MEAN, reinterpret_cast<int*>(sv) + 1))
+      FAIL("loss_join launch failed");
+  }
   return GPA_B200_OK;
 }
 
@@ -827,20 +886,10 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   char* sc = static_cast<char*>(scratch);
   bind(&p, saved);
   const float2* lse = reinterpret_cast<const float2*>(sv + p.s_lse);
-  if (p.few_rows) {
-    // The products below read W in parts, and P is measured by statistics of the same logits: the
-    // forward's differ by fp32's rounding of sums, 1e-5 of P for a logit of 100, where P - 1 may be
-    // nothing.  The labels' logits and the losses, formed once more, are left where nothing lies yet.
+  if (p.few_rows && dhidden) {  // dx takes the weight in parts
     copy_weight<float>(a, p, sc + p.w, st);
     OK_OR("loss_weight launch failed");
     p.c.w = sc + p.w;
-    float2* again = reinterpret_cast<float2*>(sc + p.again);
-    float2* to = reinterpret_cast<float2*>(sc + p.lse);
-    float *z_label = reinterpret_cast<float*>(sc + p.r), *each = reinterpret_cast<float*>(sc + p.dxp);
-    if (!tc_stats(c, again, z_label, st)) FAIL("loss_stats_tc5 launch failed");
-    if (!join(p, again, tc_stats_parts(c), z_label, to, each, nullptr, nullptr, sv, nullptr, false, st))
-      FAIL("loss_join launch failed");
-    lse = to;
   }
   void* pr = sc + p.p;
   float* dxp = reinterpret_cast<float*>(sc + p.dxp);
@@ -868,7 +917,8 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
   const bool in_place = c.width == c.pitch && (reinterpret_cast<uintptr_t>(dweight) & (p.es == 4 ? 31 : 15)) == 0;
   for (int64_t v0 = 0; v0 < c.vocab; v0 += p.piece) {
     const int64_t vn = std::min(p.piece, c.vocab - v0);
-    if (!tc_probs(c, v0, vn, lse, pr, p.piece, st)) FAIL("loss_probs_tc5 launch failed");
+    if (p.few_rows ? !few_probs(a, p, v0, vn, lse, pr, st) : !tc_probs(c, v0, vn, lse, pr, p.piece, st))
+      FAIL("loss_probs launch failed");
     if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.split.most, v0 > 0, dxp, part_stride, st))
       FAIL("loss_dx_tc5 launch failed");
     if (!dweight) continue;

@@ -528,7 +528,7 @@ def test_a_token_that_has_all_the_probability(dtype, rows, width, big):
 @pytest.mark.parametrize("rows,width,vocab", [
     (1, 1, 1), (1, 4, 5), (7, 3, 63), (8, 128, 64), (8, 6144, 700), (8, 6200, 300), (9, 130, 65), (9, 3100, 500),
     (16, 1001, 5003), (16, 3200, 129), (17, 1500, 1187), (17, 1700, 300), (31, 64, 4800), (32, 2900, 333),
-    (32, 3200, 333), (32, 127, 9999),
+    (32, 3200, 333), (32, 127, 9999), (12, 3700, 300), (32, 1792, 400), (32, 1793, 400), (8, 7168, 200), (8, 7200, 200),
 ])
 @pytest.mark.parametrize("masked", [0.0, 0.5])
 def test_few_fp32_rows(rows, width, vocab, masked):
