@@ -112,23 +112,14 @@ def _rows(t: Tensor):
     return _rows(t.contiguous())
 
 
-def _kept(tensors, as_saved):
-    """Saved tensors, checked for what the kernels take from the forward: whoever kept them
-    meanwhile (hooks on saved tensors, sharded parameters) may bring them back at another address
-    and with other strides, but not with another shape, type or device."""
-    for t, want in zip(tensors, as_saved):
-        if t is not None and (t.shape, t.dtype, t.device) != want:
-            raise RuntimeError(f"a saved tensor came back as {t.dtype} {list(t.shape)} on {t.device}, not "
-                               f"as {want[1]} {list(want[0])} on {want[2]}")
-    return tensors
+def _altered(t, shape, dtype, index):
+    """Whether a saved tensor is not what the kernels take from the forward: whoever kept it meanwhile
+    (hooks on saved tensors, sharded parameters) may bring it back at another address and with other
+    strides, but not with another shape, type or device."""
+    return t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != index)
 
 
-def _as_saved(*tensors):
-    return tuple(None if t is None else (t.shape, t.dtype, t.device) for t in tensors)
-
-
-def _stride(t):
-    return None if t is None else t.stride()
+_ALTERED = "a saved tensor came back with another shape, type or device than it was saved with"
 
 
 def _dense(t):
@@ -208,14 +199,16 @@ class _RMSNorm(torch.autograd.Function):
         ctx.save_for_backward(x, weight)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args if args[1][1] is x else None
-        ctx.as_saved, ctx.stride = _as_saved(x, weight), x.stride()
-        ctx.eps, ctx.out_dtype = eps, out_dtype
+        ctx.stride, ctx.dtype, ctx.eps, ctx.out_dtype = x.stride(), x.dtype, eps, out_dtype
         return _rms_forward(x, weight, eps, out_dtype, args)
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
-        x, weight = _kept(ctx.saved_tensors, ctx.as_saved)
+        x, weight = ctx.saved_tensors
+        shape, index = dout.shape, dout.get_device()
+        if _altered(x, shape, ctx.dtype, index) or _altered(weight, shape[-1:], torch.float32, index):
+            raise RuntimeError(_ALTERED)
         weight = _dense(weight)
         dx = torch.empty_like(x, memory_format=_DENSE)
         if not x.numel():
@@ -280,9 +273,9 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args[0] if args[1][1] is update and args[1][2] is gate else None
-        ctx.as_saved = _as_saved(stream, update, weight, post_weight, gate, scale)
-        ctx.strides = update.stride() if read else None, _stride(gate)
-        ctx.update_dtype = update.dtype
+        ctx.strides = update.stride() if read else None, None if gate is None else gate.stride()
+        ctx.dtype, ctx.update_dtype = residual.dtype, update.dtype
+        ctx.gate = None if gate is None else (gate.shape, gate.dtype)
         ctx.eps, ctx.const, ctx.out_dtype = eps, const, out_dtype
         ctx.set_materialize_grads(False)
         return stream, normed
@@ -292,8 +285,17 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dstream, dnormed):
         if dstream is None and dnormed is None:
             return (None,) * 9
-        stream, update, weight, post_weight, gate, scale = _kept(ctx.saved_tensors, ctx.as_saved)
-        stream, weight, post_weight, scale = map(_dense, (stream, weight, post_weight, scale))
+        stream, update, weight, post_weight, gate, scale = ctx.saved_tensors
+        up = dnormed if dstream is None else dstream
+        shape, index = up.shape, up.get_device()
+        vector = shape[-1:]
+        if (_altered(stream, shape, ctx.dtype, index) or _altered(weight, vector, torch.float32, index) or
+                _altered(update, shape, ctx.update_dtype, index) or
+                _altered(post_weight, vector, torch.float32, index) or
+                _altered(scale, vector, torch.float32, index) or
+                gate is not None and _altered(gate, *ctx.gate, index)):
+            raise RuntimeError(_ALTERED)
+        stream, weight, post_weight, scale = _dense(stream), _dense(weight), _dense(post_weight), _dense(scale)
         need = ctx.needs_input_grad
         dres = torch.empty_like(stream) if need[0] else None
         dupd = torch.empty_like(stream, dtype=ctx.update_dtype) if need[1] else None
@@ -307,7 +309,8 @@ class _ResidualNorm(torch.autograd.Function):
         dstream = None if dstream is None else dstream.contiguous()
         dnormed = None if dnormed is None else dnormed.contiguous()
         a, keep = ctx.args, None
-        if a is None or (_stride(update), _stride(gate)) != ctx.strides:
+        strides = None if update is None else update.stride(), None if gate is None else gate.stride()
+        if a is None or strides != ctx.strides:
             a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
                                  stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
         else:  # the tensors may have moved
@@ -433,21 +436,23 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss, saved, ctx.args = _loss_forward(hidden, weight, labels, ignore_index, reduction, True)
         # the labelled rows are packed into `saved`: hidden and labels are not needed again
         ctx.save_for_backward(weight, saved)
-        ctx.as_saved, ctx.stride = _as_saved(weight, saved), weight.stride()
-        ctx.hidden = hidden.shape, hidden.dtype
+        ctx.hidden, ctx.weight, ctx.saved = (hidden.shape, hidden.dtype), (weight.shape, weight.stride()), saved.numel()
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
     @staticmethod
     @_first_order
     def backward(ctx, dloss):
-        weight, saved = _kept(ctx.saved_tensors, ctx.as_saved)
+        weight, saved = ctx.saved_tensors
+        (shape, dtype), (weight_shape, stride) = ctx.hidden, ctx.weight
+        index = dloss.get_device()
+        if _altered(weight, weight_shape, dtype, index) or _altered(saved, (ctx.saved,), torch.uint8, index):
+            raise RuntimeError(_ALTERED)
         saved = _dense(saved)
-        shape, dtype = ctx.hidden
         lib = _lib.load()
         dev = weight.device
         a, keep = ctx.args, None
-        if a is None or weight.stride() != ctx.stride or weight.data_ptr() != a.weight:
+        if a is None or weight.stride() != stride or weight.data_ptr() != a.weight:
             a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
             if lib.gpa_b200_loss_saved_bytes(a) > saved.numel():
                 # the forward read the weight in place; where it is now that takes a copy of it
