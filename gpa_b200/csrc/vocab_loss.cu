@@ -585,15 +585,16 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   p->few_rows = f32 ? few_rows(c.n, c.width) : 0;
   p->parts_v = p->few_rows ? few_blocks(*p, c.vocab) : tc_stats_parts(c);
   // A piece is as large as its buffer allows, or somewhat smaller where the tiles of dW then
-  // come out in fewer turns of the whole GPU (the pieces' turns added up).
+  // come out in fewer turns of the whole GPU (the pieces' turns added up; one piece has the fewest).
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (c.n_pad * 2 * c.planes) / kTile);
   int64_t best = std::min(tiles_v, most), turns = INT64_MAX;
   auto turns_of = [&](int64_t t) {
     auto one = [&](int64_t v) { return (v * tiles_d + at_once - 1) / at_once; };
     return tiles_v / t * one(t) + (tiles_v % t ? one(tiles_v % t) : 0);
   };
-  for (int64_t t = best; t >= 1 && t >= std::min(tiles_v, most) / 2; --t)
-    if (turns_of(t) < turns) turns = turns_of(t), best = t;
+  if (tiles_v > most)
+    for (int64_t t = best; t >= 1 && t >= most / 2; --t)
+      if (turns_of(t) < turns) turns = turns_of(t), best = t;
   p->piece = best * kTile;
   // dx: at most one part for every 512 entries, and 256 MB of them in all beside the first; the last
   // one holds what is left.  Cut by the blocks that the first piece has, not by its tiles: every part

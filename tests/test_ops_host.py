@@ -340,3 +340,9 @@ def test_loss_backward_without_rows_needs_no_gradient_to_write():
     a = _loss_args(outer=0)
     saved, scratch = lib.gpa_b200_loss_saved_bytes(a), lib.gpa_b200_loss_scratch_bytes(a, 1)
     assert lib.gpa_b200_loss_backward(a, 32, saved, None, None, None, 32, scratch, None) == 0
+
+
+def test_a_vocabulary_that_one_piece_holds_is_one_piece():
+    for rows, vocab, dtype in ((1, 1, 1), (300, 151936, 1), (4096, 151936, 2), (2000, 100001, 0), (256, 1 << 21, 1)):
+        assert _cut(rows, rows, 64, vocab, dtype)[0] == vocab
+    assert _cut(65536, 65536, 64, 151936, 1)[0] < 151936
