@@ -565,3 +565,45 @@ def test_gradients_of_extreme_logits(lead, dtype):
     (vx, bx), (vw, bw) = want["dhidden"], want["dweight"]
     _check("dhidden", dx, (vx, bx + 2.0 ** -126 * g * wd.abs().sum(0)))
     _check("dweight", dw, (vw, bw + 2.0 ** -126 * (g * xd.abs()).sum(0)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lead", [(5,), (20,), (100,), (300,)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_captured_steps_of_every_form_replay(lead, dtype, reduction):
+    """Each form of the products, captured and replayed on new values, equals eager calls."""
+    x, w, y = _inputs(60, lead, 72, 700, dtype, 0.2)
+    other = _inputs(61, lead, 72, 700, dtype, 0.5)
+    up = torch.randn(lead if reduction == "none" else (), generator=torch.Generator().manual_seed(1)).cuda()
+
+    def step(x, w, y):
+        loss = linear_cross_entropy(x, w, y, reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), up))
+
+    held = x.clone().requires_grad_(), w.clone().requires_grad_(), y.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*held)
+    for values in (other, (x, w, y)):
+        with torch.no_grad():
+            for a, b in zip(held, values):
+                a.copy_(b)
+        graph.replay()
+        want = step(*(t.clone().requires_grad_() for t in values[:2]), values[2])
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_very_many_rows_without_labels(dtype):
+    n = (1 << 16) + 300
+    x, w, y = _inputs(62, (n,), 24, 90, dtype)
+    keep = torch.randperm(n, generator=torch.Generator().manual_seed(2))[:200].cuda()
+    few = torch.full_like(y, -100)
+    few[keep] = y[keep]
+    loss, dx, dw, up = _run(x, w, few, "mean")
+    order = few != -100
+    _, sx, sw, _ = _run(x[order], w, few[order], "mean")
+    assert torch.equal(dw, sw) and torch.equal(dx[order], sx) and not dx[~order].any()
+    loss, dx, dw, up = _run(x, w, torch.full_like(y, -100), "mean")
+    assert not loss and not dx.any() and not dw.any()
