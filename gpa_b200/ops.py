@@ -112,11 +112,19 @@ def _rows(t: Tensor):
     return _rows(t.contiguous())
 
 
+def _places(*tensors):
+    """Where the kernels find tensors, to tell whether saved ones are still there in the backward;
+    None where hooks keep them meanwhile, which may bring anything back to the same place."""
+    if torch._C._autograd._top_saved_tensors_default_hooks(False) is not None:
+        return None
+    return [None if t is None else t.data_ptr() for t in tensors]
+
+
 def _altered(t, shape, dtype, index):
     """Whether a saved tensor is not what the kernels take from the forward: whoever kept it meanwhile
     (hooks on saved tensors, sharded parameters) may bring it back at another address and with other
     strides, but not with another shape, type or device."""
-    return t is not None and (t.shape != shape or t.dtype != dtype or t.get_device() != index)
+    return t is not None and (t.shape != shape or t.dtype is not dtype or t.get_device() != index)
 
 
 _ALTERED = "a saved tensor came back with another shape, type or device than it was saved with"
@@ -198,27 +206,26 @@ class _RMSNorm(torch.autograd.Function):
         args = _rms_args(x, weight, eps, out_dtype)
         ctx.save_for_backward(x, weight)
         # the arguments serve the backward too, unless they point to a copy made for this call
-        ctx.args = args if args[1][1] is x else None
-        ctx.stride, ctx.dtype, ctx.eps, ctx.out_dtype = x.stride(), x.dtype, eps, out_dtype
+        ctx.args = args[0] if args[1][1] is x else None
+        ctx.places, ctx.stride = _places(x, weight), x.stride()
+        ctx.dtype, ctx.eps, ctx.out_dtype = x.dtype, eps, out_dtype
         return _rms_forward(x, weight, eps, out_dtype, args)
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
         x, weight = ctx.saved_tensors
-        shape, index = dout.shape, dout.get_device()
-        if _altered(x, shape, ctx.dtype, index) or _altered(weight, shape[-1:], torch.float32, index):
-            raise RuntimeError(_ALTERED)
-        weight = _dense(weight)
+        a, keep = ctx.args, None
+        if a is None or [x.data_ptr(), weight.data_ptr()] != ctx.places or x.stride() != ctx.stride:
+            shape, index = dout.shape, dout.get_device()
+            if _altered(x, shape, ctx.dtype, index) or _altered(weight, shape[-1:], torch.float32, index):
+                raise RuntimeError(_ALTERED)
+            weight = _dense(weight)
+            a, keep = _rms_args(x, weight, ctx.eps, ctx.out_dtype)
         dx = torch.empty_like(x, memory_format=_DENSE)
         if not x.numel():
             return dx, torch.zeros_like(weight), None, None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        if ctx.args and x.stride() == ctx.stride:
-            a, keep = ctx.args
-            a.update, a.weight = x.data_ptr(), weight.data_ptr()  # which may have moved
-        else:
-            a, keep = _rms_args(x, weight, ctx.eps, ctx.out_dtype)
         _norm_backward(a, x.device, None, None, dout.contiguous(), (None, dx, None, dw, None, None))
         return dx, dw, None, None
 
@@ -273,6 +280,7 @@ class _ResidualNorm(torch.autograd.Function):
         ctx.save_for_backward(stream, update if read else None, weight, post_weight, gate, scale)
         # the arguments serve the backward too, unless they point to a copy made for this call
         ctx.args = args[0] if args[1][1] is update and args[1][2] is gate else None
+        ctx.places = _places(stream, update if read else None, weight, post_weight, gate, scale)
         ctx.strides = update.stride() if read else None, None if gate is None else gate.stride()
         ctx.dtype, ctx.update_dtype = residual.dtype, update.dtype
         ctx.gate = None if gate is None else (gate.shape, gate.dtype)
@@ -285,17 +293,23 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dstream, dnormed):
         if dstream is None and dnormed is None:
             return (None,) * 9
-        stream, update, weight, post_weight, gate, scale = ctx.saved_tensors
-        up = dnormed if dstream is None else dstream
-        shape, index = up.shape, up.get_device()
-        vector = shape[-1:]
-        if (_altered(stream, shape, ctx.dtype, index) or _altered(weight, vector, torch.float32, index) or
-                _altered(update, shape, ctx.update_dtype, index) or
-                _altered(post_weight, vector, torch.float32, index) or
-                _altered(scale, vector, torch.float32, index) or
-                gate is not None and _altered(gate, *ctx.gate, index)):
-            raise RuntimeError(_ALTERED)
-        stream, weight, post_weight, scale = _dense(stream), _dense(weight), _dense(post_weight), _dense(scale)
+        saved = ctx.saved_tensors
+        stream, update, weight, post_weight, gate, scale = saved
+        a, keep = ctx.args, None
+        strides = None if update is None else update.stride(), None if gate is None else gate.stride()
+        if a is None or [None if t is None else t.data_ptr() for t in saved] != ctx.places or strides != ctx.strides:
+            up = dnormed if dstream is None else dstream
+            shape, index = up.shape, up.get_device()
+            vector = shape[-1:]
+            if (_altered(stream, shape, ctx.dtype, index) or _altered(weight, vector, torch.float32, index) or
+                    _altered(update, shape, ctx.update_dtype, index) or
+                    _altered(post_weight, vector, torch.float32, index) or
+                    _altered(scale, vector, torch.float32, index) or
+                    gate is not None and _altered(gate, *ctx.gate, index)):
+                raise RuntimeError(_ALTERED)
+            stream, weight, post_weight, scale = map(_dense, (stream, weight, post_weight, scale))
+            a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
+                                 stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
         need = ctx.needs_input_grad
         dres = torch.empty_like(stream) if need[0] else None
         dupd = torch.empty_like(stream, dtype=ctx.update_dtype) if need[1] else None
@@ -308,14 +322,6 @@ class _ResidualNorm(torch.autograd.Function):
             return dres, dupd, dw, dpw, dgate, dscale, None, None, None
         dstream = None if dstream is None else dstream.contiguous()
         dnormed = None if dnormed is None else dnormed.contiguous()
-        a, keep = ctx.args, None
-        strides = None if update is None else update.stride(), None if gate is None else gate.stride()
-        if a is None or strides != ctx.strides:
-            a, keep = _norm_args(stream, update, weight, post_weight, gate, scale, ctx.eps, ctx.const,
-                                 stream.dtype, ctx.update_dtype, ctx.out_dtype, stream.shape)
-        else:  # the tensors may have moved
-            a.update, a.weight, a.gate = _lib.ptr(update), weight.data_ptr(), _lib.ptr(gate)
-            a.post_weight, a.scale = _lib.ptr(post_weight), _lib.ptr(scale)
         _norm_backward(a, stream.device, stream, dstream, dnormed, (dres, dupd, dgate, dw, dpw, dscale))
         return dres, dupd, dw, dpw, dgate, dscale, None, None, None
 
@@ -437,6 +443,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         # the labelled rows are packed into `saved`: hidden and labels are not needed again
         ctx.save_for_backward(weight, saved)
         ctx.hidden, ctx.weight, ctx.saved = (hidden.shape, hidden.dtype), (weight.shape, weight.stride()), saved.numel()
+        ctx.places = _places(weight, saved)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
 
@@ -445,14 +452,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, dloss):
         weight, saved = ctx.saved_tensors
         (shape, dtype), (weight_shape, stride) = ctx.hidden, ctx.weight
-        index = dloss.get_device()
-        if _altered(weight, weight_shape, dtype, index) or _altered(saved, (ctx.saved,), torch.uint8, index):
-            raise RuntimeError(_ALTERED)
-        saved = _dense(saved)
         lib = _lib.load()
         dev = weight.device
         a, keep = ctx.args, None
-        if a is None or weight.stride() != stride or weight.data_ptr() != a.weight:
+        if a is None or [weight.data_ptr(), saved.data_ptr()] != ctx.places or weight.stride() != stride:
+            index = dloss.get_device()
+            if _altered(weight, weight_shape, dtype, index) or _altered(saved, (ctx.saved,), torch.uint8, index):
+                raise RuntimeError(_ALTERED)
+            saved = _dense(saved)
             a, keep = _loss_args(weight, shape, dtype, ctx.ignore_index, ctx.reduction)
             if lib.gpa_b200_loss_saved_bytes(a) > saved.numel():
                 # the forward read the weight in place; where it is now that takes a copy of it

@@ -5,6 +5,7 @@ import contextlib
 import ctypes
 import math
 import random
+import weakref
 
 import pytest
 import torch
@@ -346,3 +347,18 @@ def test_a_vocabulary_that_one_piece_holds_is_one_piece():
     for rows, vocab, dtype in ((1, 1, 1), (300, 151936, 1), (4096, 151936, 2), (2000, 100001, 0), (256, 1 << 21, 1)):
         assert _cut(rows, rows, 64, vocab, dtype)[0] == vocab
     assert _cut(65536, 65536, 64, 151936, 1)[0] < 151936
+
+
+def test_nothing_is_kept_that_hooks_on_saved_tensors_took_away(monkeypatch):
+    """What such a hook moves elsewhere is free for the allocator until the backward."""
+    _Calls(monkeypatch)
+    leaf, w, e = torch.randn(4, 32, requires_grad=True), torch.ones(32, requires_grad=True), torch.randn(50, 32)
+    for op in (lambda t: rms_norm(t, w), lambda t: residual_norm(t.detach(), t, w, post_weight=w)[0],
+               lambda t: linear_cross_entropy(t, e, torch.zeros(4, dtype=torch.long))):
+        x = leaf * 1
+        gone = weakref.ref(x)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t):
+            out = op(x)
+        del x
+        assert gone() is None
+        out.backward(torch.ones_like(out))
