@@ -523,6 +523,8 @@ __global__ void k_finish(const float* __restrict__ part, int64_t part_stride, co
 
 // ------------------------------------------------------------------ plan of a call
 constexpr int64_t kPieceBytes = int64_t(3) << 29;  // of P at a time
+// Of dW in padded rows at a time, where it takes these: 128 MB would cost 32 x 1925 x 111314 fp32 5 %.
+constexpr int64_t kPaddedBytes = int64_t(1) << 29;
 
 struct Plan {
   Call c;
@@ -531,6 +533,7 @@ struct Plan {
   int es;                  // bytes of an element of the caller's tensors
   int parts_v;             // (max, sum) pairs of a row
   int64_t piece;           // vocabulary entries of a piece (a multiple of kTile)
+  int64_t padded;          // and of dW's padded rows (likewise)
   Split split;             // of the reduction of dx
   // saved
   int64_t s_row, s_label, s_pos, s_lse, s_x, s_w, s_bytes;
@@ -635,7 +638,8 @@ const char* plan_of(const GpaLossArgs* a, Plan* p, int* code) {
   at = 0;
   p->p = take(c.planes * c.n_pad * p->piece * 2);
   p->dxp = take((int64_t)p->split.most * c.n_pad * c.pitch * 4);
-  p->dwp = take(p->piece * c.pitch * p->es);
+  p->padded = std::min(p->piece, std::max<int64_t>(1, kPaddedBytes / (c.pitch * p->es) / kTile) * kTile);
+  p->dwp = take(p->padded * c.pitch * p->es);
   p->xr = take(a->reduction == GPA_B200_LOSS_NONE ? c.planes * c.n_pad * c.pitch * 2 : 0);
   p->r = take(4 * c.n);
   p->scale = take(4);
@@ -923,12 +927,17 @@ int loss_backward(const GpaLossArgs* a, const void* saved, size_t saved_bytes, c
     if (dhidden && !tc_dx(c, pr, p.piece, v0, vn, p.split.most, v0 > 0, dxp, part_stride, st))
       FAIL("loss_dx_tc5 launch failed");
     if (!dweight) continue;
-    char* dw = static_cast<char*>(dweight) + v0 * c.width * p.es;
-    if (!tc_dw(c, pr, p.piece, v0, vn, x, up_w, in_place ? dw : sc + p.dwp, c.pitch, st)) FAIL("loss_dw_tc5 launch failed");
-    if (!in_place) {
+    const int64_t some = in_place ? vn : p.padded;
+    for (int64_t u0 = 0; u0 < vn; u0 += some) {
+      const int64_t un = std::min(some, vn - u0);
+      char* dw = static_cast<char*>(dweight) + (v0 + u0) * c.width * p.es;
+      if (!tc_dw(c, static_cast<char*>(pr) + 2 * u0, p.piece, v0 + u0, un, x, up_w, in_place ? dw : sc + p.dwp,
+                 c.pitch, st))
+        FAIL("loss_dw_tc5 launch failed");
+      if (in_place) continue;
       Launch scope("loss_unpad", st);
-      BY_TYPE(a->dtype, (k_unpad<T><<<(unsigned)((vn + 7) / 8), 256, 0, st>>>(
-                            reinterpret_cast<const T*>(sc + p.dwp), c.pitch, vn, c.width, reinterpret_cast<T*>(dw))));
+      BY_TYPE(a->dtype, (k_unpad<T><<<(unsigned)((un + 7) / 8), 256, 0, st>>>(
+                            reinterpret_cast<const T*>(sc + p.dwp), c.pitch, un, c.width, reinterpret_cast<T*>(dw))));
       OK_OR("loss_unpad launch failed");
     }
   }

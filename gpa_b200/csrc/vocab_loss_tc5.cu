@@ -1061,7 +1061,8 @@ bool tc_dw(const Call& c, const void* p, int64_t p_pitch, int64_t v0, int64_t vn
            void* dw, int64_t dw_pitch, cudaStream_t st) {
   const bool f16 = c.dtype == GPA_B200_F16;
   CUtensorMap ma, mb;
-  if (!make_map(&ma, p, p_pitch, c.planes * c.n_pad, p_pitch, kBK, f16) ||
+  // p may start inside the piece: no more columns than are read
+  if (!make_map(&ma, p, vloss::up(vn, kTile), c.planes * c.n_pad, p_pitch, kBK, f16) ||
       !make_map(&mb, x, c.pitch, c.planes * c.n_pad, c.pitch, kBK, f16))
     return false;
   Args a = base_args(c);

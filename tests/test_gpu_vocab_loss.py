@@ -607,3 +607,16 @@ def test_very_many_rows_without_labels(dtype):
     assert torch.equal(dw, sw) and torch.equal(dx[order], sx) and not dx[~order].any()
     loss, dx, dw, up = _run(x, w, torch.full_like(y, -100), "mean")
     assert not loss and not dx.any() and not dw.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [10, 50, 150])
+def test_weight_gradient_of_odd_rows_in_turns(rows, dtype):
+    """dW of rows that are no multiple of 8 channels passes through padded ones, 512 MB at a time: the
+    same values as of rows that are padded with zeros to begin with, which stay where they are."""
+    x, w, y = _inputs(rows, (rows,), 4001, 70001, dtype, 0.2)
+    loss, dx, dw, _ = _run(x, w, y, "mean")
+    wide = [torch.nn.functional.pad(t, (0, 7)) for t in (x, w)]
+    got = _run(*wide, y, "mean")
+    assert torch.equal(loss, got[0]) and torch.equal(dx, got[1][:, :-7]) and torch.equal(dw, got[2][:, :-7])
+    assert not got[1][:, -7:].any() and not got[2][:, -7:].any()

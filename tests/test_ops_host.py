@@ -362,3 +362,12 @@ def test_nothing_is_kept_that_hooks_on_saved_tensors_took_away(monkeypatch):
         del x
         assert gone() is None
         out.backward(torch.ones_like(out))
+
+
+def test_loss_workspace_does_not_grow_with_the_weight():
+    """Beside 1.5 GB of P and 256 MB of parts of dhidden: 512 MB of a wide weight's gradient at most."""
+    lib = _lib.load()
+    for rows, width, vocab, dtype in ((64, 8192, 151936, 1), (200, 4097, 151936, 1), (300, 8192, 151936, 0),
+                                      (4096, 5001, 151936, 2)):
+        a = _loss_args(outer=1, inner=rows, width=width, vocab=vocab, weight_stride=width, dtype=dtype)
+        assert lib.gpa_b200_loss_scratch_bytes(a, 1) < 2.6e9, (rows, width)
